@@ -66,8 +66,14 @@ enum {
   KH_FAM_GEMM = 3, /* [batched] matmul + epilogue tape, MFMA                  */
   KH_FAM_GEMV = 4, /* M = 1 matmul + epilogue tape                            */
   KH_FAM_RED = 5,  /* reduction over non-innermost dims                       */
-  KH_FAM_ATTN = 6  /* fused scores -> softmax -> x V (the lowering's pattern)  */
+  KH_FAM_ATTN = 6, /* fused scores -> softmax -> x V (the lowering's pattern)  */
+  KH_FAM_PAGED = 7 /* operators over a paged key/value cache (kh_paged)        */
 };
+
+/* element types of a paged cache and of the activations next to it */
+enum { KH_TYPE_F32 = 0, KH_TYPE_BF16 = 1, KH_TYPE_F16 = 2 };
+/* operators of the paged family */
+enum { KH_PAGED_ATTENTION = 0, KH_PAGED_SELECT = 1 };
 
 /* attention family: how the scores are scaled and masked before the softmax */
 enum { KH_ATTN_MASK_NONE = 0, KH_ATTN_MASK_CAUSAL = 1, KH_ATTN_MASK_ADD = 2 };
@@ -225,6 +231,22 @@ typedef struct kh_pass {
  * with cfg[6] = KH_PAIR_F16: scaled by fparams[3]. Scales are
  * powers of two; the caller guarantees that scaled values stay below 65504.
  */
+/*
+ *   PAGED (family 7; the operators of kh_paged below as launches of a plan)
+ *        variant = KH_PAGED_ATTENTION or KH_PAGED_SELECT; shape = {batch, draft,
+ *        heads, kv_heads, dim, page size}; gemm = {pages of the pool, columns
+ *        of the table, picked pages per token (0: every page is read), 0};
+ *        cfg[0] = cache type, cfg[1] = activation type (KH_TYPE_*), cfg[2] = 1:
+ *        products on the cache type's own matrix instruction, one pass;
+ *        fparams[0] = scale. Refs, strides in elements of their own type:
+ *        ATTENTION 0 q, 1 k, 2 v over (sequence, token, head, d), 3, 4 the
+ *        pages over (page, head, slot, d), 5 table over (sequence, column),
+ *        6 lengths, 7 out (as q), then refs[cfg[3]] parents over (sequence,
+ *        token) and refs[cfg[4]] the picked pages over (sequence, token, kv
+ *        head, rank), where cfg[3], cfg[4] are not 0. SELECT 0 q, 1 the
+ *        pages' means over (page, head, d), 2 table, 3 lengths, 4 out over
+ *        (sequence, token, kv head, rank). Innermost strides are 1.
+ */
 typedef struct kh_launch {
   int32_t family;
   int32_t variant;
@@ -346,6 +368,106 @@ int kh_plan_chain_timeouts(kh_plan *plan, uint64_t *timeouts);
  * normally. No counterpart in the reference. */
 int kh_plan_chain_spin(kh_plan *plan, int64_t ticks);
 int kh_plan_destroy(kh_plan *plan);
+
+/*
+ * Operators over a paged key/value cache. No counterpart in the reference,
+ * whose graphs keep no state between calls.
+ *
+ * The pages are [pages][kv_heads][page_size][dim] (any strides; dim's is 1):
+ * sequence s's token t lies in page table[s][t / page_size] at slot
+ * t % page_size, for t < lengths[s]. page_size is a power of two from 16 to
+ * 1024, dim a multiple of 8 up to 256, heads a multiple of kv_heads. A table
+ * entry outside [0, pages) holds no tokens; lengths outside [0, width *
+ * page_size] are taken as the nearest of the two.
+ *
+ * kh_paged_attention: `draft` new tokens per sequence, whose k and v (rounded
+ * to the cache's type first) are not in the cache. parents[s][i] in [-1, i)
+ * names the new token that i follows, -1 the end of the cached context; any
+ * other value marks token i, and those that follow it, as unused: their rows
+ * of `out` are zeros. parents = NULL: token i follows i - 1. Query (s, i, h)
+ * attends to the cached tokens of s - with `selected`, to those of the pages
+ * (columns of the table) selected[s][i][kv head][0..top) alone - and to the
+ * new tokens on its own path, itself included:
+ *   out = softmax(scale q . k) v.
+ * An entry of `selected` counts only where it is larger than the entry before
+ * it (the first: than -1) and below width. Sums, softmax statistics and
+ * products of fp32 activations are kept to fp32 (bf16 and fp16 caches: q and
+ * the weights split into 3 and 2 parts, whose products are exact); with
+ * act_type = cache_type = bf16 or fp16, or one_pass = 1, the weights are
+ * rounded to the cache's type for the second product (one_pass: q too).
+ *
+ * kh_paged_select: for query token (s, i) and kv head c the `top` pages with
+ * the largest (sum of the group's queries) . k_means[page][c], products and
+ * sums in 64 bits, the page of the last cached token always among them; ties
+ * go to the lower page, a NaN counts as the lowest score. selected receives
+ * the pages' columns, ascending, then -1.
+ *
+ * All pointers are device pointers on the device of `stream`; 16-byte aligned
+ * rows of q, k, v, pages and out, 4-byte aligned else. The workspace may be
+ * reused by any later call on the same stream. kh_paged_host runs the
+ * operators' meaning on the CPU over host pointers (a test instrument, as
+ * kh_plan_run_host).
+ */
+typedef struct kh_paged {
+  int32_t variant;                        /* KH_PAGED_*                             */
+  int32_t batch, draft, heads, kv_heads, dim, page_size, pages, width, top;
+  int32_t cache_type, act_type, one_pass; /* KH_TYPE_*                              */
+  float scale;
+  const void *q, *k, *v, *k_pages, *v_pages;
+  const float *k_means;
+  const int32_t *table, *lengths, *parents;
+  int32_t *selected;                      /* read by attention, written by select   */
+  void *out;
+  int64_t q_s, q_n, q_h, k_s, k_n, k_h, v_s, v_n, v_h, o_s, o_n, o_h;  /* strides in elements */
+  int64_t kp_p, kp_h, kp_t, vp_p, vp_h, vp_t, m_p, m_h;
+  int64_t table_s, parents_s, sel_s, sel_n, sel_h;
+} kh_paged;
+/* sizeof(kh_paged), sizeof(kh_cache_append_op), sizeof(kh_pool) */
+int kh_paged_sizes(size_t *sizes3);
+int kh_paged_workspace_bytes(const kh_paged *op, size_t *bytes);
+int kh_paged_run(const kh_paged *op, void *workspace, size_t workspace_bytes, void *stream);
+int kh_paged_host(const kh_paged *op);
+
+/*
+ * kh_cache_append: the rows new[rows[s][a]] of k and v (a < accept while
+ * rows[s][a] is in [0, draft); rows = NULL: rows 0 .. draft) written as tokens
+ * lengths[s] + a of sequence s, rounded to the cache's type, in each of
+ * `layers` layers; with k_means, the mean key of every page written to, over
+ * the tokens it then holds. Tokens whose page the table does not name (an
+ * entry outside [0, pages), a column outside its width, a negative length)
+ * are dropped. No page may be written through two sequences of one call.
+ */
+typedef struct kh_cache_append_op {
+  int32_t layers, batch, draft, accept, kv_heads, dim, page_size, pages, width;
+  int32_t cache_type, act_type;
+  const void *k, *v;
+  void *k_pages, *v_pages;
+  float *k_means;
+  const int32_t *table, *lengths, *rows;
+  int64_t k_l, k_s, k_n, k_h, v_l, v_s, v_n, v_h;
+  int64_t kp_l, kp_p, kp_h, kp_t, vp_l, vp_p, vp_h, vp_t, m_l, m_p, m_h;
+  int64_t table_s, rows_s;
+} kh_cache_append_op;
+int kh_cache_append(const kh_cache_append_op *op, void *stream);
+int kh_cache_append_host(const kh_cache_append_op *op);
+
+/*
+ * kh_cache_copy: in every pool, pages source[i] copied to target[i], i < n.
+ * source and target are host arrays, read before the call returns. Targets
+ * are distinct and none is a source (KH_ERR_INVALID), so the order of copies
+ * does not matter. A pool is `layers` times `pages` blocks of page_bytes bytes
+ * (a multiple of 4, 4-byte aligned) at base + layer * layer_bytes + page *
+ * page_bytes. At most KH_MAX_POOLS pools.
+ */
+#define KH_MAX_POOLS 8
+typedef struct kh_pool {
+  void *base;
+  int64_t layers, layer_bytes, page_bytes;
+} kh_pool;
+int kh_cache_copy(const kh_pool *pools, int n_pools, int32_t pages, const int32_t *source, const int32_t *target,
+                  int n, void *stream);
+int kh_cache_copy_host(const kh_pool *pools, int n_pools, int32_t pages, const int32_t *source,
+                       const int32_t *target, int n);
 
 /*
  * Measurement probes. No counterpart in the reference (its kernels are

@@ -413,6 +413,7 @@ bool run_launch_host(const kh_launch &L, float *const *ptrs, std::string &err) {
     case KH_FAM_GEMM:
     case KH_FAM_GEMV: host_matmul(L, ptrs); return true;
     case KH_FAM_ATTN: host_attn(L, ptrs); return true;
+    case KH_FAM_PAGED: host_paged_launch(L, ptrs); return true;
     default: err = "no host semantics for kernel family " + std::to_string(L.family); return false;
   }
 }

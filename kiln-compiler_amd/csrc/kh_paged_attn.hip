@@ -1,0 +1,74 @@
+// kh_paged_attn.hip - how attention over a paged cache (kh_paged_attn.hpp) is
+// dealt out: rows of an item, workgroups, workspace.
+#include <algorithm>
+
+#include "kh_paged.hpp"
+
+namespace kh {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+int passes_of(const kh_paged &p) {
+  if (p.cache_type == KH_TYPE_F32 || p.one_pass || p.act_type != KH_TYPE_F32) return 1;
+  return p.cache_type == KH_TYPE_BF16 ? 3 : 2;
+}
+
+// 16-row blocks of an item: as many as there are rows for, up to what the
+// registers of a lane hold beside a tile (q's parts, O and the tile of a
+// 256-wide head fill them with one).
+int row_blocks(const kh_paged &p) {
+  const int rows = (p.top ? 1 : p.draft) * (p.heads / p.kv_heads);
+  const int dt = padded_dim(p.dim);
+  const int most = dt == 256 ? 1 : (p.cache_type == KH_TYPE_F32 || passes_of(p) > 1) ? 2 : 4;
+  return rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+}
+
+PagedWork work_of(const kh_paged &p) {
+  PagedWork w;
+  w.p = p;
+  w.group = p.heads / p.kv_heads;
+  const int rm = 16 * row_blocks(p);
+  w.rows = (p.top ? 1 : p.draft) * w.group;
+  w.blocks = (w.rows + rm - 1) / rm;
+  w.items = p.kv_heads * w.blocks * (p.top ? p.draft : 1);
+  w.half_shift = 0;
+  while ((16 << w.half_shift) < p.page_size) ++w.half_shift;
+  w.draft_tiles = (p.draft + kPagedTile - 1) / kPagedTile;
+  w.sel_tiles = (int)(((int64_t)p.top * p.page_size + kPagedTile - 1) / kPagedTile);
+  w.rounds = 0;
+  while ((1 << w.rounds) < p.draft) ++w.rounds;
+  w.scale2 = p.scale * kLog2e;
+  // workgroups: what the chip holds at once, or a tile per wave of the most
+  // tiles the table has room for
+  const int64_t per_item = (w.sel_tiles ? w.sel_tiles : ((int64_t)p.width * p.page_size + kPagedTile - 1) / kPagedTile) + w.draft_tiles;
+  const int64_t want = (per_item * w.items * p.batch + kPagedWaves - 1) / kPagedWaves;
+  const int cap = current_device().cus * (rm == 16 && padded_dim(p.dim) <= 128 ? 2 : 1);
+  w.grid = (int)std::min<int64_t>(want, cap);
+  w.part = nullptr;
+  return w;
+}
+
+}  // namespace
+
+size_t paged_workspace_floats(const kh_paged &p) {
+  const PagedWork w = work_of(p);
+  if (w.grid <= 1) return 0;
+  return 2 * (size_t)w.grid * 16 * row_blocks(p) * (padded_dim(p.dim) + 2);
+}
+
+hipError_t launch_paged(const kh_paged &p, float *workspace, hipStream_t stream) {
+  if (p.batch == 0 || p.draft == 0) return hipSuccess;
+  PagedWork w = work_of(p);
+  w.part = workspace;
+  const int dt = padded_dim(p.dim), rt = row_blocks(p), np = passes_of(p);
+  switch (p.cache_type) {
+    case KH_TYPE_F32: return launch_paged_f32(w, np, dt, rt, stream);
+    case KH_TYPE_BF16: return launch_paged_bf16(w, np, dt, rt, stream);
+    default: return launch_paged_f16(w, np, dt, rt, stream);
+  }
+}
+
+}  // namespace kh

@@ -1,0 +1,11 @@
+// kh_paged_f16.hip - attention over a paged cache of fp16 (kh_paged_attn.hpp).
+#include "kh_paged_attn.hpp"
+
+namespace kh {
+
+hipError_t launch_paged_f16(const PagedWork &w, int passes, int dt, int rt, hipStream_t stream) {
+  return passes == 1 ? launch_typed<KH_TYPE_F16, 1>(w, dt, rt, stream)
+                     : launch_typed<KH_TYPE_F16, 2>(w, dt, rt, stream);
+}
+
+}  // namespace kh

@@ -39,6 +39,12 @@ int fail(int code, const std::string &msg) {
   return code;
 }
 
+}  // namespace
+
+int abi_fail(int code, const std::string &msg) { return fail(code, msg); }
+
+namespace {
+
 int hip_fail(hipError_t e, const char *what) {
   return fail(KH_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
@@ -189,8 +195,8 @@ int resolve(const kh_plan *p, int i, void *const *inputs, int n_in, void *const 
       default: return fail(KH_ERR_INVALID, "bad operand base");
     }
     if (base == nullptr) return fail(KH_ERR_INVALID, std::string("null device pointer for an operand of ") + L.name);
-    ptrs[j] = (kh::bf16_refs(L) >> j & 1) ? reinterpret_cast<float *>(static_cast<uint16_t *>(base) + r.offset)
-                                         : static_cast<float *>(base) + r.offset;
+    const int bytes = L.family == KH_FAM_PAGED ? kh::paged_ref_bytes(L, j) : (kh::bf16_refs(L) >> j & 1) ? 2 : 4;
+    ptrs[j] = reinterpret_cast<float *>(static_cast<char *>(base) + r.offset * bytes);
   }
   return KH_OK;
 }
@@ -302,6 +308,7 @@ int kh_plan_create(const kh_launch *launches, int n_launches, kh_plan **out) {
         case KH_FAM_GEMV: op = kh::make_gemv(L, err, unsupported); break;
         case KH_FAM_RED: op = kh::make_red(L, err, unsupported); break;
         case KH_FAM_ATTN: op = kh::make_attn(L, err, unsupported); break;
+        case KH_FAM_PAGED: op = kh::make_paged(L, err, unsupported); break;
         default: err = "unknown kernel family " + std::to_string(L.family);
       }
     }

@@ -147,6 +147,24 @@ def _compile_graph_gpu(graph: Graph, options: Options):
     return _GpuBuild(graph, options).run()
 
 
+def cache_inputs(graph: Graph) -> dict:
+    """{argument: element type} of the arguments that are a paged cache (or
+    views of which are): used in place at every call."""
+    from kiln.ir import ops
+
+    position = {a: i for i, a in enumerate(graph.args)}
+    found = {i: a.type.dtype for a, i in position.items() if a.type.dtype != "f32"}
+    for n in graph.nodes:
+        if ops.kind(n.op) != "paged":
+            continue
+        for v in n.inputs[ops.PAGED_OPERANDS[n.op]:]:
+            while v.node is not None and ops.kind(v.node.op) == "view":
+                v = v.node.inputs[0]
+            if v in position:
+                found[position[v]] = v.type.dtype
+    return found
+
+
 class _GpuBuild:
     def __init__(self, graph: Graph, options: Options):
         self.graph = graph
@@ -217,7 +235,8 @@ class _GpuBuild:
         executable = HostExecutable if interpreting() else HIPExecutable
         exe = executable(program, g.attrs.get("arena_bytes", 0), g.constants, [a.shape for a in g.args],
                             [r.shape for r in g.results], cuda_graphs=self.options.cuda_graphs,
-                            debug=self.options.debug, source_path=listing)
+                            debug=self.options.debug, source_path=listing, cache_inputs=cache_inputs(g),
+                            output_types=[r.type.dtype for r in g.results])
         if self.options.dump_mlir:
             print(f"// ----- lowered HIP plan ({listing}) -----\n{program.source}")
         families = {}
@@ -293,6 +312,13 @@ class _FnModule(torch.nn.Module):
         return self.fn(*args)
 
 
+def _returns_one(ep, module, example_inputs) -> bool:
+    if any(str(n.target).startswith("kiln.") for n in ep.graph.nodes):
+        # operators over a paged cache run on the GPU only, the examples may be elsewhere
+        return ep.call_spec.out_spec.type not in (tuple, list)
+    return not isinstance(module(*example_inputs), (tuple, list))
+
+
 def _export(module: torch.nn.Module, example_inputs):
     """(decomposed ExportedProgram, whether the module returns one tensor).
     The module runs in eval mode for the export and gets its mode back."""
@@ -301,7 +327,7 @@ def _export(module: torch.nn.Module, example_inputs):
     try:
         with torch.no_grad():
             ep = torch.export.export(module, tuple(example_inputs)).run_decompositions()
-            single = not isinstance(module(*example_inputs), (tuple, list))
+            single = _returns_one(ep, module, example_inputs)
     finally:
         module.train(training)
     return ep, single

@@ -15,6 +15,10 @@ and the HIP lowering recognises them (LayerNorm, softmax, bias + GELU):
   mean            reduce_sum, mul(1/count)
   pow(x, 2)       mul(x, x)
 
+The operators over a paged cache (kiln/hip/paged.py) are one IR op each. Their
+pages may be bf16 or fp16 and their tables int32; those are inputs of the
+compiled function (seen through views at most), everything else is float32.
+
 Python numbers become scalar constants, one per distinct value, created where
 first used. Anything without a translator raises ``Unsupported`` (a
 NotImplementedError).
@@ -29,6 +33,8 @@ from numbers import Number
 import torch
 import torch.fx
 
+import kiln.hip.paged  # noqa: F401  (registers torch.ops.kiln)
+from kiln.ir import ops
 from kiln.ir.core import Graph, TensorType, Value, verify
 
 aten = torch.ops.aten
@@ -38,11 +44,14 @@ class Unsupported(NotImplementedError):
     """The graph uses something Kiln cannot compile."""
 
 
-def static_shape(node: torch.fx.Node) -> tuple:
+_CACHE_TYPES = {torch.float32: "f32", torch.int32: "i32", torch.bfloat16: "bf16", torch.float16: "f16"}
+
+
+def static_shape(node: torch.fx.Node, dtypes=(torch.float32,)) -> tuple:
     meta = node.meta.get("val")
     if not isinstance(meta, torch.Tensor):
         raise Unsupported(f"{node.name}: no tensor metadata")
-    if meta.dtype != torch.float32:
+    if meta.dtype not in dtypes:
         raise Unsupported(f"{node.name}: only float32 is supported (got {meta.dtype})")
     dims = tuple(meta.shape)
     if any(not isinstance(d, int) for d in dims):
@@ -230,12 +239,12 @@ def _swap_axes(t, node, args, kwargs):
 @translates(aten.view.default, aten.reshape.default, aten._unsafe_view.default, aten.unsqueeze.default,
             aten.squeeze.dim, aten.squeeze.dims, aten.squeeze.default, aten.flatten.using_ints)
 def _reshape(t, node, args, kwargs):
-    return t.b("reshape", t.value(args[0]), shape=list(static_shape(node)))
+    return t.b("reshape", t.value(args[0]), shape=list(static_shape(node, _CACHE_TYPES)))
 
 
 @translates(aten.expand.default)
 def _expand(t, node, args, kwargs):
-    return t.b("expand", t.value(args[0]), shape=list(static_shape(node)))
+    return t.b("expand", t.value(args[0]), shape=list(static_shape(node, _CACHE_TYPES)))
 
 
 @translates(aten.slice.Tensor)
@@ -297,13 +306,60 @@ def _layer_norm(t, node, args, kwargs):
     return expand_layer_norm(t.b, x, len(args[1]), gamma, beta, args[4])
 
 
+def _cache_operand(t, node, operand):
+    """An operand that is the cache itself: a runtime input, or a list of
+    pages that select_pages made."""
+    v = t.value(operand)
+    source = v
+    while source.node is not None and ops.kind(source.node.op) == "view":
+        source = source.node.inputs[0]
+    weight = source.is_arg and "param" in t.graph.arg_attrs[t.graph.args.index(source)]
+    if weight or not (source.is_arg or source.node.op == "select_pages"):
+        raise Unsupported(f"{node.name}: the cache's pages, tables and lists must be inputs of the compiled function")
+    return v
+
+
+def _typed(t, node, op, inputs, attrs):
+    try:
+        return t.b(op, *inputs, **attrs)
+    except ValueError as why:   # e.g. bf16 activations
+        raise Unsupported(f"{node.name}: {why}") from None
+
+
+@translates(torch.ops.kiln.paged_attention.default)
+def _paged_attention(t, node, args, kwargs):
+    q, k, v, *cache, scale = args
+    *cache, parents, selected = cache
+    optional = [x for x in (parents, selected) if x is not None]
+    inputs = [t.value(x) for x in (q, k, v)] + [_cache_operand(t, node, x) for x in [*cache, *optional]]
+    return _typed(t, node, "paged_attention", inputs,
+                  dict(scale=float(scale), cache=inputs[3].type.dtype, parents=parents is not None,
+                       selected=selected is not None))
+
+
+@translates(torch.ops.kiln.select_pages.default)
+def _select_pages(t, node, args, kwargs):
+    q, means, table, lengths, page_size, pages = args
+    inputs = [t.value(q)] + [_cache_operand(t, node, x) for x in (means, table, lengths)]
+    return _typed(t, node, "select_pages", inputs, dict(page_size=int(page_size), pages=int(pages)))
+
+
 # -- the graph walk ---------------------------------------------------------------------------------
+
+_CACHE_OPERATORS = (torch.ops.kiln.paged_attention.default, torch.ops.kiln.select_pages.default)
+_CACHE_READERS = frozenset(_CACHE_OPERATORS + (
+    operator.getitem, aten.t.default, aten.permute.default, aten.transpose.int, aten.view.default, aten.reshape.default,
+    aten._unsafe_view.default, aten.unsqueeze.default, aten.squeeze.dim, aten.squeeze.dims, aten.squeeze.default,
+    aten.flatten.using_ints, aten.slice.Tensor, aten.select.int, aten.alias.default, aten.detach.default,
+    aten.split_with_sizes.default, aten.split.Tensor))
+
 
 class _Translator:
     def __init__(self, name: str):
         self.graph = Graph(name)
         self.b = _Builder(self.graph)
         self.env = {}
+        self.with_cache = False   # does the graph use a paged cache?
 
     def value(self, x) -> Value:
         """The IR value of an FX operand (a node's single tensor) or number."""
@@ -315,6 +371,9 @@ class _Translator:
         return v
 
     def placeholder(self, node, params):
+        if self.with_cache and node.name not in params:
+            shape = static_shape(node, _CACHE_TYPES)
+            return self.graph.add_arg(TensorType(shape, _CACHE_TYPES[node.meta["val"].dtype]), node.name)
         t = TensorType(static_shape(node))
         if node.name in params:
             target, data = params[node.name]
@@ -326,21 +385,38 @@ class _Translator:
         translate = _TRANSLATORS.get(node.target)
         if translate is None:
             raise Unsupported(f"Kiln does not support {node.target} yet")
+        if self.with_cache:
+            self.check_types(node)
         out = translate(self, node, node.args, node.kwargs)
         if isinstance(out, Value) and isinstance(node.meta.get("val"), torch.Tensor):
-            if tuple(out.shape) != static_shape(node):
-                raise AssertionError(f"{node.name}: Kiln shape {out.shape} != {static_shape(node)}")
+            dtypes = _CACHE_TYPES if self.with_cache else (torch.float32,)
+            if tuple(out.shape) != static_shape(node, dtypes):
+                raise AssertionError(f"{node.name}: Kiln shape {out.shape} != {static_shape(node, dtypes)}")
         return out
+
+    def check_types(self, node):
+        """Only views and the cache's own operators take values that are not f32."""
+        if node.target in _CACHE_READERS:
+            return
+        for x in node.all_input_nodes:
+            v = self.env.get(x)
+            if isinstance(v, Value) and v.type.dtype != "f32":
+                raise Unsupported(f"{node.name}: only float32 is supported (got {x.meta['val'].dtype})")
 
     def output(self, node):
         outs = node.args[0]
         outs = list(outs) if isinstance(outs, (list, tuple)) else [outs]
         if any(not isinstance(o, torch.fx.Node) for o in outs):
             raise Unsupported("graph returns non-tensor outputs")
-        return [self.value(o) for o in outs]
+        values = [self.value(o) for o in outs]
+        for o, v in zip(outs, values):
+            if v.type.dtype != "f32" and (v.node is None or v.node.op != "select_pages" or values.count(v) > 1):
+                raise Unsupported(f"{o.name}: only float32 results are supported, and select_pages' own")
+        return values
 
     def run(self, gm: torch.fx.GraphModule, params=None) -> Graph:
         params = params or {}
+        self.with_cache = any(node.target in _CACHE_OPERATORS for node in gm.graph.nodes)
         for node in gm.graph.nodes:
             if node.op == "placeholder":
                 self.env[node] = self.placeholder(node, params)

@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from kiln.hip import lib as kl
-from kiln.hip.runtime import host_constant
+from kiln.hip.runtime import TORCH_TYPES, check_cache_input, host_constant
 
 
 def interpreting() -> bool:
@@ -36,15 +36,17 @@ def refuse(what: str):
         raise RuntimeError(f"{what} needs the GPU path; unset KILN_HIP_INTERPRET")
 
 
-def _ptr(a: np.ndarray) -> int:
-    return a.ctypes.data
+def _ptr(a) -> int:
+    return a.data_ptr() if isinstance(a, torch.Tensor) else a.ctypes.data
 
 
 class HostExecutable:
     """The HIPExecutable interface over host memory."""
 
     def __init__(self, program, arena_bytes, constants, input_shapes, output_shapes, cuda_graphs=True,
-                 debug=False, source_path=None):
+                 debug=False, source_path=None, cache_inputs=None, output_types=None):
+        self.cache_inputs = {i: TORCH_TYPES[t] for i, t in (cache_inputs or {}).items()}
+        self.output_types = [TORCH_TYPES[t] for t in output_types or ["f32"] * len(output_shapes)]
         self.device = torch.device("cpu")
         self.program = program
         self.source_path = source_path
@@ -83,13 +85,18 @@ class HostExecutable:
         for i, (t, shape) in enumerate(zip(inputs, self.input_shapes)):
             if tuple(t.shape) != shape:
                 raise ValueError(f"Kiln was compiled for input shape {shape}, got {tuple(t.shape)} (input {i})")
+            if i in self.cache_inputs:
+                check_cache_input(t, i, shape, self.cache_inputs[i], self.device)
+                ready.append(t)
+                continue
             ready.append(np.ascontiguousarray(t.detach().cpu().numpy() if isinstance(t, torch.Tensor) else t,
                                               dtype=np.float32))
         return ready
 
     def __call__(self, *inputs):
         ins = self._prepare(inputs)
-        outs = [np.full(s, np.nan, dtype=np.float32) for s in self.output_shapes]
+        outs = [torch.full(s, float("nan")) if t == torch.float32 else torch.full(s, -7, dtype=t)
+                for s, t in zip(self.output_shapes, self.output_types)]
         in_ptrs, out_ptrs = [_ptr(a) for a in ins], [_ptr(a) for a in outs]
         if self.guards is None:
             self.plan.run_host(in_ptrs, out_ptrs)
@@ -99,4 +106,4 @@ class HostExecutable:
                 self.guards.before(i, fill)
                 one.run_host(in_ptrs, out_ptrs)
                 self.guards.after(i, differs)
-        return [torch.from_numpy(o) for o in outs]
+        return outs

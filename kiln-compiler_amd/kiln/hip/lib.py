@@ -22,7 +22,9 @@ MAX_PASSES = 8
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP, ERR_NO_DEVICE, ERR_CAPACITY = range(6)
 BASE_INPUT, BASE_OUTPUT, BASE_CONST, BASE_ARENA, BASE_WORKSPACE = range(5)
-FAM_EW, FAM_ROW, FAM_GEMM, FAM_GEMV, FAM_RED, FAM_ATTN = 1, 2, 3, 4, 5, 6
+FAM_EW, FAM_ROW, FAM_GEMM, FAM_GEMV, FAM_RED, FAM_ATTN, FAM_PAGED = 1, 2, 3, 4, 5, 6, 7
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2   # KH_TYPE_*: elements of a paged cache and of the activations next to it
+PAGED_ATTENTION, PAGED_SELECT = 0, 1      # KH_PAGED_*
 ATTN_MASK_NONE, ATTN_MASK_CAUSAL, ATTN_MASK_ADD = 0, 1, 2
 GEMV_PRO_NONE, GEMV_PRO_LAYERNORM, GEMV_PRO_ATTN = 0, 1, 2
 GEMV_CHAIN = 1   # KH_GEMV_CHAIN: kh_launch.variant flag of a GEMV launch
@@ -38,7 +40,7 @@ OP = {name: i for i, name in enumerate(OPCODES)}
 SRC_IMM = 0xFF
 
 FAMILY_NAMES = {FAM_EW: "elementwise", FAM_ROW: "row", FAM_GEMM: "gemm", FAM_GEMV: "gemv", FAM_RED: "reduce",
-                FAM_ATTN: "attention"}
+                FAM_ATTN: "attention", FAM_PAGED: "paged"}
 
 
 class Ref(ctypes.Structure):
@@ -63,6 +65,35 @@ class LaunchDesc(ctypes.Structure):
                 ("cfg", ctypes.c_int32 * 8), ("fparams", ctypes.c_float * 4), ("shape", ctypes.c_int64 * MAX_RANK),
                 ("gemm", ctypes.c_int64 * 4), ("refs", Ref * MAX_REFS), ("insns", Insn * MAX_INSNS),
                 ("passes", PassDesc * MAX_PASSES), ("name", ctypes.c_char * 32)]
+
+
+class Paged(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in
+                 ("variant", "batch", "draft", "heads", "kv_heads", "dim", "page_size", "pages", "width", "top",
+                  "cache_type", "act_type", "one_pass")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_void_p) for n in
+                   ("q", "k", "v", "k_pages", "v_pages", "k_means", "table", "lengths", "parents", "selected", "out")]
+                + [(n, ctypes.c_int64) for n in
+                   ("q_s", "q_n", "q_h", "k_s", "k_n", "k_h", "v_s", "v_n", "v_h", "o_s", "o_n", "o_h",
+                    "kp_p", "kp_h", "kp_t", "vp_p", "vp_h", "vp_t", "m_p", "m_h",
+                    "table_s", "parents_s", "sel_s", "sel_n", "sel_h")])
+
+
+class CacheAppend(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in
+                 ("layers", "batch", "draft", "accept", "kv_heads", "dim", "page_size", "pages", "width",
+                  "cache_type", "act_type")]
+                + [(n, ctypes.c_void_p) for n in
+                   ("k", "v", "k_pages", "v_pages", "k_means", "table", "lengths", "rows")]
+                + [(n, ctypes.c_int64) for n in
+                   ("k_l", "k_s", "k_n", "k_h", "v_l", "v_s", "v_n", "v_h", "kp_l", "kp_p", "kp_h", "kp_t",
+                    "vp_l", "vp_p", "vp_h", "vp_t", "m_l", "m_p", "m_h", "table_s", "rows_s")])
+
+
+class Pool(ctypes.Structure):
+    _fields_ = [("base", ctypes.c_void_p), ("layers", ctypes.c_int64), ("layer_bytes", ctypes.c_int64),
+                ("page_bytes", ctypes.c_int64)]
 
 
 def library_path() -> Path:
@@ -113,6 +144,14 @@ def load():
         "kh_plan_chain_timeouts": (ip, [vp, ctypes.POINTER(ctypes.c_uint64)]),
         "kh_plan_chain_spin": (ip, [vp, ctypes.c_int64]),
         "kh_plan_destroy": (ip, [vp]),
+        "kh_paged_sizes": (ip, [ctypes.POINTER(ctypes.c_size_t)]),
+        "kh_paged_workspace_bytes": (ip, [ctypes.POINTER(Paged), ctypes.POINTER(ctypes.c_size_t)]),
+        "kh_paged_run": (ip, [ctypes.POINTER(Paged), vp, ctypes.c_size_t, vp]),
+        "kh_paged_host": (ip, [ctypes.POINTER(Paged)]),
+        "kh_cache_append": (ip, [ctypes.POINTER(CacheAppend), vp]),
+        "kh_cache_append_host": (ip, [ctypes.POINTER(CacheAppend)]),
+        "kh_cache_copy": (ip, [ctypes.POINTER(Pool), ip, i32, ctypes.POINTER(i32), ctypes.POINTER(i32), ip, vp]),
+        "kh_cache_copy_host": (ip, [ctypes.POINTER(Pool), ip, i32, ctypes.POINTER(i32), ctypes.POINTER(i32), ip]),
         "kh_probe_attn_timeline": (ip, [vp, vp, vp, vp, ip, ip, ip, ctypes.POINTER(ctypes.c_int64), ip,
                                         ctypes.c_float, vp, vp]),
         "kh_probe_mfma_valu": (ip, [ip, ip, ip, ip, ctypes.POINTER(ctypes.c_double)]),
@@ -127,6 +166,11 @@ def load():
     mine = (ctypes.sizeof(LaunchDesc), ctypes.sizeof(Ref), ctypes.sizeof(Insn), ctypes.sizeof(PassDesc))
     if tuple(sizes) != mine:
         raise RuntimeError(f"libkiln_hip struct sizes {tuple(sizes)} != binding {mine}; rebuild")
+    paged = (ctypes.c_size_t * 3)()
+    lib.kh_paged_sizes(paged)
+    mine = (ctypes.sizeof(Paged), ctypes.sizeof(CacheAppend), ctypes.sizeof(Pool))
+    if tuple(paged) != mine:
+        raise RuntimeError(f"libkiln_hip's paged structures {tuple(paged)} != binding {mine}; rebuild")
     _lib = lib
     return lib
 
@@ -137,7 +181,9 @@ EXPORTED = ("kh_version", "kh_build_id", "kh_abi_sizes", "kh_last_error", "kh_in
             "kh_plan_run_one",
             "kh_plan_capture", "kh_plan_replay", "kh_plan_time", "kh_plan_chains", "kh_plan_chain_timeouts",
             "kh_plan_chain_spin",
-            "kh_plan_destroy", "kh_probe_attn_timeline", "kh_probe_mfma_valu")
+            "kh_plan_destroy", "kh_paged_sizes", "kh_paged_workspace_bytes", "kh_paged_run", "kh_paged_host",
+            "kh_cache_append", "kh_cache_append_host", "kh_cache_copy", "kh_cache_copy_host",
+            "kh_probe_attn_timeline", "kh_probe_mfma_valu")
 
 
 def check(rc: int, what: str = ""):

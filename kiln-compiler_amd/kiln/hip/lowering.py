@@ -1741,12 +1741,66 @@ class _Lowerer:
         self.add(d, k, f"{batch} heads x {tq} queries x {tk} keys, head dim {dh}, {what}{scale}",
                  flops=flops, nbytes=nbytes)
 
+    # paged cache ------------------------------------------------------------------------------
+
+    def lower_paged(self, k: Kernel):
+        """An operator over a paged cache: its operands as they lie. Products of
+        fp32 activations keep fp32's accuracy; in "bf16" plans those over a
+        16-bit cache run on the cache's type in one pass."""
+        (n,) = k.nodes
+        select = n.op == "select_pages"
+        q = n.inputs[0]
+        batch, draft, heads, dim = q.shape
+        d = kl.LaunchDesc()
+        d.family, d.variant = kl.FAM_PAGED, kl.PAGED_SELECT if select else kl.PAGED_ATTENTION
+        d.rank = 6
+        d.name = f"{k.name}_{'select' if select else 'paged'}".encode()[:31]
+        d.cfg[1] = kl.TYPE_F32
+
+        def ref(j, v):
+            lay = self.layouts.get(v)
+            if lay is None:
+                raise NotImplementedError(f"HIP backend: value {v} has no storage")
+            if lay.strides[-1] != 1 and lay.shape[-1] > 1:
+                raise NotImplementedError(f"HIP backend: the last dimension of operand {j} of {n.op} is not contiguous")
+            r = d.refs[j]
+            r.base, r.index = self.slot_of(lay.base)
+            r.offset = self.element_offset(v)
+            for i, s in enumerate(lay.strides):
+                r.strides[i] = s
+
+        if select:
+            means, table, lengths = n.inputs[1:]
+            pages, kv = means.shape[:2]
+            page, top = n.attrs["page_size"], n.attrs["pages"]
+            operands = [q, means, table, lengths, n.out]
+        else:
+            k_pages, table = n.inputs[3], n.inputs[5]
+            pages, kv, page, _ = k_pages.shape
+            lists = list(n.inputs[7:])
+            top = lists[-1].shape[3] if n.attrs["selected"] else 0
+            operands = [*n.inputs[:7], n.out, *lists]
+            d.cfg[0] = {"f32": kl.TYPE_F32, "bf16": kl.TYPE_BF16, "f16": kl.TYPE_F16}[n.attrs["cache"]]
+            d.cfg[2] = 1 if self.precision == "bf16" and d.cfg[0] != kl.TYPE_F32 else 0
+            d.cfg[3] = 8 if n.attrs["parents"] else 0
+            d.cfg[4] = 7 + len(lists) if n.attrs["selected"] else 0
+            d.fparams[0] = n.attrs["scale"]
+        for j, v in enumerate(operands):
+            ref(j, v)
+        d.n_refs = len(operands)
+        for i, x in enumerate((batch, draft, heads, kv, dim, page)):
+            d.shape[i] = x
+        d.gemm[0], d.gemm[1], d.gemm[2] = pages, table.shape[1], top
+        what = f"the best {top} of" if select else f"{top} picked of" if top else "over"
+        self.add(d, k, f"{batch} x {draft} tokens, {heads} heads on {kv} of {dim}, {what} up to {table.shape[1]} pages "
+                       f"of {page}" + ("" if select else f", {n.attrs['cache']}{' one pass' if d.cfg[2] else ''}"))
+
     # driver --------------------------------------------------------------------------------------
 
     def run(self) -> Program:
         for k in self.g.kernels:
             for n in k.nodes:
-                if ops.kind(n.op) not in ("elementwise", "reduction", "matmul") and k.kind != "attention":
+                if ops.kind(n.op) not in ("elementwise", "reduction", "matmul", "paged") and k.kind != "attention":
                     raise NotImplementedError(f"GPU backend: unexpected op '{n.op}' in a kernel")
         fused = self.find_ln_prologues() | self.find_attn_prologues()
         self.bf16_buffers = self.plan_bf16_storage()
@@ -1759,6 +1813,8 @@ class _Lowerer:
                 self.lower_attention(k)
             elif k.kind == "matmul":
                 self.lower_matmul(k)
+            elif k.kind == "paged":
+                self.lower_paged(k)
             elif k.kind == "reduction":
                 self.lower_reduction(k)
             else:

@@ -1,0 +1,451 @@
+"""The operators over a paged key/value cache, as functions on torch tensors.
+
+    tree_attention      N drafted tokens a sequence over its cached tokens and
+                        each other, along a tree (one token: plain decoding)
+    select_pages        the pages a cheap score picks for each drafted token
+    selected_attention  tree_attention over those pages alone
+    cache_append        new tokens' keys and values written into the pages
+    copy_pages          whole pages copied within the pools
+
+A cache's pages are ``k_pages`` and ``v_pages``, ``[pages, kv_heads,
+page_size, dim]`` in fp32, bf16 or fp16; token t of sequence s lies in page
+``table[s, t // page_size]`` at slot ``t % page_size``, for ``t < lengths[s]``
+(int32 both). ``kiln.PagedCache`` keeps such a cache and its book-keeping.
+
+The first three are also what a model given to ``kiln.compile`` or
+``torch.compile(backend=kiln.backend)`` may call: they are the operators
+``torch.ops.kiln.paged_attention`` and ``select_pages``, which the frontend
+translates. The last two change their arguments, which a compiled graph does
+not; they are called between the calls of a compiled step.
+
+Each call runs on the current stream of its tensors' device, allocates its
+result and workspace from torch's allocator (so it can be captured into a
+graph) and reads or changes nothing else. There is no CPU path; with
+``KILN_HIP_INTERPRET=1`` (tests) the library's CPU meaning runs instead.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from kiln.hip import lib as kl
+from kiln.hip.interpret import interpreting
+
+TYPES = {torch.float32: kl.TYPE_F32, torch.bfloat16: kl.TYPE_BF16, torch.float16: kl.TYPE_F16}
+
+
+# -- checks --------------------------------------------------------------------------------
+
+
+def _tensor(t, name, rank, dtypes):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.dim() != rank:
+        raise ValueError(f"{name} must have {rank} dimensions, got shape {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+
+
+def _shape(t, name, shape):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _int32(t, name, rank, shape):
+    _tensor(t, name, rank, (torch.int32,))
+    _shape(t, name, shape)
+
+
+def _no_grad(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("the paged cache's operators have no backward pass: call them under torch.no_grad()")
+
+
+def _one_device(first, *others):
+    if first.device.type != "cuda" and not interpreting():
+        raise NotImplementedError(f"the paged cache's operators run on the GPU only, got tensors on {first.device}")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"all tensors must be on one device, got {first.device} and {t.device}")
+
+
+def check_pages(k_pages, v_pages, rank=4):
+    """The pages of one layer (rank 4) or of a stack of layers (rank 5)."""
+    _tensor(k_pages, "k_pages", rank, tuple(TYPES))
+    _tensor(v_pages, "v_pages", rank, (k_pages.dtype,))
+    _shape(v_pages, "v_pages", k_pages.shape)
+
+
+def _rows_in_place(t, name):
+    """Pages are read where they are: rows along the last dimension, each at a multiple of 16 bytes."""
+    size = t.element_size()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+        raise ValueError(f"{name}: rows must be contiguous and start at multiples of 16 bytes")
+
+
+def _rows(t):
+    """A small operand whose rows start at multiples of 16 bytes: itself, or a copy."""
+    size = t.element_size()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]):
+        return t.clone(memory_format=torch.contiguous_format)   # (a new tensor is aligned, a contiguous view may not be)
+    return t
+
+
+def check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected):
+    """(sizes of the call) after checking types, shapes and their agreement."""
+    check_pages(k_pages, v_pages)
+    pages, kv_heads, page_size, dim = k_pages.shape
+    _tensor(q, "q", 4, (torch.float32,) if k_pages.dtype == torch.float32 else (torch.float32, k_pages.dtype))
+    batch, draft, heads, _ = q.shape
+    _shape(q, "q", (batch, draft, heads, dim))
+    for t, name in ((k, "k"), (v, "v")):
+        _tensor(t, name, 4, (q.dtype,))
+        _shape(t, name, (batch, draft, kv_heads, dim))
+    if kv_heads == 0 or heads % kv_heads or heads == 0:
+        raise ValueError(f"{heads} query heads do not divide over {kv_heads} heads of the cache")
+    if not isinstance(table, torch.Tensor) or table.dim() != 2:
+        raise ValueError("table must be a tensor [sequences, columns]")
+    _int32(table, "table", 2, (batch, table.shape[1]))
+    _int32(lengths, "lengths", 1, (batch,))
+    if parents is not None:
+        _int32(parents, "parents", 2, (batch, draft))
+    if selected is not None:
+        if not isinstance(selected, torch.Tensor) or selected.dim() != 4:
+            raise ValueError("selected must be a tensor [sequences, tokens, kv heads, pages]")
+        _int32(selected, "selected", 4, (batch, draft, kv_heads, selected.shape[3]))
+        if selected.shape[3] == 0:
+            raise ValueError("selected names no pages")
+    return batch, draft, heads, kv_heads, dim, page_size, pages
+
+
+def check_select(q, k_means, table, lengths, page_size, pages):
+    _tensor(q, "q", 4, tuple(TYPES))
+    _tensor(k_means, "k_means", 3, (torch.float32,))
+    batch, draft, heads, dim = q.shape
+    total, kv_heads, _ = k_means.shape
+    _shape(k_means, "k_means", (total, kv_heads, dim))
+    if kv_heads == 0 or heads % kv_heads or heads == 0:
+        raise ValueError(f"{heads} query heads do not divide over {kv_heads} heads of the cache")
+    if not isinstance(table, torch.Tensor) or table.dim() != 2:
+        raise ValueError("table must be a tensor [sequences, columns]")
+    _int32(table, "table", 2, (batch, table.shape[1]))
+    _int32(lengths, "lengths", 1, (batch,))
+    if pages < 1:
+        raise ValueError(f"pages must be at least 1, got {pages}")
+    return batch, draft, heads, kv_heads, dim, total
+
+
+def default_scale(scale, dim):
+    return 1.0 / math.sqrt(dim) if scale is None else float(scale)
+
+
+# -- running -------------------------------------------------------------------------------------
+
+
+def _columns(t):
+    """int32 operands are read with their last dimension contiguous."""
+    return t if t.stride(-1) == 1 or t.numel() == 0 else t.contiguous()
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _on_device(device, fn):
+    """fn() with `device` current (a launch goes to the current device)."""
+    if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
+        return fn()
+    with torch.cuda.device(device):
+        return fn()
+
+
+def _ready(device):
+    from kiln.hip.runtime import init_device, _ready_devices
+
+    if device.type == "cuda" and device.index not in _ready_devices:
+        # kh_init makes the device current and asks for its facts
+        with torch.cuda.device(device):
+            init_device(device)
+
+
+def _run(op: kl.Paged, device, what: str):
+    lib = kl.load()
+    if device.type != "cuda":
+        kl.check(lib.kh_paged_host(ctypes.byref(op)), what)
+        return
+    _ready(device)
+
+    def go():
+        size = ctypes.c_size_t()
+        kl.check(lib.kh_paged_workspace_bytes(ctypes.byref(op), ctypes.byref(size)), what)
+        n = size.value
+        workspace = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        rc = lib.kh_paged_run(ctypes.byref(op), workspace.data_ptr() if n else None, n, _stream(device))
+        if rc:
+            kl.check(rc, what)
+
+    _on_device(device, go)
+
+
+def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what):
+    batch, draft, heads, kv_heads, dim, page_size, pages = check_attention(
+        q, k, v, k_pages, v_pages, table, lengths, parents, selected)
+    _no_grad(q, k, v, k_pages, v_pages)
+    _one_device(q, k, v, k_pages, v_pages, table, lengths, parents, selected)
+    _rows_in_place(k_pages, "k_pages")
+    _rows_in_place(v_pages, "v_pages")
+    if pages == 0:
+        raise ValueError("the cache has no pages")
+    q, k, v, table, lengths = _rows(q), _rows(k), _rows(v), _columns(table), _columns(lengths)
+    out = torch.empty((batch, draft, heads, dim), dtype=q.dtype, device=q.device)
+    if out.numel() == 0:
+        return out
+    op = kl.Paged(kl.PAGED_ATTENTION, batch, draft, heads, kv_heads, dim, page_size, pages, table.shape[1], 0,
+                  TYPES[k_pages.dtype], TYPES[q.dtype], 0, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  k_pages.data_ptr(), v_pages.data_ptr(), None, table.data_ptr(), lengths.data_ptr(), None, None,
+                  out.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
+                  *k_pages.stride()[:3], *v_pages.stride()[:3], 0, 0, table.stride(0), 0, 0, 0, 0)
+    if parents is not None:
+        parents = _columns(parents)
+        op.parents, op.parents_s = parents.data_ptr(), parents.stride(0)
+    if selected is not None:
+        selected = _columns(selected)
+        op.selected, op.top = selected.data_ptr(), selected.shape[3]
+        op.sel_s, op.sel_n, op.sel_h = selected.stride()[:3]
+    _run(op, q.device, what)
+    return out
+
+
+def run_select(q, k_means, table, lengths, page_size, pages):
+    batch, draft, heads, kv_heads, dim, total = check_select(q, k_means, table, lengths, page_size, pages)
+    _no_grad(q, k_means)
+    _one_device(q, k_means, table, lengths)
+    _rows_in_place(k_means, "k_means")
+    q, table, lengths = _rows(q), _columns(table), _columns(lengths)
+    out = torch.empty((batch, draft, kv_heads, pages), dtype=torch.int32, device=q.device)
+    if out.numel() == 0:
+        return out
+    if total == 0:
+        raise ValueError("the cache has no pages")
+    op = kl.Paged(kl.PAGED_SELECT, batch, draft, heads, kv_heads, dim, page_size, total, table.shape[1], pages,
+                  kl.TYPE_F32, TYPES[q.dtype], 0, 1.0, q.data_ptr(), None, None, None, None, k_means.data_ptr(),
+                  table.data_ptr(), lengths.data_ptr(), None, out.data_ptr(), None)
+    op.q_s, op.q_n, op.q_h = q.stride()[:3]
+    op.m_p, op.m_h = k_means.stride()[:2]
+    op.table_s = table.stride(0)
+    op.sel_s, op.sel_n, op.sel_h = out.stride()[:3]
+    _run(op, q.device, "select_pages")
+    return out
+
+
+# -- as operators of torch, for graphs -----------------------------------------------------------
+
+
+@torch.library.custom_op("kiln::paged_attention", mutates_args=())
+def _paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                     table: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor | None,
+                     selected: torch.Tensor | None, scale: float) -> torch.Tensor:
+    with torch.no_grad():
+        return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, "paged_attention")
+
+
+@_paged_attention.register_fake
+def _(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale):
+    check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected)
+    return q.new_empty(tuple(q.shape))
+
+
+@torch.library.custom_op("kiln::select_pages", mutates_args=())
+def _select_pages(q: torch.Tensor, k_means: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, page_size: int,
+                  pages: int) -> torch.Tensor:
+    with torch.no_grad():
+        return run_select(q, k_means, table, lengths, page_size, pages)
+
+
+@_select_pages.register_fake
+def _(q, k_means, table, lengths, page_size, pages):
+    check_select(q, k_means, table, lengths, page_size, pages)
+    return q.new_empty((q.shape[0], q.shape[1], k_means.shape[1], pages), dtype=torch.int32)
+
+
+def _tracing() -> bool:
+    return torch.compiler.is_compiling()
+
+
+# -- the public functions ------------------------------------------------------------------------------
+
+
+def tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents=None, *, scale=None):
+    """Attention of drafted tokens over a paged cache and over each other.
+
+    ``q`` ``[sequences, tokens, heads, dim]``, ``k`` and ``v`` ``[sequences,
+    tokens, kv_heads, dim]``: the drafted tokens', in fp32 or the cache's
+    type; they are not in the cache yet. ``parents`` ``[sequences, tokens]``
+    (int32): the earlier drafted token that token i follows, -1 where it
+    follows the cached ones; any other value marks the token, and those that
+    follow it, as unused (rows of zeros). Without ``parents`` each token
+    follows the one before it. Query heads ``h`` share head ``h // (heads /
+    kv_heads)`` of the cache. Returns ``softmax(scale q . keys) values``,
+    shaped and typed as ``q``; ``scale`` is 1 / sqrt(dim) by default.
+
+    Drafted keys and values are rounded to the cache's type first, so a token
+    is attended to as it will be once it is appended. fp32 activations keep
+    fp32's accuracy over bf16 and fp16 caches too. Up to 256 tokens and 4096
+    sequences, dim a multiple of 8 up to 256, page_size a power of two from
+    16 to 1024. A table entry outside the pool holds no tokens.
+    """
+    scale = default_scale(scale, k_pages.shape[-1])
+    if _tracing():
+        return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale)
+    return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale, "tree_attention")
+
+
+def selected_attention(q, k, v, k_pages, v_pages, table, lengths, selected, parents=None, *, scale=None):
+    """``tree_attention`` in which token i of sequence s attends, of the
+    cached tokens, to those of the pages ``selected[s, i, kv_head]`` alone
+    (int32 ``[sequences, tokens, kv_heads, pages]``: columns of ``table``, as
+    ``select_pages`` gives them). An entry counts only where it is larger
+    than the one before it, so lists ascend and end with -1."""
+    if selected is None:
+        raise TypeError("selected must be a tensor (tree_attention reads every page)")
+    scale = default_scale(scale, k_pages.shape[-1])
+    if _tracing():
+        return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale)
+    return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, "selected_attention")
+
+
+def select_pages(q, k_means, table, lengths, *, page_size, pages):
+    """The ``pages`` pages of each sequence that a cheap score picks for each
+    drafted token and head of the cache: the largest (sum of the group's
+    queries) . ``k_means[page]`` (fp32 ``[pages of the pool, kv_heads, dim]``,
+    the mean key of each page), summed in 64 bits; the page of the last
+    cached token is always among them. Ties go to the lower column. Returns
+    int32 ``[sequences, tokens, kv_heads, pages]``: columns of ``table``,
+    ascending, then -1."""
+    if _tracing():
+        return torch.ops.kiln.select_pages(q, k_means, table, lengths, page_size, pages)
+    return run_select(q, k_means, table, lengths, int(page_size), int(pages))
+
+
+def _eager_only(what):
+    if _tracing():
+        raise NotImplementedError(f"{what} changes its arguments, which a compiled graph does not: call it between "
+                                  f"the calls of the compiled step")
+
+
+def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=None):
+    """Write new tokens behind the cached ones, in place: token
+    ``rows[s, a]`` of ``k`` and ``v`` ``[sequences, tokens, kv_heads, dim]``
+    becomes token ``lengths[s] + a`` of sequence s, rounded to the cache's
+    type. ``rows`` (int32 ``[sequences, accepted]``): the accepted path of a
+    drafted tree; a row ends at its first entry outside [0, tokens). Without
+    ``rows`` all tokens, in order. With ``k_means`` the mean key of every page
+    written to is brought up to date. ``lengths`` is not changed.
+
+    With a leading dimension of layers on ``k``, ``v`` (5 dimensions), the
+    pages (5) and ``k_means`` (4), all layers are written at once; ``table``,
+    ``lengths`` and ``rows`` hold for each. Tokens whose page the table does
+    not name are dropped. No page may belong to two of the sequences."""
+    _eager_only("cache_append")
+    rank = k_pages.dim() if isinstance(k_pages, torch.Tensor) and k_pages.dim() == 5 else 4
+    check_pages(k_pages, v_pages, rank)
+    if rank == 4:
+        k, v = (t.unsqueeze(0) if isinstance(t, torch.Tensor) else t for t in (k, v))
+        k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
+        k_means = k_means.unsqueeze(0) if isinstance(k_means, torch.Tensor) else k_means
+    layers, pages, kv_heads, page_size, dim = k_pages.shape
+    _tensor(k, "k", 5, tuple(TYPES))
+    batch, draft = k.shape[1], k.shape[2]
+    _shape(k, "k", (layers, batch, draft, kv_heads, dim))
+    _tensor(v, "v", 5, (k.dtype,))
+    _shape(v, "v", k.shape)
+    if not isinstance(table, torch.Tensor) or table.dim() != 2:
+        raise ValueError("table must be a tensor [sequences, columns]")
+    _int32(table, "table", 2, (batch, table.shape[1]))
+    _int32(lengths, "lengths", 1, (batch,))
+    if rows is not None:
+        if not isinstance(rows, torch.Tensor) or rows.dim() != 2:
+            raise ValueError("rows must be a tensor [sequences, accepted]")
+        _int32(rows, "rows", 2, (batch, rows.shape[1]))
+        rows = _columns(rows)
+    if k_means is not None:
+        _tensor(k_means, "k_means", 4, (torch.float32,))
+        _shape(k_means, "k_means", (layers, pages, kv_heads, dim))
+        if k_means.stride(-1) != 1:
+            raise ValueError("k_means: rows must be contiguous")
+    _no_grad(k, v, k_pages, v_pages, k_means)
+    _one_device(k, v, k_pages, v_pages, table, lengths, rows, k_means)
+    _rows_in_place(k_pages, "k_pages")
+    _rows_in_place(v_pages, "v_pages")
+    k, v, table, lengths = _rows(k), _rows(v), _columns(table), _columns(lengths)
+    accept = draft if rows is None else rows.shape[1]
+    if layers * batch * accept * draft == 0:
+        return
+    op = kl.CacheAppend(layers, batch, draft, accept, kv_heads, dim, page_size, pages, table.shape[1],
+                        TYPES[k_pages.dtype], TYPES[k.dtype], k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
+                        v_pages.data_ptr(), k_means.data_ptr() if k_means is not None else None, table.data_ptr(),
+                        lengths.data_ptr(), rows.data_ptr() if rows is not None else None, *k.stride()[:4],
+                        *v.stride()[:4], *k_pages.stride()[:4], *v_pages.stride()[:4],
+                        *(k_means.stride()[:3] if k_means is not None else (0, 0, 0)), table.stride(0),
+                        rows.stride(0) if rows is not None else 0)
+    lib, device = kl.load(), k.device
+    if device.type != "cuda":
+        kl.check(lib.kh_cache_append_host(ctypes.byref(op)), "cache_append")
+        return
+    _ready(device)
+    rc = _on_device(device, lambda: lib.kh_cache_append(ctypes.byref(op), _stream(device)))
+    if rc:
+        kl.check(rc, "cache_append")
+
+
+def _page_list(x, name):
+    try:
+        return (ctypes.c_int32 * len(x))(*x)
+    except (TypeError, ctypes.ArgumentError):
+        raise TypeError(f"{name} must be a sequence of page numbers") from None
+
+
+def copy_pages(pools, source, target):
+    """Copy pages within each of ``pools``, in place: page ``source[i]`` to
+    page ``target[i]``. A pool is a tensor ``[pages, ...]`` or, with 5
+    dimensions (4 for fp32 means of 5-dimensional pools: pass
+    ``means.unsqueeze(-2)``), ``[layers, pages, ...]``, contiguous within a
+    layer. ``source`` and ``target`` are sequences of ints; targets are
+    distinct and none is a source, so no order of the copies matters."""
+    _eager_only("copy_pages")
+    pools = list(pools)
+    if len(source) != len(target):
+        raise ValueError(f"{len(source)} source pages, but {len(target)} target pages")
+    descs = (kl.Pool * max(1, len(pools)))()
+    pages = None
+    for i, t in enumerate(pools):
+        if not isinstance(t, torch.Tensor) or t.dim() < 2:
+            raise TypeError("a pool is a tensor of pages")
+        stacked = t.dim() == 5
+        layer = t[0] if stacked and t.shape[0] else t
+        if stacked and not t.shape[0]:
+            raise ValueError("a pool has no layers")
+        if not layer.is_contiguous():
+            raise ValueError("a pool's pages must be contiguous within a layer")
+        if pages is not None and pages != layer.shape[0]:
+            raise ValueError(f"pools of {pages} and of {layer.shape[0]} pages")
+        pages = layer.shape[0]
+        size = t.element_size()
+        descs[i] = kl.Pool(t.data_ptr(), t.shape[0] if stacked else 1, t.stride(0) * size if stacked else 0,
+                           layer[0].numel() * size if pages else 0)
+    if not pools or len(source) == 0:
+        return
+    _no_grad(*pools)
+    _one_device(*pools)
+    src, dst = _page_list(source, "source"), _page_list(target, "target")
+    lib, device = kl.load(), pools[0].device
+    if device.type != "cuda":
+        kl.check(lib.kh_cache_copy_host(descs, len(pools), pages, src, dst, len(src)), "copy_pages")
+        return
+    _ready(device)
+    rc = _on_device(device, lambda: lib.kh_cache_copy(descs, len(pools), pages, src, dst, len(src), _stream(device)))
+    if rc:
+        kl.check(rc, "copy_pages")

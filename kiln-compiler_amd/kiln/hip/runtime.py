@@ -161,11 +161,26 @@ def host_constant(program, constants: dict, name: str) -> np.ndarray:
     return make(constants[src], offset, strides, batch, k, n).view(np.int16)
 
 
+TORCH_TYPES = {"f32": torch.float32, "i32": torch.int32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def check_cache_input(t, i, shape, dtype, device):
+    """An input that is part of a paged cache is read where it lies, so it must
+    be what the plan was made for."""
+    if t.device != device or t.dtype != dtype:
+        raise ValueError(f"input {i} is part of a paged cache and must be {dtype} on {device}, got {t.dtype} on {t.device}")
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"input {i} is part of a paged cache and must be contiguous and 16-byte aligned")
+
+
 class HIPExecutable:
-    """One compiled graph on one MI355X. Not reentrant."""
+    """One compiled graph on one MI355X. Not reentrant. ``cache_inputs``:
+    {input: element type} of those that are a paged cache, which are used in
+    place; a graph's replay works on copies of its inputs, so such a plan is
+    always launched directly. ``output_types``: the results' element types."""
 
     def __init__(self, program, arena_bytes, constants, input_shapes, output_shapes, cuda_graphs=True,
-                 debug=False, source_path=None):
+                 debug=False, source_path=None, cache_inputs=None, output_types=None):
         self.device = device()
         init_device(self.device)
         self.program = program
@@ -173,7 +188,9 @@ class HIPExecutable:
         self.input_shapes = [tuple(s) for s in input_shapes]
         self.output_shapes = [tuple(s) for s in output_shapes]
         self.kernel_names = [launch.name for launch in program.launches]
-        self.use_cuda_graphs = bool(cuda_graphs)
+        self.cache_inputs = {i: TORCH_TYPES[t] for i, t in (cache_inputs or {}).items()}
+        self.output_types = [TORCH_TYPES[t] for t in output_types or ["f32"] * len(output_shapes)]
+        self.use_cuda_graphs = bool(cuda_graphs) and not self.cache_inputs
         self.debug = debug
 
         self.plan = kl.Plan([launch.desc for launch in program.launches])
@@ -243,6 +260,10 @@ class HIPExecutable:
         for i, (t, shape) in enumerate(zip(inputs, self.input_shapes)):
             if t.shape != shape:   # (a torch.Size compares as the tuple it is)
                 raise ValueError(f"Kiln was compiled for input shape {shape}, got {tuple(t.shape)} (input {i})")
+            if i in self.cache_inputs:
+                check_cache_input(t, i, shape, self.cache_inputs[i], self.device)
+                ready.append(t)
+                continue
             if t.device != self.device or t.dtype != torch.float32 or not t.is_contiguous():
                 t = t.detach().to(device=self.device, dtype=torch.float32).contiguous()
             if t.data_ptr() % 16:   # kernels read rows as 16-byte pieces
@@ -283,8 +304,11 @@ class HIPExecutable:
         self._graph_buffers()
         self.plan.replay(current_stream_handle())
 
+    def _outputs(self):
+        return [torch.empty(s, dtype=t, device=self.device) for s, t in zip(self.output_shapes, self.output_types)]
+
     def _direct(self, inputs):
-        outputs = [torch.empty(s, device=self.device) for s in self.output_shapes]
+        outputs = self._outputs()
         self.run_into(inputs, outputs)
         return outputs
 
@@ -345,7 +369,7 @@ class HIPExecutable:
     def profile(self, *inputs, iters=20):
         """[(launch name, GPU ms per launch)], each launch timed natively."""
         inputs = self._prepare(inputs)
-        outputs = [torch.empty(s, device=self.device) for s in self.output_shapes]
+        outputs = self._outputs()
         ins, outs = [t.data_ptr() for t in inputs], [t.data_ptr() for t in outputs]
         self.run_into(inputs, outputs)
         stream = current_stream_handle()

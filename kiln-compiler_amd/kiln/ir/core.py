@@ -22,8 +22,13 @@ from typing import NamedTuple
 import numpy as np
 
 
+ELEMENT_BYTES = {"f32": 4, "i32": 4, "bf16": 2, "f16": 2}
+
+
 class TensorType(NamedTuple):
-    """Static shape and element type (only "f32" is produced)."""
+    """Static shape and element type: "f32", but for the operands of the paged
+    cache's operators (its pages may be "bf16" or "f16", tables and lists of
+    pages are "i32")."""
 
     shape: tuple
     dtype: str = "f32"
@@ -38,7 +43,7 @@ class TensorType(NamedTuple):
 
     @property
     def nbytes(self) -> int:
-        return 4 * self.numel
+        return ELEMENT_BYTES[self.dtype] * self.numel
 
     def __str__(self) -> str:
         return self.dtype + "[" + ", ".join(map(str, self.shape)) + "]"

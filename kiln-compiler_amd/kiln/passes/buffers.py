@@ -15,8 +15,10 @@ the annotations):
   * a ``copy`` kernel is added only where that is impossible: a result that
     no kernel writes (an argument, a constant, a view, a value returned
     twice), a view that strides cannot express (a reshape of a transposed
-    value), and the B operand of a matmul whose columns are not contiguous
-    (the GEMM family streams B rows along N as 16-byte vectors).
+    value), the B operand of a matmul whose columns are not contiguous (the
+    GEMM family streams B rows along N as 16-byte vectors), and the q, k or v
+    of an operator over a paged cache whose rows are not (16-byte aligned
+    vectors too).
 
 Kernels are renumbered k0, k1, ... in a topological order afterwards (copies
 are created out of order).
@@ -188,6 +190,12 @@ def _needs_copy(n, layouts):
         seen = layouts.get(b)
         if seen is not None and b.shape[-1] > 1 and seen.strides[-1] != 1:
             return 1
+    if ops.kind(n.op) == "paged":
+        for i, v in enumerate(n.inputs[:ops.PAGED_OPERANDS[n.op]]):
+            seen = layouts.get(v)
+            rows = None if seen is None else seen.strides[:-1]
+            if seen is not None and (seen.strides[-1] != 1 or seen.offset % 4 or any(s % 4 for s in rows)):
+                return i
     return None
 
 
@@ -196,6 +204,8 @@ class BufferAssignment(Pass):
 
     @staticmethod
     def _new_copy(graph: Graph, v: Value, at: int) -> Value:
+        if v.type.dtype != "f32":   # a cache or a list of pages: read in place, returned by its operator alone
+            raise NotImplementedError(f"HIP backend: a {v.type} cannot be copied")
         out = graph.add_node("copy", [v], {}, index=at)
         kernel = Kernel(f"copy{len(graph.kernels)}", "copy", [out.node])
         out.node.attrs["kernel"] = kernel.name

@@ -9,7 +9,8 @@ pinned by its tests/test_fusion.py:33-132 and the fusion.kir fixture):
   reduction    innermost-dim reductions and the elementwise ops over the same
                rows -> the row family (LayerNorm, softmax, generic tapes); a
                reduction over other dims is a kernel of its own (K-RED);
-  elementwise  a DAG of elementwise ops -> the elementwise family.
+  elementwise  a DAG of elementwise ops -> the elementwise family;
+  paged        an operator over a paged cache, always alone -> the paged family.
 
 The rules, applied to compute nodes in program order:
 
@@ -36,7 +37,7 @@ from kiln.ir import ops
 from kiln.ir.core import Graph, Kernel, Node
 from kiln.passes.manager import Pass
 
-_TRY_ORDER = {"matmul": 0, "reduction": 1, "elementwise": 2}
+_TRY_ORDER = {"matmul": 0, "reduction": 1, "elementwise": 2, "paged": 3}
 
 
 def is_row_reduction(n: Node) -> bool:
@@ -80,7 +81,7 @@ class _Kernel:
         self.start = start                       # program position of its first node
         self.matmul = node if self.kind == "matmul" else None
         self.space = None                        # (rows, inner) of a row kernel
-        self.closed = False                      # a reduction over other dims takes no company
+        self.closed = self.kind == "paged"       # ... and a reduction over other dims take no company
         self.after = set()                       # kernels that read its results
         if self.kind == "reduction":
             if is_row_reduction(node):

@@ -9,7 +9,7 @@ from kiln.ir import ops
 from kiln.ir.core import Graph, Kernel
 from kiln.passes.manager import Pass
 
-COMPUTE_KINDS = ("elementwise", "reduction", "matmul")
+COMPUTE_KINDS = ("elementwise", "reduction", "matmul", "paged")
 
 
 class OneOpPerKernel(Pass):
