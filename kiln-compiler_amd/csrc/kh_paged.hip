@@ -81,6 +81,10 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = "the pages' token stride is too large";
     return false;
   }
+  if (p.variant == KH_PAGED_ATTENTION && (std::abs(p.k_n) > most / 512 || std::abs(p.v_n) > most / 512)) {
+    err = "the new tokens' stride is too large";
+    return false;
+  }
   if (p.variant == KH_PAGED_SELECT &&
       ((int64_t)p.batch * p.kv_heads > 65535 || (p.width + 63) / 64 > (1 << 24))) {
     err = "more than 65535 (sequence, kv head) pairs";

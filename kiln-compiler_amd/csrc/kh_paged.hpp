@@ -34,6 +34,7 @@ struct PagedWork {
   int half_shift;  // page_size = 16 << half_shift
   int draft_tiles;
   int sel_tiles;   // tiles of the picked pages, 0 without
+  int whole;       // a workgroup per item, no second kernel
   int grid;        // workgroups of the first kernel
   int rounds;      // doublings that cover the longest path
   float scale2;    // scale * log2(e)

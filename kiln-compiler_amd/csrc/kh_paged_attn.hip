@@ -8,6 +8,7 @@ namespace kh {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWholeTiles = 16;
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -41,12 +42,13 @@ PagedWork work_of(const kh_paged &p) {
   w.rounds = 0;
   while ((1 << w.rounds) < p.draft) ++w.rounds;
   w.scale2 = p.scale * kLog2e;
-  // workgroups: what the chip holds at once, or a tile per wave of the most
-  // tiles the table has room for
   const int64_t per_item = (w.sel_tiles ? w.sel_tiles : ((int64_t)p.width * p.page_size + kPagedTile - 1) / kPagedTile) + w.draft_tiles;
-  const int64_t want = (per_item * w.items * p.batch + kPagedWaves - 1) / kPagedWaves;
+  const int64_t items = (int64_t)w.items * p.batch;
+  // workgroups: one per item where none can have many tiles; else what the
+  // chip holds at once, or a tile per wave of the most tiles the table has room for
+  w.whole = per_item <= kWholeTiles;
   const int cap = current_device().cus * (rm == 16 && padded_dim(p.dim) <= 128 ? 2 : 1);
-  w.grid = (int)std::min<int64_t>(want, cap);
+  w.grid = (int)(w.whole ? items : std::min<int64_t>((per_item * items + kPagedWaves - 1) / kPagedWaves, cap));
   w.part = nullptr;
   return w;
 }
@@ -55,7 +57,7 @@ PagedWork work_of(const kh_paged &p) {
 
 size_t paged_workspace_floats(const kh_paged &p) {
   const PagedWork w = work_of(p);
-  if (w.grid <= 1) return 0;
+  if (w.whole) return 0;
   return 2 * (size_t)w.grid * 16 * row_blocks(p) * (padded_dim(p.dim) + 2);
 }
 

@@ -8,14 +8,20 @@
 // ragged lengths loads every workgroup alike and one long sequence fills the
 // chip; the four waves of a workgroup take a range's tiles in turn. A range
 // that ends inside an item leaves (m, l, O) in the workspace, which a second
-// kernel joins; an item within one range is finished here.
+// kernel joins; an item within one range is finished here. Where no item can
+// have many tiles, a workgroup takes a whole item instead and one kernel is
+// enough.
 //
 // A wave holds its tile in registers: scores S^T = K Q^T, so that a lane has
 // its query's scores (lane li = lane & 15) for keys 4 g + r (g = lane >> 4),
 // which is how O^T += V^T P^T takes the weights back without a move; V^T's
 // operand needs 8 keys of one dimension per lane, which a lane makes from 8
 // rows' 16-byte pieces by 32 byte permutes. One pass over the keys with
-// running maximum and sum (base 2, fp32).
+// running maximum and sum (base 2, fp32). The next tile's K is loaded once
+// this one's scores are made, its V once this one's weights are used, into the
+// same registers: one to two tiles are in flight per wave without any for
+// themselves, and the page numbers come by scalar loads, which do not queue
+// behind them.
 //
 // fp32 activations over a 16-bit cache keep fp32's accuracy: a bf16 product's
 // three parts x = x1 + x2 + x3 of 8 bits each hold all 24 bits of q and of a
@@ -52,8 +58,13 @@ struct Plan {
   int64_t count;   // workgroups that take part
 };
 
+// int32 operands through the constant address space: a wave-uniform index
+// then becomes a scalar load (the kernels write none of them).
+typedef const __attribute__((address_space(4))) int32_t *const_ints;
+__device__ __forceinline__ const_ints ints_of(const int32_t *p) { return (const_ints)(uintptr_t)p; }
+
 __device__ __forceinline__ int clamp_len(const PagedWork &w, int s) {
-  const int n = w.p.lengths[s];
+  const int n = ints_of(w.p.lengths)[s];
   const int64_t most = (int64_t)w.p.width * w.p.page_size;
   return n < 0 ? 0 : (n > most ? (int)most : n);
 }
@@ -181,33 +192,21 @@ struct Cache<KH_TYPE_F16> {
   }
 };
 
-__device__ __forceinline__ float load_act(const void *p, int64_t i, int type) {
-  if (type == KH_TYPE_F32) return static_cast<const float *>(p)[i];
-  if (type == KH_TYPE_BF16) return (float)static_cast<const __bf16 *>(p)[i];
-  return (float)static_cast<const _Float16 *>(p)[i];
-}
-
-// n (4 or 8) adjacent activations from element i, 16-byte (8-byte) aligned
-template <int N>
-__device__ __forceinline__ void load_acts(const void *p, int64_t i, int type, float (&x)[N]) {
-  if (type == KH_TYPE_F32) {
+// n (4 or 8) adjacent activations from element i, fp32 or T, 16-byte (8-byte) aligned
+template <class T, int N>
+__device__ __forceinline__ void load_acts(const void *p, int64_t i, bool fp32, float (&x)[N]) {
+  if (sizeof(T) == 4 || fp32) {
 #pragma unroll
     for (int j = 0; j < N; j += 4) {
       const f32x4 a = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i + j);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[j + e] = a[e];
     }
-    return;
-  }
+  } else {
+    typedef T vec __attribute__((ext_vector_type(N)));
+    const vec a = *reinterpret_cast<const vec *>(static_cast<const T *>(p) + i);
 #pragma unroll
-  for (int j = 0; j < N; j += 4) {
-    const u32x2 a = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p) + i + j);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t half = (a[e / 2] >> (16 * (e & 1))) & 0xffffu;
-      x[j + e] = type == KH_TYPE_BF16 ? __uint_as_float(half << 16)
-                                      : (float)__builtin_bit_cast(_Float16, (uint16_t)half);
-    }
+    for (int j = 0; j < N; ++j) x[j] = (float)a[j];
   }
 }
 
@@ -261,8 +260,6 @@ struct Tile {
   static constexpr int VW = CT == KH_TYPE_F32 ? VD : VD / 2;   // words of VD elements
   uint32_t k[2][KS][KW];
   uint32_t v[8][VC][VW];
-  int valid[2];       // keys of each half
-  int draft;          // index of the tile among the new tokens' tiles, -1 for a cached one
 };
 
 template <int N>
@@ -281,9 +278,13 @@ __device__ __forceinline__ void load_words(const void *p, uint32_t (&x)[N]) {
   }
 }
 
-// Where the two halves of a cached tile lie.
-struct Spot {
-  int page[2], slot[2], valid[2];
+// Where a tile's halves lie (uniform over the wave): rows of `valid` keys each.
+template <class T>
+struct Source {
+  const T *k[2], *v[2];
+  int k_row, v_row;    // elements from a key to the next
+  int valid[2];
+  int draft;           // index among the new tokens' tiles, -1 for a cached one
 };
 
 // FULL: dim == DT, every lane's pieces lie inside a row.
@@ -295,8 +296,8 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
   constexpr int KS = Regs::KS, VD = Regs::VD, VC = Regs::VC;
   constexpr int RM = 16 * RT;
   constexpr int NT = DT / 16;                  // 16-wide tiles of O^T: (chunk, t)
-  constexpr bool SCALED_P = CT == KH_TYPE_F16;
   constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NP > 1;
+  constexpr float kBias = CT == KH_TYPE_F16 ? kWeightExp : 0.0f;
 
   __shared__ int first[kMaxBatch + 1];
   __shared__ int wave_sums[kWaves];
@@ -307,29 +308,42 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
   const kh_paged &p = w.p;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool act32 = p.act_type == KH_TYPE_F32;
 
-  scan_tiles(w, first, wave_sums);
-  const Plan plan = plan_of(w, first);
-  // neighbouring ranges on the same XCD: they share row blocks' keys
   int me = blockIdx.x;
-  if (me >= plan.count) return;
-  {
+  int64_t at = 0, end = 1;
+  if (!w.whole) {
+    scan_tiles(w, first, wave_sums);
+    const Plan plan = plan_of(w, first);
+    if (me >= plan.count) return;
+    // neighbouring ranges on the same XCD: they share row blocks' keys
     const int xcd = me & 7, per = (int)plan.count >> 3, rest = (int)plan.count & 7;
     me = xcd * per + min(xcd, rest) + (me >> 3);
+    at = range_start(plan, me);
+    end = range_start(plan, me + 1);
   }
-  const int64_t begin = range_start(plan, me), end = range_start(plan, me + 1);
 
   int paths_of = -1;   // sequence whose paths the LDS holds
-  int64_t at = begin;
   while (at < end) {
-    const int s = sequence_of(w, first, at);
-    const int len = clamp_len(w, s);
-    const int tiles = tiles_of(w, len);
-    const int64_t in_seq = at - (int64_t)first[s] * w.items;
-    const int item = (int)(in_seq / tiles);
-    const int t0 = (int)(in_seq - (int64_t)item * tiles);
-    const int t1 = (int)min((int64_t)tiles, t0 + (end - at));
-    at += t1 - t0;
+    int s, item, t0, t1, tiles, len;
+    if (w.whole) {
+      s = me / w.items;
+      item = me - s * w.items;
+      len = clamp_len(w, s);
+      tiles = tiles_of(w, len);
+      t0 = 0;
+      t1 = tiles;
+      at = end;
+    } else {
+      s = __builtin_amdgcn_readfirstlane(sequence_of(w, first, at));
+      len = clamp_len(w, s);
+      tiles = tiles_of(w, len);
+      const int64_t in_seq = at - (int64_t)__builtin_amdgcn_readfirstlane(first[s]) * w.items;
+      item = (int)(in_seq / tiles);
+      t0 = (int)(in_seq - (int64_t)item * tiles);
+      t1 = (int)min((int64_t)tiles, t0 + (end - at));
+      at += t1 - t0;
+    }
     const int cached = tiles - w.draft_tiles;
     // item = (kv head, [token,] row block)
     const int per_head = w.items / p.kv_heads;
@@ -345,6 +359,111 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
       paths_of = s;
     }
 
+    // -- where tile t lies; the first tile at or after t with a key, in steps of the waves
+    const T *kp = static_cast<const T *>(p.k_pages) + c * p.kp_h, *vp = static_cast<const T *>(p.v_pages) + c * p.vp_h;
+    auto find = [&](int &t, Source<T> &r) {
+      for (; t < t1; t += kWaves) {
+        if (t >= cached) {
+          r.draft = t - cached;
+          const int n0 = kTile * r.draft;
+          r.k_row = (int)p.k_n;
+          r.v_row = (int)p.v_n;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            r.valid[h] = min(max(p.draft - (n0 + 16 * h), 0), 16);
+            const int n = r.valid[h] ? n0 + 16 * h : 0;
+            r.k[h] = static_cast<const T *>(p.k) + (s * p.k_s + c * p.k_h + n * p.k_n);
+            r.v[h] = static_cast<const T *>(p.v) + (s * p.v_s + c * p.v_h + n * p.v_n);
+          }
+          return;
+        }
+        r.draft = -1;
+        r.k_row = (int)p.kp_t;
+        r.v_row = (int)p.vp_t;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int j = 2 * t + h;
+          int col = j >> w.half_shift, pos = 16 * j;
+          const int slot = (j & ((1 << w.half_shift) - 1)) * 16;
+          bool in = true;
+          if (w.sel_tiles) {
+            const int rank = col;
+            in = rank < p.top;
+            const const_ints list = ints_of(p.selected) + (s * p.sel_s + token * p.sel_n + c * p.sel_h);
+            const int before = in && rank > 0 ? list[rank - 1] : -1;
+            col = in ? list[rank] : 0;
+            in = in && col > before && col >= 0 && col < p.width;
+            pos = in ? col * p.page_size + slot : len;
+          }
+          in = in && pos < len;
+          const int page = in ? ints_of(p.table)[s * p.table_s + col] : 0;
+          in = in && page >= 0 && page < p.pages;
+          r.valid[h] = in ? min(len - pos, 16) : 0;
+          const int there = in ? page : 0;
+          r.k[h] = kp + (there * p.kp_p + (int64_t)(slot * r.k_row));
+          r.v[h] = vp + (there * p.vp_p + (int64_t)(slot * r.v_row));
+        }
+        if (r.valid[0] | r.valid[1]) return;
+      }
+    };
+
+    // a new tile of fp32 activations over a 16-bit cache is rounded as it is loaded
+    auto rounds = [&](const Source<T> &r) { return !F32 && act32 && r.draft >= 0; };
+    auto load_k = [&](const Source<T> &r, Regs &x) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = min(li, max(r.valid[h], 1) - 1) * r.k_row;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int d = 32 * ks + 8 * g, in = FULL || d < p.dim ? d : 0;
+          if (!rounds(r)) {
+            load_words(r.k[h] + (uint32_t)(row + in), x.k[h][ks]);
+          } else if constexpr (!F32) {
+            // (r.k counts elements of T, the activations are fp32: twice its size)
+            const float *y = static_cast<const float *>(p.k) + (r.k[h] - static_cast<const T *>(p.k)) + (row + in);
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(y), hi = *reinterpret_cast<const f32x4 *>(y + 4);
+            x.k[h][ks][0] = pack2<T>(lo[0], lo[1]);
+            x.k[h][ks][1] = pack2<T>(lo[2], lo[3]);
+            x.k[h][ks][2] = pack2<T>(hi[0], hi[1]);
+            x.k[h][ks][3] = pack2<T>(hi[2], hi[3]);
+          }
+        }
+      }
+    };
+    auto load_v = [&](const Source<T> &r, Regs &x) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = min(4 * g + i, max(r.valid[h], 1) - 1) * r.v_row;
+#pragma unroll
+          for (int vc = 0; vc < VC; ++vc) {
+            const int d = 16 * VD * vc + VD * li, in = FULL || d < p.dim ? d : 0;
+            if (!rounds(r)) {
+              load_words(r.v[h] + (uint32_t)(row + in), x.v[4 * h + i][vc]);
+            } else if constexpr (!F32) {
+              const float *y = static_cast<const float *>(p.v) + (r.v[h] - static_cast<const T *>(p.v)) + (row + in);
+#pragma unroll
+              for (int e = 0; e < VD; e += 4) {
+                const f32x4 z = *reinterpret_cast<const f32x4 *>(y + e);
+                x.v[4 * h + i][vc][e / 2] = pack2<T>(z[0], z[1]);
+                x.v[4 * h + i][vc][e / 2 + 1] = pack2<T>(z[2], z[3]);
+              }
+            }
+          }
+        }
+      }
+    };
+
+    Regs x;
+    Source<T> here;
+    int t = t0 + wave;
+    find(t, here);
+    if (t < t1) {
+      load_k(here, x);
+      load_v(here, x);
+    }
+
     // this lane's query rows
     int row_token[RT], row_head[RT];
     bool row_ok[RT];
@@ -358,44 +477,44 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
     }
     u32x4 q16[F32 ? 1 : NP][RT][KS];
     float q32[F32 ? RT : 1][F32 ? KS : 1][8];
-    float mult[RT];   // scores to the base-2 domain
+    float mult[RT];   // products to the base-2 domain, not negative: q takes a negative scale's sign
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float x[KS][8];
+      float y[KS][8];
       const int64_t base = s * p.q_s + row_token[rt] * p.q_n + row_head[rt] * p.q_h;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d = 32 * ks + 8 * g;
         const bool in = row_ok[rt] && (FULL || d < p.dim);
-        load_acts(p.q, base + (in ? d : 0), p.act_type, x[ks]);
+        load_acts<T>(p.q, base + (in ? d : 0), act32, y[ks]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[ks][j] = in ? x[ks][j] : 0.0f;
+        for (int j = 0; j < 8; ++j) y[ks][j] = in ? y[ks][j] : 0.0f;
       }
-      mult[rt] = w.scale2;
-      float up = 1.0f;
+      float up = w.scale2 < 0.0f ? -1.0f : 1.0f;
+      mult[rt] = fabsf(w.scale2);
       if constexpr (SCALED_Q) {
         float most = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[ks][j]));
+          for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(y[ks][j]));
         most = max16x32(most);
         // the power of two that brings the largest to [2^14, 2^15)
         int e = (int)((__float_as_uint(most) >> 23) & 255) - 127;
         e = most == 0.0f || e == 128 ? 0 : min(max(14 - e, -126), 126);
-        up = __uint_as_float((uint32_t)(e + 127) << 23);
-        mult[rt] = w.scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
+        up *= __uint_as_float((uint32_t)(e + 127) << 23);
+        mult[rt] *= __uint_as_float((uint32_t)(127 - e) << 23);
       }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[ks][j] *= up;
         if constexpr (F32) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) q32[rt][ks][j] = x[ks][j];
+          for (int j = 0; j < 8; ++j) q32[rt][ks][j] = y[ks][j];
         } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[ks][j] *= up;
           u32x4 parts[NP];
-          split8<T, NP>(x[ks], parts);
+          split8<T, NP>(y[ks], parts);
 #pragma unroll
           for (int n = 0; n < NP; ++n) q16[n][rt][ks] = parts[n];
         }
@@ -411,94 +530,15 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
 #pragma unroll
       for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
-        for (int t = 0; t < VD; ++t) o[rt][vc][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < VD; ++i) o[rt][vc][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // -- where a cached tile lies (uniform over the wave)
-    auto spot = [&](int t) {
-      Spot r;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int j = 2 * t + h;
-        int col = j >> w.half_shift, pos = 16 * j;
-        r.slot[h] = (j & ((1 << w.half_shift) - 1)) * 16;
-        bool in = true;
-        if (w.sel_tiles) {
-          const int rank = col;
-          in = rank < p.top;
-          const int32_t *list = p.selected + s * p.sel_s + token * p.sel_n + c * p.sel_h;
-          const int before = in && rank > 0 ? list[rank - 1] : -1;
-          col = in ? list[rank] : 0;
-          in = in && col > before && col >= 0 && col < p.width;
-          pos = in ? col * p.page_size + r.slot[h] : len;
-        }
-        in = in && pos < len;
-        const int page = in ? p.table[s * p.table_s + col] : 0;
-        in = in && page >= 0 && page < p.pages;
-        r.page[h] = in ? page : 0;
-        r.valid[h] = in ? min(len - pos, 16) : 0;
-      }
-      return r;
-    };
+    while (t < t1) {
+      int t_next = t + kWaves;
+      Source<T> next;
+      find(t_next, next);
 
-    auto load_cached = [&](const Spot &at_, Regs &x) {
-      x.draft = -1;
-      const T *kp = static_cast<const T *>(p.k_pages), *vp = static_cast<const T *>(p.v_pages);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        x.valid[h] = at_.valid[h];
-        const T *kb = kp + (at_.page[h] * p.kp_p + c * p.kp_h + at_.slot[h] * p.kp_t);
-        const T *vb = vp + (at_.page[h] * p.vp_p + c * p.vp_h + at_.slot[h] * p.vp_t);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int d = 32 * ks + 8 * g;
-          load_words(kb + (uint32_t)(li * (int)p.kp_t + (FULL || d < p.dim ? d : 0)), x.k[h][ks]);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int vc = 0; vc < VC; ++vc) {
-            const int d = 16 * VD * vc + VD * li;
-            load_words(vb + (uint32_t)((4 * g + r) * (int)p.vp_t + (FULL || d < p.dim ? d : 0)), x.v[4 * h + r][vc]);
-          }
-      }
-    };
-
-    // new tokens 32 j ..: their k and v rounded to the cache's type
-    auto load_new = [&](int j, Regs &x) {
-      x.draft = j;
-      auto to_words = [&](const float *y, uint32_t *out, int n) {
-        for (int e = 0; e < n; ++e)
-          if constexpr (F32) out[e] = __float_as_uint(y[e]);
-          else if (!(e & 1)) out[e / 2] = pack2<T>(y[e], y[e + 1]);
-      };
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        x.valid[h] = min(max(p.draft - (32 * j + 16 * h), 0), 16);
-        const int64_t kn = min(32 * j + 16 * h + li, p.draft - 1);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int d = 32 * ks + 8 * g;
-          float y[8];
-          load_acts(p.k, s * p.k_s + kn * p.k_n + c * p.k_h + (FULL || d < p.dim ? d : 0), p.act_type, y);
-          to_words(y, x.k[h][ks], 8);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int vc = 0; vc < VC; ++vc) {
-            const int d = 16 * VD * vc + VD * li;
-            const int64_t vn = min(32 * j + 16 * h + 4 * g + r, p.draft - 1);
-            float y[VD];
-            load_acts(p.v, s * p.v_s + vn * p.v_n + c * p.v_h + (FULL || d < p.dim ? d : 0), p.act_type, y);
-            to_words(y, x.v[4 * h + r][vc], VD);
-          }
-      }
-    };
-
-    auto compute = [&](Regs &x) {
-      // rows past a dimension's end: whatever was read meets q = 0, which needs it finite
-      if constexpr (!FULL) {
+      if constexpr (!FULL) {   // beyond dim: whatever was read meets q = 0, which needs it finite
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
           if (32 * ks + 8 * g >= p.dim) {
@@ -508,167 +548,172 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
               for (int e = 0; e < Regs::KW; ++e) x.k[h][ks][e] = 0;
           }
       }
-      // values behind the last key of a half: whatever they hold (a page's
-      // unwritten slots), their weight is 0, which needs them finite
-      if (x.valid[0] < 16 || x.valid[1] < 16) {
+      f32x4 sc[RT][2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (4 * g + (j & 3) >= x.valid[j >> 2]) {
-#pragma unroll
-            for (int vc = 0; vc < VC; ++vc)
-#pragma unroll
-              for (int e = 0; e < Regs::VW; ++e) x.v[j][vc][e] = 0;
-          }
-      }
-      uint32_t see[RT];   // which of the tile's keys this lane's rows attend to
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const uint32_t there = ((1u << x.valid[0]) - 1) | ((1u << x.valid[1]) - 1) << 16;
-        see[rt] = there;
-        if (x.draft >= 0) {
-          const int i = row_token[rt] - 32 * x.draft;   // chain: the tokens up to its own
-          see[rt] &= p.parents ? paths.bits[row_token[rt]][x.draft]
-                               : (i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1);
-        }
-      }
-      // a new token's value that is not finite must not reach rows that do not
-      // attend to it through 0 * inf: it is taken out of the product here and
-      // added by hand below
-      uint32_t odd = 0;   // keys of this lane's group with such a value
-      if (x.draft >= 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int vc = 0; vc < VC; ++vc)
-#pragma unroll
-            for (int e = 0; e < Regs::VW; ++e) {
-              const uint32_t u = x.v[j][vc][e];
-              if constexpr (F32) {
-                if ((u & 0x7f800000u) == 0x7f800000u) {
-                  x.v[j][vc][e] = 0;
-                  odd |= 1u << j;
-                }
-              } else {
-                constexpr uint32_t kExp = CT == KH_TYPE_BF16 ? 0x7f80u : 0x7c00u;
-                const bool lo = (u & kExp) == kExp, hi = (u >> 16 & kExp) == kExp;
-                if (lo || hi) {
-                  x.v[j][vc][e] = (lo ? 0u : u & 0xffffu) | (hi ? 0u : u & 0xffff0000u);
-                  odd |= 1u << j;
-                }
-              }
-            }
-      }
-
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        f32x4 sc[2];
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          sc[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          sc[rt][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
           if constexpr (F32) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
               for (int j = 0; j < 8; ++j)
-                sc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[h][ks][j]), q32[rt][ks][j], sc[h], 0, 0, 0);
+                sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[h][ks][j]), q32[rt][ks][j], sc[rt][h], 0, 0, 0);
           } else {
 #pragma unroll
             for (int n = NP - 1; n >= 0; --n)
 #pragma unroll
               for (int ks = 0; ks < KS; ++ks) {
                 const u32x4 a = {x.k[h][ks][0], x.k[h][ks][1], x.k[h][ks][2], x.k[h][ks][3]};
-                sc[h] = Cache<CT>::mma(a, q16[n][rt][ks], sc[h]);
+                sc[rt][h] = Cache<CT>::mma(a, q16[n][rt][ks], sc[rt][h]);
               }
           }
         }
-        // the running softmax of this lane's row (the four lane groups of a row agree on m)
-        float pr[8], most = -INFINITY;
+      if (t_next < t1) load_k(next, x);
+
+      uint32_t odd = 0;   // this lane group's keys with a value that is not finite (new tokens only)
+      uint32_t see[RT];
+      const bool partly = here.draft >= 0 || (here.valid[0] & here.valid[1]) < 16;
+      if (partly) {
+        // which of the tile's keys this lane's rows attend to
+        const uint32_t there = ((1u << here.valid[0]) - 1) | ((1u << here.valid[1]) - 1) << 16;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool on = see[rt] >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1;
-          pr[j] = on ? sc[j >> 2][j & 3] * mult[rt] : -INFINITY;
-          most = fmaxf(most, pr[j]);
+        for (int rt = 0; rt < RT; ++rt) {
+          see[rt] = there;
+          if (here.draft >= 0) {
+            const int i = row_token[rt] - kTile * here.draft;   // chain: the tokens up to its own
+            see[rt] &= p.parents ? paths.bits[row_token[rt]][here.draft] : (i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!(see[rt] >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1)) sc[rt][j >> 2][j & 3] = -INFINITY;
         }
-        const float m_new = fmaxf(m[rt], max16x32(most));
-        const float zero = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: every weight is 0
-        const float shrink = __builtin_amdgcn_exp2f(m[rt] - zero);
-        m[rt] = m_new;
-        l[rt] *= shrink;
+        // values behind the last key (a page's unwritten slots): their weight
+        // is 0, which needs them finite
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          pr[j] = __builtin_amdgcn_exp2f(pr[j] - zero + (SCALED_P ? kWeightExp : 0.0f));
-          l[rt] += pr[j];
-        }
-        if (__any(shrink != 1.0f)) {
+        for (int j = 0; j < 8; ++j)
+          if (4 * g + (j & 3) >= here.valid[j >> 2]) {
 #pragma unroll
-          for (int vc = 0; vc < VC; ++vc)
+            for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
-            for (int t = 0; t < VD; ++t) o[rt][vc][t] *= shrink;
-        }
-        if constexpr (F32) {
+              for (int e = 0; e < Regs::VW; ++e) x.v[j][vc][e] = 0;
+          }
+        // a new token's value that is not finite must not reach rows that do
+        // not attend to it through 0 * inf: it is taken out of the product
+        // here and added by hand below
+        if (here.draft >= 0) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
-              for (int t = 0; t < VD; ++t)
-                o[rt][vc][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][vc][t]), pr[j], o[rt][vc][t], 0, 0, 0);
-        } else {
-          u32x4 parts[NP];
-          split8<T, NP>(pr, parts);
+              for (int e = 0; e < Regs::VW; ++e) {
+                const uint32_t u = x.v[j][vc][e];
+                if constexpr (F32) {
+                  if ((u & 0x7f800000u) == 0x7f800000u) {
+                    x.v[j][vc][e] = 0;
+                    odd |= 1u << j;
+                  }
+                } else {
+                  constexpr uint32_t kExp = CT == KH_TYPE_BF16 ? 0x7f80u : 0x7c00u;
+                  const bool lo = (u & kExp) == kExp, hi = (u >> 16 & kExp) == kExp;
+                  if (lo || hi) {
+                    x.v[j][vc][e] = (lo ? 0u : u & 0xffffu) | (hi ? 0u : u & 0xffff0000u);
+                    odd |= 1u << j;
+                  }
+                }
+              }
+        }
+      }
+
+      // the running softmax of this lane's rows (the four lane groups of a row agree on m)
+      float pr[RT][8];
+      u32x4 parts[F32 ? 1 : RT][NP];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float most = sc[rt][0][0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) most = fmaxf(most, sc[rt][j >> 2][j & 3]);
+        most = max16x32(most);
+        const float m_new = fmaxf(m[rt], most == -INFINITY ? most : most * mult[rt]);
+        const float zero = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: every weight is 0
+        const float shrink = __builtin_amdgcn_exp2f(m[rt] - zero);
+        m[rt] = m_new;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = sc[rt][j >> 2][j & 3];
+          pr[rt][j] = __builtin_amdgcn_exp2f(partly && y == -INFINITY ? y : fmaf(y, mult[rt], kBias - zero));
+          sum += pr[rt][j];
+        }
+        l[rt] = fmaf(l[rt], shrink, sum);
+        if (__any(shrink != 1.0f)) {
 #pragma unroll
           for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
-            for (int t = 0; t < VD; ++t) {
-              u32x4 a;   // 8 keys of dimension t
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                a[e] = __builtin_amdgcn_perm(x.v[2 * e + 1][vc][t / 2], x.v[2 * e][vc][t / 2],
-                                             t & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-              for (int n = NP - 1; n >= 0; --n) o[rt][vc][t] = Cache<CT>::mma(a, parts[n], o[rt][vc][t]);
-            }
+            for (int i = 0; i < VD; ++i) o[rt][vc][i] *= shrink;
         }
-        if (x.draft >= 0 && __any(odd != 0)) {
-          for (int key = 0; key < 32; ++key) {   // rare: the values taken out, by hand
-            const int j = 4 * (key >> 4) + (key & 3), from = (key & 15) >> 2;
-            if (!__any(g == from && (odd >> j & 1))) continue;
+        if constexpr (!F32) split8<T, NP>(pr[rt], parts[rt]);
+      }
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int vc = 0; vc < VC; ++vc)
+#pragma unroll
+            for (int i = 0; i < VD; ++i)
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+                o[rt][vc][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][vc][i]), pr[rt][j], o[rt][vc][i], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int vc = 0; vc < VC; ++vc)
+#pragma unroll
+          for (int i = 0; i < VD; ++i) {
+            u32x4 a;   // 8 keys of dimension i
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              a[e] = __builtin_amdgcn_perm(x.v[2 * e + 1][vc][i / 2], x.v[2 * e][vc][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int n = NP - 1; n >= 0; --n) o[rt][vc][i] = Cache<CT>::mma(a, parts[rt][n], o[rt][vc][i]);
+          }
+      }
+      if (t_next < t1) load_v(next, x);
+
+      if (__builtin_expect(__any(odd != 0), 0)) {
+        for (int key = 0; key < kTile; ++key) {   // the values taken out, by hand
+          const int j = 4 * (key >> 4) + (key & 3), from = (key & 15) >> 2;
+          if (!__any(g == from && (odd >> j & 1))) continue;
+          const int n = min(kTile * here.draft + key, p.draft - 1);
+          const int64_t row = s * p.v_s + c * p.v_h + n * p.v_n;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
             float mine = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mine = e == j ? pr[e] : mine;
+            for (int e = 0; e < 8; ++e) mine = e == j ? pr[rt][e] : mine;
             const float weight = __shfl(mine, li + 16 * from);
-            const bool on = see[rt] >> key & 1;
-            const int64_t vn = min(32 * x.draft + key, p.draft - 1);
+            if (!(see[rt] >> key & 1)) continue;
+#pragma unroll
             for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
-              for (int t = 0; t < VD; ++t)
+              for (int r = 0; r < 4; ++r) {
+                const int d = 16 * VD * vc + VD * (4 * g + r);
+                float y[VD];
+                load_acts<T>(p.v, row + (FULL || d < p.dim ? d : 0), act32, y);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const int d = 16 * VD * vc + VD * (4 * g + r) + t;
-                  if (d < p.dim && on) {
-                    const float y = (float)(T)load_act(p.v, s * p.v_s + vn * p.v_n + c * p.v_h + d, p.act_type);
-                    if (!(fabsf(y) < INFINITY)) {
-#pragma unroll
-                      for (int vv = 0; vv < VC; ++vv)
-                        if (vv == vc) o[rt][vv][t][r] += weight * y;
-                    }
-                  }
+                for (int i = 0; i < VD; ++i) {
+                  const float z = (float)(T)y[i];
+                  if (!(fabsf(z) < INFINITY)) o[rt][vc][i][r] += weight * z;
                 }
+              }
           }
         }
       }
-    };
-
-    for (int t = t0 + wave; t < t1; t += kWaves) {
-      Regs x;
-      if (t < cached) {
-        const Spot here = spot(t);
-        if ((here.valid[0] | here.valid[1]) == 0) continue;
-        load_cached(here, x);
-      } else {
-        load_new(t - cached, x);
-      }
-      compute(x);
+      here = next;
+      t = t_next;
     }
 
     // -- the four waves' parts joined, in wave order
@@ -684,7 +729,7 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
 #pragma unroll
         for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
-          for (int t = 0; t < VD; ++t) o_share[to][rt][vc * VD + t][lane] = o[rt][vc][t];
+          for (int i = 0; i < VD; ++i) o_share[to][rt][vc * VD + i][lane] = o[rt][vc][i];
         if (g == 0) {
           ml_share[to][0][rt * 16 + li] = m[rt];
           ml_share[to][1][rt * 16 + li] = l[rt];
@@ -702,18 +747,22 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
 #pragma unroll
         for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
-          for (int t = 0; t < VD; ++t) o[rt][vc][t] = o[rt][vc][t] * a + o_share[from][rt][vc * VD + t][lane] * b2;
+          for (int i = 0; i < VD; ++i) o[rt][vc][i] = o[rt][vc][i] * a + o_share[from][rt][vc * VD + i][lane] * b2;
       }
     };
-    if (wave >= 2) put(wave - 2);
-    __syncthreads();
-    if (wave < 2) join(wave);
-    __syncthreads();
-    if (wave == 1) put(0);
-    __syncthreads();
+    if (t1 - t0 > 2) {   // (else waves 2 and 3 had no tile)
+      if (wave >= 2) put(wave - 2);
+      __syncthreads();
+      if (wave < 2) join(wave);
+      __syncthreads();
+    }
+    if (t1 - t0 > 1) {
+      if (wave == 1) put(0);
+      __syncthreads();
+      if (wave == 0) join(0);
+    }
     if (wave == 0) {
-      join(0);
-      const bool whole = t0 == 0 && t1 == tiles;
+      const bool done = t0 == 0 && t1 == tiles;
       // (t0 > 0: this range's first part; else its last)
       const int64_t slot = 2 * (int64_t)me + (t0 > 0 ? 0 : 1);
       float *part = w.part + slot * RM * DT;
@@ -721,11 +770,11 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         if (!row_ok[rt]) continue;
-        if (!whole && g == 0) {
+        if (!done && g == 0) {
           stats[2 * (rt * 16 + li)] = m[rt];
           stats[2 * (rt * 16 + li) + 1] = l[rt];
         }
-        const float norm = l[rt] < 0.0f ? 0.0f : 1.0f / l[rt];
+        const float norm = 1.0f / l[rt];
         const int64_t out = s * p.o_s + row_token[rt] * p.o_n + row_head[rt] * p.o_h;
 #pragma unroll
         for (int vc = 0; vc < VC; ++vc)
@@ -735,44 +784,39 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
             if (!FULL && d >= p.dim) continue;
             float y[VD];
 #pragma unroll
-            for (int t = 0; t < VD; ++t) y[t] = o[rt][vc][t][r];
-            if (!whole) {
+            for (int i = 0; i < VD; ++i) y[i] = o[rt][vc][i][r];
+            float *to = part + (rt * 16 + li) * DT + d;
+            if (done) {
 #pragma unroll
-              for (int t = 0; t < VD; t += 4)
-                *reinterpret_cast<f32x4 *>(part + (rt * 16 + li) * DT + d + t) = f32x4{y[t], y[t + 1], y[t + 2], y[t + 3]};
-              continue;
+              for (int i = 0; i < VD; ++i) y[i] = l[rt] < 0.0f ? 0.0f : y[i] * norm;
+              to = static_cast<float *>(p.out) + out + d;
             }
+            if (F32 || act32 || !done) {
 #pragma unroll
-            for (int t = 0; t < VD; ++t) y[t] = l[rt] < 0.0f ? 0.0f : y[t] * norm;
-            if (p.act_type == KH_TYPE_F32) {
+              for (int i = 0; i < VD; i += 4) *reinterpret_cast<f32x4 *>(to + i) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+            } else if constexpr (!F32) {
 #pragma unroll
-              for (int t = 0; t < VD; t += 4)
-                *reinterpret_cast<f32x4 *>(static_cast<float *>(p.out) + out + d + t) = f32x4{y[t], y[t + 1], y[t + 2], y[t + 3]};
-            } else {
-#pragma unroll
-              for (int t = 0; t < VD; t += 4) {
-                u32x2 pair;
-                if (p.act_type == KH_TYPE_BF16) pair = u32x2{pack2<__bf16>(y[t], y[t + 1]), pack2<__bf16>(y[t + 2], y[t + 3])};
-                else pair = u32x2{pack2<_Float16>(y[t], y[t + 1]), pack2<_Float16>(y[t + 2], y[t + 3])};
-                *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p.out) + out + d + t) = pair;
-              }
+              for (int i = 0; i < VD; i += 4)
+                *reinterpret_cast<u32x2 *>(static_cast<T *>(p.out) + out + d + i) = u32x2{pack2<T>(y[i], y[i + 1]), pack2<T>(y[i + 2], y[i + 3])};
             }
           }
       }
     }
-    __syncthreads();   // the shared parts are free again
+    if (at < end) __syncthreads();   // the shared parts are free again
   }
 }
 
-// The parts of the items that more than one range touched, joined: one wave
-// per row, two passes over the parts (the largest maximum, then the weighted
-// sum in range order).
+// The parts of the items that more than one range touched, joined: a
+// workgroup per row. Weights first, a part per lane, then the weighted sums,
+// every fourth part to a wave, then the waves' sums in order.
 template <int DT, int RT>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w) {
   constexpr int RM = 16 * RT;
   constexpr int PER = DT / 64;   // dimensions of a lane
   __shared__ int first[kMaxBatch + 1];
   __shared__ int wave_sums[kWaves];
+  __shared__ float sums[kWaves][DT];
+  __shared__ float weights[64];
   const kh_paged &p = w.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -787,45 +831,59 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
   const int c = item / per_head, b = item - c * per_head;
   const int token = w.sel_tiles ? b / w.blocks : 0;
   const int row0 = (w.sel_tiles ? b - token * w.blocks : b) * RM;
-  const int r = blockIdx.y * kWaves + wave;
-  if (row0 + r >= w.rows || r >= RM) return;
+  const int r = blockIdx.y;
+  if (row0 + r >= w.rows) return;
   const int n = w.sel_tiles ? token : (row0 + r) / w.group;
   const int head = c * w.group + (w.sel_tiles ? row0 + r : row0 + r - n * w.group);
   const float *stats = w.part + 2 * (int64_t)w.grid * RM * DT + 2 * r;
   // part i of the item: the last part of range w0, then the first of the others
-  auto slot = [&](int64_t i) { return 2 * (w0 + i) + (i == 0 ? 1 : 0); };
-  const int64_t count = w1 - w0 + 1;
+  auto slot = [&](int i) { return 2 * (w0 + i) + (i == 0 ? 1 : 0); };
+  const int count = (int)(w1 - w0 + 1);
   float m = -INFINITY;
-  bool unused = false;
-  for (int64_t i = lane; i < count; i += 64) {
-    m = fmaxf(m, stats[slot(i) * RM * 2]);
-    unused |= stats[slot(i) * RM * 2 + 1] < 0.0f;
-  }
+  for (int i = lane; i < count; i += 64) m = fmaxf(m, stats[slot(i) * RM * 2]);
   m = wave_max(m);
-  unused = __any(unused);
   if (m == -INFINITY) m = 0.0f;
   float l = 0.0f, o[PER];
+  bool unused = false;
 #pragma unroll
   for (int e = 0; e < PER; ++e) o[e] = 0.0f;
-#pragma unroll 4
-  for (int64_t i = 0; i < count; ++i) {
-    const int64_t at = slot(i);
-    const float a = __builtin_amdgcn_exp2f(stats[at * RM * 2] - m);
-    l += a * stats[at * RM * 2 + 1];
-    const float *part = w.part + (at * RM + r) * DT + lane * PER;
+  const bool in = lane * PER < p.dim;   // (dim is a multiple of 8, PER at most 4)
+  for (int i0 = 0; i0 < count; i0 += 64) {
+    const int here = min(count - i0, 64);
+    if (lane < here && wave == 0) {
+      const float *st = stats + slot(i0 + lane) * RM * 2;
+      weights[lane] = __builtin_amdgcn_exp2f(st[0] - m);
+      l += weights[lane] * st[1];
+      unused |= st[1] < 0.0f;
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int i = wave; i < here; i += kWaves) {
+      const float *part = w.part + (slot(i0 + i) * RM + r) * DT + (in ? lane * PER : 0);
+      const float a = weights[i];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] += lane * PER + e < p.dim ? a * part[e] : 0.0f;
+      for (int e = 0; e < PER; ++e) o[e] = fmaf(a, part[e], o[e]);
+    }
+    __syncthreads();
   }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) sums[wave][lane * PER + e] = o[e];
+  __syncthreads();
+  if (wave) return;
+  l = wave_sum(l);
+  unused = __any(unused);
   const float norm = 1.0f / l;
+  const int64_t at = s * p.o_s + n * p.o_n + head * p.o_h;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int d = lane * PER + e;
     if (d >= p.dim) continue;
-    const float y = unused ? 0.0f : o[e] * norm;
-    const int64_t at = s * p.o_s + n * p.o_n + head * p.o_h + d;
-    if (p.act_type == KH_TYPE_F32) static_cast<float *>(p.out)[at] = y;
-    else if (p.act_type == KH_TYPE_BF16) static_cast<__bf16 *>(p.out)[at] = (__bf16)y;
-    else static_cast<_Float16 *>(p.out)[at] = (_Float16)y;
+    float y = 0.0f;
+    for (int i = 0; i < kWaves; ++i) y += sums[i][d];
+    y = unused ? 0.0f : y * norm;
+    if (p.act_type == KH_TYPE_F32) static_cast<float *>(p.out)[at + d] = y;
+    else if (p.act_type == KH_TYPE_BF16) static_cast<__bf16 *>(p.out)[at + d] = (__bf16)y;
+    else static_cast<_Float16 *>(p.out)[at + d] = (_Float16)y;
   }
 }
 
@@ -833,8 +891,8 @@ template <int CT, int NP, int DT, int RT>
 void launch_both(const PagedWork &w, hipStream_t stream) {
   if (w.p.dim == DT) paged_attn_kernel<CT, NP, DT, RT, true><<<w.grid, kThreads, 0, stream>>>(w);
   else paged_attn_kernel<CT, NP, DT, RT, false><<<w.grid, kThreads, 0, stream>>>(w);
-  if (w.grid > 1) {
-    const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)((std::min(w.rows, 16 * RT) + kWaves - 1) / kWaves));
+  if (!w.whole) {
+    const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)std::min(w.rows, 16 * RT));
     paged_join_kernel<DT, RT><<<grid, kThreads, 0, stream>>>(w);
   }
 }
