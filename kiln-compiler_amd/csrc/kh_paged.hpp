@@ -31,6 +31,7 @@ struct PagedWork {
   int rows;        // query rows of an item's sequence part: draft * group, or group with picked pages
   int blocks;      // row blocks of `rows`
   int items;       // items of a sequence: kv_heads * blocks (* draft with picked pages)
+  int per_head;    // items of a kv head
   int half_shift;  // page_size = 16 << half_shift
   int draft_tiles;
   int sel_tiles;   // tiles of the picked pages, 0 without

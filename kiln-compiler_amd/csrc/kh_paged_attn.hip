@@ -8,7 +8,7 @@ namespace kh {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWholeTiles = 16;
+constexpr int kWholeTiles = 40;
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -34,7 +34,8 @@ PagedWork work_of(const kh_paged &p) {
   const int rm = 16 * row_blocks(p);
   w.rows = (p.top ? 1 : p.draft) * w.group;
   w.blocks = (w.rows + rm - 1) / rm;
-  w.items = p.kv_heads * w.blocks * (p.top ? p.draft : 1);
+  w.per_head = w.blocks * (p.top ? p.draft : 1);
+  w.items = p.kv_heads * w.per_head;
   w.half_shift = 0;
   while ((16 << w.half_shift) < p.page_size) ++w.half_shift;
   w.draft_tiles = (p.draft + kPagedTile - 1) / kPagedTile;
@@ -47,7 +48,7 @@ PagedWork work_of(const kh_paged &p) {
   // workgroups: one per item where none can have many tiles; else what the
   // chip holds at once, or a tile per wave of the most tiles the table has room for
   w.whole = per_item <= kWholeTiles;
-  const int cap = current_device().cus * (rm == 16 && padded_dim(p.dim) <= 128 ? 2 : 1);
+  const int cap = current_device().cus * (rm * padded_dim(p.dim) <= 16 * 128 ? 2 : 1);
   w.grid = (int)(w.whole ? items : std::min<int64_t>((per_item * items + kPagedWaves - 1) / kPagedWaves, cap));
   w.part = nullptr;
   return w;

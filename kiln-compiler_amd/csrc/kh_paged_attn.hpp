@@ -53,9 +53,8 @@ constexpr float kWeightExp = 14.0f;   // fp16 weights are 2^14 softmax weights
 // ---------------------------------------------------------------------------
 // The tiles of all items in a row.
 
-struct Plan {
-  int64_t total;   // tiles of the batch
-  int64_t count;   // workgroups that take part
+struct Plan {   // ranges: the first `extra` of `each` + 1 tiles, the others of `each`
+  int count, each, extra;
 };
 
 // int32 operands through the constant address space: a wave-uniform index
@@ -63,18 +62,21 @@ struct Plan {
 typedef const __attribute__((address_space(4))) int32_t *const_ints;
 __device__ __forceinline__ const_ints ints_of(const int32_t *p) { return (const_ints)(uintptr_t)p; }
 
-__device__ __forceinline__ int clamp_len(const PagedWork &w, int s) {
+template <class W>
+__device__ __forceinline__ int clamp_len(W &w, int s) {
   const int n = ints_of(w.p.lengths)[s];
   const int64_t most = (int64_t)w.p.width * w.p.page_size;
   return n < 0 ? 0 : (n > most ? (int)most : n);
 }
 
-__device__ __forceinline__ int tiles_of(const PagedWork &w, int len) {
+template <class W>
+__device__ __forceinline__ int tiles_of(W &w, int len) {
   return (w.sel_tiles ? w.sel_tiles : (len + kTile - 1) / kTile) + w.draft_tiles;
 }
 
 // first[s] = tiles of one item of the sequences before s, for s <= batch.
-__device__ __forceinline__ void scan_tiles(const PagedWork &w, int *first, int *wave_sums) {
+template <class W>
+__device__ __forceinline__ void scan_tiles(W &w, int *first, int *wave_sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = w.p.batch;
   const int per = (n + kThreads - 1) / kThreads;
@@ -99,31 +101,36 @@ __device__ __forceinline__ void scan_tiles(const PagedWork &w, int *first, int *
   __syncthreads();
 }
 
-__device__ __forceinline__ Plan plan_of(const PagedWork &w, const int *first) {
+template <class W>
+__device__ __forceinline__ Plan plan_of(W &w, const int *first) {
   Plan r;
-  r.total = (int64_t)first[w.p.batch] * w.items;
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readfirstlane(first[w.p.batch]) * (uint32_t)w.items;
   // a tile per wave at least
-  const int64_t want = (r.total + kWaves - 1) / kWaves;
-  r.count = want < w.grid ? (want < 1 ? 1 : want) : w.grid;
+  const uint32_t want = (total + kWaves - 1) / kWaves;
+  r.count = (int)min(want, (uint32_t)w.grid);
+  r.each = (int)(total / (uint32_t)r.count);
+  r.extra = (int)(total - (uint32_t)r.each * r.count);
   return r;
 }
 
-__device__ __forceinline__ int64_t range_start(const Plan &r, int64_t w) { return r.total * w / r.count; }
+__device__ __forceinline__ int range_start(const Plan &r, int w) { return r.each * w + min(w, r.extra); }
 
-// The workgroup whose range holds tile x.
-__device__ __forceinline__ int64_t range_of(const Plan &r, int64_t x) {
-  return ((x + 1) * r.count + r.total - 1) / r.total - 1;
+// The range that holds tile x.
+__device__ __forceinline__ int range_of(const Plan &r, int x) {
+  const int longer = r.extra * (r.each + 1);
+  return x < longer ? (int)((uint32_t)x / (uint32_t)(r.each + 1)) : r.extra + (int)((uint32_t)(x - longer) / (uint32_t)r.each);
 }
 
 // Which sequence tile x of the row lies in (first[] counts one item's tiles).
-__device__ __forceinline__ int sequence_of(const PagedWork &w, const int *first, int64_t x) {
+template <class W>
+__device__ __forceinline__ int sequence_of(W &w, const int *first, int x) {
   int lo = 0, hi = w.p.batch - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if ((int64_t)first[mid] * w.items <= x) lo = mid;
+    if (first[mid] * w.items <= x) lo = mid;
     else hi = mid - 1;
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // ---------------------------------------------------------------------------
@@ -136,7 +143,8 @@ struct Paths {
   int16_t next[kMaxDraft];   // the next ancestor beyond those held; -1 none, -2 the token is unused
 };
 
-__device__ void build_paths(const PagedWork &w, int s, Paths &t) {
+template <class W>
+__device__ __forceinline__ void build_paths(W &w, int s, Paths &t) {
   const int i = threadIdx.x, n = w.p.draft;
   const int32_t *parents = w.p.parents + s * w.p.parents_s;
   if (i < n) {
@@ -287,9 +295,18 @@ struct Source {
   int draft;           // index among the new tokens' tiles, -1 for a cached one
 };
 
-// FULL: dim == DT, every lane's pieces lie inside a row.
-template <int CT, int NP, int DT, int RT, bool FULL>
-__global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void paged_attn_kernel(const PagedWork w) {
+// The kernel's arguments are read where they are used, through a pointer that
+// fresh() makes opaque: hoisted to the start they would fill the scalar
+// registers and spill.
+typedef const __attribute__((address_space(4))) PagedWork const_work;
+__device__ __forceinline__ const_work &fresh() {
+  uint64_t args = (uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  return *(const_work *)(uintptr_t)args;
+}
+
+template <int CT, int NP, int DT, int RT>
+__global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_kernel(const PagedWork) {
   typedef typename Cache<CT>::T T;
   typedef Tile<CT, DT> Regs;
   constexpr bool F32 = CT == KH_TYPE_F32;
@@ -305,19 +322,18 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
   __shared__ f32x4 o_share[2][RT][NT][64];
   __shared__ float ml_share[2][2][RM];
 
-  const kh_paged &p = w.p;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool act32 = p.act_type == KH_TYPE_F32;
 
-  int me = blockIdx.x;
-  int64_t at = 0, end = 1;
-  if (!w.whole) {
+  int me = blockIdx.x, at = 0, end = 1;
+  const bool whole = fresh().whole;
+  if (!whole) {
+    const_work &w = fresh();
     scan_tiles(w, first, wave_sums);
     const Plan plan = plan_of(w, first);
     if (me >= plan.count) return;
     // neighbouring ranges on the same XCD: they share row blocks' keys
-    const int xcd = me & 7, per = (int)plan.count >> 3, rest = (int)plan.count & 7;
+    const int xcd = me & 7, per = plan.count >> 3, rest = plan.count & 7;
     me = xcd * per + min(xcd, rest) + (me >> 3);
     at = range_start(plan, me);
     end = range_start(plan, me + 1);
@@ -325,9 +341,10 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
 
   int paths_of = -1;   // sequence whose paths the LDS holds
   while (at < end) {
+    const_work &w = fresh();
     int s, item, t0, t1, tiles, len;
-    if (w.whole) {
-      s = me / w.items;
+    if (whole) {
+      s = (int)((uint32_t)me / (uint32_t)w.items);
       item = me - s * w.items;
       len = clamp_len(w, s);
       tiles = tiles_of(w, len);
@@ -335,73 +352,81 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
       t1 = tiles;
       at = end;
     } else {
-      s = __builtin_amdgcn_readfirstlane(sequence_of(w, first, at));
+      s = sequence_of(w, first, at);
       len = clamp_len(w, s);
       tiles = tiles_of(w, len);
-      const int64_t in_seq = at - (int64_t)__builtin_amdgcn_readfirstlane(first[s]) * w.items;
-      item = (int)(in_seq / tiles);
-      t0 = (int)(in_seq - (int64_t)item * tiles);
-      t1 = (int)min((int64_t)tiles, t0 + (end - at));
+      const int in_seq = at - __builtin_amdgcn_readfirstlane(first[s]) * w.items;
+      item = (int)((uint32_t)in_seq / (uint32_t)tiles);
+      t0 = in_seq - item * tiles;
+      t1 = min(tiles, t0 + (end - at));
       at += t1 - t0;
     }
     const int cached = tiles - w.draft_tiles;
     // item = (kv head, [token,] row block)
-    const int per_head = w.items / p.kv_heads;
-    const int c = item / per_head;
-    const int b = item - c * per_head;
-    const int token = w.sel_tiles ? b / w.blocks : 0;
-    const int row0 = (w.sel_tiles ? b - token * w.blocks : b) * RM;
+    const int c = (int)((uint32_t)item / (uint32_t)w.per_head);
+    const int b = item - c * w.per_head;
+    const bool sel = w.sel_tiles;
+    const int token = sel ? (int)((uint32_t)b / (uint32_t)w.blocks) : 0;
+    const int row0 = (sel ? b - token * w.blocks : b) * RM;
+    const bool act32 = w.p.act_type == KH_TYPE_F32;
 
     const bool has_draft = t1 > cached;
-    if (has_draft && p.parents && paths_of != s) {
+    const bool tree = w.p.parents != nullptr;
+    if (has_draft && tree && paths_of != s) {
       __syncthreads();   // the last item's rows have read the table
       build_paths(w, s, paths);
       paths_of = s;
     }
 
     // -- where tile t lies; the first tile at or after t with a key, in steps of the waves
-    const T *kp = static_cast<const T *>(p.k_pages) + c * p.kp_h, *vp = static_cast<const T *>(p.v_pages) + c * p.vp_h;
+    const_work &wt = fresh();
+    const T *kp = static_cast<const T *>(wt.p.k_pages) + c * wt.p.kp_h, *vp = static_cast<const T *>(wt.p.v_pages) + c * wt.p.vp_h;
+    const int64_t kp_p = wt.p.kp_p, vp_p = wt.p.vp_p;
+    const int kp_t = (int)wt.p.kp_t, vp_t = (int)wt.p.vp_t, half_shift = wt.half_shift, pages = wt.p.pages;
+    const const_ints row_of_table = ints_of(wt.p.table) + s * wt.p.table_s;
     auto find = [&](int &t, Source<T> &r) {
       for (; t < t1; t += kWaves) {
         if (t >= cached) {
+          const_work &w = fresh();
           r.draft = t - cached;
           const int n0 = kTile * r.draft;
-          r.k_row = (int)p.k_n;
-          r.v_row = (int)p.v_n;
+          r.k_row = (int)w.p.k_n;
+          r.v_row = (int)w.p.v_n;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            r.valid[h] = min(max(p.draft - (n0 + 16 * h), 0), 16);
+            r.valid[h] = min(max(w.p.draft - (n0 + 16 * h), 0), 16);
             const int n = r.valid[h] ? n0 + 16 * h : 0;
-            r.k[h] = static_cast<const T *>(p.k) + (s * p.k_s + c * p.k_h + n * p.k_n);
-            r.v[h] = static_cast<const T *>(p.v) + (s * p.v_s + c * p.v_h + n * p.v_n);
+            r.k[h] = static_cast<const T *>(w.p.k) + (s * w.p.k_s + c * w.p.k_h + n * w.p.k_n);
+            r.v[h] = static_cast<const T *>(w.p.v) + (s * w.p.v_s + c * w.p.v_h + n * w.p.v_n);
           }
           return;
         }
         r.draft = -1;
-        r.k_row = (int)p.kp_t;
-        r.v_row = (int)p.vp_t;
+        r.k_row = kp_t;
+        r.v_row = vp_t;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int j = 2 * t + h;
-          int col = j >> w.half_shift, pos = 16 * j;
-          const int slot = (j & ((1 << w.half_shift) - 1)) * 16;
+          int col = j >> half_shift, pos = 16 * j;
+          const int slot = (j & ((1 << half_shift) - 1)) * 16;
           bool in = true;
-          if (w.sel_tiles) {
+          if (sel) {
+            const_work &w = fresh();
             const int rank = col;
-            in = rank < p.top;
-            const const_ints list = ints_of(p.selected) + (s * p.sel_s + token * p.sel_n + c * p.sel_h);
+            in = rank < w.p.top;
+            const const_ints list = ints_of(w.p.selected) + (s * w.p.sel_s + token * w.p.sel_n + c * w.p.sel_h);
             const int before = in && rank > 0 ? list[rank - 1] : -1;
             col = in ? list[rank] : 0;
-            in = in && col > before && col >= 0 && col < p.width;
-            pos = in ? col * p.page_size + slot : len;
+            in = in && col > before && col >= 0 && col < w.p.width;
+            pos = in ? col * w.p.page_size + slot : len;
           }
           in = in && pos < len;
-          const int page = in ? ints_of(p.table)[s * p.table_s + col] : 0;
-          in = in && page >= 0 && page < p.pages;
+          const int page = in ? row_of_table[col] : 0;
+          in = in && page >= 0 && page < pages;
           r.valid[h] = in ? min(len - pos, 16) : 0;
           const int there = in ? page : 0;
-          r.k[h] = kp + (there * p.kp_p + (int64_t)(slot * r.k_row));
-          r.v[h] = vp + (there * p.vp_p + (int64_t)(slot * r.v_row));
+          r.k[h] = kp + (there * kp_p + (int64_t)(slot * kp_t));
+          r.v[h] = vp + (there * vp_p + (int64_t)(slot * vp_t));
         }
         if (r.valid[0] | r.valid[1]) return;
       }
@@ -409,18 +434,20 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
 
     // a new tile of fp32 activations over a 16-bit cache is rounded as it is loaded
     auto rounds = [&](const Source<T> &r) { return !F32 && act32 && r.draft >= 0; };
+    const int dim = wt.p.dim;
     auto load_k = [&](const Source<T> &r, Regs &x) {
+      const void *base = rounds(r) ? fresh().p.k : nullptr;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = min(li, max(r.valid[h], 1) - 1) * r.k_row;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const int d = 32 * ks + 8 * g, in = FULL || d < p.dim ? d : 0;
+          const int d = 32 * ks + 8 * g, in = d < dim ? d : 0;
           if (!rounds(r)) {
             load_words(r.k[h] + (uint32_t)(row + in), x.k[h][ks]);
           } else if constexpr (!F32) {
             // (r.k counts elements of T, the activations are fp32: twice its size)
-            const float *y = static_cast<const float *>(p.k) + (r.k[h] - static_cast<const T *>(p.k)) + (row + in);
+            const float *y = static_cast<const float *>(base) + (r.k[h] - static_cast<const T *>(base)) + (row + in);
             const f32x4 lo = *reinterpret_cast<const f32x4 *>(y), hi = *reinterpret_cast<const f32x4 *>(y + 4);
             x.k[h][ks][0] = pack2<T>(lo[0], lo[1]);
             x.k[h][ks][1] = pack2<T>(lo[2], lo[3]);
@@ -431,6 +458,7 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
       }
     };
     auto load_v = [&](const Source<T> &r, Regs &x) {
+      const void *base = rounds(r) ? fresh().p.v : nullptr;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -438,11 +466,11 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
           const int row = min(4 * g + i, max(r.valid[h], 1) - 1) * r.v_row;
 #pragma unroll
           for (int vc = 0; vc < VC; ++vc) {
-            const int d = 16 * VD * vc + VD * li, in = FULL || d < p.dim ? d : 0;
+            const int d = 16 * VD * vc + VD * li, in = d < dim ? d : 0;
             if (!rounds(r)) {
               load_words(r.v[h] + (uint32_t)(row + in), x.v[4 * h + i][vc]);
             } else if constexpr (!F32) {
-              const float *y = static_cast<const float *>(p.v) + (r.v[h] - static_cast<const T *>(p.v)) + (row + in);
+              const float *y = static_cast<const float *>(base) + (r.v[h] - static_cast<const T *>(base)) + (row + in);
 #pragma unroll
               for (int e = 0; e < VD; e += 4) {
                 const f32x4 z = *reinterpret_cast<const f32x4 *>(y + e);
@@ -465,15 +493,16 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
     }
 
     // this lane's query rows
+    const_work &wq = fresh();
     int row_token[RT], row_head[RT];
     bool row_ok[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = row0 + rt * 16 + li;
-      row_ok[rt] = r < w.rows;
+      row_ok[rt] = r < wq.rows;
       const int rr = row_ok[rt] ? r : 0;
-      row_token[rt] = w.sel_tiles ? token : rr / w.group;
-      row_head[rt] = c * w.group + (w.sel_tiles ? rr : rr - row_token[rt] * w.group);
+      row_token[rt] = sel ? token : (int)((uint32_t)rr / (uint32_t)wq.group);
+      row_head[rt] = c * wq.group + (sel ? rr : rr - row_token[rt] * wq.group);
     }
     u32x4 q16[F32 ? 1 : NP][RT][KS];
     float q32[F32 ? RT : 1][F32 ? KS : 1][8];
@@ -481,17 +510,17 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float y[KS][8];
-      const int64_t base = s * p.q_s + row_token[rt] * p.q_n + row_head[rt] * p.q_h;
+      const int64_t base = s * wq.p.q_s + row_token[rt] * wq.p.q_n + row_head[rt] * wq.p.q_h;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d = 32 * ks + 8 * g;
-        const bool in = row_ok[rt] && (FULL || d < p.dim);
-        load_acts<T>(p.q, base + (in ? d : 0), act32, y[ks]);
+        const bool in = row_ok[rt] && (d < dim);
+        load_acts<T>(wq.p.q, base + (in ? d : 0), act32, y[ks]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[ks][j] = in ? y[ks][j] : 0.0f;
       }
-      float up = w.scale2 < 0.0f ? -1.0f : 1.0f;
-      mult[rt] = fabsf(w.scale2);
+      float up = wq.scale2 < 0.0f ? -1.0f : 1.0f;
+      mult[rt] = fabsf(wq.scale2);
       if constexpr (SCALED_Q) {
         float most = 0.0f;
 #pragma unroll
@@ -538,10 +567,10 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
       Source<T> next;
       find(t_next, next);
 
-      if constexpr (!FULL) {   // beyond dim: whatever was read meets q = 0, which needs it finite
+      if (dim < DT) {   // beyond dim: whatever was read meets q = 0, which needs it finite
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          if (32 * ks + 8 * g >= p.dim) {
+          if (32 * ks + 8 * g >= dim) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -583,7 +612,7 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
           see[rt] = there;
           if (here.draft >= 0) {
             const int i = row_token[rt] - kTile * here.draft;   // chain: the tokens up to its own
-            see[rt] &= p.parents ? paths.bits[row_token[rt]][here.draft] : (i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1);
+            see[rt] &= tree ? paths.bits[row_token[rt]][here.draft] : (i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -684,11 +713,12 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
       if (t_next < t1) load_v(next, x);
 
       if (__builtin_expect(__any(odd != 0), 0)) {
+        const_work &w = fresh();
         for (int key = 0; key < kTile; ++key) {   // the values taken out, by hand
           const int j = 4 * (key >> 4) + (key & 3), from = (key & 15) >> 2;
           if (!__any(g == from && (odd >> j & 1))) continue;
-          const int n = min(kTile * here.draft + key, p.draft - 1);
-          const int64_t row = s * p.v_s + c * p.v_h + n * p.v_n;
+          const int n = min(kTile * here.draft + key, w.p.draft - 1);
+          const int64_t row = s * w.p.v_s + c * w.p.v_h + n * w.p.v_n;
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
             float mine = 0.0f;
@@ -702,7 +732,7 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
               for (int r = 0; r < 4; ++r) {
                 const int d = 16 * VD * vc + VD * (4 * g + r);
                 float y[VD];
-                load_acts<T>(p.v, row + (FULL || d < p.dim ? d : 0), act32, y);
+                load_acts<T>(w.p.v, row + (d < dim ? d : 0), act32, y);
 #pragma unroll
                 for (int i = 0; i < VD; ++i) {
                   const float z = (float)(T)y[i];
@@ -721,7 +751,7 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
     for (int rt = 0; rt < RT; ++rt) {
       l[rt] = sum16x32(l[rt]);
       // an unused token's rows: marked by l = -1 in the part that holds its tile
-      if (has_draft && p.parents && wave == 0 && paths.next[row_token[rt]] == -2) l[rt] = -1.0f;
+      if (has_draft && tree && wave == 0 && paths.next[row_token[rt]] == -2) l[rt] = -1.0f;
     }
     auto put = [&](int to) {
 #pragma unroll
@@ -762,6 +792,7 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
       if (wave == 0) join(0);
     }
     if (wave == 0) {
+      const_work &w = fresh();
       const bool done = t0 == 0 && t1 == tiles;
       // (t0 > 0: this range's first part; else its last)
       const int64_t slot = 2 * (int64_t)me + (t0 > 0 ? 0 : 1);
@@ -775,13 +806,13 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
           stats[2 * (rt * 16 + li) + 1] = l[rt];
         }
         const float norm = 1.0f / l[rt];
-        const int64_t out = s * p.o_s + row_token[rt] * p.o_n + row_head[rt] * p.o_h;
+        const int64_t out = s * w.p.o_s + row_token[rt] * w.p.o_n + row_head[rt] * w.p.o_h;
 #pragma unroll
         for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int d = 16 * VD * vc + VD * (4 * g + r);
-            if (!FULL && d >= p.dim) continue;
+            if (d >= dim) continue;
             float y[VD];
 #pragma unroll
             for (int i = 0; i < VD; ++i) y[i] = o[rt][vc][i][r];
@@ -789,7 +820,7 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
             if (done) {
 #pragma unroll
               for (int i = 0; i < VD; ++i) y[i] = l[rt] < 0.0f ? 0.0f : y[i] * norm;
-              to = static_cast<float *>(p.out) + out + d;
+              to = static_cast<float *>(w.p.out) + out + d;
             }
             if (F32 || act32 || !done) {
 #pragma unroll
@@ -797,7 +828,7 @@ __global__ __launch_bounds__(kThreads, (RT == 1 && DT <= 128) ? 2 : 1) void page
             } else if constexpr (!F32) {
 #pragma unroll
               for (int i = 0; i < VD; i += 4)
-                *reinterpret_cast<u32x2 *>(static_cast<T *>(p.out) + out + d + i) = u32x2{pack2<T>(y[i], y[i + 1]), pack2<T>(y[i + 2], y[i + 3])};
+                *reinterpret_cast<u32x2 *>(static_cast<T *>(w.p.out) + out + d + i) = u32x2{pack2<T>(y[i], y[i + 1]), pack2<T>(y[i + 2], y[i + 3])};
             }
           }
       }
@@ -824,11 +855,10 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
   const Plan plan = plan_of(w, first);
   const int s = blockIdx.x / w.items, item = blockIdx.x - s * w.items;
   const int tiles = tiles_of(w, clamp_len(w, s));
-  const int64_t x = (int64_t)first[s] * w.items + (int64_t)item * tiles;
-  const int64_t w0 = range_of(plan, x), w1 = range_of(plan, x + tiles - 1);
+  const int x = first[s] * w.items + item * tiles;
+  const int w0 = range_of(plan, x), w1 = range_of(plan, x + tiles - 1);
   if (w0 == w1) return;   // finished by its one range
-  const int per_head = w.items / p.kv_heads;
-  const int c = item / per_head, b = item - c * per_head;
+  const int c = item / w.per_head, b = item - c * w.per_head;
   const int token = w.sel_tiles ? b / w.blocks : 0;
   const int row0 = (w.sel_tiles ? b - token * w.blocks : b) * RM;
   const int r = blockIdx.y;
@@ -837,8 +867,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
   const int head = c * w.group + (w.sel_tiles ? row0 + r : row0 + r - n * w.group);
   const float *stats = w.part + 2 * (int64_t)w.grid * RM * DT + 2 * r;
   // part i of the item: the last part of range w0, then the first of the others
-  auto slot = [&](int i) { return 2 * (w0 + i) + (i == 0 ? 1 : 0); };
-  const int count = (int)(w1 - w0 + 1);
+  auto slot = [&](int i) { return 2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0); };
+  const int count = w1 - w0 + 1;
   float m = -INFINITY;
   for (int i = lane; i < count; i += 64) m = fmaxf(m, stats[slot(i) * RM * 2]);
   m = wave_max(m);
@@ -889,8 +919,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
 
 template <int CT, int NP, int DT, int RT>
 void launch_both(const PagedWork &w, hipStream_t stream) {
-  if (w.p.dim == DT) paged_attn_kernel<CT, NP, DT, RT, true><<<w.grid, kThreads, 0, stream>>>(w);
-  else paged_attn_kernel<CT, NP, DT, RT, false><<<w.grid, kThreads, 0, stream>>>(w);
+  paged_attn_kernel<CT, NP, DT, RT><<<w.grid, kThreads, 0, stream>>>(w);
   if (!w.whole) {
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)std::min(w.rows, 16 * RT));
     paged_join_kernel<DT, RT><<<grid, kThreads, 0, stream>>>(w);
