@@ -94,6 +94,12 @@ def _rows(t):
     return t
 
 
+def _rows_strided(t):
+    """As _rows, by the strides alone."""
+    size = t.element_size()
+    return _rows(t) if t.stride(-1) != 1 or any(s * size % 16 for s in t.stride()[:-1]) else t
+
+
 def check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected):
     """(sizes of the call) after checking types, shapes and their agreement."""
     check_pages(k_pages, v_pages)
@@ -171,73 +177,145 @@ def _ready(device):
             init_device(device)
 
 
-def _run(op: kl.Paged, device, what: str):
+def _form(*tensors):
+    """What the checks and an operator's sizes and strides depend on, of each tensor."""
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+
+
+# form of a call -> (its descriptor without addresses, workspace bytes): the
+# checks and the descriptor are worked out once per form. Forms are shapes,
+# strides and types alone; a program has few, and the oldest go first.
+_forms = {}
+MOST_FORMS = 4096
+
+
+def _remember(key, op):
+    size = ctypes.c_size_t()
+    kl.check(kl.load().kh_paged_workspace_bytes(ctypes.byref(op), ctypes.byref(size)), "paged")
+    if len(_forms) >= MOST_FORMS:
+        _forms.pop(next(iter(_forms)))
+    _forms[key] = found = (bytes(op), size.value)
+    return found
+
+
+def _launch(op: kl.Paged, size: int, device, what: str):
     lib = kl.load()
     if device.type != "cuda":
-        kl.check(lib.kh_paged_host(ctypes.byref(op)), what)
-        return
-    _ready(device)
-
-    def go():
-        size = ctypes.c_size_t()
-        kl.check(lib.kh_paged_workspace_bytes(ctypes.byref(op), ctypes.byref(size)), what)
-        n = size.value
-        workspace = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-        rc = lib.kh_paged_run(ctypes.byref(op), workspace.data_ptr() if n else None, n, _stream(device))
-        if rc:
-            kl.check(rc, what)
-
-    _on_device(device, go)
+        rc = lib.kh_paged_host(ctypes.byref(op))
+    elif device.index == torch._C._cuda_getDevice():
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+            rc = lib.kh_paged_run(ctypes.byref(op), workspace.data_ptr(), size, _stream(device))
+        else:
+            rc = lib.kh_paged_run(ctypes.byref(op), None, 0, _stream(device))
+    else:   # (a launch goes to the current device)
+        with torch.cuda.device(device):
+            return _launch(op, size, device, what)
+    if rc:
+        kl.check(rc, what)
 
 
-def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what):
+def _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale):
+    """(descriptor without addresses) of a call, checked; operands' rows are in place."""
     batch, draft, heads, kv_heads, dim, page_size, pages = check_attention(
         q, k, v, k_pages, v_pages, table, lengths, parents, selected)
-    _no_grad(q, k, v, k_pages, v_pages)
     _one_device(q, k, v, k_pages, v_pages, table, lengths, parents, selected)
     _rows_in_place(k_pages, "k_pages")
     _rows_in_place(v_pages, "v_pages")
     if pages == 0:
         raise ValueError("the cache has no pages")
-    q, k, v, table, lengths = _rows(q), _rows(k), _rows(v), _columns(table), _columns(lengths)
-    out = torch.empty((batch, draft, heads, dim), dtype=q.dtype, device=q.device)
-    if out.numel() == 0:
-        return out
-    op = kl.Paged(kl.PAGED_ATTENTION, batch, draft, heads, kv_heads, dim, page_size, pages, table.shape[1], 0,
-                  TYPES[k_pages.dtype], TYPES[q.dtype], 0, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  k_pages.data_ptr(), v_pages.data_ptr(), None, table.data_ptr(), lengths.data_ptr(), None, None,
-                  out.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
-                  *k_pages.stride()[:3], *v_pages.stride()[:3], 0, 0, table.stride(0), 0, 0, 0, 0)
+    _ready(q.device)
+    h, d = heads * dim, dim
+    return kl.Paged(kl.PAGED_ATTENTION, batch, draft, heads, kv_heads, dim, page_size, pages, table.shape[1],
+                    0 if selected is None else selected.shape[3], TYPES[k_pages.dtype], TYPES[q.dtype], 0, scale,
+                    None, None, None, None, None, None, None, None, None, None, None,
+                    *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], draft * h, h, d,
+                    *k_pages.stride()[:3], *v_pages.stride()[:3], 0, 0, table.stride(0),
+                    0 if parents is None else parents.stride(0),
+                    *((0, 0, 0) if selected is None else selected.stride()[:3]))
+
+
+def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what):
+    try:
+        key = (_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected), scale)
+    except AttributeError:
+        check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected)   # names what is no tensor
+        raise
+    found = _forms.get(key)
+    if found is None:
+        check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected)
+    if torch.is_grad_enabled():
+        _no_grad(q, k, v, k_pages, v_pages)
+    if found is None:
+        straight = [_rows_strided(t) for t in (q, k, v)] + [_columns(t) for t in (table, lengths)]
+        if any(a is not b for a, b in zip(straight, (q, k, v, table, lengths))):
+            q, k, v, table, lengths = straight
+            return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what)
+        if (parents is not None and _columns(parents) is not parents) or (selected is not None and _columns(selected) is not selected):
+            parents, selected = (None if t is None else _columns(t) for t in (parents, selected))
+            return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what)
+        op = _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale)
+        if q.numel() == 0:
+            return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        found = _remember(key, op)
+    elif q.device.type != "cuda" and not interpreting():
+        _one_device(q)
+    op = kl.Paged.from_buffer_copy(found[0])
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    at = (q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr())
+    if (at[0] | at[1] | at[2] | at[3] | at[4]) & 15:
+        _rows_in_place(k_pages, "k_pages")
+        _rows_in_place(v_pages, "v_pages")
+        return run_attention(_rows(q), _rows(k), _rows(v), k_pages, v_pages, table, lengths, parents, selected, scale, what)
+    op.q, op.k, op.v, op.k_pages, op.v_pages = at
+    op.table, op.lengths, op.out = table.data_ptr(), lengths.data_ptr(), out.data_ptr()
     if parents is not None:
-        parents = _columns(parents)
-        op.parents, op.parents_s = parents.data_ptr(), parents.stride(0)
+        op.parents = parents.data_ptr()
     if selected is not None:
-        selected = _columns(selected)
-        op.selected, op.top = selected.data_ptr(), selected.shape[3]
-        op.sel_s, op.sel_n, op.sel_h = selected.stride()[:3]
-    _run(op, q.device, what)
+        op.selected = selected.data_ptr()
+    _launch(op, found[1], q.device, what)
     return out
 
 
 def run_select(q, k_means, table, lengths, page_size, pages):
-    batch, draft, heads, kv_heads, dim, total = check_select(q, k_means, table, lengths, page_size, pages)
-    _no_grad(q, k_means)
-    _one_device(q, k_means, table, lengths)
-    _rows_in_place(k_means, "k_means")
-    q, table, lengths = _rows(q), _columns(table), _columns(lengths)
-    out = torch.empty((batch, draft, kv_heads, pages), dtype=torch.int32, device=q.device)
-    if out.numel() == 0:
-        return out
-    if total == 0:
-        raise ValueError("the cache has no pages")
-    op = kl.Paged(kl.PAGED_SELECT, batch, draft, heads, kv_heads, dim, page_size, total, table.shape[1], pages,
-                  kl.TYPE_F32, TYPES[q.dtype], 0, 1.0, q.data_ptr(), None, None, None, None, k_means.data_ptr(),
-                  table.data_ptr(), lengths.data_ptr(), None, out.data_ptr(), None)
-    op.q_s, op.q_n, op.q_h = q.stride()[:3]
-    op.m_p, op.m_h = k_means.stride()[:2]
-    op.table_s = table.stride(0)
-    op.sel_s, op.sel_n, op.sel_h = out.stride()[:3]
-    _run(op, q.device, "select_pages")
+    try:
+        key = (_form(q, k_means, table, lengths), page_size, pages)
+    except AttributeError:
+        check_select(q, k_means, table, lengths, page_size, pages)
+        raise
+    found = _forms.get(key)
+    if found is None:
+        batch, draft, heads, kv_heads, dim, total = check_select(q, k_means, table, lengths, page_size, pages)
+    if torch.is_grad_enabled():
+        _no_grad(q, k_means)
+    if found is None:
+        straight = _rows_strided(q), _columns(table), _columns(lengths)
+        if any(a is not b for a, b in zip(straight, (q, table, lengths))):
+            return run_select(straight[0], k_means, straight[1], straight[2], page_size, pages)
+        _one_device(q, k_means, table, lengths)
+        _rows_in_place(k_means, "k_means")
+        if batch * draft == 0:
+            return torch.empty((batch, draft, kv_heads, pages), dtype=torch.int32, device=q.device)
+        if total == 0:
+            raise ValueError("the cache has no pages")
+        _ready(q.device)
+        op = kl.Paged(kl.PAGED_SELECT, batch, draft, heads, kv_heads, dim, page_size, total, table.shape[1], pages,
+                      kl.TYPE_F32, TYPES[q.dtype], 0, 1.0)
+        op.q_s, op.q_n, op.q_h = q.stride()[:3]
+        op.m_p, op.m_h = k_means.stride()[:2]
+        op.table_s = table.stride(0)
+        op.sel_s, op.sel_n, op.sel_h = draft * kv_heads * pages, kv_heads * pages, pages
+        found = _remember(key, op)
+    elif q.device.type != "cuda" and not interpreting():
+        _one_device(q)
+    op = kl.Paged.from_buffer_copy(found[0])
+    out = torch.empty((op.batch, op.draft, op.kv_heads, pages), dtype=torch.int32, device=q.device)
+    op.q, op.k_means = q.data_ptr(), k_means.data_ptr()
+    if (op.q | op.k_means) & 15:
+        _rows_in_place(k_means, "k_means")
+        return run_select(_rows(q), k_means, table, lengths, page_size, pages)
+    op.table, op.lengths, op.selected = table.data_ptr(), lengths.data_ptr(), out.data_ptr()
+    _launch(op, found[1], q.device, "select_pages")
     return out
 
 
@@ -350,8 +428,52 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
     ``lengths`` and ``rows`` hold for each. Tokens whose page the table does
     not name are dropped. No page may belong to two of the sequences."""
     _eager_only("cache_append")
+    try:
+        key = _form(k, v, k_pages, v_pages, table, lengths, rows, k_means)
+    except AttributeError:
+        _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means)
+        raise
+    template = _forms.get(key)
+    if template is None:
+        op = _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means)
+        if isinstance(op, tuple):     # operands moved to where rows are in place
+            return cache_append(*op[:6], rows=op[6], k_means=k_means)
+        if op is None:
+            return
+        template = _forms[key] = bytes(op)
+        while len(_forms) > MOST_FORMS:
+            _forms.pop(next(iter(_forms)))
+    elif k.device.type != "cuda" and not interpreting():
+        _one_device(k)
+    if torch.is_grad_enabled():
+        _no_grad(k, v, k_pages, v_pages, k_means)
+    op = kl.CacheAppend.from_buffer_copy(template)
+    op.k, op.v, op.k_pages, op.v_pages = at = (k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr())
+    if (at[0] | at[1] | at[2] | at[3]) & 15:
+        _rows_in_place(k_pages, "k_pages")
+        _rows_in_place(v_pages, "v_pages")
+        return cache_append(_rows(k), _rows(v), k_pages, v_pages, table, lengths, rows=rows, k_means=k_means)
+    op.table, op.lengths = table.data_ptr(), lengths.data_ptr()
+    if rows is not None:
+        op.rows = rows.data_ptr()
+    if k_means is not None:
+        op.k_means = k_means.data_ptr()
+    lib, device = kl.load(), k.device
+    if device.type != "cuda":
+        rc = lib.kh_cache_append_host(ctypes.byref(op))
+    else:
+        rc = _on_device(device, lambda: lib.kh_cache_append(ctypes.byref(op), _stream(device)))
+    if rc:
+        kl.check(rc, "cache_append")
+
+
+def _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means):
+    """The descriptor of a call without addresses, checked; None for a call
+    that writes nothing; a tuple of operands to call with where some had to be
+    laid out anew."""
     rank = k_pages.dim() if isinstance(k_pages, torch.Tensor) and k_pages.dim() == 5 else 4
     check_pages(k_pages, v_pages, rank)
+    given = (k, v, k_pages, v_pages, table, lengths, rows)
     if rank == 4:
         k, v = (t.unsqueeze(0) if isinstance(t, torch.Tensor) else t for t in (k, v))
         k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
@@ -370,7 +492,6 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
         if not isinstance(rows, torch.Tensor) or rows.dim() != 2:
             raise ValueError("rows must be a tensor [sequences, accepted]")
         _int32(rows, "rows", 2, (batch, rows.shape[1]))
-        rows = _columns(rows)
     if k_means is not None:
         _tensor(k_means, "k_means", 4, (torch.float32,))
         _shape(k_means, "k_means", (layers, pages, kv_heads, dim))
@@ -380,25 +501,19 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
     _one_device(k, v, k_pages, v_pages, table, lengths, rows, k_means)
     _rows_in_place(k_pages, "k_pages")
     _rows_in_place(v_pages, "v_pages")
-    k, v, table, lengths = _rows(k), _rows(v), _columns(table), _columns(lengths)
+    straight = (_rows_strided(given[0]), _rows_strided(given[1]), given[2], given[3], _columns(table), _columns(lengths),
+                None if rows is None else _columns(rows))
+    if any(a is not b for a, b in zip(straight, given)):
+        return straight
     accept = draft if rows is None else rows.shape[1]
     if layers * batch * accept * draft == 0:
-        return
-    op = kl.CacheAppend(layers, batch, draft, accept, kv_heads, dim, page_size, pages, table.shape[1],
-                        TYPES[k_pages.dtype], TYPES[k.dtype], k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
-                        v_pages.data_ptr(), k_means.data_ptr() if k_means is not None else None, table.data_ptr(),
-                        lengths.data_ptr(), rows.data_ptr() if rows is not None else None, *k.stride()[:4],
-                        *v.stride()[:4], *k_pages.stride()[:4], *v_pages.stride()[:4],
-                        *(k_means.stride()[:3] if k_means is not None else (0, 0, 0)), table.stride(0),
-                        rows.stride(0) if rows is not None else 0)
-    lib, device = kl.load(), k.device
-    if device.type != "cuda":
-        kl.check(lib.kh_cache_append_host(ctypes.byref(op)), "cache_append")
-        return
-    _ready(device)
-    rc = _on_device(device, lambda: lib.kh_cache_append(ctypes.byref(op), _stream(device)))
-    if rc:
-        kl.check(rc, "cache_append")
+        return None
+    _ready(k.device)
+    return kl.CacheAppend(layers, batch, draft, accept, kv_heads, dim, page_size, pages, table.shape[1],
+                          TYPES[k_pages.dtype], TYPES[k.dtype], None, None, None, None, None, None, None, None,
+                          *k.stride()[:4], *v.stride()[:4], *k_pages.stride()[:4], *v_pages.stride()[:4],
+                          *(k_means.stride()[:3] if k_means is not None else (0, 0, 0)), table.stride(0),
+                          rows.stride(0) if rows is not None else 0)
 
 
 def _page_list(x, name):
@@ -424,18 +539,18 @@ def copy_pages(pools, source, target):
     for i, t in enumerate(pools):
         if not isinstance(t, torch.Tensor) or t.dim() < 2:
             raise TypeError("a pool is a tensor of pages")
-        stacked = t.dim() == 5
-        layer = t[0] if stacked and t.shape[0] else t
-        if stacked and not t.shape[0]:
-            raise ValueError("a pool has no layers")
-        if not layer.is_contiguous():
-            raise ValueError("a pool's pages must be contiguous within a layer")
-        if pages is not None and pages != layer.shape[0]:
-            raise ValueError(f"pools of {pages} and of {layer.shape[0]} pages")
-        pages = layer.shape[0]
-        size = t.element_size()
-        descs[i] = kl.Pool(t.data_ptr(), t.shape[0] if stacked else 1, t.stride(0) * size if stacked else 0,
-                           layer[0].numel() * size if pages else 0)
+        shape, strides, size = t.shape, t.stride(), t.element_size()
+        first = 1 if len(shape) == 5 else 0     # the dimension of pages
+        inner = 1
+        for n, step in zip(reversed(shape[first:]), reversed(strides[first:])):
+            if n > 1 and step != inner:
+                raise ValueError("a pool's pages must be contiguous within a layer")
+            inner *= n
+        if pages is not None and pages != shape[first]:
+            raise ValueError(f"pools of {pages} and of {shape[first]} pages")
+        pages = shape[first]
+        descs[i] = kl.Pool(t.data_ptr(), shape[0] if first else 1, strides[0] * size if first else 0,
+                           inner // pages * size if pages else 0)
     if not pools or len(source) == 0:
         return
     _no_grad(*pools)
