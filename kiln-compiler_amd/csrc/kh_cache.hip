@@ -68,63 +68,81 @@ __device__ __forceinline__ void store8(void *p, int64_t i, int type, float (&x)[
   }
 }
 
-// accept rows of sequence s that count: those before the first outside [0, draft)
-__device__ __forceinline__ int counted_rows(const kh_cache_append_op &a, int s, int *first_bad) {
+// How many rows of sequence s count: those before the first outside [0, draft).
+__device__ __forceinline__ int counted_rows(const kh_cache_append_op &a, int s) {
   if (!a.rows) return a.accept;
-  if (threadIdx.x == 0) *first_bad = a.accept;
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.accept; i += kThreads) {
-    const int r = a.rows[s * a.rows_s + i];
-    if (r < 0 || r >= a.draft) {
-      atomicMin(first_bad, i);
-      break;
-    }
+  for (int i = 0; i < a.accept; i += 64) {
+    const int lane = threadIdx.x & 63;
+    const int r = i + lane < a.accept ? a.rows[s * a.rows_s + i + lane] : -1;
+    const uint64_t bad = __ballot(r < 0 || r >= a.draft);
+    if (bad) return i + __builtin_ctzll(bad);
   }
-  __syncthreads();
-  return *first_bad;
+  return a.accept;
 }
 
+constexpr int kAhead = 4;   // tokens of a thread whose loads are in flight together: of those that are there
+constexpr int kPair = 2;    // ... and of the new ones, k and v of each
+
+// CT, AT: element types of the cache and of the new tokens.
+template <int CT, int AT>
 __global__ __launch_bounds__(kThreads) void append_kernel(const kh_cache_append_op a) {
-  __shared__ int first_bad;
   __shared__ float sums[kThreads][8 + 1];
   const int s = blockIdx.y / a.kv_heads, c = blockIdx.y - s * a.kv_heads, layer = blockIdx.z;
   const int64_t len = a.lengths[s];
   if (len < 0) return;
-  const int count = counted_rows(a, s, &first_bad);
   const int64_t col = len / a.page_size + blockIdx.x;
-  const int64_t start = col * a.page_size;
-  const int64_t lo = len > start ? len : start;
-  const int64_t hi = min(len + count, start + a.page_size);
-  if (lo >= hi || col >= a.width) return;
+  if (col >= a.width) return;
   const int page = a.table[s * a.table_s + col];
-  if (page < 0 || page >= a.pages) return;
+  const int count = counted_rows(a, s);
+  const int64_t first = col * a.page_size;
+  // the page's slots [lo, hi) are written, those before lo are there
+  const int lo = (int)(len > first ? len - first : 0);
+  const int hi = (int)min(len + count - first, (int64_t)a.page_size);
+  if (lo >= hi || page < 0 || page >= a.pages) return;
 
   const int chunks = a.dim / 8;                 // threads of a token
   const int side = kThreads / chunks;           // tokens at a time
   const int t = threadIdx.x / chunks, d = (threadIdx.x - t * chunks) * 8;
-  const bool works = t < side;
   float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  const int64_t k_at = layer * a.k_l + s * a.k_s + c * a.k_h + d, v_at = layer * a.v_l + s * a.v_s + c * a.v_h + d;
-  const int64_t kp_at = layer * a.kp_l + page * a.kp_p + c * a.kp_h + d;
-  const int64_t vp_at = layer * a.vp_l + page * a.vp_p + c * a.vp_h + d;
-  if (works) {
+  if (t < side) {
+    const int64_t kp_at = layer * a.kp_l + page * a.kp_p + c * a.kp_h + d;
+    const int64_t vp_at = layer * a.vp_l + page * a.vp_p + c * a.vp_h + d;
+    const int64_t k_at = layer * a.k_l + s * a.k_s + c * a.k_h + d, v_at = layer * a.v_l + s * a.v_s + c * a.v_h + d;
+    const int64_t i0 = first - len;              // slot j gets row i0 + j
     if (a.k_means) {
-      for (int64_t pos = start + t; pos < lo; pos += side) {
-        float x[8];
-        load8(a.k_pages, kp_at + (pos - start) * a.kp_t, a.cache_type, x);
+      for (int j = t; j < lo; j += kAhead * side) {
+        float x[kAhead][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += x[e];
+        for (int i = 0; i < kAhead; ++i) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+          if (j + i * side < lo) load8(a.k_pages, kp_at + (j + i * side) * a.kp_t, CT, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[e] += x[i][e];
       }
     }
-    for (int64_t pos = lo + t; pos < hi; pos += side) {
-      const int64_t i = pos - len, r = a.rows ? a.rows[s * a.rows_s + i] : i;
-      float x[8];
-      load8(a.k, k_at + r * a.k_n, a.act_type, x);
-      store8(a.k_pages, kp_at + (pos - start) * a.kp_t, a.cache_type, x);
+    for (int j = lo + t; j < hi; j += kPair * side) {
+      float x[kPair][8], y[kPair][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += x[e];
-      load8(a.v, v_at + r * a.v_n, a.act_type, x);
-      store8(a.v_pages, vp_at + (pos - start) * a.vp_t, a.cache_type, x);
+      for (int i = 0; i < kPair; ++i) {
+        if (j + i * side >= hi) continue;
+        int64_t r = i0 + j + i * side;
+        if (a.rows) r = a.rows[s * a.rows_s + r];
+        load8(a.k, k_at + r * a.k_n, AT, x[i]);
+        load8(a.v, v_at + r * a.v_n, AT, y[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kPair; ++i) {
+        const int slot = j + i * side;
+        if (slot >= hi) continue;
+        store8(a.k_pages, kp_at + slot * a.kp_t, CT, x[i]);
+        store8(a.v_pages, vp_at + slot * a.vp_t, CT, y[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += x[i][e];
+      }
     }
   }
   if (!a.k_means) return;
@@ -134,7 +152,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const kh_cache_append_
   for (int i = threadIdx.x; i < a.dim; i += kThreads) {
     float total = 0.0f;
     for (int j = 0; j < side; ++j) total += sums[j * chunks + i / 8][i & 7];
-    a.k_means[layer * a.m_l + page * a.m_p + c * a.m_h + i] = total / (float)(hi - start);
+    a.k_means[layer * a.m_l + page * a.m_p + c * a.m_h + i] = total / (float)hi;
   }
 }
 
@@ -182,7 +200,18 @@ float host_store(void *p, int64_t i, int type, float x) {
 hipError_t launch_append(const kh_cache_append_op &a, hipStream_t stream) {
   if (!a.layers || !a.batch || !a.accept) return hipSuccess;
   const unsigned pages = (unsigned)((a.accept - 1) / a.page_size + 2);
-  append_kernel<<<dim3(pages, (unsigned)a.batch * a.kv_heads, (unsigned)a.layers), kThreads, 0, stream>>>(a);
+  const dim3 grid(pages, (unsigned)a.batch * a.kv_heads, (unsigned)a.layers);
+  switch (3 * a.cache_type + a.act_type) {
+    case 0: append_kernel<0, 0><<<grid, kThreads, 0, stream>>>(a); break;
+    case 1: append_kernel<0, 1><<<grid, kThreads, 0, stream>>>(a); break;
+    case 2: append_kernel<0, 2><<<grid, kThreads, 0, stream>>>(a); break;
+    case 3: append_kernel<1, 0><<<grid, kThreads, 0, stream>>>(a); break;
+    case 4: append_kernel<1, 1><<<grid, kThreads, 0, stream>>>(a); break;
+    case 5: append_kernel<1, 2><<<grid, kThreads, 0, stream>>>(a); break;
+    case 6: append_kernel<2, 0><<<grid, kThreads, 0, stream>>>(a); break;
+    case 7: append_kernel<2, 1><<<grid, kThreads, 0, stream>>>(a); break;
+    default: append_kernel<2, 2><<<grid, kThreads, 0, stream>>>(a);
+  }
   return hipGetLastError();
 }
 
