@@ -77,6 +77,10 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = "more keys or query rows than 32-bit counts hold";
     return false;
   }
+  if (p.pages >= 1 << 27) {
+    err = "a pool of 2^27 pages or more";
+    return false;
+  }
   // (every query row of a token in a block of its own at the worst)
   const int64_t tiles = (std::max(keys, p.top ? (int64_t)p.top * p.page_size : 0) / 32 + 10) * std::max(p.batch, 1);
   if (p.variant == KH_PAGED_ATTENTION && tiles * p.kv_heads > most / (((int64_t)p.draft * (p.heads / p.kv_heads) + 15) / 16 + p.draft)) {

@@ -33,6 +33,7 @@ struct PagedWork {
   int items;       // items of a sequence: kv_heads * blocks (* draft with picked pages)
   int per_head;    // items of a kv head
   int half_shift;  // page_size = 16 << half_shift
+  int tile;        // keys of a tile
   int draft_tiles;
   int sel_tiles;   // tiles of the picked pages, 0 without
   int whole;       // a workgroup per item, no second kernel
@@ -48,6 +49,9 @@ hipError_t launch_paged_bf16(const PagedWork &w, int passes, int dt, int rt, hip
 hipError_t launch_paged_f16(const PagedWork &w, int passes, int dt, int rt, hipStream_t stream);
 
 constexpr int kPagedTile = 32;     // keys of a tile
+constexpr int kWideTile = 64;      // ... of paged_wide_kernel
+constexpr int kWideBlocks = 8;     // its rows, in 16s
+constexpr int kMaxWideBatch = 1024;
 constexpr int kPagedWaves = 4;     // waves of a workgroup
 constexpr int kMaxDraft = 256;     // new tokens of a sequence: a workgroup's table of paths fits the LDS
 constexpr int kMaxBatch = 4096;    // sequences of a call: each workgroup scans their lengths

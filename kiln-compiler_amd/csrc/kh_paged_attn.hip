@@ -8,7 +8,7 @@ namespace kh {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWholeTiles = 40;
+constexpr int kWholeKeys = 1280, kWholeWideKeys = 1024;
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -17,14 +17,16 @@ int passes_of(const kh_paged &p) {
   return p.cache_type == KH_TYPE_BF16 ? 3 : 2;
 }
 
-// 16-row blocks of an item: as many as there are rows for, up to what the
-// registers of a lane hold beside a tile (q's parts, O and the tile of a
-// 256-wide head fill them with one).
+// 16-row blocks of an item: one or two by its rows, what the registers of a
+// lane hold beside a tile (a 256-wide head's fill them with one). Many rows over
+// a 16-bit cache take paged_wide_kernel.
+constexpr int kWideRows = 48;
+
 int row_blocks(const kh_paged &p) {
   const int rows = (p.top ? 1 : p.draft) * (p.heads / p.kv_heads);
   const int dt = padded_dim(p.dim);
-  const int most = dt == 256 ? 1 : (p.cache_type == KH_TYPE_F32 || passes_of(p) > 1) ? 2 : 4;
-  return rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+  if (p.cache_type != KH_TYPE_F32 && dt < 256 && rows >= kWideRows && p.batch <= kMaxWideBatch) return kWideBlocks;
+  return rows <= 16 || dt == 256 ? 1 : 2;
 }
 
 PagedWork work_of(const kh_paged &p) {
@@ -38,17 +40,19 @@ PagedWork work_of(const kh_paged &p) {
   w.items = p.kv_heads * w.per_head;
   w.half_shift = 0;
   while ((16 << w.half_shift) < p.page_size) ++w.half_shift;
-  w.draft_tiles = (p.draft + kPagedTile - 1) / kPagedTile;
-  w.sel_tiles = (int)(((int64_t)p.top * p.page_size + kPagedTile - 1) / kPagedTile);
+  w.tile = rm == 16 * kWideBlocks ? kWideTile : kPagedTile;
+  w.draft_tiles = (p.draft + w.tile - 1) / w.tile;
+  w.sel_tiles = (int)(((int64_t)p.top * p.page_size + w.tile - 1) / w.tile);
   w.rounds = 0;
   while ((1 << w.rounds) < p.draft) ++w.rounds;
   w.scale2 = p.scale * kLog2e;
-  const int64_t per_item = (w.sel_tiles ? w.sel_tiles : ((int64_t)p.width * p.page_size + kPagedTile - 1) / kPagedTile) + w.draft_tiles;
+  const int64_t per_item = (w.sel_tiles ? w.sel_tiles : ((int64_t)p.width * p.page_size + w.tile - 1) / w.tile) + w.draft_tiles;
   const int64_t items = (int64_t)w.items * p.batch;
   // workgroups: one per item where none can have many tiles; else what the
   // chip holds at once, or a tile per wave of the most tiles the table has room for
-  w.whole = per_item <= kWholeTiles;
-  const int cap = current_device().cus * (rm * padded_dim(p.dim) <= 16 * 128 ? 2 : 1);
+  w.whole = per_item * w.tile <= (rm == 16 * kWideBlocks ? kWholeWideKeys : kWholeKeys);
+  const bool two = rm == 16 * kWideBlocks || rm * padded_dim(p.dim) <= 16 * 128;   // workgroups of a CU
+  const int cap = current_device().cus * (two ? 2 : 1);
   w.grid = (int)(w.whole ? items : std::min<int64_t>((per_item * items + kPagedWaves - 1) / kPagedWaves, cap));
   w.part = nullptr;
   return w;

@@ -71,7 +71,7 @@ __device__ __forceinline__ int clamp_len(W &w, int s) {
 
 template <class W>
 __device__ __forceinline__ int tiles_of(W &w, int len) {
-  return (w.sel_tiles ? w.sel_tiles : (len + kTile - 1) / kTile) + w.draft_tiles;
+  return (w.sel_tiles ? w.sel_tiles : (len + w.tile - 1) / w.tile) + w.draft_tiles;
 }
 
 // first[s] = tiles of one item of the sequences before s, for s <= batch.
@@ -147,10 +147,11 @@ template <class W>
 __device__ __forceinline__ void build_paths(W &w, int s, Paths &t) {
   const int i = threadIdx.x, n = w.p.draft;
   const int32_t *parents = w.p.parents + s * w.p.parents_s;
+  const int words = (n + 31) / 32;
   if (i < n) {
     const int p = parents[i];
     t.next[i] = p >= -1 && p < i ? p : -2;
-    for (int k = 0; k < w.draft_tiles; ++k) t.bits[i][k] = k == i / 32 ? 1u << (i & 31) : 0u;
+    for (int k = 0; k < words; ++k) t.bits[i][k] = k == i / 32 ? 1u << (i & 31) : 0u;
   }
   __syncthreads();
   for (int round = 0; round < w.rounds; ++round) {
@@ -161,14 +162,14 @@ __device__ __forceinline__ void build_paths(W &w, int s, Paths &t) {
       const int from = next < 0 ? i : next;
 #pragma unroll
       for (int k = 0; k < kMaxDraft / 32; ++k)
-        if (k < w.draft_tiles) got[k] = t.bits[i][k] | t.bits[from][k];
+        if (k < words) got[k] = t.bits[i][k] | t.bits[from][k];
       if (next >= 0) next = t.next[next];
     }
     __syncthreads();
     if (i < n) {
 #pragma unroll
       for (int k = 0; k < kMaxDraft / 32; ++k)
-        if (k < w.draft_tiles) t.bits[i][k] = got[k];
+        if (k < words) t.bits[i][k] = got[k];
       t.next[i] = (int16_t)next;
     }
     __syncthreads();
@@ -665,15 +666,21 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
 #pragma unroll
         for (int j = 1; j < 8; ++j) most = fmaxf(most, sc[rt][j >> 2][j & 3]);
         most = max16x32(most);
-        const float m_new = fmaxf(m[rt], most == -INFINITY ? most : most * mult[rt]);
+        // m is kBias below the largest score, so that weights reach 2^kBias; any
+        // rounding of it is the same for every key and is scaled out again
+        const float m_new = fmaxf(m[rt], most == -INFINITY ? most : fmaf(most, mult[rt], -kBias));
         const float zero = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: every weight is 0
         const float shrink = __builtin_amdgcn_exp2f(m[rt] - zero);
         m[rt] = m_new;
+        // past 2^22 a rounding of m is a factor of 2^(1/4) and more: fp16 weights could overflow
+        const bool far = CT == KH_TYPE_F16 && __any(fabsf(m_new) > 0x1p22f);
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float y = sc[rt][j >> 2][j & 3];
-          pr[rt][j] = __builtin_amdgcn_exp2f(partly && y == -INFINITY ? y : fmaf(y, mult[rt], kBias - zero));
+          float e = partly && y == -INFINITY ? y : fmaf(y, mult[rt], -zero);
+          if (far) e = e > kBias ? kBias : e;   // (a NaN stays)
+          pr[rt][j] = __builtin_amdgcn_exp2f(e);
           sum += pr[rt][j];
         }
         l[rt] = fmaf(l[rt], shrink, sum);
@@ -837,6 +844,532 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows (kWideRows and more) over a 16-bit cache: the matrix cores decide,
+// not the loads. A workgroup's four waves take 32 rows each and share a tile
+// of 64 keys in the LDS, copied while the tile before is used; 32x32x16
+// products give a lane half its row's 32 scores of a block, so a row's maximum
+// takes one exchange of lane halves instead of two, and each operand read from
+// the LDS serves 32 rows. V^T operands come from transposing LDS reads.
+
+// Chunk swizzle of K and V rows in the LDS, 16-byte chunks: a 128-bit read
+// meets in one LDS cycle rows {0-3, 12-15, 20-27}, distinct mod 16; a
+// transposing read's 32 lanes address 4 rows, 4 chunks each.
+template <int DT>
+__device__ __forceinline__ int swz_wide(int r) {
+  if constexpr (DT == 128) return r & 15;
+  else return (r >> 1) & 7;
+}
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int CT>
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (CT == KH_TYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// 64 lanes' 16 bytes at base + voff to LDS address lds + 16 lane (a wave-uniform base)
+__device__ __forceinline__ void copy_rows(const void *base, uint32_t voff, uint32_t lds) {
+  const uint64_t v = (uint64_t)(uintptr_t)base;
+  const uint64_t at = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 |
+                      (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t to = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(at), "s"(to)
+               : "memory", "m0");
+}
+
+__device__ __forceinline__ void copies_landed() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));   // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+constexpr int kWideSpots = 512;
+
+template <int CT, int NP, int DT>
+__global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork) {
+  typedef typename Cache<CT>::T T;
+  constexpr int TK = 64, NH = 4;               // keys of a tile, its parts of 16
+  constexpr int KS = DT / 16, NT = DT / 32;    // chunks of 16 dimensions in S^T, tiles of 32 in O^T
+  constexpr int RB = DT * 2, CH = RB / 16;     // bytes and chunks of a row
+  constexpr int RPI = 64 / CH;                 // rows of a copy
+  constexpr int RM = 32 * kWaves;
+  constexpr int PART = 16 * RB, SIDE = NH * PART;   // bytes of 16 keys, of a tile's K or V
+  constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NP > 1;
+  constexpr float kBias = CT == KH_TYPE_F16 ? kWeightExp : 0.0f;
+
+  __shared__ __attribute__((aligned(256))) unsigned char tiles_lds[2][2][SIDE];   // [buffer][K, V]
+  __shared__ int first[kMaxWideBatch + 1];
+  __shared__ int wave_sums[kWaves];
+  __shared__ Paths paths;
+  __shared__ uint32_t spots[kWideSpots];
+  __shared__ uint32_t odd_keys[kMaxDraft / TK][2];   // new tokens with a value that is not finite, by tile
+
+  const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  int me = blockIdx.x, at = 0, end = 1;
+  const bool whole = fresh().whole;
+  if (!whole) {
+    const_work &w = fresh();
+    scan_tiles(w, first, wave_sums);
+    const Plan plan = plan_of(w, first);
+    if (me >= plan.count) return;
+    const int xcd = me & 7, per = plan.count >> 3, rest = plan.count & 7;
+    me = xcd * per + min(xcd, rest) + (me >> 3);
+    at = range_start(plan, me);
+    end = range_start(plan, me + 1);
+  }
+  int paths_of = -1;
+  while (at < end) {
+    const_work &w = fresh();
+    int s, item, t0, t1, tiles, len;
+    if (whole) {
+      s = (int)((uint32_t)me / (uint32_t)w.items);
+      item = me - s * w.items;
+      len = clamp_len(w, s);
+      tiles = tiles_of(w, len);
+      t0 = 0;
+      t1 = tiles;
+      at = end;
+    } else {
+      s = sequence_of(w, first, at);
+      len = clamp_len(w, s);
+      tiles = tiles_of(w, len);
+      const int in_seq = at - __builtin_amdgcn_readfirstlane(first[s]) * w.items;
+      item = (int)((uint32_t)in_seq / (uint32_t)tiles);
+      t0 = in_seq - item * tiles;
+      t1 = min(tiles, t0 + (end - at));
+      at += t1 - t0;
+    }
+    const int cached = tiles - w.draft_tiles;
+    const int c = (int)((uint32_t)item / (uint32_t)w.per_head);
+    const int b = item - c * w.per_head;
+    const bool sel = w.sel_tiles;
+    const int token = sel ? (int)((uint32_t)b / (uint32_t)w.blocks) : 0;
+    const int row0 = (sel ? b - token * w.blocks : b) * RM;
+    const bool act32 = w.p.act_type == KH_TYPE_F32;
+    const bool has_draft = t1 > cached;
+    const bool tree = w.p.parents != nullptr;
+    const int dim = w.p.dim;
+    if (has_draft && tree && paths_of != s) {
+      __syncthreads();
+      build_paths(w, s, paths);
+      paths_of = s;
+    }
+
+    // places of the cached parts of tiles [c0, c1), by all threads
+    const int half_mask = (1 << w.half_shift) - 1;
+    auto stage = [&](int c0, int c1) {
+      const_work &w = fresh();
+      const int32_t *table = w.p.table + s * w.p.table_s;
+      for (int j = NH * c0 + (int)threadIdx.x; j < NH * min(c1, cached); j += kThreads) {
+        int col = j >> w.half_shift, pos = 16 * j;
+        bool in = true;
+        if (sel) {
+          const int rank = col;
+          in = rank < w.p.top;
+          const int32_t *list = w.p.selected + (s * w.p.sel_s + token * w.p.sel_n + c * w.p.sel_h);
+          const int before = in && rank > 0 ? list[rank - 1] : -1;
+          col = in ? list[rank] : 0;
+          in = in && col > before && col >= 0 && col < w.p.width;
+          pos = in ? col * w.p.page_size + (j & half_mask) * 16 : len;
+        }
+        in = in && pos < len;
+        const int page = in ? table[col] : -1;
+        in = in && page >= 0 && page < w.p.pages;
+        spots[j - NH * c0] = in ? (uint32_t)page * 32u + (uint32_t)min(len - pos, 16) : 0u;
+      }
+    };
+    stage(t0, min(t1, t0 + kWideSpots / NH));
+
+    // this lane's query row: chunk 2 ks + half of its dimensions
+    const_work &wq = fresh();
+    const int r_item = row0 + 32 * wave + row;
+    const bool row_ok = r_item < wq.rows;
+    const int rr = row_ok ? r_item : 0;
+    const int row_token = sel ? token : (int)((uint32_t)rr / (uint32_t)wq.group);
+    const int row_head = c * wq.group + (sel ? rr : rr - row_token * wq.group);
+    u32x4 q[NP][KS];
+    float mult = fabsf(wq.scale2);
+    {
+      float y[KS][8];
+      const int64_t base = s * wq.p.q_s + row_token * wq.p.q_n + row_head * wq.p.q_h;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d = 16 * ks + 8 * half;
+        const bool in = row_ok && d < dim;
+        load_acts<T>(wq.p.q, base + (in ? d : 0), act32, y[ks]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[ks][j] = in ? y[ks][j] : 0.0f;
+      }
+      float up = wq.scale2 < 0.0f ? -1.0f : 1.0f;
+      if constexpr (SCALED_Q) {
+        float most = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(y[ks][j]));
+        const float2 both = half_pair(most);
+        most = fmaxf(both.x, both.y);
+        int e = (int)((__float_as_uint(most) >> 23) & 255) - 127;   // to [2^14, 2^15)
+        e = most == 0.0f || e == 128 ? 0 : min(max(14 - e, -126), 126);
+        up *= __uint_as_float((uint32_t)(e + 127) << 23);
+        mult *= __uint_as_float((uint32_t)(127 - e) << 23);
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[ks][j] *= up;
+        u32x4 parts[NP];
+        split8<T, NP>(y[ks], parts);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) q[n][ks] = parts[n];
+      }
+    }
+
+    f32x16 o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[t][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)tiles_lds;
+    // copies of tile t into buffer `to`: wave i takes its part i, row by row in
+    // RB bytes, chunk x of row r at x ^ swz_wide(r)
+    const int crow = lane / CH, cpos = lane % CH;
+    auto fetch = [&](int t, int c0, int to) {
+      const_work &w = fresh();
+      const uint32_t k_lds = lds0 + (uint32_t)(to * 2 * SIDE + wave * PART), v_lds = k_lds + SIDE;
+      if (t < cached) {
+        const int j = NH * t + wave, slot = (j & half_mask) * 16;
+        const int page = (int)(__builtin_amdgcn_readfirstlane(spots[j - NH * c0]) >> 5);
+        const T *kb = static_cast<const T *>(w.p.k_pages) + (c * w.p.kp_h + page * w.p.kp_p + slot * w.p.kp_t);
+        const T *vb = static_cast<const T *>(w.p.v_pages) + (c * w.p.vp_h + page * w.p.vp_p + slot * w.p.vp_t);
+#pragma unroll
+        for (int i = 0; i < 16 / RPI; ++i) {
+          const int r = RPI * i + crow, d = 8 * (cpos ^ swz_wide<DT>(r)), in = d < dim ? d : 0;
+          copy_rows(kb, (uint32_t)(r * (int)w.p.kp_t + in) * 2u, k_lds + i * 1024);
+          copy_rows(vb, (uint32_t)(r * (int)w.p.vp_t + in) * 2u, v_lds + i * 1024);
+        }
+        return;
+      }
+      // new tokens: rounded to the cache's type, what is not finite in V set aside
+      const int n0 = TK * (t - cached) + 16 * wave;
+      uint32_t odd = 0;
+#pragma unroll 1
+      for (int i = 0; i < 16 / RPI; ++i) {   // (rolled: its registers would come on top of the loop's)
+        const int r = RPI * i + crow, d = 8 * (cpos ^ swz_wide<DT>(r)), in = d < dim ? d : 0;
+        const int n = n0 + r;
+        const bool there = n < w.p.draft;
+        float y[8], z[8];
+        const int64_t nn = there ? n : 0;
+        load_acts<T>(w.p.k, s * w.p.k_s + c * w.p.k_h + nn * w.p.k_n + in, act32, y);
+        load_acts<T>(w.p.v, s * w.p.v_s + c * w.p.v_h + nn * w.p.v_n + in, act32, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool fine = fabsf((float)(T)z[e]) < INFINITY;
+          if (there && !fine) odd |= 1u << r;
+          z[e] = there && fine ? z[e] : 0.0f;
+        }
+        u32x4 kw[1], vw[1];
+        split8<T, 1>(y, kw);
+        split8<T, 1>(z, vw);
+        *(lds_u32x4 *)(uintptr_t)(k_lds + i * 1024 + lane * 16) = kw[0];
+        *(lds_u32x4 *)(uintptr_t)(v_lds + i * 1024 + lane * 16) = vw[0];
+      }
+      if (odd) atomicOr(&odd_keys[t - cached][wave >> 1], odd << (16 * (wave & 1)));
+    };
+    // the tile at or after t that has a key; valid[] of its parts
+    auto find = [&](int &t, int c0, int c1, int (&valid)[NH]) {
+      for (; t < c1; ++t) {
+        if (t >= cached) {
+          const int n0 = TK * (t - cached), n = fresh().p.draft;
+#pragma unroll
+          for (int h = 0; h < NH; ++h) valid[h] = min(max(n - n0 - 16 * h, 0), 16);
+          return;
+        }
+        int any = 0;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          valid[h] = (int)(__builtin_amdgcn_readfirstlane(spots[NH * (t - c0) + h]) & 31);
+          any |= valid[h];
+        }
+        if (any) return;
+      }
+    };
+
+    if (threadIdx.x < 2 * (kMaxDraft / TK)) odd_keys[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    int buffer = 0;
+    for (int c0 = t0; c0 < t1; c0 += kWideSpots / NH) {
+      const int c1 = min(t1, c0 + kWideSpots / NH);
+      if (c0 > t0) stage(c0, c1);   // (behind the last tile's barrier: no wave reads the old places)
+      __syncthreads();
+      int t = c0, valid[NH];
+      find(t, c0, c1, valid);
+      if (t < c1) fetch(t, c0, buffer);
+      while (t < c1) {
+        int t_next = t + 1, valid_next[NH];
+        find(t_next, c0, c1, valid_next);
+        copies_landed();
+        __syncthreads();   // this tile is there, and no wave reads the other buffer
+        if (t_next < c1) fetch(t_next, c0, buffer ^ 1);
+        const uint32_t k_lds = lds0 + (uint32_t)(buffer * 2 * SIDE), v_lds = k_lds + SIDE;
+        const int draft = t >= cached ? t - cached : -1;
+        int fewest = valid[0] & valid[1] & valid[2] & valid[3];
+        const bool partly = draft >= 0 || fewest < 16;
+        if (draft < 0 && fewest < 16) {
+          // values behind the last key (a page's unwritten slots): their weight
+          // is 0, which needs them finite
+#pragma unroll
+          for (int i = 0; i < SIDE / (16 * kThreads); ++i) {
+            const int chunk = i * kThreads + (int)threadIdx.x, r = chunk / CH;
+            const int there = r < 16 ? valid[0] : r < 32 ? valid[1] : r < 48 ? valid[2] : valid[3];
+            if ((r & 15) >= there) *(lds_u32x4 *)(uintptr_t)(v_lds + chunk * 16) = u32x4{0, 0, 0, 0};
+          }
+          __syncthreads();
+        }
+        if (dim < DT) {   // K beyond dim meets q = 0, which needs it finite
+#pragma unroll
+          for (int i = 0; i < SIDE / (16 * kThreads); ++i) {
+            const int chunk = i * kThreads + (int)threadIdx.x, r = chunk / CH, x = (chunk % CH) ^ swz_wide<DT>(r);
+            if (8 * x >= dim) *(lds_u32x4 *)(uintptr_t)(k_lds + chunk * 16) = u32x4{0, 0, 0, 0};
+          }
+          __syncthreads();
+        }
+
+        // scores of the two blocks of 32 keys: register r of a lane is key 8 (r >> 2) + 4 half + (r & 3)
+        f32x16 sc[2];
+        const uint32_t k_at = k_lds + (uint32_t)row * RB + (uint32_t)(half ^ swz_wide<DT>(row)) * 16u;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[kb][r] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          u32x4 k[2];
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+            k[kb] = *(const lds_u32x4 *)(uintptr_t)((k_at ^ (uint32_t)(2 * ks * 16)) + (uint32_t)(kb * 32 * RB));
+#pragma unroll
+          for (int n = NP - 1; n >= 0; --n)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) sc[kb] = mma32<CT>(k[kb], q[n][ks], sc[kb]);
+          if (ks & 1) __builtin_amdgcn_sched_barrier(0);   // (all operands read ahead would not fit the registers)
+        }
+
+        uint32_t see[2];
+        if (partly) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            see[kb] = ((1u << valid[2 * kb]) - 1) | ((1u << valid[2 * kb + 1]) - 1) << 16;
+            if (draft >= 0) {
+              const int word = 2 * draft + kb, i = row_token - 32 * word;   // chain: the tokens up to its own
+              see[kb] &= tree ? (word < kMaxDraft / 32 ? paths.bits[row_token][word] : 0u)
+                              : (i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (!(see[kb] >> (8 * (r >> 2) + 4 * half + (r & 3)) & 1)) sc[kb][r] = -INFINITY;
+          }
+        }
+        float most = sc[0][0];
+#pragma unroll
+        for (int r = 1; r < 32; ++r) most = fmaxf(most, sc[r >> 4][r & 15]);
+        const float2 both = half_pair(most);
+        most = fmaxf(both.x, both.y);
+        // (see paged_attn_kernel: m is kBias below the largest score)
+        const float m_new = fmaxf(m, most == -INFINITY ? most : fmaf(most, mult, -kBias));
+        const float zero = m_new == -INFINITY ? 0.0f : m_new;
+        const float shrink = __builtin_amdgcn_exp2f(m - zero);
+        m = m_new;
+        const bool far = CT == KH_TYPE_F16 && __any(fabsf(m_new) > 0x1p22f);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float y = sc[kb][r];
+            float e = partly && y == -INFINITY ? y : fmaf(y, mult, -zero);
+            if (far) e = e > kBias ? kBias : e;
+            sc[kb][r] = __builtin_amdgcn_exp2f(e);
+            sum[r & 3] += sc[kb][r];
+          }
+        l = fmaf(l, shrink, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+        if (__any(shrink != 1.0f)) {
+#pragma unroll
+          for (int t2 = 0; t2 < NT; ++t2) o[t2] *= shrink;
+        }
+        // O^T += V^T P^T, 16 keys at a time: a lane's keys are its registers 8 i .. 8 i + 7,
+        // V^T's operand two transposing reads, in each of which lane (a4, b4) = (lane % 16 / 4,
+        // lane % 4) of 16 addresses dimensions 4 b4 .. + 4 of the 16 in key row a4
+        const int a4 = (lane & 15) >> 2, g1 = (lane >> 4) & 1;
+        const uint32_t v_row = (uint32_t)(4 * half + a4) * RB + (uint32_t)(lane & 1) * 8u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = sc[i >> 1][8 * (i & 1) + e];
+          u32x4 parts[NP];
+          split8<T, NP>(y, parts);
+          u32x4 v[NT];
+#pragma unroll
+          for (int t2 = 0; t2 < NT; ++t2) {
+            s16x4 x[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int r = 16 * i + 8 * j + 4 * half + a4;
+              const int chunk = (4 * t2 + 2 * g1 + ((lane & 2) >> 1)) ^ swz_wide<DT>(r);
+              x[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds_s16x4 *)(uintptr_t)(v_lds + v_row + (uint32_t)((16 * i + 8 * j) * RB + chunk * 16)));
+            }
+            v[t2] = __builtin_bit_cast(u32x4, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          }
+#pragma unroll
+          for (int n = NP - 1; n >= 0; --n)
+#pragma unroll
+            for (int t2 = 0; t2 < NT; ++t2) o[t2] = mma32<CT>(v[t2], parts[n], o[t2]);
+          if (i & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+
+        if (draft >= 0) {
+          const uint32_t odd[2] = {odd_keys[draft][0], odd_keys[draft][1]};
+          if (__builtin_expect(__any((odd[0] | odd[1]) != 0), 0)) {
+            const_work &w = fresh();
+            for (int key = 0; key < TK; ++key) {   // the values set aside, by hand
+              if (!(odd[key >> 5] >> (key & 31) & 1)) continue;
+              const int kk = key & 31, reg = 4 * (kk >> 3) + (kk & 3), from = kk >> 2 & 1;
+              float mine = 0.0f;
+#pragma unroll
+              for (int r = 0; r < 32; ++r) mine = r == 16 * (key >> 5) + reg ? sc[r >> 4][r & 15] : mine;
+              const float weight = __shfl(mine, row + 32 * from);
+              if (!((key >> 5 ? see[1] : see[0]) >> kk & 1)) continue;
+              const int64_t from_row = s * w.p.v_s + c * w.p.v_h + (int64_t)(TK * draft + key) * w.p.v_n;
+#pragma unroll
+              for (int t2 = 0; t2 < NT; ++t2)
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                  const int d = 32 * t2 + 8 * a + 4 * half;
+                  float y[4];
+                  load_acts<T>(w.p.v, from_row + (d < dim ? d : 0), act32, y);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const float z = (float)(T)y[e];
+                    if (!(fabsf(z) < INFINITY)) o[t2][4 * a + e] += weight * z;
+                  }
+                  __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < NH; ++h) valid[h] = valid_next[h];
+        t = t_next;
+        buffer ^= 1;
+      }
+      __syncthreads();   // all waves are done with this stretch's places, tiles and marks
+    }
+
+    // -- a wave's rows are its own: finished, or this range's part of them
+    const_work &we = fresh();
+    const float2 sums = half_pair(l);
+    l = sums.x + sums.y;
+    if (has_draft && tree && paths.next[row_token] == -2) l = -1.0f;   // an unused token's row
+    if (row_ok) {
+      const bool done = t0 == 0 && t1 == tiles;
+      const int64_t slot = 2 * (int64_t)me + (t0 > 0 ? 0 : 1);
+      const int r = 32 * wave + row;
+      float *to = we.part + (slot * RM + r) * DT;
+      if (!done && half == 0) {
+        float *stats = we.part + 2 * (int64_t)we.grid * RM * DT + (slot * RM + r) * 2;
+        stats[0] = m;
+        stats[1] = l;
+      }
+      const int64_t out = s * we.p.o_s + row_token * we.p.o_n + row_head * we.p.o_h;
+      if (done) to = static_cast<float *>(we.p.out) + out;
+      const float norm = done ? 1.0f / l : 1.0f;
+#pragma unroll
+      for (int t2 = 0; t2 < NT; ++t2)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const int d = 32 * t2 + 8 * a + 4 * half;
+          if (d >= dim) continue;
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = done && l < 0.0f ? 0.0f : o[t2][4 * a + e] * norm;
+          if (act32 || !done) *reinterpret_cast<f32x4 *>(to + d) = f32x4{y[0], y[1], y[2], y[3]};
+          else *reinterpret_cast<u32x2 *>(static_cast<T *>(we.p.out) + out + d) = u32x2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+        }
+    }
+  }
+}
+
+// The parts of rows that few ranges share, joined: a wave per row, in range
+// order.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(const PagedWork w) {
+  constexpr int RM = 32 * kWaves;
+  constexpr int PER = DT / 64;
+  __shared__ int first[kMaxWideBatch + 1];
+  __shared__ int wave_sums[kWaves];
+  const kh_paged &p = w.p;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  scan_tiles(w, first, wave_sums);
+  const Plan plan = plan_of(w, first);
+  const int s = blockIdx.x / w.items, item = blockIdx.x - s * w.items;
+  const int tiles = tiles_of(w, clamp_len(w, s));
+  const int x = first[s] * w.items + item * tiles;
+  const int w0 = range_of(plan, x), w1 = range_of(plan, x + tiles - 1);
+  if (w0 == w1) return;
+  const int c = item / w.per_head, b = item - c * w.per_head;
+  const int token = w.sel_tiles ? b / w.blocks : 0;
+  const int row0 = (w.sel_tiles ? b - token * w.blocks : b) * RM;
+  const bool in = lane * PER < p.dim;
+  for (int r = blockIdx.y * 16 + wave; r < min((int)blockIdx.y * 16 + 16, RM); r += kWaves) {
+    if (row0 + r >= w.rows) return;
+    const int n = w.sel_tiles ? token : (row0 + r) / w.group;
+    const int head = c * w.group + (w.sel_tiles ? row0 + r : row0 + r - n * w.group);
+    auto stat = [&](int i) { return w.part + 2 * (int64_t)w.grid * RM * DT + ((2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) * RM + r) * 2; };
+    const int count = w1 - w0 + 1;
+    float m = -INFINITY, l = 0.0f, o[PER];
+    bool unused = false;
+    for (int i = lane; i < count; i += 64) m = fmaxf(m, stat(i)[0]);
+    m = wave_max(m);
+    if (m == -INFINITY) m = 0.0f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const float a = __builtin_amdgcn_exp2f(stat(i)[0] - m), li = stat(i)[1];
+      l = fmaf(a, li, l);
+      unused |= li < 0.0f;
+      const float *part = w.part + ((2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) * RM + r) * DT + (in ? lane * PER : 0);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] = fmaf(a, part[e], o[e]);
+    }
+    const float norm = 1.0f / l;
+    const int64_t to = s * p.o_s + n * p.o_n + head * p.o_h;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int d = lane * PER + e;
+      if (d >= p.dim) continue;
+      const float y = unused ? 0.0f : o[e] * norm;
+      if (p.act_type == KH_TYPE_F32) static_cast<float *>(p.out)[to + d] = y;
+      else if (p.act_type == KH_TYPE_BF16) static_cast<__bf16 *>(p.out)[to + d] = (__bf16)y;
+      else static_cast<_Float16 *>(p.out)[to + d] = (_Float16)y;
+    }
+  }
+}
+
 // The parts of the items that more than one range touched, joined: a
 // workgroup per row. Weights first, a part per lane, then the weighted sums,
 // every fourth part to a wave, then the waves' sums in order.
@@ -926,18 +1459,29 @@ void launch_both(const PagedWork &w, hipStream_t stream) {
   }
 }
 
+template <int CT, int NP, int DT>
+void launch_wide(const PagedWork &w, hipStream_t stream) {
+  paged_wide_kernel<CT, NP, DT><<<w.grid, kThreads, 0, stream>>>(w);
+  if (!w.whole) {
+    const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)((std::min(w.rows, 32 * kWaves) + 15) / 16));
+    paged_join_rows_kernel<DT><<<grid, kThreads, 0, stream>>>(w);
+  }
+}
+
 template <int CT, int NP>
 hipError_t launch_typed(const PagedWork &w, int dt, int rt, hipStream_t stream) {
-  constexpr bool kFour = CT != KH_TYPE_F32 && NP == 1;
   if (dt == 256) launch_both<CT, NP, 256, 1>(w, stream);
-  else if (dt == 128) {
+  else if (rt == kWideBlocks) {
+    if constexpr (CT != KH_TYPE_F32) {
+      if (dt == 128) launch_wide<CT, NP, 128>(w, stream);
+      else launch_wide<CT, NP, 64>(w, stream);
+    }
+  } else if (dt == 128) {
     if (rt == 1) launch_both<CT, NP, 128, 1>(w, stream);
-    else if (rt == 2 || !kFour) launch_both<CT, NP, 128, 2>(w, stream);
-    else if constexpr (kFour) launch_both<CT, NP, 128, 4>(w, stream);
+    else launch_both<CT, NP, 128, 2>(w, stream);
   } else {
     if (rt == 1) launch_both<CT, NP, 64, 1>(w, stream);
-    else if (rt == 2 || !kFour) launch_both<CT, NP, 64, 2>(w, stream);
-    else if constexpr (kFour) launch_both<CT, NP, 64, 4>(w, stream);
+    else launch_both<CT, NP, 64, 2>(w, stream);
   }
   return hipGetLastError();
 }
