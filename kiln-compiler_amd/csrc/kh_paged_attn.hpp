@@ -507,7 +507,9 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
     }
     u32x4 q16[F32 ? 1 : NP][RT][KS];
     float q32[F32 ? RT : 1][F32 ? KS : 1][8];
-    float mult[RT];   // products to the base-2 domain, not negative: q takes a negative scale's sign
+    // products to the base-2 domain; positive, so that a masked -inf stays one: q
+    // takes a negative scale's sign, and a scale of zero is the smallest number
+    float mult[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float y[KS][8];
@@ -535,6 +537,7 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
         up *= __uint_as_float((uint32_t)(e + 127) << 23);
         mult[rt] *= __uint_as_float((uint32_t)(127 - e) << 23);
       }
+      mult[rt] = fmaxf(mult[rt], 0x1p-126f);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -668,7 +671,7 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
         most = max16x32(most);
         // m is kBias below the largest score, so that weights reach 2^kBias; any
         // rounding of it is the same for every key and is scaled out again
-        const float m_new = fmaxf(m[rt], most == -INFINITY ? most : fmaf(most, mult[rt], -kBias));
+        const float m_new = fmaxf(m[rt], fmaf(most, mult[rt], -kBias));
         const float zero = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet: every weight is 0
         const float shrink = __builtin_amdgcn_exp2f(m[rt] - zero);
         m[rt] = m_new;
@@ -677,10 +680,15 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = sc[rt][j >> 2][j & 3];
-          float e = partly && y == -INFINITY ? y : fmaf(y, mult[rt], -zero);
-          if (far) e = e > kBias ? kBias : e;   // (a NaN stays)
-          pr[rt][j] = __builtin_amdgcn_exp2f(e);
+          pr[rt][j] = fmaf(sc[rt][j >> 2][j & 3], mult[rt], -zero);
+        }
+        if (far) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pr[rt][j] = pr[rt][j] > kBias ? kBias : pr[rt][j];   // (a NaN stays)
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          pr[rt][j] = __builtin_amdgcn_exp2f(pr[rt][j]);
           sum += pr[rt][j];
         }
         l[rt] = fmaf(l[rt], shrink, sum);
@@ -853,12 +861,14 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
 // the LDS serves 32 rows. V^T operands come from transposing LDS reads.
 
 // Chunk swizzle of K and V rows in the LDS, 16-byte chunks: a 128-bit read
-// meets in one LDS cycle rows {0-3, 12-15, 20-27}, distinct mod 16; a
-// transposing read's 32 lanes address 4 rows, 4 chunks each.
+// meets in one LDS cycle rows {0-3, 12-15, 20-27}, distinct mod 16, so every
+// row mod 16 (mod 8 of each parity, two 64-wide rows to 256 bytes) has a chunk
+// of its own; a transposing read's 32 lanes address 4 adjacent rows at the same
+// 4 chunks, which a row's low bits move to other ones.
 template <int DT>
 __device__ __forceinline__ int swz_wide(int r) {
-  if constexpr (DT == 128) return r & 15;
-  else return (r >> 1) & 7;
+  if constexpr (DT == 128) return (r & 3) << 2 | (r >> 2 & 3);
+  else return (r >> 1 & 1) << 2 | (r >> 2 & 3);
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -1024,6 +1034,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
         up *= __uint_as_float((uint32_t)(e + 127) << 23);
         mult *= __uint_as_float((uint32_t)(127 - e) << 23);
       }
+      mult = fmaxf(mult, 0x1p-126f);   // (as there)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -1187,22 +1198,23 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
         const float2 both = half_pair(most);
         most = fmaxf(both.x, both.y);
         // (see paged_attn_kernel: m is kBias below the largest score)
-        const float m_new = fmaxf(m, most == -INFINITY ? most : fmaf(most, mult, -kBias));
+        const float m_new = fmaxf(m, fmaf(most, mult, -kBias));
         const float zero = m_new == -INFINITY ? 0.0f : m_new;
         const float shrink = __builtin_amdgcn_exp2f(m - zero);
         m = m_new;
         const bool far = CT == KH_TYPE_F16 && __any(fabsf(m_new) > 0x1p22f);
+#pragma unroll
+        for (int r = 0; r < 32; ++r) sc[r >> 4][r & 15] = fmaf(sc[r >> 4][r & 15], mult, -zero);
+        if (far) {
+#pragma unroll
+          for (int r = 0; r < 32; ++r) sc[r >> 4][r & 15] = sc[r >> 4][r & 15] > kBias ? kBias : sc[r >> 4][r & 15];
+        }
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float y = sc[kb][r];
-            float e = partly && y == -INFINITY ? y : fmaf(y, mult, -zero);
-            if (far) e = e > kBias ? kBias : e;
-            sc[kb][r] = __builtin_amdgcn_exp2f(e);
-            sum[r & 3] += sc[kb][r];
-          }
+        for (int r = 0; r < 32; ++r) {
+          sc[r >> 4][r & 15] = __builtin_amdgcn_exp2f(sc[r >> 4][r & 15]);
+          sum[r & 3] += sc[r >> 4][r & 15];
+        }
         l = fmaf(l, shrink, (sum[0] + sum[1]) + (sum[2] + sum[3]));
         if (__any(shrink != 1.0f)) {
 #pragma unroll
@@ -1334,7 +1346,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(const PagedWo
   const int token = w.sel_tiles ? b / w.blocks : 0;
   const int row0 = (w.sel_tiles ? b - token * w.blocks : b) * RM;
   const bool in = lane * PER < p.dim;
-  for (int r = blockIdx.y * 16 + wave; r < min((int)blockIdx.y * 16 + 16, RM); r += kWaves) {
+  const int r = blockIdx.y * kWaves + wave;
+  {
     if (row0 + r >= w.rows) return;
     const int n = w.sel_tiles ? token : (row0 + r) / w.group;
     const int head = c * w.group + (w.sel_tiles ? row0 + r : row0 + r - n * w.group);
@@ -1463,7 +1476,7 @@ template <int CT, int NP, int DT>
 void launch_wide(const PagedWork &w, hipStream_t stream) {
   paged_wide_kernel<CT, NP, DT><<<w.grid, kThreads, 0, stream>>>(w);
   if (!w.whole) {
-    const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)((std::min(w.rows, 32 * kWaves) + 15) / 16));
+    const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)((std::min(w.rows, 32 * kWaves) + kWaves - 1) / kWaves));
     paged_join_rows_kernel<DT><<<grid, kThreads, 0, stream>>>(w);
   }
 }
