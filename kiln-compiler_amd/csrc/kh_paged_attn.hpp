@@ -581,28 +581,35 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
               for (int e = 0; e < Regs::KW; ++e) x.k[h][ks][e] = 0;
           }
       }
+      // (products of different sums next to each other: each waits for the one before in its own)
       f32x4 sc[RT][2];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          sc[rt][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (F32) {
+        for (int h = 0; h < 2; ++h) sc[rt][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (F32) {
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
                 sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[h][ks][j]), q32[rt][ks][j], sc[rt][h], 0, 0, 0);
-          } else {
+      } else {
 #pragma unroll
-            for (int n = NP - 1; n >= 0; --n)
+        for (int n = NP - 1; n >= 0; --n)
 #pragma unroll
-              for (int ks = 0; ks < KS; ++ks) {
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
                 const u32x4 a = {x.k[h][ks][0], x.k[h][ks][1], x.k[h][ks][2], x.k[h][ks][3]};
                 sc[rt][h] = Cache<CT>::mma(a, q16[n][rt][ks], sc[rt][h]);
               }
-          }
-        }
+      }
       if (t_next < t1) load_k(next, x);
 
       uint32_t odd = 0;   // this lane group's keys with a value that is not finite (new tokens only)
@@ -714,15 +721,20 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
 #pragma unroll
         for (int vc = 0; vc < VC; ++vc)
 #pragma unroll
-          for (int i = 0; i < VD; ++i) {
-            u32x4 a;   // 8 keys of dimension i
+          for (int i0 = 0; i0 < VD; i0 += 4) {
+            u32x4 a[4];   // 8 keys of dimensions i0 ..
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              a[e] = __builtin_amdgcn_perm(x.v[2 * e + 1][vc][i / 2], x.v[2 * e][vc][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+              for (int e = 0; e < 4; ++e)
+                a[i][e] = __builtin_amdgcn_perm(x.v[2 * e + 1][vc][(i0 + i) / 2], x.v[2 * e][vc][(i0 + i) / 2],
+                                                i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-              for (int n = NP - 1; n >= 0; --n) o[rt][vc][i] = Cache<CT>::mma(a, parts[rt][n], o[rt][vc][i]);
+            for (int n = NP - 1; n >= 0; --n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) o[rt][vc][i0 + i] = Cache<CT>::mma(a[i], parts[rt][n], o[rt][vc][i0 + i]);
           }
       }
       if (t_next < t1) load_v(next, x);
