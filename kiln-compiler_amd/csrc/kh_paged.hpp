@@ -43,16 +43,21 @@ struct PagedWork {
   float *part;     // [workgroup][2][16 RT rows][DT], then [workgroup][2][16 RT][2] m and l
 };
 
-// The kernels of one cache type (kh_paged_attn.hpp) on `passes` passes, dt-wide heads and rt blocks of 16 rows.
-hipError_t launch_paged_f32(const PagedWork &w, int passes, int dt, int rt, hipStream_t stream);
-hipError_t launch_paged_bf16(const PagedWork &w, int passes, int dt, int rt, hipStream_t stream);
-hipError_t launch_paged_f16(const PagedWork &w, int passes, int dt, int rt, hipStream_t stream);
+// The kernels of one cache type (kh_paged_attn.hpp) and number of passes, on
+// dt-wide heads and rt blocks of 16 rows.
+hipError_t launch_paged_f32(const PagedWork &w, int dt, int rt, hipStream_t stream);
+hipError_t launch_paged_bf16(const PagedWork &w, int dt, int rt, hipStream_t stream);
+hipError_t launch_paged_bf16x3(const PagedWork &w, int dt, int rt, hipStream_t stream);
+hipError_t launch_paged_f16(const PagedWork &w, int dt, int rt, hipStream_t stream);
+hipError_t launch_paged_f16x2(const PagedWork &w, int dt, int rt, hipStream_t stream);
 
 constexpr int kPagedTile = 32;     // keys of a tile
 constexpr int kWideTile = 64;      // ... of paged_wide_kernel
 constexpr int kWideBlocks = 8;     // its rows, in 16s
 constexpr int kMaxWideBatch = 1024;
 constexpr int kPagedWaves = 4;     // waves of a workgroup
+// ... of paged_attn_kernel: eight where it takes whole items and two fit a SIMD
+constexpr int paged_waves(int dt, int rt, bool whole) { return whole && rt * dt <= 128 ? 8 : kPagedWaves; }
 constexpr int kMaxDraft = 256;     // new tokens of a sequence: a workgroup's table of paths fits the LDS
 constexpr int kMaxBatch = 4096;    // sequences of a call: each workgroup scans their lengths
 

@@ -8,7 +8,7 @@ namespace kh {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWholeKeys = 1280, kWholeWideKeys = 1024;
+constexpr int kWholeKeys = 2048, kWholeSlowKeys = 1024;   // (with eight waves, with four)
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -50,7 +50,8 @@ PagedWork work_of(const kh_paged &p) {
   const int64_t items = (int64_t)w.items * p.batch;
   // workgroups: one per item where none can have many tiles; else what the
   // chip holds at once, or a tile per wave of the most tiles the table has room for
-  w.whole = per_item * w.tile <= (rm == 16 * kWideBlocks ? kWholeWideKeys : kWholeKeys);
+  const bool eight = rm != 16 * kWideBlocks && paged_waves(padded_dim(p.dim), rm / 16, true) == 8;
+  w.whole = per_item * w.tile <= (eight ? kWholeKeys : kWholeSlowKeys);
   const bool two = rm == 16 * kWideBlocks || rm * padded_dim(p.dim) <= 16 * 128;   // workgroups of a CU
   const int cap = current_device().cus * (two ? 2 : 1);
   w.grid = (int)(w.whole ? items : std::min<int64_t>((per_item * items + kPagedWaves - 1) / kPagedWaves, cap));
@@ -70,11 +71,11 @@ hipError_t launch_paged(const kh_paged &p, float *workspace, hipStream_t stream)
   if (p.batch == 0 || p.draft == 0) return hipSuccess;
   PagedWork w = work_of(p);
   w.part = workspace;
-  const int dt = padded_dim(p.dim), rt = row_blocks(p), np = passes_of(p);
+  const int dt = padded_dim(p.dim), rt = row_blocks(p), passes = passes_of(p);
   switch (p.cache_type) {
-    case KH_TYPE_F32: return launch_paged_f32(w, np, dt, rt, stream);
-    case KH_TYPE_BF16: return launch_paged_bf16(w, np, dt, rt, stream);
-    default: return launch_paged_f16(w, np, dt, rt, stream);
+    case KH_TYPE_F32: return launch_paged_f32(w, dt, rt, stream);
+    case KH_TYPE_BF16: return passes == 1 ? launch_paged_bf16(w, dt, rt, stream) : launch_paged_bf16x3(w, dt, rt, stream);
+    default: return passes == 1 ? launch_paged_f16(w, dt, rt, stream) : launch_paged_f16x2(w, dt, rt, stream);
   }
 }
 

@@ -306,8 +306,11 @@ __device__ __forceinline__ const_work &fresh() {
   return *(const_work *)(uintptr_t)args;
 }
 
-template <int CT, int NP, int DT, int RT>
-__global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_kernel(const PagedWork) {
+// WHOLE: a workgroup per item, of eight waves where the registers allow two on
+// a SIMD (one alone waits about 1.5 us a tile for its loads); else ranges.
+template <int CT, int NP, int DT, int RT, bool WHOLE>
+__global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 : 2) void paged_attn_kernel(const PagedWork) {
+  constexpr int NW = paged_waves(DT, RT, WHOLE);
   typedef typename Cache<CT>::T T;
   typedef Tile<CT, DT> Regs;
   constexpr bool F32 = CT == KH_TYPE_F32;
@@ -317,18 +320,17 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
   constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NP > 1;
   constexpr float kBias = CT == KH_TYPE_F16 ? kWeightExp : 0.0f;
 
-  __shared__ int first[kMaxBatch + 1];
+  __shared__ int first[WHOLE ? 1 : kMaxBatch + 1];
   __shared__ int wave_sums[kWaves];
   __shared__ Paths paths;
-  __shared__ f32x4 o_share[2][RT][NT][64];
-  __shared__ float ml_share[2][2][RM];
+  __shared__ f32x4 o_share[NW / 2][RT][NT][64];
+  __shared__ float ml_share[NW / 2][2][RM];
 
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   int me = blockIdx.x, at = 0, end = 1;
-  const bool whole = fresh().whole;
-  if (!whole) {
+  if constexpr (!WHOLE) {
     const_work &w = fresh();
     scan_tiles(w, first, wave_sums);
     const Plan plan = plan_of(w, first);
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
   while (at < end) {
     const_work &w = fresh();
     int s, item, t0, t1, tiles, len;
-    if (whole) {
+    if constexpr (WHOLE) {
       s = (int)((uint32_t)me / (uint32_t)w.items);
       item = me - s * w.items;
       len = clamp_len(w, s);
@@ -386,7 +388,7 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
     const int kp_t = (int)wt.p.kp_t, vp_t = (int)wt.p.vp_t, half_shift = wt.half_shift, pages = wt.p.pages;
     const const_ints row_of_table = ints_of(wt.p.table) + s * wt.p.table_s;
     auto find = [&](int &t, Source<T> &r) {
-      for (; t < t1; t += kWaves) {
+      for (; t < t1; t += NW) {
         if (t >= cached) {
           const_work &w = fresh();
           r.draft = t - cached;
@@ -567,7 +569,7 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
     }
 
     while (t < t1) {
-      int t_next = t + kWaves;
+      int t_next = t + NW;
       Source<T> next;
       find(t_next, next);
 
@@ -773,7 +775,7 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
       t = t_next;
     }
 
-    // -- the four waves' parts joined, in wave order
+    // -- the waves' parts joined, in a fixed order
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       l[rt] = sum16x32(l[rt]);
@@ -807,20 +809,17 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
           for (int i = 0; i < VD; ++i) o[rt][vc][i] = o[rt][vc][i] * a + o_share[from][rt][vc * VD + i][lane] * b2;
       }
     };
-    if (t1 - t0 > 2) {   // (else waves 2 and 3 had no tile)
-      if (wave >= 2) put(wave - 2);
+#pragma unroll
+    for (int step = NW / 2; step; step /= 2) {
+      if (t1 - t0 <= step) continue;   // (waves from `step` on had no tile)
+      if (wave >= step && wave < 2 * step) put(wave - step);
       __syncthreads();
-      if (wave < 2) join(wave);
-      __syncthreads();
-    }
-    if (t1 - t0 > 1) {
-      if (wave == 1) put(0);
-      __syncthreads();
-      if (wave == 0) join(0);
+      if (wave < step) join(wave);
+      if (step > 1) __syncthreads();
     }
     if (wave == 0) {
       const_work &w = fresh();
-      const bool done = t0 == 0 && t1 == tiles;
+      const bool done = WHOLE || (t0 == 0 && t1 == tiles);
       // (t0 > 0: this range's first part; else its last)
       const int64_t slot = 2 * (int64_t)me + (t0 > 0 ? 0 : 1);
       float *part = w.part + slot * RM * DT;
@@ -860,7 +859,7 @@ __global__ __launch_bounds__(kThreads, RT * DT <= 128 ? 2 : 1) void paged_attn_k
           }
       }
     }
-    if (at < end) __syncthreads();   // the shared parts are free again
+    if (!WHOLE && at < end) __syncthreads();   // the shared parts are free again
   }
 }
 
@@ -1477,8 +1476,10 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
 
 template <int CT, int NP, int DT, int RT>
 void launch_both(const PagedWork &w, hipStream_t stream) {
-  paged_attn_kernel<CT, NP, DT, RT><<<w.grid, kThreads, 0, stream>>>(w);
-  if (!w.whole) {
+  if (w.whole) {
+    paged_attn_kernel<CT, NP, DT, RT, true><<<w.grid, 64 * paged_waves(DT, RT, true), 0, stream>>>(w);
+  } else {
+    paged_attn_kernel<CT, NP, DT, RT, false><<<w.grid, kThreads, 0, stream>>>(w);
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)std::min(w.rows, 16 * RT));
     paged_join_kernel<DT, RT><<<grid, kThreads, 0, stream>>>(w);
   }
@@ -1494,7 +1495,7 @@ void launch_wide(const PagedWork &w, hipStream_t stream) {
 }
 
 template <int CT, int NP>
-hipError_t launch_typed(const PagedWork &w, int dt, int rt, hipStream_t stream) {
+hipError_t launch_passes(const PagedWork &w, int dt, int rt, hipStream_t stream) {
   if (dt == 256) launch_both<CT, NP, 256, 1>(w, stream);
   else if (rt == kWideBlocks) {
     if constexpr (CT != KH_TYPE_F32) {

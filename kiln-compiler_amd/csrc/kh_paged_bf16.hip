@@ -1,11 +1,10 @@
-// kh_paged_bf16.hip - attention over a paged cache of bf16 (kh_paged_attn.hpp).
+// kh_paged_bf16.hip - attention over a paged cache of bf16, products in one pass (kh_paged_attn.hpp).
 #include "kh_paged_attn.hpp"
 
 namespace kh {
 
-hipError_t launch_paged_bf16(const PagedWork &w, int passes, int dt, int rt, hipStream_t stream) {
-  return passes == 1 ? launch_typed<KH_TYPE_BF16, 1>(w, dt, rt, stream)
-                     : launch_typed<KH_TYPE_BF16, 3>(w, dt, rt, stream);
+hipError_t launch_paged_bf16(const PagedWork &w, int dt, int rt, hipStream_t stream) {
+  return launch_passes<KH_TYPE_BF16, 1>(w, dt, rt, stream);
 }
 
 }  // namespace kh
