@@ -87,7 +87,7 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = "more keys and query rows than 32-bit counts hold";
     return false;
   }
-  if (p.variant == KH_PAGED_ATTENTION && ((int64_t)p.kp_t * 16 + p.dim > most / 8 || (int64_t)p.vp_t * 16 + p.dim > most / 8)) {
+  if (p.variant == KH_PAGED_ATTENTION && (p.kp_t > most / 8 / p.page_size - p.dim || p.vp_t > most / 8 / p.page_size - p.dim)) {
     err = "the pages' token stride is too large";
     return false;
   }

@@ -8,7 +8,15 @@ namespace kh {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWholeKeys = 2048, kWholeSlowKeys = 1024;   // (with eight waves, with four)
+
+// Whole items or ranges. A whole item of n keys takes eight waves about 8 us +
+// n / 110 ns whatever else runs, ranges and their join 14 us and the time that
+// the chip's loads take: one sequence of 8 heads, 1000 keys 17.1 (whole) and
+// 17.8 us (ranges), 2000 keys 26.1 and 14.1. With an item for half the compute
+// units whole items lose little of the chip: 128 items of 2000 keys 30.1 and
+// 33.1 us, of 4000 keys 50.0 and 52.2, 512 items of 4000 keys 194 and 195. Four
+// waves (many rows, wide heads) take about twice as long a key.
+constexpr int kWholeKeys = 1280, kWholeManyKeys = 4096, kWholeSlowKeys = 1024;
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -51,7 +59,8 @@ PagedWork work_of(const kh_paged &p) {
   // workgroups: one per item where none can have many tiles; else what the
   // chip holds at once, or a tile per wave of the most tiles the table has room for
   const bool eight = rm != 16 * kWideBlocks && paged_waves(padded_dim(p.dim), rm / 16, true) == 8;
-  w.whole = per_item * w.tile <= (eight ? kWholeKeys : kWholeSlowKeys);
+  const int64_t most_whole = !eight ? kWholeSlowKeys : 2 * items >= current_device().cus ? kWholeManyKeys : kWholeKeys;
+  w.whole = per_item * w.tile <= most_whole;
   const bool two = rm == 16 * kWideBlocks || rm * padded_dim(p.dim) <= 16 * 128;   // workgroups of a CU
   const int cap = current_device().cus * (two ? 2 : 1);
   w.grid = (int)(w.whole ? items : std::min<int64_t>((per_item * items + kPagedWaves - 1) / kPagedWaves, cap));

@@ -203,8 +203,6 @@ class PagedCache:
             while len(have) * self.page_size < self._length[s] + n:
                 have.append(take())
             plans.append(have)
-        if source:
-            paged.copy_pages(self._pools(), source, target)
         table = torch.full((len(seqs), max(len(p) for p in plans)), -1, dtype=torch.int32)
         for i, p in enumerate(plans):
             table[i, :len(p)] = torch.tensor(p, dtype=torch.int32)
@@ -217,6 +215,8 @@ class PagedCache:
                     path[i, :len(r)] = torch.tensor(r, dtype=torch.int32)
             path = self._upload(path)
         try:
+            if source:
+                paged.copy_pages(self._pools(), source, target)
             paged.cache_append(k, v, self.k, self.v, self._upload(table), self._upload(lengths), rows=path,
                                k_means=self.means)
         except Exception:

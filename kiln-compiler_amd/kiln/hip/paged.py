@@ -26,6 +26,7 @@ graph) and reads or changes nothing else. There is no CPU path; with
 
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 
@@ -518,9 +519,12 @@ def _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means):
 
 def _page_list(x, name):
     try:
-        return (ctypes.c_int32 * len(x))(*x)
-    except (TypeError, ctypes.ArgumentError):
-        raise TypeError(f"{name} must be a sequence of page numbers") from None
+        numbers = array.array("i", x)
+    except TypeError:
+        raise TypeError(f"{name} must be a sequence of page numbers (ints)") from None
+    except OverflowError:
+        raise ValueError(f"{name} holds a number that no page has") from None
+    return (ctypes.c_int32 * len(numbers)).from_buffer(numbers)
 
 
 def copy_pages(pools, source, target):

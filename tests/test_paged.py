@@ -162,6 +162,8 @@ def test_refusals_of_append_and_copy(interpreting):
         kiln.copy_pages([pool.t()], [0], [1])
     with pytest.raises(TypeError):
         kiln.copy_pages([pool], ["a"], [1])
+    with pytest.raises(ValueError):
+        kiln.copy_pages([pool], [2 ** 32], [1])
     assert torch.equal(pool, torch.arange(40.0).view(10, 4))
     kiln.copy_pages([pool], [1, 3, 1], [0, 2, 9])
     assert torch.equal(pool[[0, 2, 9]], torch.arange(40.0).view(10, 4)[[1, 3, 1]])
@@ -445,3 +447,42 @@ def test_c_entries_refuse(interpreting):
     launch.n_refs = 8
     launch.cfg[4] = 11
     assert lib.kh_plan_create(kl.ctypes.byref(launch), 1, kl.ctypes.byref(handle)) == kl.ERR_INVALID
+
+
+def test_strides_past_32_bits_are_refused(interpreting):
+    op = kl.Paged(kl.PAGED_ATTENTION, 1, 1, 1, 1, 64, 1024, 4, 2, 0, kl.TYPE_F32, kl.TYPE_F32, 0, 1.0)
+    size = kl.ctypes.c_size_t()
+    lib = kl.load()
+    assert lib.kh_paged_workspace_bytes(op, size) == kl.OK
+    op.kp_t = 2 ** 20
+    assert lib.kh_paged_workspace_bytes(op, size) == kl.ERR_UNSUPPORTED
+    op.kp_t, op.k_n = 0, 2 ** 24
+    assert lib.kh_paged_workspace_bytes(op, size) == kl.ERR_UNSUPPORTED
+    op.k_n, op.pages = 0, 2 ** 27
+    assert lib.kh_paged_workspace_bytes(op, size) == kl.ERR_UNSUPPORTED
+    op.pages, op.batch, op.width = 4, 4096, 2 ** 20
+    assert lib.kh_paged_workspace_bytes(op, size) == kl.ERR_UNSUPPORTED
+
+
+def test_a_cache_whose_append_fails_is_as_before(interpreting, monkeypatch):
+    from kiln.hip import paged
+
+    cache = kiln.PagedCache(1, 6, 16, 2, 8, dtype=torch.float32)
+    a = cache.open()
+    k = torch.randn(1, 1, 20, 2, 8)
+    cache.append([a], k, k)
+    b, = cache.fork(a)
+
+    def fails(*args, **more):
+        raise RuntimeError("a launch failed")
+
+    for name in ("copy_pages", "cache_append"):
+        with monkeypatch.context() as m:
+            m.setattr(paged, name, fails)
+            with pytest.raises(RuntimeError):
+                cache.append([b], k, k)
+        consistent(cache)
+        assert cache.length(b) == 20 and cache.pages_of(b) == cache.pages_of(a) and cache.free_pages == 4
+    cache.append([b], k, k)
+    consistent(cache)
+    assert torch.equal(content(cache, b)[0][:, :, :20], content(cache, a)[0])
