@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const kh_cache_append_
   const int64_t len = a.lengths[s];
   if (len < 0) return;
   const int64_t col = len / a.page_size + blockIdx.x;
-  if (col >= a.width) return;
+  if (col >= a.width || col * a.page_size >= len + a.accept) return;   // (before rows are counted)
   const int page = a.table[s * a.table_s + col];
   const int count = counted_rows(a, s);
   const int64_t first = col * a.page_size;
@@ -179,7 +179,18 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(const CopyArgs a) {
   char *base = static_cast<char *>(pool.base) + layer * pool.layer_bytes + at;
   const T *from = reinterpret_cast<const T *>(base + a.source[blockIdx.y] * pool.page_bytes);
   T *to = reinterpret_cast<T *>(base + a.target[blockIdx.y] * pool.page_bytes);
-  for (int64_t j = threadIdx.x; j < n; j += kThreads) to[j] = from[j];
+  // (the whole chunk in flight; each byte is read and written once: past the caches)
+  T x[kChunk / kThreads / sizeof(T)];
+#pragma unroll
+  for (int i = 0; i < (int)(kChunk / kThreads / sizeof(T)); ++i) {
+    const int64_t j = (int64_t)i * kThreads + threadIdx.x;
+    if (j < n) x[i] = __builtin_nontemporal_load(from + j);
+  }
+#pragma unroll
+  for (int i = 0; i < (int)(kChunk / kThreads / sizeof(T)); ++i) {
+    const int64_t j = (int64_t)i * kThreads + threadIdx.x;
+    if (j < n) __builtin_nontemporal_store(x[i], to + j);
+  }
 }
 
 // -- CPU meaning ----------------------------------------------------------------

@@ -80,18 +80,21 @@ template <int DG>
 __global__ __launch_bounds__(kThreads) void scores_kernel(const kh_paged p, uint64_t *keys) {
   __shared__ __attribute__((aligned(16))) double sums[kTokens][64 * DG];
   const int s = blockIdx.y / p.kv_heads, c = blockIdx.y - s * p.kv_heads;
-  const int held = held_pages(p, s);
   const int b0 = blockIdx.x * kPagesPerGroup;
+  const int lane16 = threadIdx.x & 15, sub = threadIdx.x >> 4;   // 16 pages at a time
+  int named[kPagesPerGroup / 16];   // (asked for along with the length)
+#pragma unroll
+  for (int r = 0; r < kPagesPerGroup / 16; ++r) named[r] = p.table[s * p.table_s + min(b0 + 16 * r + sub, p.width - 1)];
+  const int held = held_pages(p, s);
   if (b0 >= held) return;
   const int group = p.heads / p.kv_heads;
-  const int lane16 = threadIdx.x & 15, sub = threadIdx.x >> 4;   // 16 pages at a time
   // this lane's part of its pages' means: dimensions 4 lane16 .. + 4 of every 64
   constexpr int kRounds = kPagesPerGroup / 16;
   f32x4 mean[kRounds][DG];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const int b = b0 + 16 * r + sub;
-    const int page = b < held ? p.table[s * p.table_s + b] : -1;
+    const int page = b < held ? named[r] : -1;
     const bool there = page >= 0 && page < p.pages;   // else: every score 0
     const float *at = p.k_means + (there ? page * p.m_p + c * p.m_h : 0);
 #pragma unroll

@@ -161,12 +161,12 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _on_device(device, fn):
-    """fn() with `device` current (a launch goes to the current device)."""
-    if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
-        return fn()
+def _on_device(device, entry, *args):
+    """entry(*args, stream) with `device` current (a launch goes to the current device)."""
+    if device.index == torch._C._cuda_getDevice():
+        return entry(*args, _stream(device))
     with torch.cuda.device(device):
-        return fn()
+        return entry(*args, _stream(device))
 
 
 def _ready(device):
@@ -238,14 +238,22 @@ def _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected
 
 def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what):
     try:
-        key = (_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected), scale)
+        key = (q.shape, q.dtype, q.stride(), q.get_device(), k.shape, k.dtype, k.stride(), k.get_device(),
+               v.shape, v.dtype, v.stride(), v.get_device(), k_pages.shape, k_pages.dtype, k_pages.stride(),
+               k_pages.get_device(), v_pages.shape, v_pages.dtype, v_pages.stride(), v_pages.get_device(),
+               table.shape, table.dtype, table.stride(), table.get_device(), lengths.shape, lengths.dtype,
+               lengths.stride(), lengths.get_device(),
+               None if parents is None else (parents.shape, parents.dtype, parents.stride(), parents.get_device()),
+               None if selected is None else (selected.shape, selected.dtype, selected.stride(), selected.get_device()),
+               scale)
     except AttributeError:
         check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected)   # names what is no tensor
         raise
     found = _forms.get(key)
     if found is None:
         check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad
+                                    or v_pages.requires_grad):
         _no_grad(q, k, v, k_pages, v_pages)
     if found is None:
         straight = [_rows_strided(t) for t in (q, k, v)] + [_columns(t) for t in (table, lengths)]
@@ -262,7 +270,7 @@ def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, 
     elif q.device.type != "cuda" and not interpreting():
         _one_device(q)
     op = kl.Paged.from_buffer_copy(found[0])
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     at = (q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr())
     if (at[0] | at[1] | at[2] | at[3] | at[4]) & 15:
         _rows_in_place(k_pages, "k_pages")
@@ -287,7 +295,7 @@ def run_select(q, k_means, table, lengths, page_size, pages):
     found = _forms.get(key)
     if found is None:
         batch, draft, heads, kv_heads, dim, total = check_select(q, k_means, table, lengths, page_size, pages)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (q.requires_grad or k_means.requires_grad):
         _no_grad(q, k_means)
     if found is None:
         straight = _rows_strided(q), _columns(table), _columns(lengths)
@@ -310,7 +318,7 @@ def run_select(q, k_means, table, lengths, page_size, pages):
     elif q.device.type != "cuda" and not interpreting():
         _one_device(q)
     op = kl.Paged.from_buffer_copy(found[0])
-    out = torch.empty((op.batch, op.draft, op.kv_heads, pages), dtype=torch.int32, device=q.device)
+    out = table.new_empty((op.batch, op.draft, op.kv_heads, pages))
     op.q, op.k_means = q.data_ptr(), k_means.data_ptr()
     if (op.q | op.k_means) & 15:
         _rows_in_place(k_means, "k_means")
@@ -446,7 +454,8 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
             _forms.pop(next(iter(_forms)))
     elif k.device.type != "cuda" and not interpreting():
         _one_device(k)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+                                    or (k_means is not None and k_means.requires_grad)):
         _no_grad(k, v, k_pages, v_pages, k_means)
     op = kl.CacheAppend.from_buffer_copy(template)
     op.k, op.v, op.k_pages, op.v_pages = at = (k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr())
@@ -463,7 +472,7 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
     if device.type != "cuda":
         rc = lib.kh_cache_append_host(ctypes.byref(op))
     else:
-        rc = _on_device(device, lambda: lib.kh_cache_append(ctypes.byref(op), _stream(device)))
+        rc = _on_device(device, lib.kh_cache_append, ctypes.byref(op))
     if rc:
         kl.check(rc, "cache_append")
 
@@ -527,17 +536,8 @@ def _page_list(x, name):
     return (ctypes.c_int32 * len(numbers)).from_buffer(numbers)
 
 
-def copy_pages(pools, source, target):
-    """Copy pages within each of ``pools``, in place: page ``source[i]`` to
-    page ``target[i]``. A pool is a tensor ``[pages, ...]`` or, with 5
-    dimensions (4 for fp32 means of 5-dimensional pools: pass
-    ``means.unsqueeze(-2)``), ``[layers, pages, ...]``, contiguous within a
-    layer. ``source`` and ``target`` are sequences of ints; targets are
-    distinct and none is a source, so no order of the copies matters."""
-    _eager_only("copy_pages")
-    pools = list(pools)
-    if len(source) != len(target):
-        raise ValueError(f"{len(source)} source pages, but {len(target)} target pages")
+def _pool_forms(pools):
+    """(the pools' descriptors without addresses, their number of pages), checked."""
     descs = (kl.Pool * max(1, len(pools)))()
     pages = None
     for i, t in enumerate(pools):
@@ -553,18 +553,51 @@ def copy_pages(pools, source, target):
         if pages is not None and pages != shape[first]:
             raise ValueError(f"pools of {pages} and of {shape[first]} pages")
         pages = shape[first]
-        descs[i] = kl.Pool(t.data_ptr(), shape[0] if first else 1, strides[0] * size if first else 0,
+        descs[i] = kl.Pool(None, shape[0] if first else 1, strides[0] * size if first else 0,
                            inner // pages * size if pages else 0)
-    if not pools or len(source) == 0:
+    return bytes(descs), pages
+
+
+def copy_pages(pools, source, target):
+    """Copy pages within each of ``pools``, in place: page ``source[i]`` to
+    page ``target[i]``. A pool is a tensor ``[pages, ...]`` or, with 5
+    dimensions (4 for fp32 means of 5-dimensional pools: pass
+    ``means.unsqueeze(-2)``), ``[layers, pages, ...]``, contiguous within a
+    layer. ``source`` and ``target`` are sequences of ints; targets are
+    distinct and none is a source, so no order of the copies matters."""
+    _eager_only("copy_pages")
+    pools = list(pools)
+    if len(source) != len(target):
+        raise ValueError(f"{len(source)} source pages, but {len(target)} target pages")
+    try:
+        key = _form(*pools)
+    except AttributeError:
+        raise TypeError("a pool is a tensor of pages") from None
+    found = _forms.get(key)
+    if found is None:
+        found = _pool_forms(pools)
+        if not pools or len(source) == 0:
+            return
+        _one_device(*pools)
+        _ready(pools[0].device)
+        _forms[key] = found
+        while len(_forms) > MOST_FORMS:
+            _forms.pop(next(iter(_forms)))
+    elif pools[0].device.type != "cuda" and not interpreting():
+        _one_device(*pools)
+    if len(source) == 0:
         return
-    _no_grad(*pools)
-    _one_device(*pools)
+    if torch.is_grad_enabled():
+        _no_grad(*pools)
+    template, pages = found
+    descs = (kl.Pool * len(pools)).from_buffer_copy(template)
+    for desc, t in zip(descs, pools):
+        desc.base = t.data_ptr()
     src, dst = _page_list(source, "source"), _page_list(target, "target")
     lib, device = kl.load(), pools[0].device
     if device.type != "cuda":
         kl.check(lib.kh_cache_copy_host(descs, len(pools), pages, src, dst, len(src)), "copy_pages")
         return
-    _ready(device)
-    rc = _on_device(device, lambda: lib.kh_cache_copy(descs, len(pools), pages, src, dst, len(src), _stream(device)))
+    rc = _on_device(device, lib.kh_cache_copy, descs, len(pools), pages, src, dst, len(src))
     if rc:
         kl.check(rc, "copy_pages")
