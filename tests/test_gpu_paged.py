@@ -433,3 +433,41 @@ def test_another_cards_tensors_are_refused():
         kiln.tree_attention(**dict(p, table=p["table"].cpu()))
     with pytest.raises(NotImplementedError):
         kiln.tree_attention(**{k: v.cpu() for k, v in p.items()})
+
+
+@pytest.mark.parametrize("cache,act", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("dim,group", [(64, 1), (80, 2), (128, 1), (128, 4)])
+def test_many_rows(cache, act, dim, group):
+    # 48 rows of an item and more share tiles: one block, two, several; ranges and whole items
+    draft = 70
+    for lengths, page in (((1100, 0), 16), ((63, 130), 128)):
+        p = ref.problem(gen(group), draft=draft, heads=group * 2, kv=2, dim=dim, lengths=lengths, page=page, cache=cache,
+                        act=act, device="cuda")
+        used = torch.zeros(len(p["k_pages"]), page, dtype=torch.bool)
+        for s, n in enumerate(lengths):
+            for t in range(n):
+                used[p["table"][s, t // page].cpu(), t % page] = True
+        at = [x.cuda() for x in (~used).nonzero(as_tuple=True)]
+        for pages in (p["k_pages"], p["v_pages"]):
+            pages[at[0], :, at[1]] = math.nan      # a page's unwritten slots
+        p["parents"][0, 40] = 50                    # unused
+        p["v"][1, 33, 0, 5] = -math.inf
+        p["v"][1, 66, 1] = math.nan
+        check(p)
+        p["parents"] = None
+        check({k: v for k, v in p.items() if k != "parents"})
+
+
+@pytest.mark.parametrize("heads", [96, 320])
+def test_many_heads_of_a_picked_page(heads):
+    p = ref.problem(gen(14), draft=2, heads=heads, kv=1, lengths=(700, 90), cache=torch.float16, act=torch.float16, dim=128,
+                    device="cuda")
+    sel = torch.tensor([[0, 3, 4, -1], [1, 2, 5, 43]], dtype=torch.int32, device="cuda").view(1, 2, 1, 4).expand(2, 2, 1, 4)
+    got = kiln.selected_attention(**p, selected=sel)
+    torch.testing.assert_close(got.double().cpu(), ref.attention(**p, selected=sel.cpu()), **tolerance(torch.float16))
+
+
+def test_many_sequences():
+    p = ref.problem(gen(15), batch=1500, draft=1, heads=1, kv=1, lengths=[i % 40 for i in range(1500)], cache=torch.bfloat16,
+                    columns=200, device="cuda")
+    check(p)
