@@ -13,6 +13,11 @@
 // (sign and exponent first; counts in the LDS), until a digit's bin is taken
 // whole; then one ordered sweep writes the columns, ties in order of column.
 // Up to 2048 scores stay in registers meanwhile.
+//
+// Measured: 16 sequences of up to 512 pages, 8 heads of 128 (17 MB of means)
+// 13.5 and 6.4 us; 13 tokens over 1024 pages, 2 sequences, 13.2 (38 with the dot
+// products' lane sums through the LDS) and 8.2; 125 pages of 12 heads of 64 4.4
+// and 5.4. Both are chains of a few dependent loads, not their bytes.
 #include <algorithm>
 
 #include "kh_paged.hpp"
