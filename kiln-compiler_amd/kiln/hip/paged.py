@@ -101,6 +101,11 @@ def _rows_strided(t):
     return _rows(t) if t.stride(-1) != 1 or any(s * size % 16 for s in t.stride()[:-1]) else t
 
 
+def _head_dim(dim):
+    if dim % 8 or not 0 < dim <= 256:
+        raise NotImplementedError(f"head dimension {dim}: multiples of 8 up to 256 have kernels")
+
+
 def check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected):
     """(sizes of the call) after checking types, shapes and their agreement."""
     check_pages(k_pages, v_pages)
@@ -108,6 +113,7 @@ def check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected
     _tensor(q, "q", 4, (torch.float32,) if k_pages.dtype == torch.float32 else (torch.float32, k_pages.dtype))
     batch, draft, heads, _ = q.shape
     _shape(q, "q", (batch, draft, heads, dim))
+    _head_dim(dim)
     for t, name in ((k, "k"), (v, "v")):
         _tensor(t, name, 4, (q.dtype,))
         _shape(t, name, (batch, draft, kv_heads, dim))
@@ -134,6 +140,7 @@ def check_select(q, k_means, table, lengths, page_size, pages):
     batch, draft, heads, dim = q.shape
     total, kv_heads, _ = k_means.shape
     _shape(k_means, "k_means", (total, kv_heads, dim))
+    _head_dim(dim)
     if kv_heads == 0 or heads % kv_heads or heads == 0:
         raise ValueError(f"{heads} query heads do not divide over {kv_heads} heads of the cache")
     if not isinstance(table, torch.Tensor) or table.dim() != 2:
@@ -489,6 +496,7 @@ def _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means):
         k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
         k_means = k_means.unsqueeze(0) if isinstance(k_means, torch.Tensor) else k_means
     layers, pages, kv_heads, page_size, dim = k_pages.shape
+    _head_dim(dim)
     _tensor(k, "k", 5, tuple(TYPES))
     batch, draft = k.shape[1], k.shape[2]
     _shape(k, "k", (layers, batch, draft, kv_heads, dim))

@@ -99,10 +99,18 @@ def test_refusals_of_attention(interpreting, change, error):
 
 
 def test_refusals_of_sizes(interpreting):
-    for sizes in (dict(dim=12), dict(dim=264), dict(page=8, lengths=(20, 9)), dict(page=48, lengths=(20, 9)),
+    for sizes in (dict(dim=12), dict(dim=10), dict(dim=12, cache=torch.float16), dict(dim=20, cache=torch.bfloat16, act=torch.bfloat16),
+                  dict(dim=264), dict(page=8, lengths=(20, 9)), dict(page=48, lengths=(20, 9)),
                   dict(draft=257), dict(page=2048, lengths=(20, 9))):
         with pytest.raises(NotImplementedError):
             kiln.tree_attention(**operands(**sizes))
+    for dim in (4, 10, 260):
+        pages, k = torch.zeros(4, 2, 16, dim, dtype=torch.float16), torch.zeros(1, 3, 2, dim)
+        with pytest.raises(NotImplementedError):
+            kiln.cache_append(k, k, pages, pages.clone(), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+        with pytest.raises(NotImplementedError):
+            kiln.select_pages(k, pages.float().mean(2), torch.zeros(1, 2, dtype=torch.int32),
+                              torch.zeros(1, dtype=torch.int32), page_size=16, pages=1)
     p = operands()
     with pytest.raises(ValueError):    # token rows that do not lie together
         kiln.tree_attention(**dict(p, k_pages=p["k_pages"].transpose(2, 3).contiguous().transpose(2, 3)))
