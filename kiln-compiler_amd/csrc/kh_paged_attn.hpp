@@ -26,8 +26,10 @@
 // fp32 activations over a 16-bit cache keep fp32's accuracy: a bf16 product's
 // three parts x = x1 + x2 + x3 of 8 bits each hold all 24 bits of q and of a
 // weight, and K and V are exact, so three passes lose nothing; fp16 parts
-// hold 11 bits each, two passes 22, with q scaled by a power of two per row
-// and the weights by 2^14 to stay clear of fp16's subnormals.
+// hold 11 bits each, two passes are off by 2^-21, with q scaled by a power of
+// two per row and the weights by 2^14 to stay clear of fp16's subnormals. The
+// parts of a number all have its sign and none is 0 alone, so that an infinite
+// key or value gives what it gives in one product (split8).
 //
 // What bounds it, measured (one MI355X; a 2 GiB copy moves 4.9 TB/s, reads and
 // writes together): long caches the reading of K and V - 131072 bf16 tokens of
@@ -239,20 +241,52 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-// x as NP parts of type T, the first the nearest to x, each next the nearest
-// to what the ones before leave.
-template <class T, int NP>
+// x's leading bits as a T, toward zero, as a float
+template <class T>
+__device__ __forceinline__ float leading(float x) {
+  if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  else return (float)__builtin_amdgcn_cvt_pkrtz(x, x)[0];
+}
+
+// x as NP parts of type T: the leading bits of x, those of what is left, and
+// last the nearest to that. No part has the other sign, and none is 0 under an
+// x that T can tell from 0 (the smallest normal of bf16 or the smallest
+// subnormal of fp16 stands in): an infinite key or value then meets no part
+// that makes a NaN of it (0 inf, inf - inf), as it would not meet x.
+// One part is the nearest to x. SIGNED: x may be negative.
+template <class T, int NP, bool SIGNED>
 __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&out)[NP]) {
+  if constexpr (NP == 1) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m) out[0][m] = pack2<T>(x[2 * m], x[2 * m + 1]);
+    return;
+  }
+  constexpr float kLeast = std::is_same<T, __bf16>::value ? 0x1p-126f : 0x1p-24f;
   float rest[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = x[j];
+  for (int j = 0; j < 8; ++j) rest[j] = SIGNED ? fabsf(x[j]) : x[j];
 #pragma unroll
   for (int part = 0; part < NP; ++part) {
-#pragma unroll
-    for (int m = 0; m < 4; ++m) out[part][m] = pack2<T>(rest[2 * m], rest[2 * m + 1]);
     if (part + 1 < NP) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) rest[j] -= (float)(T)rest[j];
+      for (int m = 0; m < 4; ++m) {
+        const float a = rest[2 * m], b = rest[2 * m + 1];
+        if constexpr (std::is_same<T, __bf16>::value)
+          out[part][m] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+        else
+          out[part][m] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+      }
+      // (the median: not below kLeast, nor above x where x is)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rest[j] = __builtin_amdgcn_fmed3f(rest[j] - leading<T>(rest[j]), kLeast, rest[j]);
+    } else {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) out[part][m] = pack2<T>(rest[2 * m], rest[2 * m + 1]);
+    }
+    if constexpr (SIGNED) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        out[part][m] |= __float_as_uint(x[2 * m]) >> 31 << 15 | (__float_as_uint(x[2 * m + 1]) & 0x80000000u);
     }
   }
 }
@@ -562,7 +596,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           for (int j = 0; j < 8; ++j) q32[rt][ks][j] = y[ks][j];
         } else {
           u32x4 parts[NP];
-          split8<T, NP>(y[ks], parts);
+          split8<T, NP, true>(y[ks], parts);
 #pragma unroll
           for (int n = 0; n < NP; ++n) q16[n][rt][ks] = parts[n];
         }
@@ -720,7 +754,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
             for (int i = 0; i < VD; ++i) o[rt][vc][i] *= shrink;
         }
-        if constexpr (!F32) split8<T, NP>(pr[rt], parts[rt]);
+        if constexpr (!F32) split8<T, NP, false>(pr[rt], parts[rt]);
       }
       if constexpr (F32) {
 #pragma unroll
@@ -1073,7 +1107,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[ks][j] *= up;
         u32x4 parts[NP];
-        split8<T, NP>(y[ks], parts);
+        split8<T, NP, true>(y[ks], parts);
 #pragma unroll
         for (int n = 0; n < NP; ++n) q[n][ks] = parts[n];
       }
@@ -1125,8 +1159,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
           z[e] = there && fine ? z[e] : 0.0f;
         }
         u32x4 kw[1], vw[1];
-        split8<T, 1>(y, kw);
-        split8<T, 1>(z, vw);
+        split8<T, 1, true>(y, kw);
+        split8<T, 1, true>(z, vw);
         *(lds_u32x4 *)(uintptr_t)(k_lds + i * 1024 + lane * 16) = kw[0];
         *(lds_u32x4 *)(uintptr_t)(v_lds + i * 1024 + lane * 16) = vw[0];
       }
@@ -1264,7 +1298,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = sc[i >> 1][8 * (i & 1) + e];
           u32x4 parts[NP];
-          split8<T, NP>(y, parts);
+          split8<T, NP, false>(y, parts);
           u32x4 v[NT];
 #pragma unroll
           for (int t2 = 0; t2 < NT; ++t2) {
