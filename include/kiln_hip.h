@@ -392,9 +392,10 @@ int kh_plan_destroy(kh_plan *plan);
  * An entry of `selected` counts only where it is larger than the entry before
  * it (the first: than -1) and below width. Sums, softmax statistics and
  * products of fp32 activations are kept to fp32 (bf16 and fp16 caches: q and
- * the weights split into 3 and 2 parts, whose products are exact); with
- * act_type = cache_type = bf16 or fp16, or one_pass = 1, the weights are
- * rounded to the cache's type for the second product (one_pass: q too).
+ * the weights split into 3 and 2 parts, whose products are exact). With
+ * act_type = cache_type = bf16 or fp16 the first product is exact and the
+ * weights are two parts of the cache's type, 2^-15 or 2^-21 of a weight off.
+ * one_pass = 1: q and the weights are rounded to the cache's type.
  *
  * kh_paged_select: for query token (s, i) and kv head c the `top` pages with
  * the largest (sum of the group's queries) . k_means[page][c], products and

@@ -43,12 +43,15 @@ struct PagedWork {
   float *part;     // [workgroup][2][16 RT rows][DT], then [workgroup][2][16 RT][2] m and l
 };
 
-// The kernels of one cache type (kh_paged_attn.hpp) and number of passes, on
-// dt-wide heads and rt blocks of 16 rows.
+// The kernels of one cache type (kh_paged_attn.hpp) and number of parts of q and
+// of the weights (1 and 1; x3, x2: as many of both; w2: 1 and 2), on dt-wide
+// heads and rt blocks of 16 rows.
 hipError_t launch_paged_f32(const PagedWork &w, int dt, int rt, hipStream_t stream);
 hipError_t launch_paged_bf16(const PagedWork &w, int dt, int rt, hipStream_t stream);
+hipError_t launch_paged_bf16w2(const PagedWork &w, int dt, int rt, hipStream_t stream);
 hipError_t launch_paged_bf16x3(const PagedWork &w, int dt, int rt, hipStream_t stream);
 hipError_t launch_paged_f16(const PagedWork &w, int dt, int rt, hipStream_t stream);
+hipError_t launch_paged_f16w2(const PagedWork &w, int dt, int rt, hipStream_t stream);
 hipError_t launch_paged_f16x2(const PagedWork &w, int dt, int rt, hipStream_t stream);
 
 constexpr int kPagedTile = 32;     // keys of a tile

@@ -20,11 +20,6 @@ constexpr int kWholeKeys = 1280, kWholeManyKeys = 4096, kWholeSlowKeys = 1024;
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-int passes_of(const kh_paged &p) {
-  if (p.cache_type == KH_TYPE_F32 || p.one_pass || p.act_type != KH_TYPE_F32) return 1;
-  return p.cache_type == KH_TYPE_BF16 ? 3 : 2;
-}
-
 // 16-row blocks of an item: one or two by its rows, what the registers of a
 // lane hold beside a tile (a 256-wide head's fill them with one). Many rows over
 // a 16-bit cache take paged_wide_kernel: from half as many as its 128, where two
@@ -82,11 +77,13 @@ hipError_t launch_paged(const kh_paged &p, float *workspace, hipStream_t stream)
   if (p.batch == 0 || p.draft == 0) return hipSuccess;
   PagedWork w = work_of(p);
   w.part = workspace;
-  const int dt = padded_dim(p.dim), rt = row_blocks(p), passes = passes_of(p);
+  const int dt = padded_dim(p.dim), rt = row_blocks(p);
+  const bool fp32 = p.act_type == KH_TYPE_F32;
   switch (p.cache_type) {
     case KH_TYPE_F32: return launch_paged_f32(w, dt, rt, stream);
-    case KH_TYPE_BF16: return passes == 1 ? launch_paged_bf16(w, dt, rt, stream) : launch_paged_bf16x3(w, dt, rt, stream);
-    default: return passes == 1 ? launch_paged_f16(w, dt, rt, stream) : launch_paged_f16x2(w, dt, rt, stream);
+    case KH_TYPE_BF16:
+      return (p.one_pass ? launch_paged_bf16 : fp32 ? launch_paged_bf16x3 : launch_paged_bf16w2)(w, dt, rt, stream);
+    default: return (p.one_pass ? launch_paged_f16 : fp32 ? launch_paged_f16x2 : launch_paged_f16w2)(w, dt, rt, stream);
   }
 }
 

@@ -27,7 +27,11 @@
 // three parts x = x1 + x2 + x3 of 8 bits each hold all 24 bits of q and of a
 // weight, and K and V are exact, so three passes lose nothing; fp16 parts
 // hold 11 bits each, two passes are off by 2^-21, with q scaled by a power of
-// two per row and the weights by 2^14 to stay clear of fp16's subnormals. The
+// two per row and the weights by 2^14 to stay clear of fp16's subnormals. Under
+// 16-bit activations q is exact as it is and the weights are two parts: 16 bits
+// of bf16 and 22 of fp16, so that nothing rounds by as much as the result's own
+// 8 or 11 do. NQ and NW: parts of q and of the weights; one and one rounds
+// both to the cache's type (a plan whose products are bf16 asks for that). The
 // parts of a number all have its sign and none is 0 alone, so that an infinite
 // key or value gives what it gives in one product (split8).
 //
@@ -355,23 +359,23 @@ __device__ __forceinline__ const_work &fresh() {
 
 // WHOLE: a workgroup per item, of eight waves where the registers allow two on
 // a SIMD (one alone waits about 1.5 us a tile for its loads); else ranges.
-template <int CT, int NP, int DT, int RT, bool WHOLE>
+template <int CT, int NQ, int NW, int DT, int RT, bool WHOLE>
 __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 : 2) void paged_attn_kernel(const PagedWork) {
-  constexpr int NW = paged_waves(DT, RT, WHOLE);
+  constexpr int WAVES = paged_waves(DT, RT, WHOLE);
   typedef typename Cache<CT>::T T;
   typedef Tile<CT, DT> Regs;
   constexpr bool F32 = CT == KH_TYPE_F32;
   constexpr int KS = Regs::KS, VD = Regs::VD, VC = Regs::VC;
   constexpr int RM = 16 * RT;
   constexpr int NT = DT / 16;                  // 16-wide tiles of O^T: (chunk, t)
-  constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NP > 1;
+  constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NQ > 1;
   constexpr float kBias = CT == KH_TYPE_F16 ? kWeightExp : 0.0f;
 
   __shared__ int first[WHOLE ? 1 : kMaxBatch + 1];
   __shared__ int wave_sums[kWaves];
   __shared__ Paths paths;
-  __shared__ f32x4 o_share[NW / 2][RT][NT][64];
-  __shared__ float ml_share[NW / 2][2][RM];
+  __shared__ f32x4 o_share[WAVES / 2][RT][NT][64];
+  __shared__ float ml_share[WAVES / 2][2][RM];
 
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -435,7 +439,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     const int kp_t = (int)wt.p.kp_t, vp_t = (int)wt.p.vp_t, half_shift = wt.half_shift, pages = wt.p.pages;
     const const_ints row_of_table = ints_of(wt.p.table) + s * wt.p.table_s;
     auto find = [&](int &t, Source<T> &r) {
-      for (; t < t1; t += NW) {
+      for (; t < t1; t += WAVES) {
         if (t >= cached) {
           const_work &w = fresh();
           r.draft = t - cached;
@@ -554,7 +558,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       row_token[rt] = sel ? token : (int)((uint32_t)rr / (uint32_t)wq.group);
       row_head[rt] = c * wq.group + (sel ? rr : rr - row_token[rt] * wq.group);
     }
-    u32x4 q16[F32 ? 1 : NP][RT][KS];
+    u32x4 q16[F32 ? 1 : NQ][RT][KS];
     float q32[F32 ? RT : 1][F32 ? KS : 1][8];
     // products to the base-2 domain; positive, so that a masked -inf stays one: q
     // takes a negative scale's sign, and a scale of zero is the smallest number
@@ -595,10 +599,10 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
           for (int j = 0; j < 8; ++j) q32[rt][ks][j] = y[ks][j];
         } else {
-          u32x4 parts[NP];
-          split8<T, NP, true>(y[ks], parts);
+          u32x4 parts[NQ];
+          split8<T, NQ, true>(y[ks], parts);
 #pragma unroll
-          for (int n = 0; n < NP; ++n) q16[n][rt][ks] = parts[n];
+          for (int n = 0; n < NQ; ++n) q16[n][rt][ks] = parts[n];
         }
       }
     }
@@ -616,7 +620,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     }
 
     while (t < t1) {
-      int t_next = t + NW;
+      int t_next = t + WAVES;
       Source<T> next;
       find(t_next, next);
 
@@ -648,7 +652,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
                 sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[h][ks][j]), q32[rt][ks][j], sc[rt][h], 0, 0, 0);
       } else {
 #pragma unroll
-        for (int n = NP - 1; n >= 0; --n)
+        for (int n = NQ - 1; n >= 0; --n)
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -718,7 +722,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 
       // the running softmax of this lane's rows (the four lane groups of a row agree on m)
       float pr[RT][8];
-      u32x4 parts[F32 ? 1 : RT][NP];
+      u32x4 parts[F32 ? 1 : RT][NW];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         float most = sc[rt][0][0];
@@ -754,7 +758,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
             for (int i = 0; i < VD; ++i) o[rt][vc][i] *= shrink;
         }
-        if constexpr (!F32) split8<T, NP, false>(pr[rt], parts[rt]);
+        if constexpr (!F32) split8<T, NW, false>(pr[rt], parts[rt]);
       }
       if constexpr (F32) {
 #pragma unroll
@@ -779,7 +783,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
                 a[i][e] = __builtin_amdgcn_perm(x.v[2 * e + 1][vc][(i0 + i) / 2], x.v[2 * e][vc][(i0 + i) / 2],
                                                 i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-            for (int n = NP - 1; n >= 0; --n)
+            for (int n = NW - 1; n >= 0; --n)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -857,7 +861,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       }
     };
 #pragma unroll
-    for (int step = NW / 2; step; step /= 2) {
+    for (int step = WAVES / 2; step; step /= 2) {
       if (t1 - t0 <= step) continue;   // (waves from `step` on had no tile)
       if (wave >= step && wave < 2 * step) put(wave - step);
       __syncthreads();
@@ -970,7 +974,7 @@ __device__ __forceinline__ void copies_landed() {
 
 constexpr int kWideSpots = 512;
 
-template <int CT, int NP, int DT>
+template <int CT, int NQ, int NW, int DT>
 __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork) {
   typedef typename Cache<CT>::T T;
   constexpr int TK = 64, NH = 4;               // keys of a tile, its parts of 16
@@ -979,7 +983,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
   constexpr int RPI = 64 / CH;                 // rows of a copy
   constexpr int RM = 32 * kWaves;
   constexpr int PART = 16 * RB, SIDE = NH * PART;   // bytes of 16 keys, of a tile's K or V
-  constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NP > 1;
+  constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NQ > 1;
   constexpr float kBias = CT == KH_TYPE_F16 ? kWeightExp : 0.0f;
 
   __shared__ __attribute__((aligned(256))) unsigned char tiles_lds[2][2][SIDE];   // [buffer][K, V]
@@ -1074,7 +1078,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
     const int rr = row_ok ? r_item : 0;
     const int row_token = sel ? token : (int)((uint32_t)rr / (uint32_t)wq.group);
     const int row_head = c * wq.group + (sel ? rr : rr - row_token * wq.group);
-    u32x4 q[NP][KS];
+    u32x4 q[NQ][KS];
     float mult = fabsf(wq.scale2);
     {
       float y[KS][8];
@@ -1106,10 +1110,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
       for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[ks][j] *= up;
-        u32x4 parts[NP];
-        split8<T, NP, true>(y[ks], parts);
+        u32x4 parts[NQ];
+        split8<T, NQ, true>(y[ks], parts);
 #pragma unroll
-        for (int n = 0; n < NP; ++n) q[n][ks] = parts[n];
+        for (int n = 0; n < NQ; ++n) q[n][ks] = parts[n];
       }
     }
 
@@ -1238,7 +1242,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
           for (int kb = 0; kb < 2; ++kb)
             k[kb] = *(const lds_u32x4 *)(uintptr_t)((k_at ^ (uint32_t)(2 * ks * 16)) + (uint32_t)(kb * 32 * RB));
 #pragma unroll
-          for (int n = NP - 1; n >= 0; --n)
+          for (int n = NQ - 1; n >= 0; --n)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) sc[kb] = mma32<CT>(k[kb], q[n][ks], sc[kb]);
           if (ks & 1) __builtin_amdgcn_sched_barrier(0);   // (all operands read ahead would not fit the registers)
@@ -1297,8 +1301,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
           float y[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = sc[i >> 1][8 * (i & 1) + e];
-          u32x4 parts[NP];
-          split8<T, NP, false>(y, parts);
+          u32x4 parts[NW];
+          split8<T, NW, false>(y, parts);
           u32x4 v[NT];
 #pragma unroll
           for (int t2 = 0; t2 < NT; ++t2) {
@@ -1313,7 +1317,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
             v[t2] = __builtin_bit_cast(u32x4, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
           }
 #pragma unroll
-          for (int n = NP - 1; n >= 0; --n)
+          for (int n = NW - 1; n >= 0; --n)
 #pragma unroll
             for (int t2 = 0; t2 < NT; ++t2) o[t2] = mma32<CT>(v[t2], parts[n], o[t2]);
           if (i & 1) __builtin_amdgcn_sched_barrier(0);
@@ -1530,40 +1534,40 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
   }
 }
 
-template <int CT, int NP, int DT, int RT>
+template <int CT, int NQ, int NW, int DT, int RT>
 void launch_both(const PagedWork &w, hipStream_t stream) {
   if (w.whole) {
-    paged_attn_kernel<CT, NP, DT, RT, true><<<w.grid, 64 * paged_waves(DT, RT, true), 0, stream>>>(w);
+    paged_attn_kernel<CT, NQ, NW, DT, RT, true><<<w.grid, 64 * paged_waves(DT, RT, true), 0, stream>>>(w);
   } else {
-    paged_attn_kernel<CT, NP, DT, RT, false><<<w.grid, kThreads, 0, stream>>>(w);
+    paged_attn_kernel<CT, NQ, NW, DT, RT, false><<<w.grid, kThreads, 0, stream>>>(w);
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)std::min(w.rows, 16 * RT));
     paged_join_kernel<DT, RT><<<grid, kThreads, 0, stream>>>(w);
   }
 }
 
-template <int CT, int NP, int DT>
+template <int CT, int NQ, int NW, int DT>
 void launch_wide(const PagedWork &w, hipStream_t stream) {
-  paged_wide_kernel<CT, NP, DT><<<w.grid, kThreads, 0, stream>>>(w);
+  paged_wide_kernel<CT, NQ, NW, DT><<<w.grid, kThreads, 0, stream>>>(w);
   if (!w.whole) {
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)((std::min(w.rows, 32 * kWaves) + kWaves - 1) / kWaves));
     paged_join_rows_kernel<DT><<<grid, kThreads, 0, stream>>>(w);
   }
 }
 
-template <int CT, int NP>
+template <int CT, int NQ, int NW>
 hipError_t launch_passes(const PagedWork &w, int dt, int rt, hipStream_t stream) {
-  if (dt == 256) launch_both<CT, NP, 256, 1>(w, stream);
+  if (dt == 256) launch_both<CT, NQ, NW, 256, 1>(w, stream);
   else if (rt == kWideBlocks) {
     if constexpr (CT != KH_TYPE_F32) {
-      if (dt == 128) launch_wide<CT, NP, 128>(w, stream);
-      else launch_wide<CT, NP, 64>(w, stream);
+      if (dt == 128) launch_wide<CT, NQ, NW, 128>(w, stream);
+      else launch_wide<CT, NQ, NW, 64>(w, stream);
     }
   } else if (dt == 128) {
-    if (rt == 1) launch_both<CT, NP, 128, 1>(w, stream);
-    else launch_both<CT, NP, 128, 2>(w, stream);
+    if (rt == 1) launch_both<CT, NQ, NW, 128, 1>(w, stream);
+    else launch_both<CT, NQ, NW, 128, 2>(w, stream);
   } else {
-    if (rt == 1) launch_both<CT, NP, 64, 1>(w, stream);
-    else launch_both<CT, NP, 64, 2>(w, stream);
+    if (rt == 1) launch_both<CT, NQ, NW, 64, 1>(w, stream);
+    else launch_both<CT, NQ, NW, 64, 2>(w, stream);
   }
   return hipGetLastError();
 }

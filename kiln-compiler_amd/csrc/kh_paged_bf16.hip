@@ -4,7 +4,7 @@
 namespace kh {
 
 hipError_t launch_paged_bf16(const PagedWork &w, int dt, int rt, hipStream_t stream) {
-  return launch_passes<KH_TYPE_BF16, 1>(w, dt, rt, stream);
+  return launch_passes<KH_TYPE_BF16, 1, 1>(w, dt, rt, stream);
 }
 
 }  // namespace kh

@@ -4,7 +4,7 @@
 namespace kh {
 
 hipError_t launch_paged_f16x2(const PagedWork &w, int dt, int rt, hipStream_t stream) {
-  return launch_passes<KH_TYPE_F16, 2>(w, dt, rt, stream);
+  return launch_passes<KH_TYPE_F16, 2, 2>(w, dt, rt, stream);
 }
 
 }  // namespace kh

@@ -387,7 +387,9 @@ def tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents=None, *, s
 
     Drafted keys and values are rounded to the cache's type first, so a token
     is attended to as it will be once it is appended. fp32 activations keep
-    fp32's accuracy over bf16 and fp16 caches too. Up to 256 tokens and 4096
+    fp32's accuracy over bf16 and fp16 caches too; 16-bit ones are exact in
+    the scores, their softmax weights keep 16 bits (bf16) or 22 (fp16), sums
+    are fp32, and the result is rounded once. Up to 256 tokens and 4096
     sequences, dim a multiple of 8 up to 256, page_size a power of two from
     16 to 1024. A table entry outside the pool holds no tokens.
     """
