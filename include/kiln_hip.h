@@ -404,7 +404,8 @@ int kh_plan_destroy(kh_plan *plan);
  * the pages' columns, ascending, then -1.
  *
  * All pointers are device pointers on the device of `stream`; 16-byte aligned
- * rows of q, k, v, pages and out, 4-byte aligned else. The workspace may be
+ * rows of q, k, v, pages and out, 4-byte aligned else; the token strides k_n,
+ * v_n, kp_t and vp_t are not negative. The workspace may be
  * reused by any later call on the same stream. kh_paged_host runs the
  * operators' meaning on the CPU over host pointers (a test instrument, as
  * kh_plan_run_host).

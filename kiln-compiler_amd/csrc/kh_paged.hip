@@ -91,7 +91,7 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = "the pages' token stride is too large";
     return false;
   }
-  if (p.variant == KH_PAGED_ATTENTION && (std::abs(p.k_n) > most / 512 || std::abs(p.v_n) > most / 512)) {
+  if (p.variant == KH_PAGED_ATTENTION && (p.k_n > most / 512 || p.v_n > most / 512)) {
     err = "the new tokens' stride is too large";
     return false;
   }
@@ -113,8 +113,13 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     }
     return true;
   }
+  // (row offsets inside a tile are unsigned 32-bit counts)
   if (p.kp_t < 0 || p.vp_t < 0) {
     err = "negative token stride of the pages";
+    return false;
+  }
+  if (p.k_n < 0 || p.v_n < 0) {
+    err = "negative token stride of the new tokens";
     return false;
   }
   if (!aligned_strides({p.k_s, p.k_n, p.k_h, p.v_s, p.v_n, p.v_h, p.o_s, p.o_n, p.o_h}, ab)) {
