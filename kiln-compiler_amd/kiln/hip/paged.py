@@ -16,7 +16,10 @@ The first three are also what a model given to ``kiln.compile`` or
 ``torch.compile(backend=kiln.backend)`` may call: they are the operators
 ``torch.ops.kiln.paged_attention`` and ``select_pages``, which the frontend
 translates. The last two change their arguments, which a compiled graph does
-not; they are called between the calls of a compiled step.
+not; they are called between the calls of a compiled step. Where a tracer or a
+dispatch mode watches (``torch.jit.trace``, ``make_fx``, a flop counter), a call
+goes through its operator in ``torch.ops.kiln``, which those see;
+``torch.jit.trace`` does not keep the last two, which refuse it.
 
 Each call runs on the current stream of its tensors' device, allocates its
 result and workspace from torch's allocator (so it can be captured into a
@@ -365,8 +368,34 @@ def _(q, k_means, table, lengths, page_size, pages):
     return q.new_empty((q.shape[0], q.shape[1], k_means.shape[1], pages), dtype=torch.int32)
 
 
-def _tracing() -> bool:
-    return torch.compiler.is_compiling()
+@torch.library.custom_op("kiln::cache_append", mutates_args=("k_pages", "v_pages", "k_means"))
+def _cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                  lengths: torch.Tensor, rows: torch.Tensor | None, k_means: torch.Tensor | None) -> None:
+    with torch.no_grad():
+        run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means)
+
+
+@_cache_append.register_fake
+def _(k, v, k_pages, v_pages, table, lengths, rows, k_means):
+    pass
+
+
+@torch.library.custom_op("kiln::copy_pages", mutates_args=("pools",))
+def _copy_pages(pools: list[torch.Tensor], source: list[int], target: list[int]) -> None:
+    with torch.no_grad():
+        run_copy(pools, source, target)
+
+
+@_copy_pages.register_fake
+def _(pools, source, target):
+    pass
+
+
+def _watched() -> bool:
+    """Whether a compiler, a tracer or a dispatch mode is to see the call: not
+    what it allocates, but the operator."""
+    return (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
+            or torch._C._len_torch_dispatch_stack() > 0)
 
 
 # -- the public functions ------------------------------------------------------------------------------
@@ -394,7 +423,7 @@ def tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents=None, *, s
     16 to 1024. A table entry outside the pool holds no tokens.
     """
     scale = default_scale(scale, k_pages.shape[-1])
-    if _tracing():
+    if _watched():
         return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale)
     return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale, "tree_attention")
 
@@ -408,7 +437,7 @@ def selected_attention(q, k, v, k_pages, v_pages, table, lengths, selected, pare
     if selected is None:
         raise TypeError("selected must be a tensor (tree_attention reads every page)")
     scale = default_scale(scale, k_pages.shape[-1])
-    if _tracing():
+    if _watched():
         return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale)
     return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, "selected_attention")
 
@@ -421,15 +450,17 @@ def select_pages(q, k_means, table, lengths, *, page_size, pages):
     cached token is always among them. Ties go to the lower column. Returns
     int32 ``[sequences, tokens, kv_heads, pages]``: columns of ``table``,
     ascending, then -1."""
-    if _tracing():
-        return torch.ops.kiln.select_pages(q, k_means, table, lengths, page_size, pages)
+    if _watched():
+        return torch.ops.kiln.select_pages(q, k_means, table, lengths, int(page_size), int(pages))
     return run_select(q, k_means, table, lengths, int(page_size), int(pages))
 
 
 def _eager_only(what):
-    if _tracing():
+    if torch.compiler.is_compiling():
         raise NotImplementedError(f"{what} changes its arguments, which a compiled graph does not: call it between "
                                   f"the calls of the compiled step")
+    if torch._C._get_tracing_state() is not None:   # (torch.jit.trace drops an operator without results)
+        raise NotImplementedError(f"{what} changes its arguments, which torch.jit.trace does not record")
 
 
 def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=None):
@@ -446,6 +477,13 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
     ``lengths`` and ``rows`` hold for each. Tokens whose page the table does
     not name are dropped. No page may belong to two of the sequences."""
     _eager_only("cache_append")
+    if _watched():
+        _no_grad(k, v, k_pages, v_pages, k_means)
+        return torch.ops.kiln.cache_append(k, v, k_pages, v_pages, table, lengths, rows, k_means)
+    run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means)
+
+
+def run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means):
     try:
         key = _form(k, v, k_pages, v_pages, table, lengths, rows, k_means)
     except AttributeError:
@@ -455,7 +493,7 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
     if template is None:
         op = _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means)
         if isinstance(op, tuple):     # operands moved to where rows are in place
-            return cache_append(*op[:6], rows=op[6], k_means=k_means)
+            return run_append(*op, k_means)
         if op is None:
             return
         template = _forms[key] = bytes(op)
@@ -471,7 +509,7 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
     if (at[0] | at[1] | at[2] | at[3]) & 15:
         _rows_in_place(k_pages, "k_pages")
         _rows_in_place(v_pages, "v_pages")
-        return cache_append(_rows(k), _rows(v), k_pages, v_pages, table, lengths, rows=rows, k_means=k_means)
+        return run_append(_rows(k), _rows(v), k_pages, v_pages, table, lengths, rows, k_means)
     op.table, op.lengths = table.data_ptr(), lengths.data_ptr()
     if rows is not None:
         op.rows = rows.data_ptr()
@@ -577,6 +615,13 @@ def copy_pages(pools, source, target):
     distinct and none is a source, so no order of the copies matters."""
     _eager_only("copy_pages")
     pools = list(pools)
+    if _watched():
+        _no_grad(*pools)
+        return torch.ops.kiln.copy_pages(pools, [int(x) for x in source], [int(x) for x in target])
+    run_copy(pools, source, target)
+
+
+def run_copy(pools, source, target):
     if len(source) != len(target):
         raise ValueError(f"{len(source)} source pages, but {len(target)} target pages")
     try:

@@ -43,3 +43,110 @@ def test_negative_token_strides_are_refused(stride):
     launch.refs[at[0]].strides[at[1]] = -64
     handle = ctypes.c_void_p()
     assert kl.load().kh_plan_create(ctypes.byref(launch), 1, ctypes.byref(handle)) == kl.ERR_INVALID
+
+
+# -- tracers and dispatch modes ------------------------------------------------------------------
+
+
+def attention_calls():
+    p = ref.problem(gen(), lengths=(70, 17))
+    means = p["k_pages"].mean(2)
+    names = list(p)
+
+    def tree(*args):
+        return kiln.tree_attention(**dict(zip(names, args)))
+
+    def picked(*args):
+        p = dict(zip(names, args))
+        sel = kiln.select_pages(p["q"], args[-1], p["table"], p["lengths"], page_size=16, pages=2)
+        return kiln.selected_attention(**p, selected=sel)
+
+    return [(tree, tuple(p.values())), (picked, (*p.values(), means))]
+
+
+def append_call():
+    k_pages, v_pages = (torch.randn(9, 3, 16, 8, generator=gen(s)) for s in (1, 2))
+    table, lengths = torch.tensor([[4, 2], [0, 7]], dtype=torch.int32), torch.tensor([14, 3], dtype=torch.int32)
+    rows = torch.tensor([[0, 2, 4, 6], [9, 1, -1, 3]], dtype=torch.int32)
+    k, v = (torch.randn(2, 11, 3, 8, generator=gen(s)) for s in (3, 4))
+
+    def append(k, v, k_pages, v_pages, means):
+        kiln.cache_append(k, v, k_pages, v_pages, table, lengths, rows=rows, k_means=means)
+        kiln.copy_pages([k_pages, v_pages], [4, 0], [1, 3])
+        return k_pages + v_pages
+
+    return append, (k, v, k_pages, v_pages, k_pages.mean(2))
+
+
+@pytest.mark.parametrize("how", ["jit", "make_fx"])
+@pytest.mark.parametrize("which", [0, 1], ids=["tree", "picked"])
+def test_traces_hold_the_operators(how, which):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    fn, args = attention_calls()[which]
+    traced = torch.jit.trace(fn, args) if how == "jit" else make_fx(fn)(*args)
+    assert "paged_attention" in str(traced.graph)
+    other = [t.clone() for t in args]
+    other[0].mul_(-0.7)
+    other[6].sub_(9)
+    assert torch.equal(traced(*other), fn(*other))
+
+
+def test_traces_hold_what_changes_the_cache():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    fn, args = append_call()
+    traced = make_fx(fn)(*[t.clone() for t in args])
+    assert "cache_append" in str(traced.graph) and "copy_pages" in str(traced.graph)
+    mine, want = [t.clone() for t in args], [t.clone() for t in args]
+    for x in (mine, want):
+        x[0].mul_(-2)
+    out = traced(*mine)
+    assert torch.equal(out, fn(*want))
+    assert all(torch.equal(a, b) for a, b in zip(mine, want)) and not torch.equal(mine[2], args[2])
+
+
+def test_a_trace_that_would_drop_them_is_refused():
+    fn, args = append_call()
+    for call in (fn, lambda pool: kiln.copy_pages([pool], [0], [1]) or pool):
+        before = [t.clone() for t in args]
+        with pytest.raises(NotImplementedError, match="trace"):
+            torch.jit.trace(call, args if call is fn else args[2:3])
+        assert all(torch.equal(a, b) for a, b in zip(args, before))
+
+
+def test_dispatch_modes_see_the_operators():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Names(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    for fn, args in attention_calls():
+        want = fn(*args)
+        with Names() as mode:
+            got = fn(*args)
+        assert torch.equal(got, want) and "kiln.paged_attention.default" in mode.seen
+    fn, args = append_call()
+    mine = [t.clone() for t in args]
+    want = fn(*args)
+    with Names() as mode:
+        got = fn(*mine)
+    assert torch.equal(got, want) and {"kiln.cache_append.default", "kiln.copy_pages.default"} <= set(mode.seen)
+    assert all(torch.equal(a, b) for a, b in zip(mine, args))
+
+
+def test_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode() as mode:
+        for fn, args in attention_calls():
+            out = fn(*[mode.from_tensor(t) for t in args] if not isinstance(args[0], torch._subclasses.FakeTensor) else args)
+            assert out.shape == args[0].shape and isinstance(out, torch._subclasses.FakeTensor)
+        fn, args = append_call()
+        fn(*args)
