@@ -34,6 +34,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from kiln.hip import lib as kl
 from kiln.hip.interpret import interpreting
@@ -66,6 +67,13 @@ def _int32(t, name, rank, shape):
 def _no_grad(*tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError("the paged cache's operators have no backward pass: call them under torch.no_grad()")
+
+
+def _no_tangent(*tensors):
+    """Where a level of forward mode is open (no_grad does not close it)."""
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the paged cache's operators have no forward-mode derivative: pass the primal tensors "
+                                  "(torch.autograd.forward_ad.unpack_dual)")
 
 
 def _one_device(first, *others):
@@ -391,11 +399,18 @@ def _(pools, source, target):
     pass
 
 
-def _watched() -> bool:
+def _watched(*tensors) -> bool:
     """Whether a compiler, a tracer or a dispatch mode is to see the call: not
-    what it allocates, but the operator."""
-    return (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
-            or torch._C._len_torch_dispatch_stack() > 0)
+    what it allocates, but the operator. ``tensors``: those that a derivative
+    could be asked of."""
+    if torch.compiler.is_compiling():
+        return True
+    if forward_ad._current_level >= 0:
+        _no_tangent(*tensors)
+    if torch._C._get_tracing_state() is None and not torch._C._len_torch_dispatch_stack():
+        return False
+    _no_grad(*tensors)
+    return True
 
 
 # -- the public functions ------------------------------------------------------------------------------
@@ -423,7 +438,7 @@ def tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents=None, *, s
     16 to 1024. A table entry outside the pool holds no tokens.
     """
     scale = default_scale(scale, k_pages.shape[-1])
-    if _watched():
+    if _watched(q, k, v, k_pages, v_pages):
         return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale)
     return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale, "tree_attention")
 
@@ -437,7 +452,7 @@ def selected_attention(q, k, v, k_pages, v_pages, table, lengths, selected, pare
     if selected is None:
         raise TypeError("selected must be a tensor (tree_attention reads every page)")
     scale = default_scale(scale, k_pages.shape[-1])
-    if _watched():
+    if _watched(q, k, v, k_pages, v_pages):
         return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale)
     return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, "selected_attention")
 
@@ -450,7 +465,7 @@ def select_pages(q, k_means, table, lengths, *, page_size, pages):
     cached token is always among them. Ties go to the lower column. Returns
     int32 ``[sequences, tokens, kv_heads, pages]``: columns of ``table``,
     ascending, then -1."""
-    if _watched():
+    if _watched(q, k_means):
         return torch.ops.kiln.select_pages(q, k_means, table, lengths, int(page_size), int(pages))
     return run_select(q, k_means, table, lengths, int(page_size), int(pages))
 
@@ -477,8 +492,7 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
     ``lengths`` and ``rows`` hold for each. Tokens whose page the table does
     not name are dropped. No page may belong to two of the sequences."""
     _eager_only("cache_append")
-    if _watched():
-        _no_grad(k, v, k_pages, v_pages, k_means)
+    if _watched(k, v, k_pages, v_pages, k_means):
         return torch.ops.kiln.cache_append(k, v, k_pages, v_pages, table, lengths, rows, k_means)
     run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means)
 
@@ -615,8 +629,7 @@ def copy_pages(pools, source, target):
     distinct and none is a source, so no order of the copies matters."""
     _eager_only("copy_pages")
     pools = list(pools)
-    if _watched():
-        _no_grad(*pools)
+    if _watched(*pools):
         return torch.ops.kiln.copy_pages(pools, [int(x) for x in source], [int(x) for x in target])
     run_copy(pools, source, target)
 

@@ -150,3 +150,48 @@ def test_fake_tensors():
             assert out.shape == args[0].shape and isinstance(out, torch._subclasses.FakeTensor)
         fn, args = append_call()
         fn(*args)
+
+
+# -- autograd -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_forward_mode_is_refused(no_grad):
+    """A dual tensor's tangent would be lost; tensors without one go through."""
+    import torch.autograd.forward_ad as fw
+
+    p = ref.problem(gen(), lengths=(70, 17))
+    means = p["k_pages"].mean(2)
+
+    def attend(p):
+        return kiln.tree_attention(**p)
+
+    def pick(q, means):
+        return kiln.select_pages(q, means, p["table"], p["lengths"], page_size=16, pages=2)
+
+    def append(k, v, k_pages, v_pages, m):
+        return kiln.cache_append(k, v, k_pages, v_pages, p["table"], p["lengths"], k_means=m)
+
+    def copy(pool):
+        return kiln.copy_pages([pool], [0], [1])
+
+    want, picked = attend(p), pick(p["q"], means)
+    with fw.dual_level(), torch.set_grad_enabled(not no_grad):
+        def dual(t):
+            return fw.make_dual(t.clone(), torch.ones_like(t))
+
+        for name in ("q", "k", "v", "k_pages", "v_pages"):
+            with pytest.raises(NotImplementedError, match="forward"):
+                attend(dict(p, **{name: dual(p[name])}))
+        for args in ((dual(p["q"]), means), (p["q"], dual(means))):
+            with pytest.raises(NotImplementedError, match="forward"):
+                pick(*args)
+        args = [p["k"], p["v"], p["k_pages"], p["v_pages"], means]
+        for i in range(5):
+            mine = [t.clone() for t in args]
+            mine[i] = dual(args[i])
+            with pytest.raises(NotImplementedError, match="forward"):
+                append(*mine)
+        with pytest.raises(NotImplementedError, match="forward"):
+            copy(dual(means))
+        assert torch.equal(attend(p), want) and torch.equal(pick(p["q"], means), picked)
