@@ -23,7 +23,8 @@ goes through its operator in ``torch.ops.kiln``, which those see;
 
 Each call runs on the current stream of its tensors' device, allocates its
 result and workspace from torch's allocator (so it can be captured into a
-graph) and reads or changes nothing else. There is no CPU path; with
+graph) and reads or changes nothing else; what it changes counts as changed in
+place for autograd. There is no CPU path; with
 ``KILN_HIP_INTERPRET=1`` (tests) the library's CPU meaning runs instead.
 """
 
@@ -35,6 +36,7 @@ import math
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from kiln.hip import lib as kl
 from kiln.hip.interpret import interpreting
@@ -536,6 +538,7 @@ def run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means):
         rc = _on_device(device, lib.kh_cache_append, ctypes.byref(op))
     if rc:
         kl.check(rc, "cache_append")
+    increment_version((k_pages, v_pages) if k_means is None else (k_pages, v_pages, k_means))
 
 
 def _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means):
@@ -664,8 +667,9 @@ def run_copy(pools, source, target):
     src, dst = _page_list(source, "source"), _page_list(target, "target")
     lib, device = kl.load(), pools[0].device
     if device.type != "cuda":
-        kl.check(lib.kh_cache_copy_host(descs, len(pools), pages, src, dst, len(src)), "copy_pages")
-        return
-    rc = _on_device(device, lib.kh_cache_copy, descs, len(pools), pages, src, dst, len(src))
+        rc = lib.kh_cache_copy_host(descs, len(pools), pages, src, dst, len(src))
+    else:
+        rc = _on_device(device, lib.kh_cache_copy, descs, len(pools), pages, src, dst, len(src))
     if rc:
         kl.check(rc, "copy_pages")
+    increment_version(pools)

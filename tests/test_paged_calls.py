@@ -195,3 +195,39 @@ def test_forward_mode_is_refused(no_grad):
         with pytest.raises(NotImplementedError, match="forward"):
             copy(dual(means))
         assert torch.equal(attend(p), want) and torch.equal(pick(p["q"], means), picked)
+
+
+@pytest.mark.parametrize("seen", [False, True], ids=["alone", "dispatch mode"])
+def test_what_changed_counts_as_changed(seen):
+    """Values saved for a backward pass and changed before it: torch's error, no gradient of other values."""
+    from torch.utils.flop_counter import FlopCounterMode
+
+    fn, (k, v, k_pages, v_pages, means) = append_call()
+    table, lengths = torch.tensor([[4, 2], [0, 7]], dtype=torch.int32), torch.tensor([14, 3], dtype=torch.int32)
+
+    def run(call):
+        if not seen:
+            return call()
+        with FlopCounterMode(display=False):
+            return call()
+
+    for call, changed in ((lambda: kiln.cache_append(k, v, k_pages, v_pages, table, lengths, k_means=means), (k_pages, v_pages, means)),
+                          (lambda: kiln.copy_pages([k_pages, v_pages], [4], [1]), (k_pages, v_pages))):
+        for t in changed:
+            x = torch.ones((), requires_grad=True)
+            y = (x * t.view(-1)[5:]).sum()      # saves a view
+            before = [t._version for t in changed]
+            run(call)
+            assert all(t._version > n for t, n in zip(changed, before))
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+    before = k_pages._version, v_pages._version
+    for refused in (lambda: kiln.copy_pages([k_pages, v_pages], [4], [4]), lambda: kiln.copy_pages([k_pages, v_pages], [], [])):
+        try:
+            refused()
+        except ValueError:
+            pass
+    assert (k_pages._version, v_pages._version) == before
+    with torch.inference_mode():                # (such tensors count no versions)
+        kiln.copy_pages([k_pages.clone()], [4], [1])
+        kiln.cache_append(k, v, k_pages.clone(), v_pages.clone(), table, lengths)
