@@ -184,42 +184,40 @@ class PagedCache:
 
         def take():
             if not self._free:
-                for page in taken:
-                    heapq.heappush(self._free, page)
                 raise MemoryError(f"the cache has no free page left ({self.pages} pages)")
             taken.append(heapq.heappop(self._free))
             return taken[-1]
 
-        for s, n in zip(seqs, counts):
-            have = list(self._pages[s])
-            at = self._length[s] // self.page_size
-            if n and at < len(have):           # the last page has room (only it can: truncate drops those behind)
-                old = have[at]
-                if refs.setdefault(old, self._refs[old]) > 1:
-                    refs[old] -= 1
-                    have[at] = take()
-                    source.append(old)
-                    target.append(have[at])
-            while len(have) * self.page_size < self._length[s] + n:
-                have.append(take())
-            plans.append(have)
-        table = torch.full((len(seqs), max(len(p) for p in plans)), -1, dtype=torch.int32)
-        for i, p in enumerate(plans):
-            table[i, :len(p)] = torch.tensor(p, dtype=torch.int32)
-        lengths = torch.tensor([self._length[s] for s in seqs], dtype=torch.int32)
-        path = None
-        if rows is not None:
-            path = torch.full((len(seqs), max(counts)), -1, dtype=torch.int32)
-            for i, r in enumerate(rows):
-                if r:
-                    path[i, :len(r)] = torch.tensor(r, dtype=torch.int32)
-            path = self._upload(path)
         try:
+            for s, n in zip(seqs, counts):
+                have = list(self._pages[s])
+                at = self._length[s] // self.page_size
+                if n and at < len(have):           # the last page has room (only it can: truncate drops those behind)
+                    old = have[at]
+                    if refs.setdefault(old, self._refs[old]) > 1:
+                        refs[old] -= 1
+                        have[at] = take()
+                        source.append(old)
+                        target.append(have[at])
+                while len(have) * self.page_size < self._length[s] + n:
+                    have.append(take())
+                plans.append(have)
+            table = torch.full((len(seqs), max(len(p) for p in plans)), -1, dtype=torch.int32)
+            for i, p in enumerate(plans):
+                table[i, :len(p)] = torch.tensor(p, dtype=torch.int32)
+            lengths = torch.tensor([self._length[s] for s in seqs], dtype=torch.int32)
+            path = None
+            if rows is not None:
+                path = torch.full((len(seqs), max(counts)), -1, dtype=torch.int32)
+                for i, r in enumerate(rows):
+                    if r:
+                        path[i, :len(r)] = torch.tensor(r, dtype=torch.int32)
+                path = self._upload(path)
             if source:
                 paged.copy_pages(self._pools(), source, target)
             paged.cache_append(k, v, self.k, self.v, self._upload(table), self._upload(lengths), rows=path,
                                k_means=self.means)
-        except Exception:
+        except BaseException:
             for page in taken:                 # nothing names them yet
                 heapq.heappush(self._free, page)
             raise

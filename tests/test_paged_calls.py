@@ -231,3 +231,34 @@ def test_what_changed_counts_as_changed(seen):
     with torch.inference_mode():                # (such tensors count no versions)
         kiln.copy_pages([k_pages.clone()], [4], [1])
         kiln.cache_append(k, v, k_pages.clone(), v_pages.clone(), table, lengths)
+
+
+# -- kiln.PagedCache ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("upload", [0, 1, 2])
+@pytest.mark.parametrize("error", [RuntimeError, MemoryError, KeyboardInterrupt])
+def test_an_append_that_fails_on_its_way_gives_its_pages_back(monkeypatch, upload, error):
+    """The accepted rows, the table or the lengths do not reach the device."""
+    cache = kiln.PagedCache(1, 6, 16, 2, 8, dtype=torch.float32)
+    a = cache.open()
+    k = torch.randn(1, 1, 20, 2, 8, generator=gen())
+    cache.append([a], k, k)
+    b, = cache.fork(a)
+    before = cache.k.clone(), list(cache._refs), sorted(cache._free), cache.pages_of(b)
+    done = []
+
+    def fails(t):
+        done.append(t)
+        if len(done) > upload:
+            raise error("no more")
+        return t
+
+    with monkeypatch.context() as m:
+        m.setattr(cache, "_upload", fails)
+        with pytest.raises(error):
+            cache.append([b], k, k, rows=[list(range(20))])
+    assert sorted(cache._free) == before[2] and cache._refs == before[1] and cache.pages_of(b) == before[3]
+    assert cache.length(b) == 20 and torch.equal(cache.k[:, list(before[3])], before[0][:, list(before[3])])
+    cache.append([b], k, k)
+    assert cache.length(b) == 40 and cache.free_pages == 2
