@@ -203,20 +203,25 @@ def _form(*tensors):
     return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
 
 
-# form of a call -> (its descriptor without addresses, workspace bytes): the
-# checks and the descriptor are worked out once per form. Forms are shapes,
-# strides and types alone; a program has few, and the oldest go first.
+# (operator, form of a call) -> its descriptor without addresses, and what
+# belongs to it: the checks and the descriptor are worked out once per form.
+# Forms are shapes, strides and types alone; a program has few, and the oldest
+# go first.
 _forms = {}
 MOST_FORMS = 4096
+
+
+def _keep(key, found):
+    while len(_forms) >= MOST_FORMS:
+        _forms.pop(next(iter(_forms)), None)
+    _forms[key] = found
+    return found
 
 
 def _remember(key, op):
     size = ctypes.c_size_t()
     kl.check(kl.load().kh_paged_workspace_bytes(ctypes.byref(op), ctypes.byref(size)), "paged")
-    if len(_forms) >= MOST_FORMS:
-        _forms.pop(next(iter(_forms)))
-    _forms[key] = found = (bytes(op), size.value)
-    return found
+    return _keep(key, (bytes(op), size.value))
 
 
 def _launch(op: kl.Paged, size: int, device, what: str):
@@ -258,7 +263,7 @@ def _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected
 
 def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what):
     try:
-        key = (q.shape, q.dtype, q.stride(), q.get_device(), k.shape, k.dtype, k.stride(), k.get_device(),
+        key = ("attention", q.shape, q.dtype, q.stride(), q.get_device(), k.shape, k.dtype, k.stride(), k.get_device(),
                v.shape, v.dtype, v.stride(), v.get_device(), k_pages.shape, k_pages.dtype, k_pages.stride(),
                k_pages.get_device(), v_pages.shape, v_pages.dtype, v_pages.stride(), v_pages.get_device(),
                table.shape, table.dtype, table.stride(), table.get_device(), lengths.shape, lengths.dtype,
@@ -308,7 +313,7 @@ def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, 
 
 def run_select(q, k_means, table, lengths, page_size, pages):
     try:
-        key = (_form(q, k_means, table, lengths), page_size, pages)
+        key = ("select", _form(q, k_means, table, lengths), page_size, pages)
     except AttributeError:
         check_select(q, k_means, table, lengths, page_size, pages)
         raise
@@ -501,7 +506,7 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
 
 def run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means):
     try:
-        key = _form(k, v, k_pages, v_pages, table, lengths, rows, k_means)
+        key = ("append", _form(k, v, k_pages, v_pages, table, lengths, rows, k_means))
     except AttributeError:
         _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means)
         raise
@@ -512,9 +517,7 @@ def run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means):
             return run_append(*op, k_means)
         if op is None:
             return
-        template = _forms[key] = bytes(op)
-        while len(_forms) > MOST_FORMS:
-            _forms.pop(next(iter(_forms)))
+        template = _keep(key, bytes(op))
     elif k.device.type != "cuda" and not interpreting():
         _one_device(k)
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad
@@ -641,7 +644,7 @@ def run_copy(pools, source, target):
     if len(source) != len(target):
         raise ValueError(f"{len(source)} source pages, but {len(target)} target pages")
     try:
-        key = _form(*pools)
+        key = ("copy", _form(*pools))
     except AttributeError:
         raise TypeError("a pool is a tensor of pages") from None
     found = _forms.get(key)
@@ -651,9 +654,7 @@ def run_copy(pools, source, target):
             return
         _one_device(*pools)
         _ready(pools[0].device)
-        _forms[key] = found
-        while len(_forms) > MOST_FORMS:
-            _forms.pop(next(iter(_forms)))
+        _keep(key, found)
     elif pools[0].device.type != "cuda" and not interpreting():
         _one_device(*pools)
     if len(source) == 0:

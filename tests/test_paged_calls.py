@@ -262,3 +262,21 @@ def test_an_append_that_fails_on_its_way_gives_its_pages_back(monkeypatch, uploa
     assert cache.length(b) == 20 and torch.equal(cache.k[:, list(before[3])], before[0][:, list(before[3])])
     cache.append([b], k, k)
     assert cache.length(b) == 40 and cache.free_pages == 2
+
+
+# -- calls whose forms are kept ---------------------------------------------------------------------
+
+
+def test_forms_of_different_operators():
+    """Tensors of the same shapes, strides and types in another operator's places."""
+    k, pages, means = torch.randn(9, 5, 9, 8, generator=gen()), torch.zeros(9, 9, 16, 8), torch.zeros(9, 9, 8)
+    table, lengths = torch.arange(9, dtype=torch.int32).view(9, 1), torch.zeros(9, dtype=torch.int32)
+    rows = torch.zeros(9, 4, dtype=torch.int32)
+    args = (k, k.clone(), pages, pages.clone(), table, lengths)
+    kiln.cache_append(*args, rows=rows, k_means=means)
+    assert means.abs().sum() > 0
+    with pytest.raises(TypeError, match="pool"):      # lengths are no pool: as without the append before
+        kiln.copy_pages([*args, rows, means], [0], [1])
+    pools = [*args[:5], rows, means]
+    kiln.copy_pages(pools, [0], [1])
+    assert all(torch.equal(t[1], t[0]) for t in pools)
