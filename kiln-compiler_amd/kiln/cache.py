@@ -13,7 +13,9 @@ copied when one of them writes to it. The device work - appending, copying
 pages - is ``kiln.cache_append`` and ``kiln.copy_pages`` on the current
 stream; a caller that works on several streams orders them itself, as for any
 tensor. Calls that need more pages than are free raise MemoryError and change
-nothing. Not thread-safe.
+nothing. A graph being captured would replay device work without its
+book-keeping: ``batch``, ``append`` and ``compact`` refuse that (the operators
+on tables made before can be captured). Not thread-safe.
 """
 
 from __future__ import annotations
@@ -123,12 +125,18 @@ class PagedCache:
         del self._pages[seq][keep:]
         self._length[seq] = length
 
+    def _not_captured(self, what):
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"PagedCache.{what} while a graph is captured: its replay would not repeat the "
+                               f"book-keeping; call it before, or between replays")
+
     # -- the device's view ------------------------------------------------------------------
 
     def batch(self, seqs, columns=None):
         """(table, lengths) of the sequences, as the operators take them: int32
         ``[sequences, columns]`` (as many as the longest needs, or ``columns``)
         and ``[sequences]``, uploaded without waiting for the device."""
+        self._not_captured("batch")
         rows = [self._pages[self._known(s)] for s in seqs]
         need = max([1] + [len(r) for r in rows])
         columns = need if columns is None else columns
@@ -156,6 +164,7 @@ class PagedCache:
         i the tokens ``rows[i]`` (a list of ints: a drafted tree's accepted
         path). Pages are taken as needed; a page that other sequences have too
         is copied before it is written to."""
+        self._not_captured("append")
         seqs = list(seqs)
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence is named twice")
@@ -234,6 +243,7 @@ class PagedCache:
     def compact(self) -> int:
         """Move the pages in use to the front of the pool; returns how many
         there are. Tables made before by ``batch`` name the old places."""
+        self._not_captured("compact")
         used = self.pages - len(self._free)
         holes = sorted(p for p in self._free if p < used)
         moved = [p for p in range(used, self.pages) if self._refs[p]]

@@ -280,3 +280,22 @@ def test_forms_of_different_operators():
     pools = [*args[:5], rows, means]
     kiln.copy_pages(pools, [0], [1])
     assert all(torch.equal(t[1], t[0]) for t in pools)
+
+
+def test_the_cache_refuses_to_be_captured(monkeypatch):
+    cache = kiln.PagedCache(1, 6, 16, 2, 8, dtype=torch.float32)
+    a = cache.open()
+    k = torch.randn(1, 1, 20, 2, 8, generator=gen())
+    cache.append([a], k, k)
+    b = cache.open()
+    cache.append([b], k, k)
+    cache.free(a)
+    before = cache.k.clone(), cache.pages_of(b), cache.free_pages
+    with monkeypatch.context() as m:
+        m.setattr(cache, "device", torch.device("cuda"))
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        for call in (lambda: cache.append([b], k, k), lambda: cache.batch([b]), cache.compact):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    assert torch.equal(cache.k, before[0]) and cache.pages_of(b) == before[1] and cache.free_pages == before[2]
+    assert cache.compact() == 2
