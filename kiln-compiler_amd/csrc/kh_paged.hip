@@ -87,6 +87,10 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = "more keys and query rows than 32-bit counts hold";
     return false;
   }
+  if (p.variant == KH_PAGED_ATTENTION && paged_threads(p) > (int64_t)std::numeric_limits<uint32_t>::max()) {
+    err = "more sequences, heads and tokens than one launch has room for (2^32 work items)";
+    return false;
+  }
   if (p.variant == KH_PAGED_ATTENTION && (p.kp_t > most / 8 / p.page_size - p.dim || p.vp_t > most / 8 / p.page_size - p.dim)) {
     err = "the pages' token stride is too large";
     return false;

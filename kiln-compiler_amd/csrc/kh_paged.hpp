@@ -16,6 +16,8 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported);
 bool check_paged_pointers(const kh_paged &p, std::string &err);
 
 size_t paged_workspace_floats(const kh_paged &p);
+// Work items of the largest of an attention's launches.
+int64_t paged_threads(const kh_paged &p);
 hipError_t launch_paged(const kh_paged &p, float *workspace, hipStream_t stream);
 size_t select_workspace_floats(const kh_paged &p);
 hipError_t launch_select(const kh_paged &p, float *workspace, hipStream_t stream);

@@ -73,6 +73,14 @@ size_t paged_workspace_floats(const kh_paged &p) {
   return 2 * (size_t)w.grid * 16 * row_blocks(p) * (padded_dim(p.dim) + 2);
 }
 
+int64_t paged_threads(const kh_paged &p) {
+  if (p.batch == 0 || p.draft == 0) return 0;
+  const PagedWork w = work_of(p);
+  const int rt = row_blocks(p);
+  const int waves = rt == kWideBlocks ? kPagedWaves : paged_waves(padded_dim(p.dim), rt, w.whole);
+  return (int64_t)p.batch * w.items * 64 * (w.whole ? waves : kPagedWaves);   // (ranges: the join)
+}
+
 hipError_t launch_paged(const kh_paged &p, float *workspace, hipStream_t stream) {
   if (p.batch == 0 || p.draft == 0) return hipSuccess;
   PagedWork w = work_of(p);

@@ -299,3 +299,19 @@ def test_the_cache_refuses_to_be_captured(monkeypatch):
                 call()
     assert torch.equal(cache.k, before[0]) and cache.pages_of(b) == before[1] and cache.free_pages == before[2]
     assert cache.compact() == 2
+
+
+def test_more_items_than_a_launch_holds_are_refused():
+    """A workgroup of eight waves per (sequence, head, token): 2^32 work items are one too many."""
+    size = ctypes.c_size_t()
+    for draft, batch, rc in ((15, 4096, kl.OK), (16, 4096, kl.ERR_UNSUPPORTED), (16, 4095, kl.OK)):
+        op = kl.Paged(kl.PAGED_ATTENTION, batch, draft, 128, 128, 8, 16, 4, 2, 2, kl.TYPE_BF16, kl.TYPE_BF16, 0, 1.0)
+        assert kl.load().kh_paged_workspace_bytes(op, size) == rc
+    for draft, rc in ((31, kl.OK), (32, kl.ERR_UNSUPPORTED)):     # (heads of 256: four waves)
+        op = kl.Paged(kl.PAGED_ATTENTION, 4096, draft, 128, 128, 256, 16, 4, 2, 2, kl.TYPE_BF16, kl.TYPE_BF16, 0, 1.0)
+        assert kl.load().kh_paged_workspace_bytes(op, size) == rc
+    p = ref.problem(gen(), batch=4096, draft=16, heads=128, kv=128, dim=8, lengths=[0] * 4096, spare=4, columns=2, tree=False,
+                    cache=torch.bfloat16, act=torch.bfloat16)
+    p["q"], p["k"], p["v"] = (t[:, :, :1, :].expand(4096, 16, 128, 8) for t in (p["q"], p["k"], p["v"]))
+    with pytest.raises(NotImplementedError, match="launch"):
+        kiln.selected_attention(**p, selected=torch.zeros(1, 1, 1, 2, dtype=torch.int32).expand(4096, 16, 128, 2))
