@@ -57,6 +57,7 @@ class PagedCache:
         self.page_size = page_size
         self.pages = pages
         self.k = torch.zeros((layers, pages, kv_heads, page_size, dim), dtype=dtype, device=self.device)
+        self.device = self.k.device              # ("cuda" alone follows the current device)
         self.v = torch.zeros_like(self.k)
         self.means = torch.zeros((layers, pages, kv_heads, dim), dtype=torch.float32, device=self.device) if means else None
         self._free = list(range(pages))          # a heap: the lowest free page is taken first

@@ -34,3 +34,11 @@ def test_the_cache_refuses_to_be_captured():
         assert torch.equal(out, want)
     cache.append([a], k, k)
     assert cache.length(a) == 40
+
+
+def test_a_device_without_a_number_is_the_current_one():
+    cache = kiln.PagedCache(1, 6, 16, 2, 8, device="cuda")
+    assert cache.device == cache.k.device == torch.device("cuda", torch.cuda.current_device())
+    a = cache.open()
+    table, lengths = cache.batch([a])
+    assert table.device == lengths.device == cache.device
