@@ -392,6 +392,8 @@ class _Translator:
             dtypes = _CACHE_TYPES if self.with_cache else (torch.float32,)
             if tuple(out.shape) != static_shape(node, dtypes):
                 raise AssertionError(f"{node.name}: Kiln shape {out.shape} != {static_shape(node, dtypes)}")
+            if out.type.dtype != _CACHE_TYPES[node.meta["val"].dtype]:   # e.g. a sum into another type
+                raise Unsupported(f"{node.name}: only float32 is supported (got {node.meta['val'].dtype})")
         return out
 
     def check_types(self, node):

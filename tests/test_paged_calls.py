@@ -315,3 +315,27 @@ def test_more_items_than_a_launch_holds_are_refused():
     p["q"], p["k"], p["v"] = (t[:, :, :1, :].expand(4096, 16, 128, 8) for t in (p["q"], p["k"], p["v"]))
     with pytest.raises(NotImplementedError, match="launch"):
         kiln.selected_attention(**p, selected=torch.zeros(1, 1, 1, 2, dtype=torch.int32).expand(4096, 16, 128, 2))
+
+
+# -- models ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("change", [lambda y: y.sum(-1, dtype=torch.float16), lambda y: y.mean(-1, dtype=torch.bfloat16),
+                                    lambda y: y.half(), lambda y: y.sum(-1, dtype=torch.int32)])
+def test_models_that_change_the_type_are_refused(change):
+    """Beside a cache too: everything but the cache's own operands is float32."""
+    from kiln.frontend.fx_import import Unsupported, import_exported
+
+    p = ref.problem(gen(), lengths=(40, 17), dim=16)
+
+    class Model(torch.nn.Module):
+        def forward(self, q, k_pages, table, lengths):
+            return change(kiln.tree_attention(q, q[:, :, :2], q[:, :, :2], k_pages, k_pages, table, lengths))
+
+    class Plain(torch.nn.Module):
+        def forward(self, q):
+            return change(q)
+
+    for model, args in ((Model(), (p["q"], p["k_pages"], p["table"], p["lengths"])), (Plain(), (p["q"],))):
+        with pytest.raises(Unsupported):
+            import_exported(torch.export.export(model.eval(), args).run_decompositions())
