@@ -36,10 +36,13 @@ import math
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.graph import increment_version
 
 from kiln.hip import lib as kl
 from kiln.hip.interpret import interpreting
+
+# asked at every call
+_is_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+_increment_version = torch._C._increment_version
 
 TYPES = {torch.float32: kl.TYPE_F32, torch.bfloat16: kl.TYPE_BF16, torch.float16: kl.TYPE_F16}
 
@@ -414,7 +417,7 @@ def _watched(*tensors) -> bool:
         return True
     if forward_ad._current_level >= 0:
         _no_tangent(*tensors)
-    if torch._C._get_tracing_state() is None and not torch._C._len_torch_dispatch_stack():
+    if not (_dispatch_modes() or _is_tracing()):
         return False
     _no_grad(*tensors)
     return True
@@ -477,11 +480,12 @@ def select_pages(q, k_means, table, lengths, *, page_size, pages):
     return run_select(q, k_means, table, lengths, int(page_size), int(pages))
 
 
-def _eager_only(what):
+def _recorded(what):
+    """Refuse what does not keep a call that changes its arguments."""
     if torch.compiler.is_compiling():
         raise NotImplementedError(f"{what} changes its arguments, which a compiled graph does not: call it between "
                                   f"the calls of the compiled step")
-    if torch._C._get_tracing_state() is not None:   # (torch.jit.trace drops an operator without results)
+    if _is_tracing():   # (torch.jit.trace drops an operator without results)
         raise NotImplementedError(f"{what} changes its arguments, which torch.jit.trace does not record")
 
 
@@ -498,8 +502,8 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, *, rows=None, k_means=N
     pages (5) and ``k_means`` (4), all layers are written at once; ``table``,
     ``lengths`` and ``rows`` hold for each. Tokens whose page the table does
     not name are dropped. No page may belong to two of the sequences."""
-    _eager_only("cache_append")
     if _watched(k, v, k_pages, v_pages, k_means):
+        _recorded("cache_append")
         return torch.ops.kiln.cache_append(k, v, k_pages, v_pages, table, lengths, rows, k_means)
     run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means)
 
@@ -541,7 +545,7 @@ def run_append(k, v, k_pages, v_pages, table, lengths, rows, k_means):
         rc = _on_device(device, lib.kh_cache_append, ctypes.byref(op))
     if rc:
         kl.check(rc, "cache_append")
-    increment_version((k_pages, v_pages) if k_means is None else (k_pages, v_pages, k_means))
+    _increment_version((k_pages, v_pages) if k_means is None else (k_pages, v_pages, k_means))
 
 
 def _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means):
@@ -633,9 +637,9 @@ def copy_pages(pools, source, target):
     ``means.unsqueeze(-2)``), ``[layers, pages, ...]``, contiguous within a
     layer. ``source`` and ``target`` are sequences of ints; targets are
     distinct and none is a source, so no order of the copies matters."""
-    _eager_only("copy_pages")
     pools = list(pools)
     if _watched(*pools):
+        _recorded("copy_pages")
         return torch.ops.kiln.copy_pages(pools, [int(x) for x in source], [int(x) for x in target])
     run_copy(pools, source, target)
 
@@ -673,4 +677,4 @@ def run_copy(pools, source, target):
         rc = _on_device(device, lib.kh_cache_copy, descs, len(pools), pages, src, dst, len(src))
     if rc:
         kl.check(rc, "copy_pages")
-    increment_version(pools)
+    _increment_version(pools)
