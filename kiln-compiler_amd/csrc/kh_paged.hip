@@ -72,7 +72,8 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
   }
   const int64_t most = std::numeric_limits<int32_t>::max();
   const int64_t keys = (int64_t)p.width * p.page_size;
-  if (keys > most || (keys / 32 + 9) * std::max(p.batch, 1) > most || (int64_t)p.top * p.page_size > most ||
+  // (a length and a tile's keys are added in 32 bits)
+  if (keys > most - std::max(kPagedTile, kWideTile) || (keys / 32 + 9) * std::max(p.batch, 1) > most || (int64_t)p.top * p.page_size > most ||
       (int64_t)p.batch * p.draft * p.heads > most / 2 || p.top > (1 << 20)) {
     err = "more keys or query rows than 32-bit counts hold";
     return false;

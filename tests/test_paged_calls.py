@@ -301,6 +301,16 @@ def test_the_cache_refuses_to_be_captured(monkeypatch):
     assert cache.compact() == 2
 
 
+@pytest.mark.parametrize("variant", [kl.PAGED_ATTENTION, kl.PAGED_SELECT])
+def test_tables_whose_last_tile_passes_32_bits_are_refused(variant):
+    """Tiles of a sequence are counted as (length + keys of a tile - 1) / keys of a tile, in 32 bits."""
+    size = ctypes.c_size_t()
+    for page, width, rc in ((16, 2 ** 27 - 1, kl.ERR_UNSUPPORTED), (16, 2 ** 27 - 4, kl.ERR_UNSUPPORTED), (16, 2 ** 27 - 8, kl.OK),
+                            (1024, 2 ** 21 - 1, kl.OK), (1024, 2 ** 21, kl.ERR_UNSUPPORTED)):
+        op = kl.Paged(variant, 1, 1, 1, 1, 64, page, 4, width, variant, kl.TYPE_F32, kl.TYPE_F32, 0, 1.0)
+        assert kl.load().kh_paged_workspace_bytes(op, size) == rc, (page, width)
+
+
 def test_more_items_than_a_launch_holds_are_refused():
     """A workgroup of eight waves per (sequence, head, token): 2^32 work items are one too many."""
     size = ctypes.c_size_t()
