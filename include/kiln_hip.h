@@ -432,7 +432,7 @@ int kh_paged_host(const kh_paged *op);
 
 /*
  * kh_cache_append: the rows new[rows[s][a]] of k and v (a < accept while
- * rows[s][a] is in [0, draft); rows = NULL: rows 0 .. draft) written as tokens
+ * rows[s][a] is in [0, draft); rows = NULL: rows 0 .. accept) written as tokens
  * lengths[s] + a of sequence s, rounded to the cache's type, in each of
  * `layers` layers; with k_means, the mean key of every page written to, over
  * the tokens it then holds. Tokens whose page the table does not name (an

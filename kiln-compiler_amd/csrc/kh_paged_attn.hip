@@ -9,13 +9,16 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Whole items or ranges. A whole item of n keys takes eight waves about 8 us +
-// n / 110 ns whatever else runs, ranges and their join 14 us and the time that
-// the chip's loads take: one sequence of 8 heads, 1000 keys 17.1 (whole) and
-// 17.8 us (ranges), 2000 keys 26.1 and 14.1. With an item for half the compute
-// units whole items lose little of the chip: 128 items of 2000 keys 30.1 and
-// 33.1 us, of 4000 keys 50.0 and 52.2, 512 items of 4000 keys 194 and 195. Four
-// waves (many rows, wide heads) take about twice as long a key.
+// Whole items or ranges. A whole item of n keys takes eight waves about 8 us
+// and 9 ns a key whatever else runs, ranges and their join 14 us and the time
+// that the chip's loads take: one sequence of 8 heads of 128, bf16, 1000 keys
+// 17.7 (whole) and 18.1 us (ranges), 1280 keys 19.7 and 18.2, 2000 keys 26.2
+// and 14.3. With an item for half the compute units whole items lose little of
+// the chip: 128 items of 1000 keys 20.6 and 27.6 us, of 2000 keys 30.9 and 33.3,
+// of 4000 keys 51.3 and 53.3, 512 items of 4000 keys 193 and 194 (fp32
+// activations 198 and 194). Four waves (many rows, wide heads) take about twice
+// as long a key. The number of keys is that of the table's columns: lengths are
+// on the device, so short sequences under a wide table run as ranges.
 constexpr int kWholeKeys = 1280, kWholeManyKeys = 4096, kWholeSlowKeys = 1024;
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }

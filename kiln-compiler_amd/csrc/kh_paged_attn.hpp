@@ -37,13 +37,13 @@
 //
 // What bounds it, measured (one MI355X; a 2 GiB copy moves 4.9 TB/s, reads and
 // writes together): long caches the reading of K and V - 131072 bf16 tokens of
-// 8 heads of 128, one fp32 query of 32 heads, 102 us (5.2 TB/s) and 7 us for
-// the join; 32 sequences of 0 to 8192 tokens 121 us (4.7 TB/s) and 7; 48 pages
+// 8 heads of 128, one fp32 query of 32 heads, 104 us (5.2 TB/s) and 7 us for
+// the join; 32 sequences of 0 to 8192 tokens 122 us (4.7 TB/s) and 7; 48 pages
 // of 128 tokens picked for each of 13 tokens 102 us (653 MB, 6.4 TB/s: tokens
 // share pages). Short ones latency: a launch, the length, the first loads and
 // one tile are 7 us, each further tile of a wave 1.5 us (a K load's latency and
 // the products behind it), which is why a whole item takes eight waves: 27-token
-// trees over 1024 tokens, 12 heads of 64, 30.6 us with four, 23.2 with eight.
+// trees over 1024 tokens, 12 heads of 64, 30.6 us with four, 23.8 with eight.
 // Tiles of 64 keys for 64-wide heads, and page numbers staged in the LDS, were
 // both slower (32.7 us there; 137 for the 32 sequences): the first tile waits
 // longer, and nothing that comes after was waiting for them.
@@ -923,13 +923,15 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 // the LDS serves 32 rows. V^T operands come from transposing LDS reads.
 //
 // Measured: 4 sequences of 3604 to 32768 tokens, 64 drafted tokens of 8 heads a
-// group (512 rows over 4 fp16 heads of 128) 143 us and 13 for the join, where
-// paged_attn_kernel on 64 rows a wave took 369 and 26; its matrix instructions
-// are busy 22% of the time, VALU 30%, the LDS 12% (no conflicts). Tried without
-// gain: the second block's exponentials between the first block's products (146
-// us; fp32 activations slower), eight waves of 256 rows with two tiles copied
-// ahead (150 us): the waits are each wave's own chain from LDS read to product
-// to maximum to weight to product.
+// group (512 rows over 4 fp16 heads of 128) 174 us and 13 for the join (weights in
+// one part 146, where paged_attn_kernel on 64 rows a wave took 369). K and V are
+// fetched once for each of an item's four row blocks, 562 MiB for 142: equal
+// ranges cut the blocks at different keys, so they do not meet in an XCD's L2.
+// That is 3.4 TB/s; at 2.4 GHz the matrix instructions are busy 26% of the
+// time, VALU 35% (10.6 for each of them), the LDS 9% (no conflicts). Tried
+// without gain, with weights in one part: the second block's exponentials
+// between the first block's products (146 us; fp32 activations slower), eight
+// waves of 256 rows with two tiles copied ahead (150 us).
 
 // Chunk swizzle of K and V rows in the LDS, 16-byte chunks: a 128-bit read
 // meets in one LDS cycle rows {0-3, 12-15, 20-27}, distinct mod 16, so every

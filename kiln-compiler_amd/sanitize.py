@@ -33,7 +33,7 @@ SAN_BUILD = build.BUILD.with_name("_build_asan")
 SAN_FLAGS = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
              "-Xarch_host", "-fno-sanitize-recover=undefined", "-Xarch_host", "-fno-omit-frame-pointer",
              "-Xarch_host", "-g"]
-TESTS = ["tests/test_interpret.py", "tests/test_lowering.py", "tests/test_paged.py"]
+TESTS = ["tests/test_interpret.py", "tests/test_lowering.py", "tests/test_paged.py", "tests/test_paged_calls.py"]
 
 
 def asan_runtime() -> str:
