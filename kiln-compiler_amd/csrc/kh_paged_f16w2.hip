@@ -1,4 +1,5 @@
-// kh_paged_f16w2.hip - attention over a paged cache of fp16, fp16 activations: scores in one pass, weights in two parts (kh_paged_attn.hpp).
+// kh_paged_f16w2.hip - attention over a paged cache of fp16, fp16 activations: scores in one pass, weights in two
+// parts (kh_paged_attn.hpp).
 #include "kh_paged_attn.hpp"
 
 namespace kh {
