@@ -70,8 +70,10 @@ enum {
   KH_FAM_PAGED = 7 /* operators over a paged key/value cache (kh_paged)        */
 };
 
-/* element types of a paged cache and of the activations next to it */
-enum { KH_TYPE_F32 = 0, KH_TYPE_BF16 = 1, KH_TYPE_F16 = 2 };
+/* element types of a paged cache and of the activations next to it;
+ * KH_TYPE_MX4 (a cache alone): 4 bits an element, 32 adjacent dimensions under
+ * one power of two (kh_cache_append below says how they lie) */
+enum { KH_TYPE_F32 = 0, KH_TYPE_BF16 = 1, KH_TYPE_F16 = 2, KH_TYPE_MX4 = 3 };
 /* operators of the paged family */
 enum { KH_PAGED_ATTENTION = 0, KH_PAGED_SELECT = 1 };
 
@@ -238,7 +240,7 @@ typedef struct kh_pass {
  *        of the table, picked pages per token (0: every page is read), 0};
  *        cfg[0] = cache type, cfg[1] = activation type (KH_TYPE_*), cfg[2] = 1:
  *        products on the cache type's own matrix instruction, one pass;
- *        fparams[0] = scale. Refs, strides in elements of their own type:
+ *        cfg[5] = window, cfg[6] = sinks of ATTENTION; fparams[0] = scale. Refs, strides in elements of their own type:
  *        ATTENTION 0 q, 1 k, 2 v over (sequence, token, head, d), 3, 4 the
  *        pages over (page, head, slot, d), 5 table over (sequence, column),
  *        6 lengths, 7 out (as q), then refs[cfg[3]] parents over (sequence,
@@ -389,13 +391,19 @@ int kh_plan_destroy(kh_plan *plan);
  * (columns of the table) selected[s][i][kv head][0..top) alone - and to the
  * new tokens on its own path, itself included:
  *   out = softmax(scale q . k) v.
+ * With window > 0 (not beside `selected`) a new token at position p = lengths[s]
+ * + the number of its ancestors attends, of these, to the tokens at positions
+ * above p - window and below `sinks` alone; pages without such tokens are not
+ * read. 4-bit pages (KH_TYPE_MX4) take activations of every type; new tokens
+ * are rounded to 4 bits as kh_cache_append does.
  * An entry of `selected` counts only where it is larger than the entry before
  * it (the first: than -1) and below width. Sums, softmax statistics and
  * products of fp32 activations are kept to fp32 (bf16 and fp16 caches: q and
  * the weights split into 3 and 2 parts, whose products are exact). With
  * act_type = cache_type = bf16 or fp16 the first product is exact and the
  * weights are two parts of the cache's type, 2^-15 or 2^-21 of a weight off.
- * one_pass = 1: q and the weights are rounded to the cache's type.
+ * one_pass = 1: q and the weights are rounded to the cache's type (over 4-bit
+ * pages q to bf16, the weights to two parts of it).
  *
  * kh_paged_select: for query token (s, i) and kv head c the `top` pages with
  * the largest (sum of the group's queries) . k_means[page][c], products and
@@ -423,9 +431,12 @@ typedef struct kh_paged {
   int64_t q_s, q_n, q_h, k_s, k_n, k_h, v_s, v_n, v_h, o_s, o_n, o_h;  /* strides in elements */
   int64_t kp_p, kp_h, kp_t, vp_p, vp_h, vp_t, m_p, m_h;
   int64_t table_s, parents_s, sel_s, sel_n, sel_h;
+  int32_t window, sinks;                  /* 0: every token is in the window        */
 } kh_paged;
 /* sizeof(kh_paged), sizeof(kh_cache_append_op), sizeof(kh_pool) */
 int kh_paged_sizes(size_t *sizes3);
+/* sizeof(kh_cache_read_op) */
+int kh_decode_sizes(size_t *sizes1);
 int kh_paged_workspace_bytes(const kh_paged *op, size_t *bytes);
 int kh_paged_run(const kh_paged *op, void *workspace, size_t workspace_bytes, void *stream);
 int kh_paged_host(const kh_paged *op);
@@ -438,6 +449,20 @@ int kh_paged_host(const kh_paged *op);
  * the tokens it then holds. Tokens whose page the table does not name (an
  * entry outside [0, pages), a column outside its width, a negative length)
  * are dropped. No page may be written through two sequences of one call.
+ *
+ * KH_TYPE_MX4 (dim a multiple of 32): a block is 32 adjacent dimensions of a
+ * token, its elements a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6 (codes 0-7,
+ * 8 more with the sign) times 2^(e - 127), e its scale byte: the smallest from
+ * 2 to 252 for which the largest |x| is below 7 times it (or 252), 255 (NaN)
+ * where an x is not finite; elements go to the nearest, ties to the even code. A page of a
+ * head is page_size * 17 dim / 32 bytes, kp_p, kp_h (and vp_p, vp_h) count
+ * bytes and kp_t, vp_t nothing: first the codes, element (t, d) the low half
+ * (d even) or high half of byte
+ *   keys    t dim/2 + d/2
+ *   values  (t/16) 8 dim + ((t%16)/4 dim/8 + d/8) 16 + (t%4) 4 + (d%8)/2
+ * then, from byte page_size dim/2 on, the scale bytes, of (t, d) byte
+ *   keys    t dim/32 + d/32
+ *   values  (t/16) dim/2 + ((t%16)/4 dim/32 + d/32) 4 + t%4
  */
 typedef struct kh_cache_append_op {
   int32_t layers, batch, draft, accept, kv_heads, dim, page_size, pages, width;
@@ -452,6 +477,24 @@ typedef struct kh_cache_append_op {
 } kh_cache_append_op;
 int kh_cache_append(const kh_cache_append_op *op, void *stream);
 int kh_cache_append_host(const kh_cache_append_op *op);
+
+/*
+ * kh_cache_read: tokens starts[s] + a (a < tokens, while below ends[s]) of every
+ * sequence s as dense rows, k and v [layers][batch][tokens][kv_heads][dim] of
+ * out_type (not KH_TYPE_MX4), each value rounded once; zeros where no token is:
+ * behind ends[s], in front of token 0, or where the table names no page.
+ */
+typedef struct kh_cache_read_op {
+  int32_t layers, batch, tokens, kv_heads, dim, page_size, pages, width;
+  int32_t cache_type, out_type;
+  const void *k_pages, *v_pages;
+  void *k, *v;
+  const int32_t *table, *starts, *ends;
+  int64_t kp_l, kp_p, kp_h, kp_t, vp_l, vp_p, vp_h, vp_t;
+  int64_t table_s;
+} kh_cache_read_op;
+int kh_cache_read(const kh_cache_read_op *op, void *stream);
+int kh_cache_read_host(const kh_cache_read_op *op);
 
 /*
  * kh_cache_copy: in every pool, pages source[i] copied to target[i], i < n.

@@ -6,6 +6,7 @@
 #include <limits>
 #include <vector>
 
+#include "kh_mx4.hpp"
 #include "kh_paged.hpp"
 
 namespace kh {
@@ -13,6 +14,9 @@ namespace kh {
 int abi_fail(int code, const std::string &msg);   // kh_plan.hip: sets kh_last_error
 hipError_t launch_append(const kh_cache_append_op &a, hipStream_t stream);
 void host_append(const kh_cache_append_op &a);
+hipError_t launch_read(const kh_cache_read_op &a, hipStream_t stream);
+int64_t read_blocks(const kh_cache_read_op &a);
+void host_read(const kh_cache_read_op &a);
 hipError_t launch_copy(const kh_pool *pools, int n_pools, const int32_t *source, const int32_t *target, int n,
                        hipStream_t stream);
 
@@ -20,7 +24,14 @@ namespace {
 
 bool type_ok(int t) { return t == KH_TYPE_F32 || t == KH_TYPE_BF16 || t == KH_TYPE_F16; }
 
+bool cache_type_ok(int t) { return type_ok(t) || t == KH_TYPE_MX4; }
+
 bool page_size_ok(int n) { return n >= 16 && n <= 1024 && (n & (n - 1)) == 0; }
+
+std::string dim_error(int dim, int cache_type) {
+  return "head dimension " + std::to_string(dim) +
+         (cache_type == KH_TYPE_MX4 ? " (multiples of 32 up to 256 have kernels over 4-bit pages)" : " (multiples of 8 up to 256 have kernels)");
+}
 
 // Rows of `bytes`-byte elements that start at multiples of 16 bytes.
 bool aligned_strides(std::initializer_list<int64_t> strides, int bytes) {
@@ -45,13 +56,18 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = "heads must be a multiple of kv_heads";
     return false;
   }
-  if (!type_ok(p.cache_type) || !type_ok(p.act_type)) {
+  if (!cache_type_ok(p.cache_type) || !type_ok(p.act_type) || (p.variant == KH_PAGED_SELECT && p.cache_type == KH_TYPE_MX4)) {
     err = "unknown element type";
     return false;
   }
+  if (p.window < 0 || p.sinks < 0 || (p.window == 0 && p.sinks > 0) || (p.window > 0 && (p.top > 0 || p.variant != KH_PAGED_ATTENTION))) {
+    err = "a window of " + std::to_string(p.window) + " tokens and " + std::to_string(p.sinks) + " first ones (picked pages take none)";
+    return false;
+  }
   unsupported = true;
-  if (p.dim % 8 || p.dim > 256) {
-    err = "head dimension " + std::to_string(p.dim) + " (multiples of 8 up to 256 have kernels)";
+  const bool mx = p.cache_type == KH_TYPE_MX4;
+  if (p.dim % (mx ? kMxBlock : 8) || p.dim > 256) {
+    err = dim_error(p.dim, p.cache_type);
     return false;
   }
   if (!page_size_ok(p.page_size)) {
@@ -66,14 +82,15 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = std::to_string(p.batch) + " sequences (at most " + std::to_string(kMaxBatch) + ")";
     return false;
   }
-  if (p.variant == KH_PAGED_ATTENTION && p.act_type != KH_TYPE_F32 && p.act_type != p.cache_type) {
+  if (p.variant == KH_PAGED_ATTENTION && p.act_type != KH_TYPE_F32 && p.act_type != p.cache_type && !mx) {
     err = "activations are fp32 or of the cache's type";
     return false;
   }
   const int64_t most = std::numeric_limits<int32_t>::max();
   const int64_t keys = (int64_t)p.width * p.page_size;
   // (a length and a tile's keys are added in 32 bits)
-  if (keys > most - std::max(kPagedTile, kWideTile) || (keys / 32 + 9) * std::max(p.batch, 1) > most || (int64_t)p.top * p.page_size > most ||
+  // (and under a window a new token's depth)
+  if (keys > most - std::max(kPagedTile, kWideTile) - (p.window ? kMaxDraft : 0) || (keys / 32 + 9) * std::max(p.batch, 1) > most || (int64_t)p.top * p.page_size > most ||
       (int64_t)p.batch * p.draft * p.heads > most / 2 || p.top > (1 << 20)) {
     err = "more keys or query rows than 32-bit counts hold";
     return false;
@@ -92,7 +109,7 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = "more sequences, heads and tokens than one launch has room for (2^32 work items)";
     return false;
   }
-  if (p.variant == KH_PAGED_ATTENTION && (p.kp_t > most / 8 / p.page_size - p.dim || p.vp_t > most / 8 / p.page_size - p.dim)) {
+  if (p.variant == KH_PAGED_ATTENTION && !mx && (p.kp_t > most / 8 / p.page_size - p.dim || p.vp_t > most / 8 / p.page_size - p.dim)) {
     err = "the pages' token stride is too large";
     return false;
   }
@@ -119,7 +136,7 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     return true;
   }
   // (row offsets inside a tile are unsigned 32-bit counts)
-  if (p.kp_t < 0 || p.vp_t < 0) {
+  if (!mx && (p.kp_t < 0 || p.vp_t < 0)) {
     err = "negative token stride of the pages";
     return false;
   }
@@ -131,7 +148,7 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     err = "k, v, out: rows must start at multiples of 16 bytes";
     return false;
   }
-  if (!aligned_strides({p.kp_p, p.kp_h, p.kp_t, p.vp_p, p.vp_h, p.vp_t}, cb)) {
+  if (!aligned_strides({p.kp_p, p.kp_h, p.vp_p, p.vp_h}, cb) || (!mx && !aligned_strides({p.kp_t, p.vp_t}, cb))) {
     err = "pages: rows must start at multiples of 16 bytes";
     return false;
   }
@@ -174,6 +191,10 @@ kh_paged paged_of_launch(const kh_launch &L) {
   p.cache_type = L.cfg[0];
   p.act_type = L.cfg[1];
   p.one_pass = L.cfg[2];
+  if (p.variant == KH_PAGED_ATTENTION) {
+    p.window = L.cfg[5];
+    p.sinks = L.cfg[6];
+  }
   p.scale = L.fparams[0];
   auto strides = [&](int j, std::initializer_list<int64_t *> to) {
     int i = 0;
@@ -278,8 +299,27 @@ double value(const void *p, int64_t i, int type) {
   return (double)(float)static_cast<const _Float16 *>(p)[i];
 }
 
+// A page's element (t, d), the page's head at element `at`.
+double page_value(const kh_paged &p, bool keys, int64_t at, int64_t t, int d) {
+  const void *pages = keys ? p.k_pages : p.v_pages;
+  if (p.cache_type != KH_TYPE_MX4) return value(pages, at + t * (keys ? p.kp_t : p.vp_t) + d, p.cache_type);
+  const uint8_t *b = static_cast<const uint8_t *>(pages) + at;
+  const int s = (int)t;
+  const uint32_t code = b[keys ? mx_key_code(s, d, p.dim) : mx_value_code(s, d, p.dim)] >> (4 * (d & 1)) & 15u;
+  return mx_value(code, b[keys ? mx_key_scale(s, d, p.dim, p.page_size) : mx_value_scale(s, d, p.dim, p.page_size)]);
+}
+
+// x[0 .. dim) of a new token as the cache will hold it.
+void round_row(std::vector<double> &x, int type) {
+  if (type != KH_TYPE_MX4) return;
+  std::vector<float> y(x.begin(), x.end());
+  for (size_t b = 0; b + kMxBlock <= y.size(); b += kMxBlock) mx_round(&y[b]);
+  std::copy(y.begin(), y.end(), x.begin());
+}
+
 double rounded(double x, int type) {
   if (type == KH_TYPE_F32) return x;
+  if (type == KH_TYPE_MX4) return x;   // (a row at a time: round_row)
   if (type == KH_TYPE_BF16) return (double)(float)(__bf16)(float)x;
   return (double)(float)(_Float16)(float)x;
 }
@@ -348,16 +388,19 @@ void host_attention(const kh_paged &p) {
       for (int c = 0; c < p.kv_heads; ++c) {
         keys.clear();
         values.clear();
+        const int64_t mine = len + (int64_t)path.size() - 1;   // the token's position
+        auto in_window = [&](int64_t pos) { return !p.window || pos < p.sinks || pos > mine - p.window; };
         auto cached = [&](int64_t col) {
           const int page = p.table[s * p.table_s + col];
           if (page < 0 || page >= p.pages) return;
           for (int64_t pos = col * p.page_size; pos < std::min(len, (col + 1) * p.page_size); ++pos) {
+            if (!in_window(pos)) continue;
             keys.emplace_back();
             values.emplace_back();
             for (int d = 0; d < p.dim; ++d) {
               const int64_t slot = pos - col * p.page_size;
-              keys.back().push_back(value(p.k_pages, page * p.kp_p + c * p.kp_h + slot * p.kp_t + d, p.cache_type));
-              values.back().push_back(value(p.v_pages, page * p.vp_p + c * p.vp_h + slot * p.vp_t + d, p.cache_type));
+              keys.back().push_back(page_value(p, true, (int64_t)page * p.kp_p + c * p.kp_h, slot, d));
+              values.back().push_back(page_value(p, false, (int64_t)page * p.vp_p + c * p.vp_h, slot, d));
             }
           }
         };
@@ -368,20 +411,24 @@ void host_attention(const kh_paged &p) {
         } else {
           for (int64_t col = 0; col * p.page_size < len; ++col) cached(col);
         }
-        for (int i : path) {
+        for (size_t a = 0; a < path.size(); ++a) {   // (ancestor a is at position len + a)
+          const int i = path[a];
+          if (!in_window(len + (int64_t)a)) continue;
           keys.emplace_back();
           values.emplace_back();
           for (int d = 0; d < p.dim; ++d) {
             keys.back().push_back(rounded(value(p.k, s * p.k_s + i * p.k_n + c * p.k_h + d, p.act_type), p.cache_type));
             values.back().push_back(rounded(value(p.v, s * p.v_s + i * p.v_n + c * p.v_h + d, p.act_type), p.cache_type));
           }
+          round_row(keys.back(), p.cache_type);
+          round_row(values.back(), p.cache_type);
         }
         for (int h = c * group; h < (c + 1) * group; ++h) {
           std::fill(out.begin(), out.end(), 0.0);
           if (used) {
             for (int d = 0; d < p.dim; ++d) {
               q[(size_t)d] = value(p.q, s * p.q_s + n * p.q_n + h * p.q_h + d, p.act_type);
-              if (p.one_pass) q[(size_t)d] = rounded(q[(size_t)d], p.cache_type);
+              if (p.one_pass) q[(size_t)d] = rounded(q[(size_t)d], p.cache_type == KH_TYPE_MX4 ? KH_TYPE_BF16 : p.cache_type);
             }
             double most = -INFINITY, total = 0.0;
             score.assign(keys.size(), 0.0);
@@ -426,26 +473,54 @@ void host_paged_launch(const kh_launch &L, float *const *ptrs) {
 
 namespace {
 
+int check_page(int dim, int page_size, int cache_type) {
+  if (dim % (cache_type == KH_TYPE_MX4 ? kMxBlock : 8) || dim > 256) return abi_fail(KH_ERR_UNSUPPORTED, dim_error(dim, cache_type));
+  if (!page_size_ok(page_size))
+    return abi_fail(KH_ERR_UNSUPPORTED, "page size " + std::to_string(page_size) + " (powers of two from 16 to 1024 have kernels)");
+  return KH_OK;
+}
+
 int check_append(const kh_cache_append_op *a) {
   if (!a) return abi_fail(KH_ERR_INVALID, "null argument");
   if (a->layers < 0 || a->batch < 0 || a->draft < 0 || a->accept < 0 || a->kv_heads < 1 || a->dim < 1 || a->pages < 1 ||
-      a->width < 0 || !type_ok(a->cache_type) || !type_ok(a->act_type))
+      a->width < 0 || !cache_type_ok(a->cache_type) || !type_ok(a->act_type))
     return abi_fail(KH_ERR_INVALID, "bad sizes or types");
   if (!a->rows && a->accept > a->draft) return abi_fail(KH_ERR_INVALID, "more tokens to append than there are");
-  if (a->dim % 8 || a->dim > 256)
-    return abi_fail(KH_ERR_UNSUPPORTED, "head dimension " + std::to_string(a->dim) + " (multiples of 8 up to 256 have kernels)");
-  if (!page_size_ok(a->page_size))
-    return abi_fail(KH_ERR_UNSUPPORTED, "page size " + std::to_string(a->page_size) + " (powers of two from 16 to 1024 have kernels)");
+  const int rc = check_page(a->dim, a->page_size, a->cache_type);
+  if (rc != KH_OK) return rc;
   if ((int64_t)a->batch * a->kv_heads > 65535 || a->layers > 65535)
     return abi_fail(KH_ERR_UNSUPPORTED, "more than 65535 (sequence, kv head) pairs or layers");
   const int ab = type_bytes(a->act_type), cb = type_bytes(a->cache_type);
   if (!aligned_strides({a->k_l, a->k_s, a->k_n, a->k_h, a->v_l, a->v_s, a->v_n, a->v_h}, ab) ||
-      !aligned_strides({a->kp_l, a->kp_p, a->kp_h, a->kp_t, a->vp_l, a->vp_p, a->vp_h, a->vp_t}, cb))
+      !aligned_strides({a->kp_l, a->kp_p, a->kp_h, a->vp_l, a->vp_p, a->vp_h}, cb) ||
+      (a->cache_type != KH_TYPE_MX4 && !aligned_strides({a->kp_t, a->vp_t}, cb)))
     return abi_fail(KH_ERR_INVALID, "rows must start at multiples of 16 bytes");
   if (!a->layers || !a->batch || !a->accept) return KH_OK;
   auto odd = [](const void *x, int n) { return x == nullptr || (uintptr_t)x % n; };
   if (odd(a->k, 16) || odd(a->v, 16) || odd(a->k_pages, 16) || odd(a->v_pages, 16) || odd(a->lengths, 4) ||
       (a->width > 0 && odd(a->table, 4)) || (a->rows && odd(a->rows, 4)) || (a->k_means && odd(a->k_means, 4)))
+    return abi_fail(KH_ERR_INVALID, "a null or unaligned pointer");
+  return KH_OK;
+}
+
+int check_read(const kh_cache_read_op *a) {
+  if (!a) return abi_fail(KH_ERR_INVALID, "null argument");
+  if (a->layers < 0 || a->batch < 0 || a->tokens < 0 || a->kv_heads < 1 || a->dim < 1 || a->pages < 1 || a->width < 0 ||
+      !cache_type_ok(a->cache_type) || !type_ok(a->out_type))
+    return abi_fail(KH_ERR_INVALID, "bad sizes or types");
+  const int rc = check_page(a->dim, a->page_size, a->cache_type);
+  if (rc != KH_OK) return rc;
+  if (a->batch > 65535 || a->layers > 65535) return abi_fail(KH_ERR_UNSUPPORTED, "more than 65535 sequences or layers");
+  if (read_blocks(*a) * 256 > (int64_t)std::numeric_limits<uint32_t>::max())
+    return abi_fail(KH_ERR_UNSUPPORTED, "more tokens than one launch has room for (2^32 work items)");
+  const int cb = type_bytes(a->cache_type);
+  if (!aligned_strides({a->kp_l, a->kp_p, a->kp_h, a->vp_l, a->vp_p, a->vp_h}, cb) ||
+      (a->cache_type != KH_TYPE_MX4 && !aligned_strides({a->kp_t, a->vp_t}, cb)))
+    return abi_fail(KH_ERR_INVALID, "rows must start at multiples of 16 bytes");
+  if (!a->layers || !a->batch || !a->tokens) return KH_OK;
+  auto odd = [](const void *x, int n) { return x == nullptr || (uintptr_t)x % n; };
+  if (odd(a->k, 16) || odd(a->v, 16) || odd(a->k_pages, 16) || odd(a->v_pages, 16) || odd(a->starts, 4) || odd(a->ends, 4) ||
+      (a->width > 0 && odd(a->table, 4)))
     return abi_fail(KH_ERR_INVALID, "a null or unaligned pointer");
   return KH_OK;
 }
@@ -561,6 +636,28 @@ int kh_cache_append_host(const kh_cache_append_op *op) {
   return kh::guarded([&] {
     const int rc = kh::check_append(op);
     if (rc == KH_OK) kh::host_append(*op);
+    return rc;
+  });
+}
+
+int kh_decode_sizes(size_t *sizes1) {
+  if (!sizes1) return kh::abi_fail(KH_ERR_INVALID, "null argument");
+  sizes1[0] = sizeof(kh_cache_read_op);
+  return KH_OK;
+}
+
+int kh_cache_read(const kh_cache_read_op *op, void *stream) {
+  return kh::guarded([&] {
+    const int rc = kh::check_read(op);
+    if (rc != KH_OK) return rc;
+    return kh::hip_status(kh::launch_read(*op, static_cast<hipStream_t>(stream)), "kh_cache_read");
+  });
+}
+
+int kh_cache_read_host(const kh_cache_read_op *op) {
+  return kh::guarded([&] {
+    const int rc = kh::check_read(op);
+    if (rc == KH_OK) kh::host_read(*op);
     return rc;
   });
 }

@@ -54,6 +54,9 @@ hipError_t launch_paged_bf16w2(const PagedWork &w, int dt, int rt, hipStream_t s
 hipError_t launch_paged_bf16x3(const PagedWork &w, int dt, int rt, hipStream_t stream);
 hipError_t launch_paged_f16(const PagedWork &w, int dt, int rt, hipStream_t stream);
 hipError_t launch_paged_f16w2(const PagedWork &w, int dt, int rt, hipStream_t stream);
+hipError_t launch_paged_mx4w2(const PagedWork &w, int dt, int rt, hipStream_t stream);   // bf16 activations
+hipError_t launch_paged_mx4x2(const PagedWork &w, int dt, int rt, hipStream_t stream);   // fp16 ones
+hipError_t launch_paged_mx4x3(const PagedWork &w, int dt, int rt, hipStream_t stream);   // fp32 ones
 hipError_t launch_paged_f16x2(const PagedWork &w, int dt, int rt, hipStream_t stream);
 
 constexpr int kPagedTile = 32;     // keys of a tile
@@ -66,6 +69,7 @@ constexpr int paged_waves(int dt, int rt, bool whole) { return whole && rt * dt 
 constexpr int kMaxDraft = 256;     // new tokens of a sequence: a workgroup's table of paths fits the LDS
 constexpr int kMaxBatch = 4096;    // sequences of a call: each workgroup scans their lengths
 
-inline int type_bytes(int t) { return t == KH_TYPE_F32 ? 4 : 2; }
+// (4-bit pages are counted in bytes)
+inline int type_bytes(int t) { return t == KH_TYPE_F32 ? 4 : t == KH_TYPE_MX4 ? 1 : 2; }
 
 }  // namespace kh

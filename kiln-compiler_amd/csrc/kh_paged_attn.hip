@@ -33,7 +33,7 @@ constexpr int kWideRows = 48;
 int row_blocks(const kh_paged &p) {
   const int rows = (p.top ? 1 : p.draft) * (p.heads / p.kv_heads);
   const int dt = padded_dim(p.dim);
-  if (p.cache_type != KH_TYPE_F32 && dt < 256 && rows >= kWideRows && p.batch <= kMaxWideBatch) return kWideBlocks;
+  if (p.cache_type != KH_TYPE_F32 && p.cache_type != KH_TYPE_MX4 && dt < 256 && rows >= kWideRows && p.batch <= kMaxWideBatch) return kWideBlocks;
   return rows <= 16 || dt == 256 ? 1 : 2;
 }
 
@@ -54,7 +54,10 @@ PagedWork work_of(const kh_paged &p) {
   w.rounds = 0;
   while ((1 << w.rounds) < p.draft) ++w.rounds;
   w.scale2 = p.scale * kLog2e;
-  const int64_t per_item = (w.sel_tiles ? w.sel_tiles : ((int64_t)p.width * p.page_size + w.tile - 1) / w.tile) + w.draft_tiles;
+  int64_t cached = ((int64_t)p.width * p.page_size + w.tile - 1) / w.tile;
+  // (a window's keys, those before it in its first tile, and the sinks')
+  if (p.window) cached = std::min(cached, ((int64_t)p.window + w.tile - 2) / w.tile + 1 + ((int64_t)p.sinks + w.tile - 1) / w.tile);
+  const int64_t per_item = (w.sel_tiles ? w.sel_tiles : cached) + w.draft_tiles;
   const int64_t items = (int64_t)w.items * p.batch;
   // workgroups: one per item where none can have many tiles; else what the
   // chip holds at once, or a tile per wave of the most tiles the table has room for
@@ -92,6 +95,8 @@ hipError_t launch_paged(const kh_paged &p, float *workspace, hipStream_t stream)
   const bool fp32 = p.act_type == KH_TYPE_F32;
   switch (p.cache_type) {
     case KH_TYPE_F32: return launch_paged_f32(w, dt, rt, stream);
+    case KH_TYPE_MX4:
+      return (p.act_type == KH_TYPE_F16 ? launch_paged_mx4x2 : fp32 && !p.one_pass ? launch_paged_mx4x3 : launch_paged_mx4w2)(w, dt, rt, stream);
     case KH_TYPE_BF16:
       return (p.one_pass ? launch_paged_bf16 : fp32 ? launch_paged_bf16x3 : launch_paged_bf16w2)(w, dt, rt, stream);
     default: return (p.one_pass ? launch_paged_f16 : fp32 ? launch_paged_f16x2 : launch_paged_f16w2)(w, dt, rt, stream);

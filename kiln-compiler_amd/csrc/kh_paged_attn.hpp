@@ -53,6 +53,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "kh_mx4.hpp"
 #include "kh_paged.hpp"
 
 namespace kh {
@@ -88,20 +89,58 @@ __device__ __forceinline__ int clamp_len(W &w, int s) {
   return n < 0 ? 0 : (n > most ? (int)most : n);
 }
 
-template <class W>
+// The tiles of the cached tokens that count: all of them, or under a window
+// those of the first `sinks` tokens and those from the first key that the
+// shallowest new token sees; tile t is tile t of the sequence below `head`, t +
+// skip from there on.
+// (WIN: whether there may be a window; kernels are built with and without, as
+// its few scalars would not fit beside the others.)
+struct Span {
+  int tiles, head, skip;
+};
+
+template <bool WIN, class W>
+__device__ __forceinline__ Span span_of(W &w, int len) {
+  const int all = (len + w.tile - 1) / w.tile;
+  Span r = {all, all, 0};
+  if (WIN && w.p.window) {
+    const int from = max(len - w.p.window + 1, 0) / w.tile;
+    r.head = (min(w.p.sinks, len) + w.tile - 1) / w.tile;
+    r.skip = max(from - r.head, 0);
+    r.tiles = all - r.skip;
+  }
+  return r;
+}
+
+// Do new tokens differ in which keys they see of the 32 (64) from `pos` on, or
+// see none of some? (A new token's window starts at len + depth - window + 1.)
+template <bool WIN, class W>
+__device__ __forceinline__ bool on_edge(W &w, int len, int pos, int keys) {
+  return WIN && w.p.window && pos + keys > w.p.sinks && pos <= len - w.p.window + w.p.draft - 1;
+}
+
+// Bits of the 32 keys from `pos` on that lie in the window or are sinks: `first`
+// is the window's first key.
+__device__ __forceinline__ uint32_t window_bits(int first, int sinks, int pos) {
+  const int lo = first - pos, hi = sinks - pos;
+  const uint32_t in = lo <= 0 ? ~0u : lo >= 32 ? 0u : ~0u << lo;
+  return in | (hi <= 0 ? 0u : hi >= 32 ? ~0u : (1u << hi) - 1);
+}
+
+template <bool WIN, class W>
 __device__ __forceinline__ int tiles_of(W &w, int len) {
-  return (w.sel_tiles ? w.sel_tiles : (len + w.tile - 1) / w.tile) + w.draft_tiles;
+  return (w.sel_tiles ? w.sel_tiles : span_of<WIN>(w, len).tiles) + w.draft_tiles;
 }
 
 // first[s] = tiles of one item of the sequences before s, for s <= batch.
-template <class W>
+template <bool WIN, class W>
 __device__ __forceinline__ void scan_tiles(W &w, int *first, int *wave_sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = w.p.batch;
   const int per = (n + kThreads - 1) / kThreads;
   const int lo = threadIdx.x * per;
   int sum = 0;
-  for (int i = lo; i < min(lo + per, n); ++i) sum += tiles_of(w, clamp_len(w, i));
+  for (int i = lo; i < min(lo + per, n); ++i) sum += tiles_of<WIN>(w, clamp_len(w, i));
   int run = sum;   // inclusive over the wave
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -114,7 +153,7 @@ __device__ __forceinline__ void scan_tiles(W &w, int *first, int *wave_sums) {
   for (int i = 0; i < wave; ++i) at += wave_sums[i];
   for (int i = lo; i < min(lo + per, n); ++i) {
     first[i] = at;
-    at += tiles_of(w, clamp_len(w, i));
+    at += tiles_of<WIN>(w, clamp_len(w, i));
   }
   if (lo < n && lo + per >= n) first[n] = at;
   __syncthreads();
@@ -160,10 +199,11 @@ __device__ __forceinline__ int sequence_of(W &w, const int *first, int x) {
 struct Paths {
   uint32_t bits[kMaxDraft][kMaxDraft / 32];
   int16_t next[kMaxDraft];   // the next ancestor beyond those held; -1 none, -2 the token is unused
+  int16_t depth[kMaxDraft];  // ancestors of the token (under a window)
 };
 
-template <class W>
-__device__ __forceinline__ void build_paths(W &w, int s, Paths &t) {
+template <bool WIN, class W>
+__device__ __forceinline__ void build_paths(W &w, int s, int len, Paths &t) {
   const int i = threadIdx.x, n = w.p.draft;
   const int32_t *parents = w.p.parents + s * w.p.parents_s;
   const int words = (n + 31) / 32;
@@ -193,6 +233,22 @@ __device__ __forceinline__ void build_paths(W &w, int s, Paths &t) {
     }
     __syncthreads();
   }
+  if (WIN && w.p.window) {
+    if (i < n) {
+      int depth = -1;
+      for (int k = 0; k < words; ++k) depth += __builtin_popcount(t.bits[i][k]);
+      t.depth[i] = (int16_t)depth;
+      if (w.p.window < n) {   // ancestors out of the window: the path is walked again
+        for (int k = 0; k < words; ++k) t.bits[i][k] = 0u;
+        int j = i;
+        for (int back = 0; back <= depth; ++back) {
+          if (back < w.p.window || len + depth - back < w.p.sinks) t.bits[i][j / 32] |= 1u << (j & 31);
+          j = max(parents[j], 0);
+        }
+      }
+    }
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -219,6 +275,13 @@ struct Cache<KH_TYPE_F16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
+
+// 4-bit pages: values are bf16 ones (kh_mx4.hpp), the products bf16's
+template <>
+struct Cache<KH_TYPE_MX4> : Cache<KH_TYPE_BF16> {};
+// elements that pages are counted in
+template <int CT>
+using PageElement = std::conditional_t<CT == KH_TYPE_MX4, uint8_t, typename Cache<CT>::T>;
 
 // n (4 or 8) adjacent activations from element i, fp32 or T, 16-byte (8-byte) aligned
 template <class T, int N>
@@ -322,6 +385,22 @@ struct Tile {
   uint32_t v[8][VC][VW];
 };
 
+// 4-bit pages: K: codes of the DT / 4 dimensions from DT / 4 g on of key 16 h + li
+// (one 16-byte load where DT is 128), their blocks' scale bytes in a word; V:
+// codes of 8 dimensions of 4 keys (16 bytes that lie together; heads of 64: of
+// which this lane uses 4, its neighbour the others) and the keys' scales.
+template <int DT>
+struct Tile<KH_TYPE_MX4, DT> {
+  static constexpr int KS = DT / 32;
+  static constexpr int VD = DT >= 128 ? 8 : 4;
+  static constexpr int VC = DT / (16 * VD);
+  static constexpr int PD = DT / 4;                        // adjacent dimensions of a lane's key
+  static constexpr int PW = PD < 32 ? 2 : 4;               // words of one block's share of them
+  static constexpr int PB = PD < 32 ? 1 : PD / 32;         // blocks
+  uint32_t k[2][PB][PW], ke[2];
+  uint32_t v[2][VC][4], ve[2][VC];
+};
+
 template <int N>
 __device__ __forceinline__ void load_words(const void *p, uint32_t (&x)[N]) {
   if constexpr (N == 2) {
@@ -339,12 +418,16 @@ __device__ __forceinline__ void load_words(const void *p, uint32_t (&x)[N]) {
 }
 
 // Where a tile's halves lie (uniform over the wave): rows of `valid` keys each.
+// 4-bit pages: k and v are the page's of the head, slot the half's first token.
 template <class T>
 struct Source {
   const T *k[2], *v[2];
   int k_row, v_row;    // elements from a key to the next
+  int slot[2];
   int valid[2];
   int draft;           // index among the new tokens' tiles, -1 for a cached one
+  int pos;             // a cached tile's first key
+  bool edge;           // not every row sees the same of its keys
 };
 
 // The kernel's arguments are read where they are used, through a pointer that
@@ -359,12 +442,14 @@ __device__ __forceinline__ const_work &fresh() {
 
 // WHOLE: a workgroup per item, of eight waves where the registers allow two on
 // a SIMD (one alone waits about 1.5 us a tile for its loads); else ranges.
-template <int CT, int NQ, int NW, int DT, int RT, bool WHOLE>
+template <int CT, int NQ, int NW, int DT, int RT, bool WHOLE, bool WIN>
 __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 : 2) void paged_attn_kernel(const PagedWork) {
   constexpr int WAVES = paged_waves(DT, RT, WHOLE);
   typedef typename Cache<CT>::T T;
   typedef Tile<CT, DT> Regs;
-  constexpr bool F32 = CT == KH_TYPE_F32;
+  typedef PageElement<CT> E;
+  constexpr bool F32 = CT == KH_TYPE_F32, MX = CT == KH_TYPE_MX4;
+  typedef std::conditional_t<MX && NQ == 2, _Float16, T> A;   // 16-bit activations
   constexpr int KS = Regs::KS, VD = Regs::VD, VC = Regs::VC;
   constexpr int RM = 16 * RT;
   constexpr int NT = DT / 16;                  // 16-wide tiles of O^T: (chunk, t)
@@ -383,7 +468,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
   int me = blockIdx.x, at = 0, end = 1;
   if constexpr (!WHOLE) {
     const_work &w = fresh();
-    scan_tiles(w, first, wave_sums);
+    scan_tiles<WIN>(w, first, wave_sums);
     const Plan plan = plan_of(w, first);
     if (me >= plan.count) return;
     // neighbouring ranges on the same XCD: they share row blocks' keys
@@ -401,14 +486,14 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       s = (int)((uint32_t)me / (uint32_t)w.items);
       item = me - s * w.items;
       len = clamp_len(w, s);
-      tiles = tiles_of(w, len);
+      tiles = tiles_of<WIN>(w, len);
       t0 = 0;
       t1 = tiles;
       at = end;
     } else {
       s = sequence_of(w, first, at);
       len = clamp_len(w, s);
-      tiles = tiles_of(w, len);
+      tiles = tiles_of<WIN>(w, len);
       const int in_seq = at - __builtin_amdgcn_readfirstlane(first[s]) * w.items;
       item = (int)((uint32_t)in_seq / (uint32_t)tiles);
       t0 = in_seq - item * tiles;
@@ -416,6 +501,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       at += t1 - t0;
     }
     const int cached = tiles - w.draft_tiles;
+    const Span span = span_of<WIN>(w, len);
     // item = (kv head, [token,] row block)
     const int c = (int)((uint32_t)item / (uint32_t)w.per_head);
     const int b = item - c * w.per_head;
@@ -426,23 +512,24 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 
     const bool has_draft = t1 > cached;
     const bool tree = w.p.parents != nullptr;
-    if (has_draft && tree && paths_of != s) {
+    if ((has_draft || WIN) && tree && paths_of != s) {
       __syncthreads();   // the last item's rows have read the table
-      build_paths(w, s, paths);
+      build_paths<WIN>(w, s, len, paths);
       paths_of = s;
     }
 
     // -- where tile t lies; the first tile at or after t with a key, in steps of the waves
     const_work &wt = fresh();
-    const T *kp = static_cast<const T *>(wt.p.k_pages) + c * wt.p.kp_h, *vp = static_cast<const T *>(wt.p.v_pages) + c * wt.p.vp_h;
+    const E *kp = static_cast<const E *>(wt.p.k_pages) + c * wt.p.kp_h, *vp = static_cast<const E *>(wt.p.v_pages) + c * wt.p.vp_h;
     const int64_t kp_p = wt.p.kp_p, vp_p = wt.p.vp_p;
     const int kp_t = (int)wt.p.kp_t, vp_t = (int)wt.p.vp_t, half_shift = wt.half_shift, pages = wt.p.pages;
     const const_ints row_of_table = ints_of(wt.p.table) + s * wt.p.table_s;
-    auto find = [&](int &t, Source<T> &r) {
+    auto find = [&](int &t, Source<E> &r) {
       for (; t < t1; t += WAVES) {
         if (t >= cached) {
           const_work &w = fresh();
           r.draft = t - cached;
+          if constexpr (WIN) r.edge = false;
           const int n0 = kTile * r.draft;
           r.k_row = (int)w.p.k_n;
           r.v_row = (int)w.p.v_n;
@@ -450,17 +537,25 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           for (int h = 0; h < 2; ++h) {
             r.valid[h] = min(max(w.p.draft - (n0 + 16 * h), 0), 16);
             const int n = r.valid[h] ? n0 + 16 * h : 0;
-            r.k[h] = static_cast<const T *>(w.p.k) + (s * w.p.k_s + c * w.p.k_h + n * w.p.k_n);
-            r.v[h] = static_cast<const T *>(w.p.v) + (s * w.p.v_s + c * w.p.v_h + n * w.p.v_n);
+            if constexpr (!MX) {
+              r.k[h] = static_cast<const T *>(w.p.k) + (s * w.p.k_s + c * w.p.k_h + n * w.p.k_n);
+              r.v[h] = static_cast<const T *>(w.p.v) + (s * w.p.v_s + c * w.p.v_h + n * w.p.v_n);
+            }
+            if constexpr (MX) r.slot[h] = n;
           }
           return;
         }
         r.draft = -1;
         r.k_row = kp_t;
         r.v_row = vp_t;
+        const int real = t < span.head ? t : t + span.skip;
+        if constexpr (WIN) {
+          r.pos = kTile * real;
+          r.edge = on_edge<WIN>(fresh(), len, r.pos, kTile);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int j = 2 * t + h;
+          const int j = 2 * real + h;
           int col = j >> half_shift, pos = 16 * j;
           const int slot = (j & ((1 << half_shift) - 1)) * 16;
           bool in = true;
@@ -479,17 +574,64 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           in = in && page >= 0 && page < pages;
           r.valid[h] = in ? min(len - pos, 16) : 0;
           const int there = in ? page : 0;
-          r.k[h] = kp + (there * kp_p + (int64_t)(slot * kp_t));
-          r.v[h] = vp + (there * vp_p + (int64_t)(slot * vp_t));
+          if constexpr (MX) {
+            r.slot[h] = slot;
+            r.k[h] = kp + there * kp_p;
+            r.v[h] = vp + there * vp_p;
+          } else {
+            r.k[h] = kp + (there * kp_p + (int64_t)(slot * kp_t));
+            r.v[h] = vp + (there * vp_p + (int64_t)(slot * vp_t));
+          }
         }
         if (r.valid[0] | r.valid[1]) return;
       }
     };
 
     // a new tile of fp32 activations over a 16-bit cache is rounded as it is loaded
-    auto rounds = [&](const Source<T> &r) { return !F32 && act32 && r.draft >= 0; };
+    auto rounds = [&](const Source<E> &r) { return !F32 && !MX && act32 && r.draft >= 0; };
     const int dim = wt.p.dim;
-    auto load_k = [&](const Source<T> &r, Regs &x) {
+    const int page_size = wt.p.page_size;
+    auto load_k = [&](const Source<E> &r, Regs &x) {
+      if constexpr (MX) {
+        constexpr int PD = Regs::PD, PW = Regs::PW, PB = Regs::PB;
+        if (r.draft >= 0) {   // new tokens: as the cache will hold them
+          const_work &w = fresh();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int64_t base = s * w.p.k_s + c * w.p.k_h + (int64_t)(r.slot[h] + min(li, max(r.valid[h], 1) - 1)) * w.p.k_n;
+            x.ke[h] = 0;
+#pragma unroll
+            for (int b = 0; b < PB; ++b) {
+              float y[8 * PW];
+#pragma unroll
+              for (int e = 0; e < PW; ++e) {
+                const int d = PD * g + 8 * (PW * b + e), in = d < dim ? d : 0;
+                load_acts<A>(w.p.k, base + in, act32, reinterpret_cast<float (&)[8]>(y[8 * e]));
+              }
+              uint32_t most = mx_most(y);
+              if constexpr (PD < 32) most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+              const uint32_t e8 = mx_scale_of(most);
+              x.ke[h] |= e8 << (8 * b);
+#pragma unroll
+              for (int e = 0; e < PW; ++e) x.k[h][b][e] = mx_pack(reinterpret_cast<float (&)[8]>(y[8 * e]), e8);
+            }
+          }
+          return;
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int t = r.slot[h] + min(li, max(r.valid[h], 1) - 1);
+            x.ke[h] = 0;
+#pragma unroll
+            for (int b = 0; b < PB; ++b) {
+              const int d = PD * g + 32 * b, in = d < dim ? d : 0;
+              load_words(r.k[h] + (uint32_t)mx_key_code(t, in, dim), x.k[h][b]);
+              x.ke[h] |= (uint32_t)r.k[h][(uint32_t)mx_key_scale(t, in, dim, page_size)] << (8 * b);
+            }
+          }
+          return;
+        }
+      } else {
       const void *base = rounds(r) ? fresh().p.k : nullptr;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -510,8 +652,46 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           }
         }
       }
+      }
     };
-    auto load_v = [&](const Source<T> &r, Regs &x) {
+    auto load_v = [&](const Source<E> &r, Regs &x) {
+      if constexpr (MX) {
+        constexpr int PAIR = VD == 8 ? 1 : 2;   // lanes of a chunk of 8 dimensions
+        if (r.draft >= 0) {
+          const_work &w = fresh();
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int vc = 0; vc < VC; ++vc) {
+              const int d = 16 * VD * vc + 8 * (li / PAIR), in = d < dim ? d : 0;
+              x.ve[h][vc] = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int64_t base = s * w.p.v_s + c * w.p.v_h + (int64_t)(r.slot[h] + min(4 * g + i, max(r.valid[h], 1) - 1)) * w.p.v_n;
+                float y[8];
+                load_acts<A>(w.p.v, base + in, act32, y);
+                uint32_t most = mx_most(y);
+                most = max(most, (uint32_t)__shfl_xor((int)most, PAIR));
+                most = max(most, (uint32_t)__shfl_xor((int)most, 2 * PAIR));
+                const uint32_t e8 = mx_scale_of(most);
+                x.ve[h][vc] |= e8 << (8 * i);
+                x.v[h][vc][i] = mx_pack(y, e8);
+              }
+            }
+          return;
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int vc = 0; vc < VC; ++vc) {
+              const int d = 16 * VD * vc + 8 * (li / PAIR), in = d < dim ? d : 0;
+              const int t = r.slot[h] + 4 * g;
+              load_words(r.v[h] + (uint32_t)mx_value_code(t, in, dim), x.v[h][vc]);
+              x.ve[h][vc] = *reinterpret_cast<const uint32_t *>(r.v[h] + (uint32_t)mx_value_scale(t, in, dim, page_size));
+            }
+          return;
+        }
+      } else {
       const void *base = rounds(r) ? fresh().p.v : nullptr;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -535,10 +715,11 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           }
         }
       }
+      }
     };
 
     Regs x;
-    Source<T> here;
+    Source<E> here;
     int t = t0 + wave;
     find(t, here);
     if (t < t1) {
@@ -569,9 +750,9 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       const int64_t base = s * wq.p.q_s + row_token[rt] * wq.p.q_n + row_head[rt] * wq.p.q_h;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int d = 32 * ks + 8 * g;
+        const int d = MX ? DT / 4 * g + 8 * ks : 32 * ks + 8 * g;
         const bool in = row_ok[rt] && (d < dim);
-        load_acts<T>(wq.p.q, base + (in ? d : 0), act32, y[ks]);
+        load_acts<A>(wq.p.q, base + (in ? d : 0), act32, y[ks]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[ks][j] = in ? y[ks][j] : 0.0f;
       }
@@ -621,10 +802,10 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 
     while (t < t1) {
       int t_next = t + WAVES;
-      Source<T> next;
+      Source<E> next;
       find(t_next, next);
 
-      if (dim < DT) {   // beyond dim: whatever was read meets q = 0, which needs it finite
+      if constexpr (!MX) if (dim < DT) {   // beyond dim: whatever was read meets q = 0, which needs it finite
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
           if (32 * ks + 8 * g >= dim) {
@@ -650,6 +831,24 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
               for (int h = 0; h < 2; ++h)
                 sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[h][ks][j]), q32[rt][ks][j], sc[rt][h], 0, 0, 0);
+      } else if constexpr (MX) {
+        // (dimensions beyond dim hold the first block's values, which meet q = 0)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          u32x4 a[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t word = x.k[h][ks / Regs::PW][ks % Regs::PW];
+            const float scale = mx_scale(x.ke[h] >> (8 * (ks / Regs::PW)) & 255u);
+            a[h] = u32x4{mx_pair<0>(word, scale), mx_pair<1>(word, scale), mx_pair<2>(word, scale), mx_pair<3>(word, scale)};
+          }
+#pragma unroll
+          for (int n = NQ - 1; n >= 0; --n)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) sc[rt][h] = Cache<CT>::mma(a[h], q16[n][rt][ks], sc[rt][h]);
+        }
       } else {
 #pragma unroll
         for (int n = NQ - 1; n >= 0; --n)
@@ -665,9 +864,10 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       }
       if (t_next < t1) load_k(next, x);
 
-      uint32_t odd = 0;   // this lane group's keys with a value that is not finite (new tokens only)
+      uint32_t odd = 0;   // this lane group's keys with a value that is not finite (where rows see different keys)
       uint32_t see[RT];
-      const bool partly = here.draft >= 0 || (here.valid[0] & here.valid[1]) < 16;
+      const bool masked = here.draft >= 0 || (WIN && here.edge);   // rows see different keys
+      const bool partly = masked || (here.valid[0] & here.valid[1]) < 16;
       if (partly) {
         // which of the tile's keys this lane's rows attend to
         const uint32_t there = ((1u << here.valid[0]) - 1) | ((1u << here.valid[1]) - 1) << 16;
@@ -677,11 +877,35 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           if (here.draft >= 0) {
             const int i = row_token[rt] - kTile * here.draft;   // chain: the tokens up to its own
             see[rt] &= tree ? paths.bits[row_token[rt]][here.draft] : (i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1);
+            if (WIN && !tree) {   // (a tree's bits know the window)
+              const_work &w = fresh();
+              see[rt] &= window_bits(row_token[rt] - w.p.window + 1, w.p.sinks - len, kTile * here.draft);
+            }
+          } else if (WIN && here.edge) {
+            const_work &w = fresh();
+            const int depth = tree ? (int)paths.depth[row_token[rt]] : row_token[rt];
+            see[rt] &= window_bits(len - w.p.window + 1 + depth, w.p.sinks, here.pos);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (!(see[rt] >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1)) sc[rt][j >> 2][j & 3] = -INFINITY;
         }
+        if constexpr (MX) {
+          // values behind the last key, and new ones or ones that not every row
+          // sees, of a block that is NaN: any scale will do for a weight of 0, and
+          // NaN is added by hand below
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int vc = 0; vc < VC; ++vc) {
+              const uint32_t e8 = x.ve[j >> 2][vc] >> (8 * (j & 3)) & 255u;
+              const bool behind = 4 * g + (j & 3) >= here.valid[j >> 2];
+              if (e8 == 255u && (behind || masked)) {
+                x.ve[j >> 2][vc] ^= (255u ^ 127u) << (8 * (j & 3));
+                if (!behind) odd |= 1u << (8 * vc + j);
+              }
+            }
+        } else {
         // values behind the last key (a page's unwritten slots): their weight
         // is 0, which needs them finite
 #pragma unroll
@@ -695,7 +919,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
         // a new token's value that is not finite must not reach rows that do
         // not attend to it through 0 * inf: it is taken out of the product
         // here and added by hand below
-        if (here.draft >= 0) {
+        if (masked) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -717,6 +941,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
                   }
                 }
               }
+        }
         }
       }
 
@@ -776,12 +1001,24 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
           for (int i0 = 0; i0 < VD; i0 += 4) {
             u32x4 a[4];   // 8 keys of dimensions i0 ..
+            uint32_t pairs[8][2];   // two dimensions each
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if constexpr (MX) {
+                const float scale = mx_scale(x.ve[j >> 2][vc] >> (8 * (j & 3)) & 255u);
+                const uint32_t word = x.v[j >> 2][vc][j & 3] >> (VD == 8 ? 0 : 16 * (li & 1));
+                pairs[j][0] = i0 ? mx_pair<2>(word, scale) : mx_pair<0>(word, scale);
+                pairs[j][1] = i0 ? mx_pair<3>(word, scale) : mx_pair<1>(word, scale);
+              } else {
+                pairs[j][0] = x.v[j][vc][i0 / 2];
+                pairs[j][1] = x.v[j][vc][i0 / 2 + 1];
+              }
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                a[i][e] = __builtin_amdgcn_perm(x.v[2 * e + 1][vc][(i0 + i) / 2], x.v[2 * e][vc][(i0 + i) / 2],
-                                                i & 1 ? 0x07060302u : 0x05040100u);
+                a[i][e] = __builtin_amdgcn_perm(pairs[2 * e + 1][i / 2], pairs[2 * e][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
             for (int n = NW - 1; n >= 0; --n)
 #pragma unroll
@@ -796,6 +1033,21 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
         const_work &w = fresh();
         for (int key = 0; key < kTile; ++key) {   // the values taken out, by hand
           const int j = 4 * (key >> 4) + (key & 3), from = (key & 15) >> 2;
+          if constexpr (MX) {   // (all of a block at once: bit 8 vc + j of the lane that holds it)
+            if (!__any(g == from && (odd & (0x01010101u << j)) != 0)) continue;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t theirs = (uint32_t)__shfl((int)odd, 4 * g + r + 16 * from);
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int vc = 0; vc < VC; ++vc)
+                  if ((theirs >> (8 * vc + j) & 1) && (see[rt] >> key & 1)) {
+#pragma unroll
+                    for (int i = 0; i < VD; ++i) o[rt][vc][i][r] = NAN;
+                  }
+            }
+          } else {
           if (!__any(g == from && (odd >> j & 1))) continue;
           const int n = min(kTile * here.draft + key, w.p.draft - 1);
           const int64_t row = s * w.p.v_s + c * w.p.v_h + n * w.p.v_n;
@@ -812,13 +1064,18 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
               for (int r = 0; r < 4; ++r) {
                 const int d = 16 * VD * vc + VD * (4 * g + r);
                 float y[VD];
-                load_acts<T>(w.p.v, row + (d < dim ? d : 0), act32, y);
+                if (!WIN || here.draft >= 0) {
+                  load_acts<T>(w.p.v, row + (d < dim ? d : 0), act32, y);
+                } else {   // (a cached one)
+                  load_acts<T>(key & 16 ? here.v[1] : here.v[0], (int64_t)(key & 15) * here.v_row + (d < dim ? d : 0), false, y);
+                }
 #pragma unroll
                 for (int i = 0; i < VD; ++i) {
                   const float z = (float)(T)y[i];
                   if (!(fabsf(z) < INFINITY)) o[rt][vc][i][r] += weight * z;
                 }
               }
+          }
           }
         }
       }
@@ -905,7 +1162,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
             } else if constexpr (!F32) {
 #pragma unroll
               for (int i = 0; i < VD; i += 4)
-                *reinterpret_cast<u32x2 *>(static_cast<T *>(w.p.out) + out + d + i) = u32x2{pack2<T>(y[i], y[i + 1]), pack2<T>(y[i + 2], y[i + 3])};
+                *reinterpret_cast<u32x2 *>(static_cast<A *>(w.p.out) + out + d + i) = u32x2{pack2<A>(y[i], y[i + 1]), pack2<A>(y[i + 2], y[i + 3])};
             }
           }
       }
@@ -976,7 +1233,7 @@ __device__ __forceinline__ void copies_landed() {
 
 constexpr int kWideSpots = 512;
 
-template <int CT, int NQ, int NW, int DT>
+template <int CT, int NQ, int NW, int DT, bool WIN>
 __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork) {
   typedef typename Cache<CT>::T T;
   constexpr int TK = 64, NH = 4;               // keys of a tile, its parts of 16
@@ -994,6 +1251,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
   __shared__ Paths paths;
   __shared__ uint32_t spots[kWideSpots];
   __shared__ uint32_t odd_keys[kMaxDraft / TK][2];   // new tokens with a value that is not finite, by tile
+  __shared__ uint32_t odd_edge[WIN ? 2 : 1];         // keys of a tile on a window's edge with such a value
 
   const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1002,7 +1260,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
   const bool whole = fresh().whole;
   if (!whole) {
     const_work &w = fresh();
-    scan_tiles(w, first, wave_sums);
+    scan_tiles<WIN>(w, first, wave_sums);
     const Plan plan = plan_of(w, first);
     if (me >= plan.count) return;
     const int xcd = me & 7, per = plan.count >> 3, rest = plan.count & 7;
@@ -1018,14 +1276,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
       s = (int)((uint32_t)me / (uint32_t)w.items);
       item = me - s * w.items;
       len = clamp_len(w, s);
-      tiles = tiles_of(w, len);
+      tiles = tiles_of<WIN>(w, len);
       t0 = 0;
       t1 = tiles;
       at = end;
     } else {
       s = sequence_of(w, first, at);
       len = clamp_len(w, s);
-      tiles = tiles_of(w, len);
+      tiles = tiles_of<WIN>(w, len);
       const int in_seq = at - __builtin_amdgcn_readfirstlane(first[s]) * w.items;
       item = (int)((uint32_t)in_seq / (uint32_t)tiles);
       t0 = in_seq - item * tiles;
@@ -1042,9 +1300,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
     const bool has_draft = t1 > cached;
     const bool tree = w.p.parents != nullptr;
     const int dim = w.p.dim;
-    if (has_draft && tree && paths_of != s) {
+    const Span span = span_of<WIN>(w, len);
+    if ((has_draft || WIN) && tree && paths_of != s) {
       __syncthreads();
-      build_paths(w, s, paths);
+      build_paths<WIN>(w, s, len, paths);
       paths_of = s;
     }
 
@@ -1053,7 +1312,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
     auto stage = [&](int c0, int c1) {
       const_work &w = fresh();
       const int32_t *table = w.p.table + s * w.p.table_s;
-      for (int j = NH * c0 + (int)threadIdx.x; j < NH * min(c1, cached); j += kThreads) {
+      for (int at = NH * c0 + (int)threadIdx.x; at < NH * min(c1, cached); at += kThreads) {
+        const int j = at < NH * span.head ? at : at + NH * span.skip;
         int col = j >> w.half_shift, pos = 16 * j;
         bool in = true;
         if (sel) {
@@ -1068,7 +1328,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
         in = in && pos < len;
         const int page = in ? table[col] : -1;
         in = in && page >= 0 && page < w.p.pages;
-        spots[j - NH * c0] = in ? (uint32_t)page * 32u + (uint32_t)min(len - pos, 16) : 0u;
+        spots[at - NH * c0] = in ? (uint32_t)page * 32u + (uint32_t)min(len - pos, 16) : 0u;
       }
     };
     stage(t0, min(t1, t0 + kWideSpots / NH));
@@ -1134,8 +1394,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
       const_work &w = fresh();
       const uint32_t k_lds = lds0 + (uint32_t)(to * 2 * SIDE + wave * PART), v_lds = k_lds + SIDE;
       if (t < cached) {
-        const int j = NH * t + wave, slot = (j & half_mask) * 16;
-        const int page = (int)(__builtin_amdgcn_readfirstlane(spots[j - NH * c0]) >> 5);
+        const int j = NH * (t < span.head ? t : t + span.skip) + wave, slot = (j & half_mask) * 16;
+        const int page = (int)(__builtin_amdgcn_readfirstlane(spots[NH * (t - c0) + wave]) >> 5);
         const T *kb = static_cast<const T *>(w.p.k_pages) + (c * w.p.kp_h + page * w.p.kp_p + slot * w.p.kp_t);
         const T *vb = static_cast<const T *>(w.p.v_pages) + (c * w.p.vp_h + page * w.p.vp_p + slot * w.p.vp_t);
 #pragma unroll
@@ -1209,7 +1469,35 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
         const uint32_t k_lds = lds0 + (uint32_t)(buffer * 2 * SIDE), v_lds = k_lds + SIDE;
         const int draft = t >= cached ? t - cached : -1;
         int fewest = valid[0] & valid[1] & valid[2] & valid[3];
-        const bool partly = draft >= 0 || fewest < 16;
+        const int pos = TK * (t < span.head ? t : t + span.skip);
+        const bool edge = WIN && draft < 0 && on_edge<WIN>(fresh(), len, pos, TK);
+        const bool partly = draft >= 0 || edge || fewest < 16;
+        if (WIN && edge) {
+          // a value that is not finite must not reach rows that do not see its
+          // key: set aside, as a new token's is
+          if (threadIdx.x < 2) odd_edge[threadIdx.x] = 0;
+          __syncthreads();
+#pragma unroll 1
+          for (int i = 0; i < SIDE / (16 * kThreads); ++i) {
+            const int chunk = i * kThreads + (int)threadIdx.x, r = chunk / CH;
+            u32x4 x = *(lds_u32x4 *)(uintptr_t)(v_lds + chunk * 16);
+            constexpr uint32_t kExp = CT == KH_TYPE_BF16 ? 0x7f80u : 0x7c00u;
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool lo = (x[e] & kExp) == kExp, hi = (x[e] >> 16 & kExp) == kExp;
+              odd |= lo | hi;
+              x[e] = (lo ? 0u : x[e] & 0xffffu) | (hi ? 0u : x[e] & 0xffff0000u);
+            }
+            const int there = r < 16 ? valid[0] : r < 32 ? valid[1] : r < 48 ? valid[2] : valid[3];
+            const int d = 8 * ((chunk % CH) ^ swz_wide<DT>(r));
+            if (odd) {
+              *(lds_u32x4 *)(uintptr_t)(v_lds + chunk * 16) = x;
+              if ((r & 15) < there && d < dim) atomicOr(&odd_edge[r >> 5], 1u << (r & 31));
+            }
+          }
+          __syncthreads();
+        }
         if (draft < 0 && fewest < 16) {
           // values behind the last key (a page's unwritten slots): their weight
           // is 0, which needs them finite
@@ -1259,6 +1547,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
               const int word = 2 * draft + kb, i = row_token - 32 * word;   // chain: the tokens up to its own
               see[kb] &= tree ? (word < kMaxDraft / 32 ? paths.bits[row_token][word] : 0u)
                               : (i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1);
+              if (WIN && !tree) {   // (a tree's bits know the window)
+                const_work &w = fresh();
+                see[kb] &= window_bits(row_token - w.p.window + 1, w.p.sinks - len, 32 * word);
+              }
+            } else if (WIN && edge) {
+              const_work &w = fresh();
+              const int depth = tree ? (int)paths.depth[row_token] : row_token;
+              see[kb] &= window_bits(len - w.p.window + 1 + depth, w.p.sinks, pos + 32 * kb);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -1325,8 +1621,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
           if (i & 1) __builtin_amdgcn_sched_barrier(0);
         }
 
-        if (draft >= 0) {
-          const uint32_t odd[2] = {odd_keys[draft][0], odd_keys[draft][1]};
+        if (draft >= 0 || (WIN && edge)) {
+          const uint32_t *set_aside = !WIN || draft >= 0 ? odd_keys[draft] : odd_edge;
+          const uint32_t odd[2] = {set_aside[0], set_aside[1]};
           if (__builtin_expect(__any((odd[0] | odd[1]) != 0), 0)) {
             const_work &w = fresh();
             for (int key = 0; key < TK; ++key) {   // the values set aside, by hand
@@ -1337,14 +1634,19 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
               for (int r = 0; r < 32; ++r) mine = r == 16 * (key >> 5) + reg ? sc[r >> 4][r & 15] : mine;
               const float weight = __shfl(mine, row + 32 * from);
               if (!((key >> 5 ? see[1] : see[0]) >> kk & 1)) continue;
-              const int64_t from_row = s * w.p.v_s + c * w.p.v_h + (int64_t)(TK * draft + key) * w.p.v_n;
+              int64_t from_row = s * w.p.v_s + c * w.p.v_h + (int64_t)(TK * draft + key) * w.p.v_n;
+              if (WIN && draft < 0) {   // a cached one
+                const int64_t page = spots[NH * (t - c0) + (key >> 4)] >> 5;
+                const int slot = ((pos + key) & (w.p.page_size - 1));
+                from_row = c * w.p.vp_h + page * w.p.vp_p + slot * w.p.vp_t;
+              }
 #pragma unroll
               for (int t2 = 0; t2 < NT; ++t2)
 #pragma unroll
                 for (int a = 0; a < 4; ++a) {
                   const int d = 32 * t2 + 8 * a + 4 * half;
                   float y[4];
-                  load_acts<T>(w.p.v, from_row + (d < dim ? d : 0), act32, y);
+                  load_acts<T>(!WIN || draft >= 0 ? w.p.v : w.p.v_pages, from_row + (d < dim ? d : 0), (!WIN || draft >= 0) && act32, y);
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
                     const float z = (float)(T)y[e];
@@ -1408,10 +1710,10 @@ __global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(const PagedWo
   const kh_paged &p = w.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  scan_tiles(w, first, wave_sums);
+  scan_tiles<true>(w, first, wave_sums);
   const Plan plan = plan_of(w, first);
   const int s = blockIdx.x / w.items, item = blockIdx.x - s * w.items;
-  const int tiles = tiles_of(w, clamp_len(w, s));
+  const int tiles = tiles_of<true>(w, clamp_len(w, s));
   const int x = first[s] * w.items + item * tiles;
   const int w0 = range_of(plan, x), w1 = range_of(plan, x + tiles - 1);
   if (w0 == w1) return;
@@ -1470,10 +1772,10 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
   const kh_paged &p = w.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  scan_tiles(w, first, wave_sums);
+  scan_tiles<true>(w, first, wave_sums);
   const Plan plan = plan_of(w, first);
   const int s = blockIdx.x / w.items, item = blockIdx.x - s * w.items;
-  const int tiles = tiles_of(w, clamp_len(w, s));
+  const int tiles = tiles_of<true>(w, clamp_len(w, s));
   const int x = first[s] * w.items + item * tiles;
   const int w0 = range_of(plan, x), w1 = range_of(plan, x + tiles - 1);
   if (w0 == w1) return;   // finished by its one range
@@ -1536,41 +1838,47 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
   }
 }
 
-template <int CT, int NQ, int NW, int DT, int RT>
+template <int CT, int NQ, int NW, int DT, int RT, bool WIN>
 void launch_both(const PagedWork &w, hipStream_t stream) {
   if (w.whole) {
-    paged_attn_kernel<CT, NQ, NW, DT, RT, true><<<w.grid, 64 * paged_waves(DT, RT, true), 0, stream>>>(w);
+    paged_attn_kernel<CT, NQ, NW, DT, RT, true, WIN><<<w.grid, 64 * paged_waves(DT, RT, true), 0, stream>>>(w);
   } else {
-    paged_attn_kernel<CT, NQ, NW, DT, RT, false><<<w.grid, kThreads, 0, stream>>>(w);
+    paged_attn_kernel<CT, NQ, NW, DT, RT, false, WIN><<<w.grid, kThreads, 0, stream>>>(w);
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)std::min(w.rows, 16 * RT));
     paged_join_kernel<DT, RT><<<grid, kThreads, 0, stream>>>(w);
   }
 }
 
-template <int CT, int NQ, int NW, int DT>
+template <int CT, int NQ, int NW, int DT, bool WIN>
 void launch_wide(const PagedWork &w, hipStream_t stream) {
-  paged_wide_kernel<CT, NQ, NW, DT><<<w.grid, kThreads, 0, stream>>>(w);
+  paged_wide_kernel<CT, NQ, NW, DT, WIN><<<w.grid, kThreads, 0, stream>>>(w);
   if (!w.whole) {
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)((std::min(w.rows, 32 * kWaves) + kWaves - 1) / kWaves));
     paged_join_rows_kernel<DT><<<grid, kThreads, 0, stream>>>(w);
   }
 }
 
-template <int CT, int NQ, int NW>
-hipError_t launch_passes(const PagedWork &w, int dt, int rt, hipStream_t stream) {
-  if (dt == 256) launch_both<CT, NQ, NW, 256, 1>(w, stream);
+template <int CT, int NQ, int NW, bool WIN>
+void launch_sizes(const PagedWork &w, int dt, int rt, hipStream_t stream) {
+  if (dt == 256) launch_both<CT, NQ, NW, 256, 1, WIN>(w, stream);
   else if (rt == kWideBlocks) {
-    if constexpr (CT != KH_TYPE_F32) {
-      if (dt == 128) launch_wide<CT, NQ, NW, 128>(w, stream);
-      else launch_wide<CT, NQ, NW, 64>(w, stream);
+    if constexpr (CT != KH_TYPE_F32 && CT != KH_TYPE_MX4) {
+      if (dt == 128) launch_wide<CT, NQ, NW, 128, WIN>(w, stream);
+      else launch_wide<CT, NQ, NW, 64, WIN>(w, stream);
     }
   } else if (dt == 128) {
-    if (rt == 1) launch_both<CT, NQ, NW, 128, 1>(w, stream);
-    else launch_both<CT, NQ, NW, 128, 2>(w, stream);
+    if (rt == 1) launch_both<CT, NQ, NW, 128, 1, WIN>(w, stream);
+    else launch_both<CT, NQ, NW, 128, 2, WIN>(w, stream);
   } else {
-    if (rt == 1) launch_both<CT, NQ, NW, 64, 1>(w, stream);
-    else launch_both<CT, NQ, NW, 64, 2>(w, stream);
+    if (rt == 1) launch_both<CT, NQ, NW, 64, 1, WIN>(w, stream);
+    else launch_both<CT, NQ, NW, 64, 2, WIN>(w, stream);
   }
+}
+
+template <int CT, int NQ, int NW>
+hipError_t launch_passes(const PagedWork &w, int dt, int rt, hipStream_t stream) {
+  if (w.p.window) launch_sizes<CT, NQ, NW, true>(w, dt, rt, stream);
+  else launch_sizes<CT, NQ, NW, false>(w, dt, rt, stream);
   return hipGetLastError();
 }
 

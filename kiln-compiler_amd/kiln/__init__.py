@@ -17,7 +17,8 @@ HIP kernel family from libkiln_hip.so, replayed as one hipGraph.
 from kiln.api import CompiledModule, Options, Report, compile, compile_graph
 from kiln.backend import backend, stats
 from kiln.cache import PagedCache
-from kiln.hip.paged import cache_append, copy_pages, select_pages, selected_attention, tree_attention
+from kiln.hip.paged import cache_append, cache_read, copy_pages, select_pages, selected_attention, tree_attention
 
 __all__ = ["compile", "compile_graph", "Options", "Report", "CompiledModule", "backend", "stats",
-           "PagedCache", "tree_attention", "select_pages", "selected_attention", "cache_append", "copy_pages"]
+           "PagedCache", "tree_attention", "select_pages", "selected_attention", "cache_append", "cache_read",
+           "copy_pages"]

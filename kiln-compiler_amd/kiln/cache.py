@@ -31,18 +31,25 @@ from kiln.hip.interpret import interpreting
 class PagedCache:
     """The pages ``k`` and ``v`` ``[layers, pages, kv_heads, page_size, dim]``,
     with ``means=True`` the pages' mean keys ``means`` ``[layers, pages,
-    kv_heads, dim]`` (what ``select_pages`` reads), and their book-keeping."""
+    kv_heads, dim]`` (what ``select_pages`` reads), and their book-keeping.
+    ``dtype``: fp32, bf16, fp16, or ``torch.float4_e2m1fn_x2`` for pages of 4
+    bits (uint8 ``[layers, pages, kv_heads, page_size, 17 * dim // 32]``: codes
+    and the scales of every 32 dimensions, kiln/hip/paged.py)."""
 
     def __init__(self, layers, pages, page_size, kv_heads, dim, dtype=torch.bfloat16, means=False, device=None):
         for name, n in (("layers", layers), ("pages", pages), ("kv_heads", kv_heads)):
             if n < 1:
                 raise ValueError(f"{name} must be at least 1, got {n}")
-        if dtype not in paged.TYPES:
-            raise TypeError(f"dtype must be one of {', '.join(map(str, paged.TYPES))}, got {dtype}")
+        packed = dtype == torch.float4_e2m1fn_x2
+        if dtype not in paged.TYPES and not packed:
+            raise TypeError(f"dtype must be one of {', '.join(map(str, paged.TYPES))}, {torch.float4_e2m1fn_x2}, got {dtype}")
         if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
             raise NotImplementedError(f"page_size {page_size}: powers of two from 16 to 1024 have kernels")
         if dim < 8 or dim % 8 or dim > 256:
             raise NotImplementedError(f"dim {dim}: multiples of 8 up to 256 have kernels")
+        if packed and dim % paged.BLOCK:
+            raise NotImplementedError(f"dim {dim}: multiples of {paged.BLOCK} up to 256 have kernels over 4-bit pages")
+        row = dim // paged.BLOCK * paged.BLOCK_BYTES if packed else dim   # elements of a token's row
         if device is None:
             from kiln.hip.runtime import device as gpu
 
@@ -51,12 +58,14 @@ class PagedCache:
         if self.device.type == "cuda":
             from kiln.hip.runtime import check_memory
 
-            size = torch.empty(0, dtype=dtype).element_size()
-            need = layers * pages * kv_heads * dim * (2 * page_size * size + (4 if means else 0))
+            size = 1 if packed else torch.empty(0, dtype=dtype).element_size()
+            need = layers * pages * kv_heads * (2 * page_size * size * row + (4 * dim if means else 0))
             check_memory(self.device, need, f"the cache's {pages} pages")
         self.page_size = page_size
         self.pages = pages
-        self.k = torch.zeros((layers, pages, kv_heads, page_size, dim), dtype=dtype, device=self.device)
+        self.dim = dim
+        self.k = torch.zeros((layers, pages, kv_heads, page_size, row), dtype=torch.uint8 if packed else dtype,
+                             device=self.device)
         self.device = self.k.device              # ("cuda" alone follows the current device)
         self.v = torch.zeros_like(self.k)
         self.means = torch.zeros((layers, pages, kv_heads, dim), dtype=torch.float32, device=self.device) if means else None
@@ -171,7 +180,8 @@ class PagedCache:
             raise ValueError("a sequence is named twice")
         for s in seqs:
             self._known(s)
-        layers, _, kv_heads, _, dim = self.k.shape
+        layers, _, kv_heads, _, _ = self.k.shape
+        dim = self.dim
         if k.dim() != 5 or tuple(k.shape) != (layers, len(seqs), k.shape[2], kv_heads, dim):
             raise ValueError(f"k must have shape ({layers}, {len(seqs)}, tokens, {kv_heads}, {dim}), got {tuple(k.shape)}")
         if v.shape != k.shape or v.dtype != k.dtype:
@@ -238,6 +248,16 @@ class PagedCache:
         for s, n, have in zip(seqs, counts, plans):
             self._pages[s] = have
             self._length[s] += n
+
+    def read(self, seqs, dtype=None):
+        """The tokens of ``seqs`` as dense tensors ``(k, v)``, ``[layers,
+        sequences, longest, kv_heads, dim]``, zeros behind each one's last:
+        what ``append`` takes, of another cache too. ``dtype`` as for
+        ``kiln.cache_read``."""
+        seqs = list(seqs)
+        table, lengths = self.batch(seqs)
+        return paged.cache_read(self.k, self.v, table, torch.zeros_like(lengths), lengths,
+                                tokens=max([0] + [self._length[s] for s in seqs]), dtype=dtype)
 
     # -- pages --------------------------------------------------------------------------------------
 

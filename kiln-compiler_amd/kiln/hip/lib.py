@@ -23,7 +23,7 @@ MAX_PASSES = 8
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP, ERR_NO_DEVICE, ERR_CAPACITY = range(6)
 BASE_INPUT, BASE_OUTPUT, BASE_CONST, BASE_ARENA, BASE_WORKSPACE = range(5)
 FAM_EW, FAM_ROW, FAM_GEMM, FAM_GEMV, FAM_RED, FAM_ATTN, FAM_PAGED = 1, 2, 3, 4, 5, 6, 7
-TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2   # KH_TYPE_*: elements of a paged cache and of the activations next to it
+TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_MX4 = 0, 1, 2, 3   # KH_TYPE_*: elements of a paged cache and of the activations next to it
 PAGED_ATTENTION, PAGED_SELECT = 0, 1      # KH_PAGED_*
 ATTN_MASK_NONE, ATTN_MASK_CAUSAL, ATTN_MASK_ADD = 0, 1, 2
 GEMV_PRO_NONE, GEMV_PRO_LAYERNORM, GEMV_PRO_ATTN = 0, 1, 2
@@ -77,7 +77,8 @@ class Paged(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in
                    ("q_s", "q_n", "q_h", "k_s", "k_n", "k_h", "v_s", "v_n", "v_h", "o_s", "o_n", "o_h",
                     "kp_p", "kp_h", "kp_t", "vp_p", "vp_h", "vp_t", "m_p", "m_h",
-                    "table_s", "parents_s", "sel_s", "sel_n", "sel_h")])
+                    "table_s", "parents_s", "sel_s", "sel_n", "sel_h")]
+                + [("window", ctypes.c_int32), ("sinks", ctypes.c_int32)])
 
 
 class CacheAppend(ctypes.Structure):
@@ -89,6 +90,14 @@ class CacheAppend(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in
                    ("k_l", "k_s", "k_n", "k_h", "v_l", "v_s", "v_n", "v_h", "kp_l", "kp_p", "kp_h", "kp_t",
                     "vp_l", "vp_p", "vp_h", "vp_t", "m_l", "m_p", "m_h", "table_s", "rows_s")])
+
+
+class CacheRead(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in
+                 ("layers", "batch", "tokens", "kv_heads", "dim", "page_size", "pages", "width", "cache_type", "out_type")]
+                + [(n, ctypes.c_void_p) for n in ("k_pages", "v_pages", "k", "v", "table", "starts", "ends")]
+                + [(n, ctypes.c_int64) for n in
+                   ("kp_l", "kp_p", "kp_h", "kp_t", "vp_l", "vp_p", "vp_h", "vp_t", "table_s")])
 
 
 class Pool(ctypes.Structure):
@@ -150,6 +159,9 @@ def load():
         "kh_paged_host": (ip, [ctypes.POINTER(Paged)]),
         "kh_cache_append": (ip, [ctypes.POINTER(CacheAppend), vp]),
         "kh_cache_append_host": (ip, [ctypes.POINTER(CacheAppend)]),
+        "kh_decode_sizes": (ip, [ctypes.POINTER(ctypes.c_size_t)]),
+        "kh_cache_read": (ip, [ctypes.POINTER(CacheRead), vp]),
+        "kh_cache_read_host": (ip, [ctypes.POINTER(CacheRead)]),
         "kh_cache_copy": (ip, [ctypes.POINTER(Pool), ip, i32, ctypes.POINTER(i32), ctypes.POINTER(i32), ip, vp]),
         "kh_cache_copy_host": (ip, [ctypes.POINTER(Pool), ip, i32, ctypes.POINTER(i32), ctypes.POINTER(i32), ip]),
         "kh_probe_attn_timeline": (ip, [vp, vp, vp, vp, ip, ip, ip, ctypes.POINTER(ctypes.c_int64), ip,
@@ -171,6 +183,10 @@ def load():
     mine = (ctypes.sizeof(Paged), ctypes.sizeof(CacheAppend), ctypes.sizeof(Pool))
     if tuple(paged) != mine:
         raise RuntimeError(f"libkiln_hip's paged structures {tuple(paged)} != binding {mine}; rebuild")
+    decode = (ctypes.c_size_t * 1)()
+    lib.kh_decode_sizes(decode)
+    if tuple(decode) != (ctypes.sizeof(CacheRead),):
+        raise RuntimeError(f"libkiln_hip's structures of decoding {tuple(decode)} != binding; rebuild")
     _lib = lib
     return lib
 
@@ -182,7 +198,7 @@ EXPORTED = ("kh_version", "kh_build_id", "kh_abi_sizes", "kh_last_error", "kh_in
             "kh_plan_capture", "kh_plan_replay", "kh_plan_time", "kh_plan_chains", "kh_plan_chain_timeouts",
             "kh_plan_chain_spin",
             "kh_plan_destroy", "kh_paged_sizes", "kh_paged_workspace_bytes", "kh_paged_run", "kh_paged_host",
-            "kh_cache_append", "kh_cache_append_host", "kh_cache_copy", "kh_cache_copy_host",
+            "kh_cache_append", "kh_cache_append_host", "kh_decode_sizes", "kh_cache_read", "kh_cache_read_host", "kh_cache_copy", "kh_cache_copy_host",
             "kh_probe_attn_timeline", "kh_probe_mfma_valu")
 
 

@@ -5,12 +5,21 @@
     select_pages        the pages a cheap score picks for each drafted token
     selected_attention  tree_attention over those pages alone
     cache_append        new tokens' keys and values written into the pages
+    cache_read          cached tokens' keys and values as dense tensors
     copy_pages          whole pages copied within the pools
 
 A cache's pages are ``k_pages`` and ``v_pages``, ``[pages, kv_heads,
 page_size, dim]`` in fp32, bf16 or fp16; token t of sequence s lies in page
 ``table[s, t // page_size]`` at slot ``t % page_size``, for ``t < lengths[s]``
 (int32 both). ``kiln.PagedCache`` keeps such a cache and its book-keeping.
+
+Pages of 4 bits are uint8, ``[pages, kv_heads, page_size, 17 * dim // 32]``, dim
+a multiple of 32: 32 adjacent dimensions of a token share a power of two, an
+element is a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6 times it (17 / 64 of the
+bytes of bf16). The last two dimensions are one block of bytes, whose order is
+the kernels' own (include/kiln_hip.h, kh_cache_append): ``cache_append`` writes
+it, ``cache_read`` gives the values. A block with a value that is not finite is
+NaN.
 
 The first three are also what a model given to ``kiln.compile`` or
 ``torch.compile(backend=kiln.backend)`` may call: they are the operators
@@ -45,6 +54,9 @@ _is_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatc
 _increment_version = torch._C._increment_version
 
 TYPES = {torch.float32: kl.TYPE_F32, torch.bfloat16: kl.TYPE_BF16, torch.float16: kl.TYPE_F16}
+CACHE_TYPES = {**TYPES, torch.uint8: kl.TYPE_MX4}
+BLOCK = 32           # dimensions under one power of two in 4-bit pages
+BLOCK_BYTES = 17     # and their bytes: 32 codes and the scale
 
 
 # -- checks --------------------------------------------------------------------------------
@@ -91,14 +103,26 @@ def _one_device(first, *others):
 
 def check_pages(k_pages, v_pages, rank=4):
     """The pages of one layer (rank 4) or of a stack of layers (rank 5)."""
-    _tensor(k_pages, "k_pages", rank, tuple(TYPES))
+    _tensor(k_pages, "k_pages", rank, tuple(CACHE_TYPES))
     _tensor(v_pages, "v_pages", rank, (k_pages.dtype,))
     _shape(v_pages, "v_pages", k_pages.shape)
+    if k_pages.dtype == torch.uint8 and (k_pages.shape[-1] % BLOCK_BYTES or not k_pages.shape[-1]):
+        raise ValueError(f"4-bit pages have 17 bytes a token for every 32 dimensions, got {k_pages.shape[-1]}")
+
+
+def page_dim(k_pages):
+    """The head dimension of pages."""
+    return k_pages.shape[-1] // BLOCK_BYTES * BLOCK if k_pages.dtype == torch.uint8 else k_pages.shape[-1]
 
 
 def _rows_in_place(t, name):
-    """Pages are read where they are: rows along the last dimension, each at a multiple of 16 bytes."""
+    """Pages are read where they are: rows along the last dimension, each at a multiple of 16 bytes; 4-bit pages
+    of a head in one block."""
     size = t.element_size()
+    if t.dtype == torch.uint8:
+        if t.stride(-1) != 1 or t.stride(-2) != t.shape[-1] or t.data_ptr() % 16 or any(s % 16 for s, n in zip(t.stride()[:-2], t.shape) if n > 1):
+            raise ValueError(f"{name}: 4-bit pages of a head must be contiguous and start at multiples of 16 bytes")
+        return
     if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
         raise ValueError(f"{name}: rows must be contiguous and start at multiples of 16 bytes")
 
@@ -122,11 +146,13 @@ def _head_dim(dim):
         raise NotImplementedError(f"head dimension {dim}: multiples of 8 up to 256 have kernels")
 
 
-def check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected):
+def check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, window=0, sinks=0):
     """(sizes of the call) after checking types, shapes and their agreement."""
     check_pages(k_pages, v_pages)
-    pages, kv_heads, page_size, dim = k_pages.shape
-    _tensor(q, "q", 4, (torch.float32,) if k_pages.dtype == torch.float32 else (torch.float32, k_pages.dtype))
+    pages, kv_heads, page_size, _ = k_pages.shape
+    dim = page_dim(k_pages)
+    _tensor(q, "q", 4, tuple(TYPES) if k_pages.dtype == torch.uint8 else
+            (torch.float32,) if k_pages.dtype == torch.float32 else (torch.float32, k_pages.dtype))
     batch, draft, heads, _ = q.shape
     _shape(q, "q", (batch, draft, heads, dim))
     _head_dim(dim)
@@ -147,6 +173,10 @@ def check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected
         _int32(selected, "selected", 4, (batch, draft, kv_heads, selected.shape[3]))
         if selected.shape[3] == 0:
             raise ValueError("selected names no pages")
+        if window:
+            raise ValueError("picked pages take no window")
+    if not 0 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31 or (sinks and not window):
+        raise ValueError(f"a window of {window} tokens and {sinks} sinks")
     return batch, draft, heads, kv_heads, dim, page_size, pages
 
 
@@ -169,7 +199,7 @@ def check_select(q, k_means, table, lengths, page_size, pages):
 
 
 def default_scale(scale, dim):
-    return 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    return 1.0 / math.sqrt(max(dim, 1)) if scale is None else float(scale)
 
 
 # -- running -------------------------------------------------------------------------------------
@@ -244,10 +274,10 @@ def _launch(op: kl.Paged, size: int, device, what: str):
         kl.check(rc, what)
 
 
-def _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale):
+def _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, window, sinks):
     """(descriptor without addresses) of a call, checked; operands' rows are in place."""
     batch, draft, heads, kv_heads, dim, page_size, pages = check_attention(
-        q, k, v, k_pages, v_pages, table, lengths, parents, selected)
+        q, k, v, k_pages, v_pages, table, lengths, parents, selected, window, sinks)
     _one_device(q, k, v, k_pages, v_pages, table, lengths, parents, selected)
     _rows_in_place(k_pages, "k_pages")
     _rows_in_place(v_pages, "v_pages")
@@ -256,15 +286,15 @@ def _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected
     _ready(q.device)
     h, d = heads * dim, dim
     return kl.Paged(kl.PAGED_ATTENTION, batch, draft, heads, kv_heads, dim, page_size, pages, table.shape[1],
-                    0 if selected is None else selected.shape[3], TYPES[k_pages.dtype], TYPES[q.dtype], 0, scale,
+                    0 if selected is None else selected.shape[3], CACHE_TYPES[k_pages.dtype], TYPES[q.dtype], 0, scale,
                     None, None, None, None, None, None, None, None, None, None, None,
                     *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], draft * h, h, d,
                     *k_pages.stride()[:3], *v_pages.stride()[:3], 0, 0, table.stride(0),
                     0 if parents is None else parents.stride(0),
-                    *((0, 0, 0) if selected is None else selected.stride()[:3]))
+                    *((0, 0, 0) if selected is None else selected.stride()[:3]), window, sinks)
 
 
-def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what):
+def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what, window=0, sinks=0):
     try:
         key = ("attention", q.shape, q.dtype, q.stride(), q.get_device(), k.shape, k.dtype, k.stride(), k.get_device(),
                v.shape, v.dtype, v.stride(), v.get_device(), k_pages.shape, k_pages.dtype, k_pages.stride(),
@@ -273,13 +303,13 @@ def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, 
                lengths.stride(), lengths.get_device(),
                None if parents is None else (parents.shape, parents.dtype, parents.stride(), parents.get_device()),
                None if selected is None else (selected.shape, selected.dtype, selected.stride(), selected.get_device()),
-               scale)
+               scale, window, sinks)
     except AttributeError:
         check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected)   # names what is no tensor
         raise
     found = _forms.get(key)
     if found is None:
-        check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected)
+        check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, window, sinks)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad
                                     or v_pages.requires_grad):
         _no_grad(q, k, v, k_pages, v_pages)
@@ -287,11 +317,11 @@ def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, 
         straight = [_rows_strided(t) for t in (q, k, v)] + [_columns(t) for t in (table, lengths)]
         if any(a is not b for a, b in zip(straight, (q, k, v, table, lengths))):
             q, k, v, table, lengths = straight
-            return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what)
+            return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what, window, sinks)
         if (parents is not None and _columns(parents) is not parents) or (selected is not None and _columns(selected) is not selected):
             parents, selected = (None if t is None else _columns(t) for t in (parents, selected))
-            return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what)
-        op = _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale)
+            return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, what, window, sinks)
+        op = _attention_form(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, window, sinks)
         if q.numel() == 0:
             return torch.empty(q.shape, dtype=q.dtype, device=q.device)
         found = _remember(key, op)
@@ -303,7 +333,8 @@ def run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, 
     if (at[0] | at[1] | at[2] | at[3] | at[4]) & 15:
         _rows_in_place(k_pages, "k_pages")
         _rows_in_place(v_pages, "v_pages")
-        return run_attention(_rows(q), _rows(k), _rows(v), k_pages, v_pages, table, lengths, parents, selected, scale, what)
+        return run_attention(_rows(q), _rows(k), _rows(v), k_pages, v_pages, table, lengths, parents, selected, scale, what,
+                             window, sinks)
     op.q, op.k, op.v, op.k_pages, op.v_pages = at
     op.table, op.lengths, op.out = table.data_ptr(), lengths.data_ptr(), out.data_ptr()
     if parents is not None:
@@ -362,14 +393,15 @@ def run_select(q, k_means, table, lengths, page_size, pages):
 @torch.library.custom_op("kiln::paged_attention", mutates_args=())
 def _paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                      table: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor | None,
-                     selected: torch.Tensor | None, scale: float) -> torch.Tensor:
+                     selected: torch.Tensor | None, scale: float, window: int = 0, sinks: int = 0) -> torch.Tensor:
     with torch.no_grad():
-        return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, "paged_attention")
+        return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, "paged_attention",
+                             window, sinks)
 
 
 @_paged_attention.register_fake
-def _(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale):
-    check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected)
+def _(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, window=0, sinks=0):
+    check_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, window, sinks)
     return q.new_empty(tuple(q.shape))
 
 
@@ -396,6 +428,19 @@ def _cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pag
 @_cache_append.register_fake
 def _(k, v, k_pages, v_pages, table, lengths, rows, k_means):
     pass
+
+
+@torch.library.custom_op("kiln::cache_read", mutates_args=())
+def _cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
+                ends: torch.Tensor, tokens: int, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    with torch.no_grad():
+        return run_read(k_pages, v_pages, table, starts, ends, tokens, dtype)
+
+
+@_cache_read.register_fake
+def _(k_pages, v_pages, table, starts, ends, tokens, dtype):
+    shape = check_read(k_pages, v_pages, table, starts, ends, tokens)
+    return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
 
 
 @torch.library.custom_op("kiln::copy_pages", mutates_args=("pools",))
@@ -426,18 +471,24 @@ def _watched(*tensors) -> bool:
 # -- the public functions ------------------------------------------------------------------------------
 
 
-def tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents=None, *, scale=None):
+def tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents=None, *, scale=None, window=None, sinks=0):
     """Attention of drafted tokens over a paged cache and over each other.
 
     ``q`` ``[sequences, tokens, heads, dim]``, ``k`` and ``v`` ``[sequences,
     tokens, kv_heads, dim]``: the drafted tokens', in fp32 or the cache's
-    type; they are not in the cache yet. ``parents`` ``[sequences, tokens]``
+    type (any of the three over 4-bit pages); they are not in the cache yet. ``parents`` ``[sequences, tokens]``
     (int32): the earlier drafted token that token i follows, -1 where it
     follows the cached ones; any other value marks the token, and those that
     follow it, as unused (rows of zeros). Without ``parents`` each token
     follows the one before it. Query heads ``h`` share head ``h // (heads /
     kv_heads)`` of the cache. Returns ``softmax(scale q . keys) values``,
     shaped and typed as ``q``; ``scale`` is 1 / sqrt(dim) by default.
+
+    With ``window`` (at least 1) a token at position p - ``lengths[s]`` and the
+    number of its ancestors - attends, of these tokens, to those at positions
+    above p - ``window`` and to the sequence's first ``sinks`` alone. Pages
+    behind the window are not read: their columns may name no page
+    (``PagedCache.release``).
 
     Drafted keys and values are rounded to the cache's type first, so a token
     is attended to as it will be once it is appended. fp32 activations keep
@@ -447,10 +498,13 @@ def tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents=None, *, s
     sequences, dim a multiple of 8 up to 256, page_size a power of two from
     16 to 1024. A table entry outside the pool holds no tokens.
     """
-    scale = default_scale(scale, k_pages.shape[-1])
+    scale = default_scale(scale, page_dim(k_pages))
+    if window is not None and window < 1:
+        raise ValueError(f"a window holds at least the token itself, got {window}")
+    window, sinks = 0 if window is None else int(window), int(sinks)
     if _watched(q, k, v, k_pages, v_pages):
-        return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale)
-    return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale, "tree_attention")
+        return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale, window, sinks)
+    return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale, "tree_attention", window, sinks)
 
 
 def selected_attention(q, k, v, k_pages, v_pages, table, lengths, selected, parents=None, *, scale=None):
@@ -461,7 +515,7 @@ def selected_attention(q, k, v, k_pages, v_pages, table, lengths, selected, pare
     than the one before it, so lists ascend and end with -1."""
     if selected is None:
         raise TypeError("selected must be a tensor (tree_attention reads every page)")
-    scale = default_scale(scale, k_pages.shape[-1])
+    scale = default_scale(scale, page_dim(k_pages))
     if _watched(q, k, v, k_pages, v_pages):
         return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale)
     return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, selected, scale, "selected_attention")
@@ -559,7 +613,8 @@ def _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means):
         k, v = (t.unsqueeze(0) if isinstance(t, torch.Tensor) else t for t in (k, v))
         k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
         k_means = k_means.unsqueeze(0) if isinstance(k_means, torch.Tensor) else k_means
-    layers, pages, kv_heads, page_size, dim = k_pages.shape
+    layers, pages, kv_heads, page_size, _ = k_pages.shape
+    dim = page_dim(k_pages)
     _head_dim(dim)
     _tensor(k, "k", 5, tuple(TYPES))
     batch, draft = k.shape[1], k.shape[2]
@@ -592,10 +647,98 @@ def _append_form(k, v, k_pages, v_pages, table, lengths, rows, k_means):
         return None
     _ready(k.device)
     return kl.CacheAppend(layers, batch, draft, accept, kv_heads, dim, page_size, pages, table.shape[1],
-                          TYPES[k_pages.dtype], TYPES[k.dtype], None, None, None, None, None, None, None, None,
+                          CACHE_TYPES[k_pages.dtype], TYPES[k.dtype], None, None, None, None, None, None, None, None,
                           *k.stride()[:4], *v.stride()[:4], *k_pages.stride()[:4], *v_pages.stride()[:4],
                           *(k_means.stride()[:3] if k_means is not None else (0, 0, 0)), table.stride(0),
                           rows.stride(0) if rows is not None else 0)
+
+
+def cache_read(k_pages, v_pages, table, starts, ends, *, tokens, dtype=None):
+    """Cached tokens as dense tensors ``(k, v)``, ``[sequences, tokens,
+    kv_heads, dim]``: token ``starts[s] + a`` of sequence s (int32) in row a,
+    while it is below ``ends[s]`` (int32; what ``lengths`` is to the other
+    operators); zeros behind, and where the table names no page. ``dtype``
+    (fp32, bf16 or fp16): the pages' own by default, bf16 for 4-bit pages,
+    which holds their values exactly; others are rounded once. With a leading
+    dimension of layers on the pages (5 dimensions) all layers are read at
+    once, ``[layers, sequences, tokens, kv_heads, dim]``: what ``cache_append``
+    takes, of another cache too."""
+    dtype = _read_type(k_pages, dtype)
+    if _watched(k_pages, v_pages):
+        return torch.ops.kiln.cache_read(k_pages, v_pages, table, starts, ends, int(tokens), dtype)
+    return run_read(k_pages, v_pages, table, starts, ends, int(tokens), dtype)
+
+
+def _read_type(k_pages, dtype):
+    if dtype is not None and dtype not in TYPES:
+        raise TypeError(f"dtype must be one of {', '.join(map(str, TYPES))}, got {dtype}")
+    if not isinstance(k_pages, torch.Tensor):
+        raise TypeError(f"k_pages must be a tensor, got {type(k_pages).__name__}")
+    return (torch.bfloat16 if k_pages.dtype == torch.uint8 else k_pages.dtype) if dtype is None else dtype
+
+
+def check_read(k_pages, v_pages, table, starts, ends, tokens):
+    rank = k_pages.dim() if k_pages.dim() == 5 else 4
+    check_pages(k_pages, v_pages, rank)
+    _head_dim(page_dim(k_pages))
+    if not isinstance(table, torch.Tensor) or table.dim() != 2:
+        raise ValueError("table must be a tensor [sequences, columns]")
+    _int32(table, "table", 2, tuple(table.shape))
+    _int32(starts, "starts", 1, table.shape[:1])
+    _int32(ends, "ends", 1, table.shape[:1])
+    if not 0 <= tokens < 2 ** 31:
+        raise ValueError(f"cannot read {tokens} tokens")
+    return (*k_pages.shape[:rank - 4], table.shape[0], tokens, k_pages.shape[-3], page_dim(k_pages))
+
+
+def run_read(k_pages, v_pages, table, starts, ends, tokens, dtype):
+    try:
+        key = ("read", _form(k_pages, v_pages, table, starts, ends), tokens, dtype)
+    except AttributeError:
+        check_read(k_pages, v_pages, table, starts, ends, tokens)
+        raise
+    found = _forms.get(key)
+    if found is None:
+        shape = check_read(k_pages, v_pages, table, starts, ends, tokens)
+        _no_grad(k_pages, v_pages)
+        _one_device(k_pages, v_pages, table, starts, ends)
+        _rows_in_place(k_pages, "k_pages")
+        _rows_in_place(v_pages, "v_pages")
+        straight = tuple(_columns(t) for t in (table, starts, ends))
+        if any(a is not b for a, b in zip(straight, (table, starts, ends))):
+            return run_read(k_pages, v_pages, *straight, tokens, dtype)
+        rank = k_pages.dim()
+        ks, vs = k_pages.stride(), v_pages.stride()
+        if math.prod(shape) == 0:
+            return tuple(torch.empty(shape, dtype=dtype, device=k_pages.device) for _ in "kv")
+        if k_pages.shape[-4] == 0:
+            raise ValueError("the cache has no pages")
+        _ready(k_pages.device)
+        op = kl.CacheRead(k_pages.shape[0] if rank == 5 else 1, table.shape[0], tokens, k_pages.shape[-3], shape[-1],
+                          k_pages.shape[-2], k_pages.shape[-4], table.shape[1], CACHE_TYPES[k_pages.dtype], TYPES[dtype],
+                          None, None, None, None, None, None, None, ks[0] if rank == 5 else 0, *ks[rank - 4:-1],
+                          vs[0] if rank == 5 else 0, *vs[rank - 4:-1], table.stride(0))
+        found = _keep(key, (bytes(op), shape))
+    elif k_pages.device.type != "cuda" and not interpreting():
+        _one_device(k_pages)
+    if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad):
+        _no_grad(k_pages, v_pages)
+    op = kl.CacheRead.from_buffer_copy(found[0])
+    op.k_pages, op.v_pages = at = (k_pages.data_ptr(), v_pages.data_ptr())
+    if (at[0] | at[1]) & 15:
+        _rows_in_place(k_pages, "k_pages")
+        _rows_in_place(v_pages, "v_pages")
+    device = k_pages.device
+    k, v = (torch.empty(found[1], dtype=dtype, device=device) for _ in "kv")
+    op.k, op.v, op.table, op.starts, op.ends = k.data_ptr(), v.data_ptr(), table.data_ptr(), starts.data_ptr(), ends.data_ptr()
+    lib = kl.load()
+    if device.type != "cuda":
+        rc = lib.kh_cache_read_host(ctypes.byref(op))
+    else:
+        rc = _on_device(device, lib.kh_cache_read, ctypes.byref(op))
+    if rc:
+        kl.check(rc, "cache_read")
+    return k, v
 
 
 def _page_list(x, name):

@@ -1,0 +1,250 @@
+"""The 4-bit cache, dense reads and windows on the GPU against their definitions
+in 64 bits.
+
+Pages, codes and dense values are compared for equality. Attention: the bounds
+of test_gpu_paged.py, whose scores and weights are made the same way: values of
+4-bit pages are bf16 ones, at most 6 times the largest of a block's new tokens
+here (|v| < 6 of normal inputs), and products of fp32 activations take three
+bf16 parts, of fp16 ones two (16 bits of q, which has 11, and of the weights):
+1e-4 for fp32, and half a step of the result and of each weight more for 16-bit
+activations."""
+
+import math
+
+import pytest
+import torch
+
+import kiln
+import packed_reference as ref
+import test_packed
+
+pytestmark = pytest.mark.gpu
+
+ACTS = [torch.float32, torch.bfloat16, torch.float16]
+CACHES = [(torch.uint8, a) for a in ACTS] + [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
+                                             (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)]
+IDS = ["fp4-fp32", "fp4-bf16", "fp4-fp16", "fp32", "bf16-fp32", "fp16-fp32", "bf16", "fp16"]
+
+
+def gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def tolerance(act):
+    if act == torch.float32:
+        return dict(rtol=0.0, atol=1e-4)
+    half = torch.finfo(act).eps / 2
+    return dict(rtol=half, atol=1e-4 + 2 * 6 * half)
+
+
+def check(p, selected=None, **more):
+    if selected is None:
+        got = kiln.tree_attention(**p, **more)
+    else:
+        got = kiln.selected_attention(**p, selected=selected)
+        more = dict(selected=selected)
+    want = ref.attention(**p, **more)
+    assert got.dtype == p["q"].dtype and got.shape == p["q"].shape
+    torch.testing.assert_close(got.double().cpu(), want, equal_nan=True, **tolerance(got.dtype))
+    return got
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_blocks(act):
+    x = test_packed.blocks().to(act)
+    n = len(x)
+    k = x.view(1, n, 1, 32).cuda()
+    kp, vp = (torch.zeros(-(-n // 16), 1, 16, 17, dtype=torch.uint8, device="cuda") for _ in "kv")
+    table = torch.arange(len(kp), dtype=torch.int32, device="cuda")[None]
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kiln.cache_append(k, k.flip(1), kp, vp, table, zero)
+    want = torch.zeros(len(kp) * 16, 32, dtype=act)
+    want[:n] = x
+    assert torch.equal(kp[:, 0].cpu().flatten()[:n // 16 * 272], ref.pack(want.view(-1, 16, 32), True).flatten()[:n // 16 * 272])
+    got_k, got_v = kiln.cache_read(kp, vp, table, zero, zero + n, tokens=n, dtype=torch.float32)
+    want = ref.rounded(x)
+    assert torch.equal(got_k.cpu().double().view(n, 32).nan_to_num(nan=99.0), want.nan_to_num(nan=99.0))
+    assert torch.equal(got_v.cpu().double().view(n, 32).flip(0).nan_to_num(nan=99.0), want.nan_to_num(nan=99.0))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("layers,dim,page", [(1, 32, 16), (3, 96, 32), (2, 256, 64), (1, 64, 1024)])
+def test_append_and_read(act, layers, dim, page):
+    g = gen(dim)
+    batch, n, kv, pages = 4, 45, 3, 24
+    k_pages, v_pages = (torch.cat([ref.fast_pack(torch.randn(pages, kv, page, dim, generator=g), keys)[None] for _ in range(layers)])
+                        .cuda() for keys in (True, False))
+    means = torch.randn(layers, pages, kv, dim, generator=g).cuda()
+    table = torch.randperm(pages, generator=g).to(torch.int32).view(4, 6).cuda()
+    table[3, 1] = -1
+    lengths = torch.tensor([0, page - 1, 2 * page + 3, page - 5], dtype=torch.int32, device="cuda")
+    k = torch.randn(layers, batch, n, kv, dim, generator=g).to(act).cuda()
+    v = torch.randn(layers, batch, n, kv, dim, generator=g).to(act).cuda()
+    k[0, 0, 2, 1, 5] = math.inf
+    v[0, 1, 3, 0, 31] = math.nan
+    rows = torch.full((batch, 20), -1, dtype=torch.int32)
+    rows[0] = torch.arange(20) * 2
+    rows[1, :7] = torch.tensor([3, 3, 44, 0, 1, -1, 9])     # ends at the sixth
+    rows[3, :9] = torch.arange(9)
+    for r in (None, rows.cuda()):
+        mine = [t.clone() for t in (k_pages, v_pages, means)]
+        kiln.cache_append(k, v, mine[0], mine[1], table, lengths, rows=r, k_means=mine[2])
+        want = ref.append(k, v, k_pages, v_pages, table, lengths, r, means)
+        assert torch.equal(mine[0].cpu(), want[0]) and torch.equal(mine[1].cpu(), want[1])
+        # sums of at most 1024 values below 8 in fp32: each addition off by 2^-24 of a sum below 2^8
+        torch.testing.assert_close(mine[2].double().cpu(), want[2], rtol=0, atol=1024 * 2 ** -16 / page * 2 ** -8 + 1e-5, equal_nan=True)
+        without = [t.clone() for t in (k_pages, v_pages)]
+        kiln.cache_append(k, v, *without, table, lengths, rows=r)
+        assert torch.equal(without[0].cpu(), want[0]) and torch.equal(without[1].cpu(), want[1])
+    starts = torch.tensor([0, -3, page + 1, 2 * page - 2], dtype=torch.int32, device="cuda")
+    ends = torch.tensor([page + 3, 10 ** 6, page + 9, 5], dtype=torch.int32, device="cuda")
+    for dtype in ACTS:
+        got = kiln.cache_read(*mine[:2], table, starts, ends, tokens=page + 70, dtype=dtype)
+        for a, b in zip(got, ref.read(*mine[:2], table, starts, ends, page + 70)):
+            assert torch.equal(a.cpu().nan_to_num(nan=99.0), b.to(dtype).nan_to_num(nan=99.0))
+
+
+@pytest.mark.parametrize("cache", ACTS)
+def test_read_of_other_types(cache):
+    g = gen(5)
+    k_pages, v_pages = (torch.randn(2, 9, 3, 16, 40, generator=g).to(cache).cuda() for _ in "kv")
+    table = torch.tensor([[4, 2, -1], [0, 7, 8]], dtype=torch.int32, device="cuda")
+    starts, ends = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([3, 0], [40, 17]))
+    for dtype in (None, *ACTS):
+        got = kiln.cache_read(k_pages, v_pages, table, starts, ends, tokens=50, dtype=dtype)
+        for a, b in zip(got, ref.read(k_pages, v_pages, table, starts, ends, 50)):
+            assert torch.equal(a.cpu(), b.to(dtype or cache))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 256])
+@pytest.mark.parametrize("heads,kv,draft", [(2, 2, 1), (4, 1, 5), (6, 2, 33)])
+def test_types_heads_dims(act, dim, heads, kv, draft):
+    check(ref.problem(gen(dim), act=act, draft=draft, heads=heads, kv=kv, dim=dim, device="cuda"))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("page", [16, 32, 128, 1024])
+@pytest.mark.parametrize("lengths", [(0, 0), (1, 0), (15, 16), (31, 33), (129, 1000), (2049, 5)], ids=str)
+def test_lengths_and_pages(act, page, lengths):
+    check(ref.problem(gen(page), act=act, lengths=lengths, page=page, device="cuda"))
+
+
+@pytest.mark.parametrize("draft", [1, 2, 31, 32, 33, 64, 100, 256])
+@pytest.mark.parametrize("tree", [True, False], ids=["tree", "chain"])
+def test_drafts(draft, tree):
+    check(ref.problem(gen(draft), draft=draft, heads=3, kv=1, tree=tree, lengths=(50, 0), device="cuda"))
+    check(ref.problem(gen(draft), act=torch.float16, draft=draft, heads=8, kv=1, tree=tree, lengths=(50, 3), dim=128, device="cuda"))
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_long_and_ragged(act):
+    # ranges that end inside an item, and many items in one range
+    lengths = (5000, 0, 1, 700, 33, 2600, 64, 16)
+    check(ref.problem(gen(1), act=act, batch=8, draft=2, heads=4, kv=2, lengths=lengths, device="cuda"))
+    check(ref.problem(gen(2), act=act, batch=40, draft=1, heads=2, kv=1, lengths=[7 * i for i in range(40)], device="cuda"))
+    check(ref.problem(gen(3), act=act, batch=3, draft=20, heads=8, kv=2, dim=128, lengths=(3000, 1111, 2), device="cuda"))
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_picked_pages(act):
+    p = ref.problem(gen(3), act=act, batch=3, draft=5, heads=6, kv=2, lengths=(300, 0, 41), device="cuda")
+    means = ref.unpack(p["k_pages"], True).mean(2).float().cuda()
+    for top in (1, 7):
+        check(p, selected=kiln.select_pages(p["q"], means, p["table"], p["lengths"], page_size=16, pages=top))
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_what_is_masked_does_not_reach(act):
+    for dim in (64, 128, 256):
+        p = ref.problem(gen(5), act=act, draft=6, lengths=(37, 16), spare=3, dim=dim, device="cuda")
+        for s, n in enumerate((37, 16)):      # slots behind the last token: NaN blocks
+            for t in range(n, -(-n // 16) * 16):
+                page = int(p["table"][s, t // 16])
+                for pages, keys in ((p["k_pages"], True), (p["v_pages"], False)):
+                    for d in range(0, dim, 32):
+                        at = ref.places(t % 16, d, dim, 16, keys)[1]
+                        pages[page].view(2, -1)[:, at] = 255
+        p["parents"] = torch.tensor([[-1, 0, 0, 1, 2, 4], [-1, -1, -1, -1, -1, -1]], dtype=torch.int32, device="cuda")
+        p["v"][0, 1, 0, 3] = math.inf      # reaches tokens 1 and 3 of the first sequence alone
+        p["v"][0, 4, 1] = math.nan         # tokens 4, 5
+        p["k"][1, 2] = math.nan            # token 2 of the second
+        got = check(p)
+        assert torch.isfinite(got[0, [0, 2]]).all() and torch.isfinite(got[1, [0, 1, 3, 4, 5]]).all()
+        if dim > 32:
+            assert torch.isfinite(got[0, 3, 0, 32:]).all()     # (the other blocks of that value)
+        p["v"][0, 1, 0, 3] = 0.0
+        at = ref.places(5, 0, dim, 16, False)[1]
+        p["v_pages"][int(p["table"][0, 1])].view(2, -1)[:, at] = 255   # a cached value: every row
+        check(p)
+
+
+def test_unused_rows_are_zeros():
+    p = ref.problem(gen(4), draft=40, lengths=(20, 0), device="cuda")
+    p["parents"][0, 7] = 9          # follows a later token
+    p["parents"][0, 20] = -5
+    p["parents"][1, 0] = 0          # follows itself: every token of the sequence that leads to it is unused
+    p["k"][0, 7] = math.nan
+    p["v"][1, 0] = math.inf
+    for more in (dict(), dict(window=5, sinks=2)):
+        got = check(p, **more)
+        assert (got[0, 7] == 0).all() and (got[0, 20] == 0).all() and (got[1, 0] == 0).all()
+
+
+def test_tables_that_name_no_page():
+    p = ref.problem(gen(7), lengths=(100, 64), device="cuda")
+    p["table"][0, 2] = -1
+    p["table"][0, 3] = len(p["k_pages"])
+    p["table"][1, 0] = 2 ** 31 - 1
+    check(p)
+    p["lengths"][0] = 10 ** 6        # beyond the table: what the table has
+    p["lengths"][1] = -3
+    check(p)
+    check(p, window=20, sinks=3)
+
+
+# -- windows ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cache,act", CACHES, ids=IDS)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (2, 1), (17, 0), (33, 4), (64, 40), (200, 16), (5000, 0)])
+def test_windows(cache, act, window, sinks):
+    for draft, tree, dim in ((1, False, 64), (7, True, 128), (40, True, 64), (40, False, 128)):
+        check(ref.problem(gen(window), cache=cache, act=act, batch=3, draft=draft, heads=4, kv=2, dim=dim, tree=tree,
+                          lengths=(430, 0, 61), device="cuda"), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("cache,act", CACHES, ids=IDS)
+def test_long_windows(cache, act):
+    # ranges, and (many rows) the kernel that shares tiles
+    for draft, heads, dim in ((1, 4, 64), (3, 4, 256), (33, 4, 128), (70, 2, 64)):
+        check(ref.problem(gen(9), cache=cache, act=act, batch=2, draft=draft, heads=heads, kv=2, dim=dim, page=64,
+                          lengths=(6000, 2100), device="cuda"), window=1900, sinks=70)
+
+
+@pytest.mark.parametrize("cache,act", CACHES, ids=IDS)
+@pytest.mark.parametrize("draft,heads", [(6, 4), (33, 4)], ids=["few", "many"])
+def test_what_is_behind_the_window_does_not_reach(cache, act, draft, heads):
+    # pages that no token sees hold NaN or are not named; a value that only the first tokens still see reaches only them
+    p = ref.problem(gen(11), cache=cache, act=act, draft=draft, heads=heads, kv=2, dim=64, lengths=(200, 90), tree=False, device="cuda")
+    window, sinks = 50, 5
+    first = 200 - window + 1                   # token 0's first key; token 1 does not see it
+    spoilt = [(0, t) for t in range(sinks, first)] + [(0, first), (1, 90 - window + 1)]
+    for s, t in spoilt:
+        page, slot = int(p["table"][s, t // 16]), t % 16
+        if cache == torch.uint8:
+            for pages, keys in ((p["k_pages"], True), (p["v_pages"], False)):
+                for d in (0, 32):
+                    pages[page].view(2, -1)[:, ref.places(slot, d, 64, 16, keys)[1]] = 255
+        else:
+            p["v_pages"][page, :, slot] = math.inf
+            p["k_pages"][page, :, slot] = math.nan if t < first - 3 else 0.0
+    got = check(p, window=window, sinks=sinks)
+    assert torch.isfinite(got[:, 1:]).all() and not torch.isfinite(got[:, 0]).any()
+    p["table"][0, 1:(first - 1) // 16] = -1
+    assert torch.equal(check(p, window=window, sinks=sinks)[:, 1:], got[:, 1:])
+
+
+def test_window_of_everything():
+    p = ref.problem(gen(12), cache=torch.bfloat16, act=torch.bfloat16, draft=5, lengths=(300, 7), device="cuda")
+    assert torch.equal(kiln.tree_attention(**p, window=10 ** 6), kiln.tree_attention(**p))

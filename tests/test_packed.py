@@ -1,0 +1,228 @@
+"""The 4-bit cache, dense reads and windows on the CPU: the meaning of the
+operators (KILN_HIP_INTERPRET=1: the library's CPU meaning) against their
+definitions, refusals, and kiln.PagedCache over 4-bit pages.
+
+What 4 bits hold is exact in both, so pages, codes and values are compared for
+equality; the CPU meaning of attention works in 64 bits and rounds its result
+once: half a step of it, and 2^-24 of the largest value for what exp and the
+sums differ by."""
+
+import math
+import random
+
+import pytest
+import torch
+
+import kiln
+import packed_reference as ref
+import paged_reference
+
+FP4 = torch.float4_e2m1fn_x2
+
+
+@pytest.fixture()
+def interpreting(monkeypatch):
+    monkeypatch.setenv("KILN_HIP_INTERPRET", "1")
+
+
+def gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def half(act):
+    return dict(rtol=torch.finfo(act).eps / 2, atol=12 * 2 ** -24)
+
+
+def blocks():
+    """Rows of 32 with every code, ties, the borders of a scale, the smallest and the largest, zeros, signs."""
+    g = gen(3)
+    rows = [torch.randn(32, generator=g) * 10.0 ** (i - 12) for i in range(26)]
+    grid = torch.tensor([0, .25, .5, .75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, 6.999])
+    both = torch.cat([grid, -grid])
+    rows += [both, both * 2.0 ** 100, both * 2.0 ** -100, both * 2.0 ** -124, both * 2.0 ** -130, torch.nextafter(both, both * 2),
+             torch.nextafter(both, both * 0), torch.zeros(32), -torch.zeros(32)]
+    for top in (7.0, 6.9999995, 3.5, 4.0, torch.finfo(torch.float32).max, 2.0 ** -126, 2.0 ** -149, 1.75 * 2.0 ** -124):
+        row = torch.linspace(-0.9, 0.9, 32) * top
+        row[7] = top
+        rows.append(row)
+    return torch.stack(rows)
+
+
+@pytest.mark.parametrize("act", [torch.float32, torch.bfloat16, torch.float16])
+def test_blocks(interpreting, act):
+    x = blocks().to(act)
+    n = len(x)
+    k = x.view(1, n, 1, 32)
+    kp, vp = (torch.zeros(-(-n // 16), 1, 16, 17, dtype=torch.uint8) for _ in "kv")
+    table = torch.arange(len(kp), dtype=torch.int32)[None]
+    zero = torch.zeros(1, dtype=torch.int32)
+    kiln.cache_append(k, k.flip(1), kp, vp, table, zero)
+    got_k, got_v = kiln.cache_read(kp, vp, table, zero, zero + n, tokens=n, dtype=torch.float32)
+    want = ref.rounded(x)
+    # (fp32 activations may be past fp16's range: infinite there, a NaN block)
+    assert torch.equal(got_k.double().view(n, 32).nan_to_num(nan=99.0), want.nan_to_num(nan=99.0))
+    assert torch.equal(got_v.double().view(n, 32).flip(0).nan_to_num(nan=99.0), want.nan_to_num(nan=99.0))
+
+
+def test_half_a_step():
+    # 1/6 of the block's largest at the most: half a step of the top binade is 1, of a largest of 6 (below 7: 1/7 beyond)
+    x = blocks()
+    x = x[(x.abs().amax(1) > 2.0 ** -120) & torch.isfinite(x).all(1)]
+    assert bool(((ref.rounded(x) - x.double()).abs() <= x.double().abs().amax(1, keepdim=True) / 3.5).all())
+
+
+@pytest.mark.parametrize("dim,page", [(32, 16), (96, 32), (256, 16)])
+def test_append_and_read(interpreting, dim, page):
+    g = gen(dim)
+    k_pages, v_pages = (ref.fast_pack(torch.randn(2, 9, 3, page, dim, generator=g), keys) for keys in (True, False))
+    means = torch.randn(2, 9, 3, dim, generator=g)
+    table = torch.tensor([[4, 2, -1], [0, 7, 8], [1, 3, 99]], dtype=torch.int32)
+    lengths = torch.tensor([page - 2, 2 * page - 1, 5], dtype=torch.int32)
+    k, v = (torch.randn(2, 3, 21, 3, dim, generator=g) for _ in range(2))
+    rows = torch.tensor([[0, 2, 2, 20, 5], [9, 1, -1, 3, 4], [-1, 0, 0, 0, 0]], dtype=torch.int32)
+    for r in (None, rows):
+        want = ref.append(k, v, k_pages, v_pages, table, lengths, r, means)
+        got = [t.clone() for t in (k_pages, v_pages, means)]
+        kiln.cache_append(k, v, got[0], got[1], table, lengths, rows=r, k_means=got[2])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        torch.testing.assert_close(got[2].double(), want[2], rtol=2 ** -24, atol=0)
+    starts = torch.tensor([0, -3, page + 1], dtype=torch.int32)
+    ends = torch.tensor([page + 3, 10 ** 6, page + 9], dtype=torch.int32)
+    for dtype in (None, torch.float32, torch.float16):
+        got = kiln.cache_read(k_pages, v_pages, table, starts, ends, tokens=3 * page + 7, dtype=dtype)
+        for a, b in zip(got, ref.read(k_pages, v_pages, table, starts, ends, 3 * page + 7)):
+            assert a.dtype == (dtype or torch.bfloat16) and torch.equal(a.double(), b)
+    one = kiln.cache_read(k_pages[1], v_pages[1], table, starts, ends, tokens=5)
+    assert torch.equal(one[0], kiln.cache_read(k_pages, v_pages, table, starts, ends, tokens=5)[0][1])
+
+
+@pytest.mark.parametrize("cache", [torch.float32, torch.bfloat16, torch.float16])
+def test_read_of_other_types(interpreting, cache):
+    g = gen(5)
+    k_pages, v_pages = (torch.randn(2, 9, 3, 16, 40, generator=g).to(cache) for _ in "kv")
+    table = torch.tensor([[4, 2, -1], [0, 7, 8]], dtype=torch.int32)
+    starts, ends = torch.tensor([3, 0], dtype=torch.int32), torch.tensor([40, 17], dtype=torch.int32)
+    for dtype in (None, torch.float32, torch.bfloat16, torch.float16):
+        got = kiln.cache_read(k_pages, v_pages, table, starts, ends, tokens=50, dtype=dtype)
+        for a, b in zip(got, ref.read(k_pages, v_pages, table, starts, ends, 50)):
+            assert torch.equal(a, b.to(dtype or cache))
+
+
+ACTS = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dim", [32, 64, 96])
+def test_attention_meaning(interpreting, act, dim):
+    p = ref.problem(gen(), act=act, batch=3, draft=7, heads=6, kv=2, lengths=(70, 0, 33), dim=dim)
+    p["parents"][0, 3] = 5     # unused, and what follows it
+    p["table"][0, 1] = 99      # no such page
+    torch.testing.assert_close(kiln.tree_attention(**p).double(), ref.attention(**p), **half(act))
+    for window, sinks in ((1, 0), (3, 0), (5, 2), (40, 17), (1000, 3)):
+        more = dict(window=window, sinks=sinks)
+        torch.testing.assert_close(kiln.tree_attention(**p, **more).double(), ref.attention(**p, **more), **half(act))
+        chain = dict(p, parents=None, **more)
+        torch.testing.assert_close(kiln.tree_attention(**chain).double(), ref.attention(**chain), **half(act))
+    sel = torch.tensor([[0, 2, 4], [1, 1, 3]], dtype=torch.int32).expand(3, 7, 2, 3).contiguous()
+    torch.testing.assert_close(kiln.selected_attention(**p, selected=sel).double(), ref.attention(**p, selected=sel), **half(act))
+
+
+@pytest.mark.parametrize("cache,act", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+def test_window_meaning(interpreting, cache, act):
+    p = ref.problem(gen(2), cache=cache, act=act, batch=3, draft=9, heads=4, kv=2, lengths=(70, 0, 33))
+    for window, sinks in ((1, 0), (1, 100), (4, 1), (17, 0), (33, 20), (2 ** 31 - 1, 2 ** 31 - 1)):
+        more = dict(window=window, sinks=sinks)
+        torch.testing.assert_close(kiln.tree_attention(**p, **more).double(), ref.attention(**p, **more), **half(act))
+    whole = kiln.tree_attention(**p)
+    assert torch.equal(kiln.tree_attention(**p, window=80), whole)      # (a window that holds everything)
+
+
+# -- refusals -----------------------------------------------------------------------------------
+
+
+def test_refusals(interpreting):
+    p = ref.problem(gen())
+    for change, more, error in (
+            (dict(k_pages=p["k_pages"][..., :33].contiguous(), v_pages=p["v_pages"][..., :33].contiguous()), {}, ValueError),
+            (dict(k_pages=p["k_pages"][..., :0], v_pages=p["v_pages"][..., :0]), {}, ValueError),
+            (dict(q=p["q"].double()), {}, TypeError),
+            (dict(k=p["k"].half()), {}, TypeError),
+            (dict(v_pages=p["v_pages"].float()), {}, TypeError),
+            (dict(k_pages=p["k_pages"].transpose(2, 3).contiguous().transpose(2, 3)), {}, ValueError),
+            ({}, dict(window=0), ValueError),
+            ({}, dict(window=-1), ValueError),
+            ({}, dict(sinks=4), ValueError),
+            ({}, dict(window=4, sinks=-1), ValueError),
+            ({}, dict(window=2 ** 31), ValueError)):
+        with pytest.raises(error):
+            kiln.tree_attention(**dict(p, **change), **more)
+    with pytest.raises(NotImplementedError):     # 288 dimensions
+        kiln.tree_attention(**ref.problem(gen(), dim=288))
+    with pytest.raises(ValueError):
+        torch.ops.kiln.paged_attention(*[p[n] for n in ("q", "k", "v", "k_pages", "v_pages", "table", "lengths", "parents")],
+                                       torch.zeros(2, 3, 2, 1, dtype=torch.int32), 1.0, 4, 0)
+    zero = torch.zeros(2, dtype=torch.int32)
+    read = dict(k_pages=p["k_pages"], v_pages=p["v_pages"], table=p["table"], starts=zero, ends=zero + 4, tokens=4)
+    for change, error in ((dict(tokens=-1), ValueError), (dict(dtype=torch.float64), TypeError), (dict(dtype=torch.uint8), TypeError),
+                          (dict(starts=zero.long()), TypeError), (dict(ends=zero[:1]), ValueError), (dict(table=None), ValueError),
+                          (dict(v_pages=p["v_pages"][:1]), ValueError), (dict(k_pages=None), TypeError),
+                          (dict(k_pages=p["k_pages"][:, :, :15], v_pages=p["v_pages"][:, :, :15]), (ValueError, NotImplementedError))):
+        with pytest.raises(error):
+            kiln.cache_read(**dict(read, **change))
+    with pytest.raises(NotImplementedError):
+        kiln.cache_read(**dict(read, k_pages=torch.zeros(2, 1, 16, 64, requires_grad=True), v_pages=torch.zeros(2, 1, 16, 64)))
+    assert kiln.cache_read(**dict(read, tokens=0))[0].shape == (2, 0, 2, 64)
+    with pytest.raises(NotImplementedError):     # 48 dimensions: no block ends there
+        kiln.PagedCache(1, 4, 16, 1, 48, dtype=FP4)
+
+
+def test_no_cpu_path():
+    p = ref.problem(gen())
+    with pytest.raises(NotImplementedError):
+        kiln.tree_attention(**p, window=4)
+    with pytest.raises(NotImplementedError):
+        kiln.cache_read(p["k_pages"], p["v_pages"], p["table"], p["lengths"], p["lengths"], tokens=3)
+
+
+# -- kiln.PagedCache ---------------------------------------------------------------------------------
+
+
+def test_packed_cache_keeps_what_it_is_given(interpreting):
+    rng, g = random.Random(1), gen(1)
+    cache = kiln.PagedCache(2, 24, 16, 2, 32, dtype=FP4, means=True)
+    assert cache.k.dtype == torch.uint8 and cache.k.shape == (2, 24, 2, 16, 17)
+    held = {}
+    for step in range(30):
+        seqs = list(held)
+        what = rng.choice(["open", "append", "append", "fork", "truncate", "compact"])
+        if what == "open" and len(seqs) < 4:
+            held[cache.open()] = (torch.zeros(2, 0, 2, 32), torch.zeros(2, 0, 2, 32))
+        elif what == "append" and seqs:
+            some = rng.sample(seqs, rng.randint(1, len(seqs)))
+            k, v = (torch.randn(2, len(some), 3, 2, 32, generator=g) for _ in range(2))
+            cache.append(some, k, v)
+            for i, s in enumerate(some):
+                held[s] = tuple(torch.cat([old, ref.rounded(t[:, i]).float()], 1) for old, t in zip(held[s], (k, v)))
+        elif what == "fork" and seqs and len(seqs) < 6:
+            s = rng.choice(seqs)
+            held[cache.fork(s)[0]] = held[s]
+        elif what == "truncate" and seqs:
+            s = rng.choice(seqs)
+            n = rng.randint(0, cache.length(s))
+            cache.truncate(s, n)
+            held[s] = tuple(t[:, :n] for t in held[s])
+        elif what == "compact":
+            cache.compact()
+        if held:
+            for got, i in zip(cache.read(list(held), dtype=torch.float32), (0, 1)):
+                for j, s in enumerate(held):
+                    assert torch.equal(got[:, j, :cache.length(s)], held[s][i])
+                    assert not got[:, j, cache.length(s):].any()
+    # into another cache, of another type
+    seqs = list(held)
+    other = kiln.PagedCache(2, 24, 32, 2, 32, dtype=torch.bfloat16)
+    there = [other.open() for _ in seqs]
+    k, v = cache.read(seqs)
+    other.append(there, k, v, rows=[list(range(cache.length(s))) for s in seqs])
+    for a, b in zip(other.read(there), (k, v)):
+        assert torch.equal(a, b)
