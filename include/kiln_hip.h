@@ -435,8 +435,8 @@ typedef struct kh_paged {
 } kh_paged;
 /* sizeof(kh_paged), sizeof(kh_cache_append_op), sizeof(kh_pool) */
 int kh_paged_sizes(size_t *sizes3);
-/* sizeof(kh_cache_read_op) */
-int kh_decode_sizes(size_t *sizes1);
+/* sizeof(kh_cache_read_op), sizeof(kh_verify_op) */
+int kh_decode_sizes(size_t *sizes2);
 int kh_paged_workspace_bytes(const kh_paged *op, size_t *bytes);
 int kh_paged_run(const kh_paged *op, void *workspace, size_t workspace_bytes, void *stream);
 int kh_paged_host(const kh_paged *op);
@@ -495,6 +495,38 @@ typedef struct kh_cache_read_op {
 } kh_cache_read_op;
 int kh_cache_read(const kh_cache_read_op *op, void *stream);
 int kh_cache_read_host(const kh_cache_read_op *op);
+
+/*
+ * kh_verify: which of a sequence's drafted tokens the target model keeps, and
+ * the token after them. tokens [batch][draft] is a tree, parents[s][i] in
+ * [0, i) the token that i > 0 follows (NULL: i - 1); a token with another
+ * parent, or outside [0, vocab), is never kept. Token 0 is the root: it is kept
+ * where its parent is -1; any other value marks an unused sequence (nothing
+ * kept, next -1). target[s][i] is the target's distribution after token i,
+ * drafted[s][i] (NULL: none) the one that the children of i were drawn from,
+ * uniforms[s][i] a number in [0, 1). With `drafted` the children c of the
+ * current token are asked in order: with r = target's row and R = 1 at first, c
+ * is kept where u[c] R q(c) < r(c), q = drafted's row; where not, r becomes
+ * max(r - R q, 0) and R its sum. A kept child is the current token from then on.
+ * When none is left, next is the first x whose running sum of r passes u[0] of
+ * the whole (r = target's row where R is 0). Without `drafted`, x is drawn so
+ * from target's row with u[current]; a child that is x is kept and is the
+ * current token, else next = x. All in 64 bits; a probability that is not above
+ * 0 counts as 0, and next is -1 where a row has no weight or an infinite one.
+ * rows [batch][draft]: the kept tokens, then -1; counts [batch]: their number.
+ * The workspace as kh_paged_run's.
+ */
+typedef struct kh_verify_op {
+  int32_t batch, draft, vocab, type;      /* KH_TYPE_* of target and drafted   */
+  int32_t tokens_wide, uniforms_wide;     /* int64 and double, not int32, float */
+  const void *tokens, *target, *uniforms, *drafted;
+  const int32_t *parents;
+  int32_t *rows, *counts, *next;
+  int64_t tokens_s, target_s, target_n, uniforms_s, drafted_s, drafted_n, parents_s;  /* strides in elements */
+} kh_verify_op;
+int kh_verify_workspace_bytes(const kh_verify_op *op, size_t *bytes);
+int kh_verify_run(const kh_verify_op *op, void *workspace, size_t workspace_bytes, void *stream);
+int kh_verify_host(const kh_verify_op *op);
 
 /*
  * kh_cache_copy: in every pool, pages source[i] copied to target[i], i < n.

@@ -640,9 +640,10 @@ int kh_cache_append_host(const kh_cache_append_op *op) {
   });
 }
 
-int kh_decode_sizes(size_t *sizes1) {
-  if (!sizes1) return kh::abi_fail(KH_ERR_INVALID, "null argument");
-  sizes1[0] = sizeof(kh_cache_read_op);
+int kh_decode_sizes(size_t *sizes2) {
+  if (!sizes2) return kh::abi_fail(KH_ERR_INVALID, "null argument");
+  sizes2[0] = sizeof(kh_cache_read_op);
+  sizes2[1] = sizeof(kh_verify_op);
   return KH_OK;
 }
 

@@ -18,7 +18,8 @@ from kiln.api import CompiledModule, Options, Report, compile, compile_graph
 from kiln.backend import backend, stats
 from kiln.cache import PagedCache
 from kiln.hip.paged import cache_append, cache_read, copy_pages, select_pages, selected_attention, tree_attention
+from kiln.hip.verify import verify_tokens
 
 __all__ = ["compile", "compile_graph", "Options", "Report", "CompiledModule", "backend", "stats",
            "PagedCache", "tree_attention", "select_pages", "selected_attention", "cache_append", "cache_read",
-           "copy_pages"]
+           "copy_pages", "verify_tokens"]

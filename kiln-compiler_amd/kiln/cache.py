@@ -73,6 +73,7 @@ class PagedCache:
         self._refs = [0] * pages                 # sequences that have the page
         self._pages = {}                         # sequence -> its pages, in order
         self._length = {}                        # sequence -> its tokens
+        self._gone = {}                          # sequence -> the tokens before this one may be released
         self._next = 0
 
     # -- sequences ----------------------------------------------------------------------
@@ -85,7 +86,7 @@ class PagedCache:
         return self._length[self._known(seq)]
 
     def pages_of(self, seq) -> tuple:
-        """The sequence's pages, in order."""
+        """The sequence's pages, in order; -1 for those that were released."""
         return tuple(self._pages[self._known(seq)])
 
     def _known(self, seq):
@@ -96,7 +97,7 @@ class PagedCache:
     def open(self) -> int:
         """A new, empty sequence."""
         seq, self._next = self._next, self._next + 1
-        self._pages[seq], self._length[seq] = [], 0
+        self._pages[seq], self._length[seq], self._gone[seq] = [], 0, 0
         return seq
 
     def fork(self, seq, n=1) -> list:
@@ -108,13 +109,16 @@ class PagedCache:
         for _ in range(n):
             new = self.open()
             self._pages[new] = list(self._pages[seq])
-            self._length[new] = self._length[seq]
+            self._length[new], self._gone[new] = self._length[seq], self._gone[seq]
             for page in self._pages[new]:
-                self._refs[page] += 1
+                if page >= 0:
+                    self._refs[page] += 1
             made.append(new)
         return made
 
     def _drop(self, page):
+        if page < 0:
+            return
         self._refs[page] -= 1
         if not self._refs[page]:
             heapq.heappush(self._free, page)
@@ -123,17 +127,39 @@ class PagedCache:
         """Forget ``seq``; its pages that no other sequence has become free."""
         for page in self._pages[self._known(seq)]:
             self._drop(page)
-        del self._pages[seq], self._length[seq]
+        del self._pages[seq], self._length[seq], self._gone[seq]
 
     def truncate(self, seq, length):
-        """Keep the first ``length`` tokens of ``seq``."""
+        """Keep the first ``length`` tokens of ``seq``. Where pages were
+        released, only so far back that the window of the next token still
+        holds what it held."""
         if not 0 <= length <= self._length[self._known(seq)]:
             raise ValueError(f"cannot keep {length} of {self._length[seq]} tokens")
+        if 0 < length < self._gone[seq]:
+            raise ValueError(f"cannot keep {length} tokens: pages of the window before them were released")
         keep = -(-length // self.page_size)
         for page in self._pages[seq][keep:]:
             self._drop(page)
         del self._pages[seq][keep:]
         self._length[seq] = length
+        if not length:
+            self._gone[seq] = 0
+
+    def release(self, seq, *, window, sinks=0):
+        """Give back the pages of ``seq`` that no token appended from now on
+        can see through ``tree_attention(..., window=window, sinks=sinks)``:
+        those behind the window of the next token, but for the first
+        ``sinks`` tokens'. Its length stays; ``batch`` names -1 in their place,
+        and ``read`` gives zeros."""
+        have = self._pages[self._known(seq)]
+        if window < 1 or sinks < 0:
+            raise ValueError(f"a window of {window} tokens and {sinks} sinks")
+        first = self._length[seq] - window + 1           # the next token's first key
+        for column in range(-(-sinks // self.page_size), max(0, first) // self.page_size):
+            if have[column] >= 0:
+                self._drop(have[column])
+                have[column] = -1
+                self._gone[seq] = self._length[seq]
 
     def _not_captured(self, what):
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
@@ -272,7 +298,7 @@ class PagedCache:
             paged.copy_pages(self._pools(), moved, holes)
             place = dict(zip(moved, holes))
             for seq, have in self._pages.items():
-                self._pages[seq] = [place.get(p, p) for p in have]
+                self._pages[seq] = [place.get(p, p) for p in have]   # (-1 stays)
             for old, new in place.items():
                 self._refs[new], self._refs[old] = self._refs[old], 0
         self._free = list(range(used, self.pages))

@@ -100,6 +100,13 @@ class CacheRead(ctypes.Structure):
                    ("kp_l", "kp_p", "kp_h", "kp_t", "vp_l", "vp_p", "vp_h", "vp_t", "table_s")])
 
 
+class Verify(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("batch", "draft", "vocab", "type", "tokens_wide", "uniforms_wide")]
+                + [(n, ctypes.c_void_p) for n in ("tokens", "target", "uniforms", "drafted", "parents", "rows", "counts", "next")]
+                + [(n, ctypes.c_int64) for n in
+                   ("tokens_s", "target_s", "target_n", "uniforms_s", "drafted_s", "drafted_n", "parents_s")])
+
+
 class Pool(ctypes.Structure):
     _fields_ = [("base", ctypes.c_void_p), ("layers", ctypes.c_int64), ("layer_bytes", ctypes.c_int64),
                 ("page_bytes", ctypes.c_int64)]
@@ -162,6 +169,9 @@ def load():
         "kh_decode_sizes": (ip, [ctypes.POINTER(ctypes.c_size_t)]),
         "kh_cache_read": (ip, [ctypes.POINTER(CacheRead), vp]),
         "kh_cache_read_host": (ip, [ctypes.POINTER(CacheRead)]),
+        "kh_verify_workspace_bytes": (ip, [ctypes.POINTER(Verify), ctypes.POINTER(ctypes.c_size_t)]),
+        "kh_verify_run": (ip, [ctypes.POINTER(Verify), vp, ctypes.c_size_t, vp]),
+        "kh_verify_host": (ip, [ctypes.POINTER(Verify)]),
         "kh_cache_copy": (ip, [ctypes.POINTER(Pool), ip, i32, ctypes.POINTER(i32), ctypes.POINTER(i32), ip, vp]),
         "kh_cache_copy_host": (ip, [ctypes.POINTER(Pool), ip, i32, ctypes.POINTER(i32), ctypes.POINTER(i32), ip]),
         "kh_probe_attn_timeline": (ip, [vp, vp, vp, vp, ip, ip, ip, ctypes.POINTER(ctypes.c_int64), ip,
@@ -183,9 +193,9 @@ def load():
     mine = (ctypes.sizeof(Paged), ctypes.sizeof(CacheAppend), ctypes.sizeof(Pool))
     if tuple(paged) != mine:
         raise RuntimeError(f"libkiln_hip's paged structures {tuple(paged)} != binding {mine}; rebuild")
-    decode = (ctypes.c_size_t * 1)()
+    decode = (ctypes.c_size_t * 2)()
     lib.kh_decode_sizes(decode)
-    if tuple(decode) != (ctypes.sizeof(CacheRead),):
+    if tuple(decode) != (ctypes.sizeof(CacheRead), ctypes.sizeof(Verify)):
         raise RuntimeError(f"libkiln_hip's structures of decoding {tuple(decode)} != binding; rebuild")
     _lib = lib
     return lib
@@ -198,7 +208,8 @@ EXPORTED = ("kh_version", "kh_build_id", "kh_abi_sizes", "kh_last_error", "kh_in
             "kh_plan_capture", "kh_plan_replay", "kh_plan_time", "kh_plan_chains", "kh_plan_chain_timeouts",
             "kh_plan_chain_spin",
             "kh_plan_destroy", "kh_paged_sizes", "kh_paged_workspace_bytes", "kh_paged_run", "kh_paged_host",
-            "kh_cache_append", "kh_cache_append_host", "kh_decode_sizes", "kh_cache_read", "kh_cache_read_host", "kh_cache_copy", "kh_cache_copy_host",
+            "kh_cache_append", "kh_cache_append_host", "kh_decode_sizes", "kh_cache_read", "kh_cache_read_host", "kh_verify_workspace_bytes",
+            "kh_verify_run", "kh_verify_host", "kh_cache_copy", "kh_cache_copy_host",
             "kh_probe_attn_timeline", "kh_probe_mfma_valu")
 
 

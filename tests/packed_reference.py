@@ -192,3 +192,69 @@ def read(k_pages, v_pages, table, starts, ends, tokens):
                 k[:, s, a] = k_pages[:, int(table[s, p // ps]), :, p % ps]
                 v[:, s, a] = v_pages[:, int(table[s, p // ps]), :, p % ps]
     return k, v
+
+
+def weights(row):
+    x = row.double().cpu()
+    return torch.where(x > 0, x, 0.0)
+
+
+def drawn(w, u):
+    """The first index whose running sum passes u of the whole."""
+    whole = float(w.sum())
+    if not whole < math.inf or whole <= 0:
+        return -1
+    past = (torch.cumsum(w, 0) > max(u, 0.0) * whole).nonzero()
+    return int(past[0]) if len(past) else int(w.nonzero()[-1])
+
+
+def verify(tokens, target, uniforms, parents=None, draft=None):
+    """(rows, counts, after), lists."""
+    batch, n, vocab = target.shape
+    out = [], [], []
+    for s in range(batch):
+        follows = list(range(-1, n - 1)) if parents is None else parents[s].tolist()
+        token, u = tokens[s].tolist(), uniforms[s].double().tolist()
+        path, after = [], -1
+        if follows[0] == -1:
+            path, w, whole = [0], weights(target[s, 0]), 1.0
+            choice = drawn(w, u[0])
+            for i in range(1, n):
+                if follows[i] != path[-1] or not 0 <= token[i] < vocab:
+                    continue
+                if draft is None:
+                    if token[i] != choice:
+                        continue
+                else:
+                    q = draft[s, path[-1]].double().cpu()
+                    if not u[i] * whole * float(q[token[i]]) < float(w[token[i]]):
+                        w = weights(w - whole * q)
+                        whole = float(w.sum())
+                        continue
+                path.append(i)
+                w, whole = weights(target[s, i]), 1.0
+                choice = drawn(w, u[i])
+            after = choice if draft is None else drawn(w if float(w.sum()) > 0 else weights(target[s, path[-1]]), u[0])
+        out[0].append(path + [-1] * (n - len(path)))
+        out[1].append(len(path))
+        out[2].append(after)
+    return out
+
+
+def drafted(gen, batch, n, vocab, dtype=torch.float32, tree=True, probs=True, noise=0.7, device="cpu", root=True):
+    """Operands of verify_tokens: a noisy draft's tokens, so that some are kept and some are not."""
+    target = 2 * torch.randn(batch, n, vocab, generator=gen)
+    draft = (target + noise * torch.randn(batch, n, vocab, generator=gen)).softmax(-1).to(dtype)
+    target = target.softmax(-1).to(dtype)
+    parents = None
+    up = (torch.arange(n) - 1).clamp(min=0).expand(batch, n)
+    if tree:
+        back = 1 + (torch.randn(batch, n, generator=gen).abs() * 2).long()
+        up = (torch.arange(n) - back).clamp(min=0)
+        parents = up.to(torch.int32).clone()
+        parents[:, 0] = -1
+    rows = draft[torch.arange(batch)[:, None], up].float()
+    tokens = torch.multinomial(rows.flatten(0, 1), 1, generator=gen).view(batch, n)
+    p = dict(tokens=tokens, target=target, uniforms=torch.rand(batch, n, generator=gen), parents=parents,
+             draft=draft if probs else None)
+    return {name: None if t is None else t.to(device) for name, t in p.items()}

@@ -226,3 +226,52 @@ def test_packed_cache_keeps_what_it_is_given(interpreting):
     other.append(there, k, v, rows=[list(range(cache.length(s))) for s in seqs])
     for a, b in zip(other.read(there), (k, v)):
         assert torch.equal(a, b)
+
+
+def test_release(interpreting):
+    cache = kiln.PagedCache(1, 12, 16, 1, 32, dtype=torch.float32)
+    a = cache.open()
+    k = torch.randn(1, 1, 100, 1, 32, generator=gen(8))
+    cache.append([a], k, k)
+    whole = cache.read([a])[0]
+    cache.release(a, window=101)                  # everything is in it
+    assert cache.free_pages == 5 and -1 not in cache.pages_of(a)
+    cache.release(a, window=40, sinks=17)         # keys 61 .. and 0 .. 16 are seen: page 2 alone is not
+    assert [p < 0 for p in cache.pages_of(a)] == [False, False, True, False, False, False, False] and cache.free_pages == 6
+    assert cache.length(a) == 100
+    got = cache.read([a])[0]
+    assert torch.equal(got[:, :, :32], whole[:, :, :32]) and not got[:, :, 32:48].any() and torch.equal(got[:, :, 48:], whole[:, :, 48:])
+    q = torch.randn(1, 3, 2, 32, generator=gen(9))
+    new = torch.randn(1, 3, 1, 32, generator=gen(10))
+    fresh = kiln.PagedCache(1, 12, 16, 1, 32, dtype=torch.float32)
+    b = fresh.open()
+    fresh.append([b], k, k)
+    for more in (dict(window=40, sinks=17), dict(window=3)):
+        out = [kiln.tree_attention(q, new, new, c.k[0], c.v[0], *c.batch([s]), **more) for c, s in ((cache, a), (fresh, b))]
+        assert torch.equal(*out)
+    (c,) = cache.fork(a)                          # shares what is left
+    cache.release(c, window=20)
+    assert [p < 0 for p in cache.pages_of(c)] == [True] * 5 + [False, False] and cache.free_pages == 6
+    for length in (1, 99):
+        with pytest.raises(ValueError):
+            cache.truncate(a, length)
+    cache.append([a], k[:, :, :30], k[:, :, :30])
+    cache.truncate(a, 100)
+    cache.append([a, c], k[:, :, :2].expand(1, 2, 2, 1, 32), k[:, :, :2].expand(1, 2, 2, 1, 32))
+    assert cache.length(a) == cache.length(c) == 102
+    assert torch.equal(cache.read([a])[0][:, :, 100:], k[:, :, :2])
+    used = cache.compact()
+    assert used == 12 - cache.free_pages and all(p < used for s in (a, c) for p in cache.pages_of(s))
+    assert torch.equal(cache.read([a])[0][:, :, 48:100], whole[:, :, 48:])
+    cache.free(a)
+    cache.truncate(c, 0)
+    assert cache.free_pages == 12 and cache.read([c])[0].shape[2] == 0
+    cache.append([c], k, k)                       # (anew: nothing of it is gone)
+    cache.truncate(c, 3)
+    for window, sinks in ((0, 0), (-1, 0), (3, -1)):
+        with pytest.raises(ValueError):
+            cache.release(c, window=window, sinks=sinks)
+    with pytest.raises(ValueError):
+        cache.release(99, window=3)
+    cache.release(c, window=1)
+    assert cache.free_pages == 11                 # (the last page has room)
