@@ -86,12 +86,6 @@ __device__ __forceinline__ int counted_rows(const kh_cache_append_op &a, int s) 
   return a.accept;
 }
 
-// The largest of a quad of lanes.
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
-  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
-}
-
 constexpr int kAhead = 4;   // tokens of a thread whose loads are in flight together: of those that are there
 constexpr int kPair = 2;    // ... and of the new ones, k and v of each
 

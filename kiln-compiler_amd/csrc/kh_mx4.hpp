@@ -27,6 +27,7 @@
 namespace kh {
 
 constexpr int kMxBlock = 32;
+constexpr uint32_t kMxMost = 252;   // the largest scale byte of numbers: what is above stands for NaN
 
 // Byte offsets inside a page of a head, of token t's element d (its low half
 // where d is even) and of its block's scale byte.
@@ -47,14 +48,14 @@ __host__ __device__ inline int mx_value_scale(int t, int d, int dim, int page_si
 __host__ __device__ inline uint32_t mx_scale_of(uint32_t most) {
   if (most >= 0x7f800000u) return 255u;
   const int e = (int)(most >> 23) - 2 + ((most & 0x7fffffu) >= 0x600000u ? 1 : 0);
-  return e < 2 ? 2u : e > 252 ? 252u : (uint32_t)e;
+  return e < 2 ? 2u : e > (int)kMxMost ? kMxMost : (uint32_t)e;
 }
 
 // -- on the CPU -------------------------------------------------------------------
 
 inline float mx_value(uint32_t code, uint32_t e) {
   static const float level[8] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f};
-  if (e == 255) return std::nanf("");
+  if (e > kMxMost) return std::nanf("");
   const float x = std::ldexp(level[code & 7], (int)e - 127);
   return code & 8 ? -x : x;
 }
@@ -86,8 +87,12 @@ inline void mx_round(float *x) {
 typedef __bf16 mx_bf16x2 __attribute__((ext_vector_type(2)));
 typedef float mx_f32x2 __attribute__((ext_vector_type(2)));
 
-// The power of two of a scale byte, NaN of 255.
-__device__ __forceinline__ float mx_scale(uint32_t e) { return __uint_as_float(e == 255u ? 0x7fc00000u : e << 23); }
+// The power of two of a scale byte, or NaN.
+__device__ __forceinline__ float mx_scale(uint32_t e) { return __uint_as_float(e > kMxMost ? 0x7fc00000u : e << 23); }
+
+// ... left to the conversions, which take an exponent of 255 for NaN (253 and 254,
+// which no writer makes, for 2^126 and 2^127)
+__device__ __forceinline__ float mx_scale_raw(uint32_t e) { return __uint_as_float(e << 23); }
 
 // Codes 2 i and 2 i + 1 of a word as a pair of bf16, exact.
 template <int I>
@@ -109,6 +114,12 @@ __device__ __forceinline__ uint32_t mx_most(const float (&x)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
   return m;
+}
+
+// The largest of a quad of lanes.
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
 }
 
 // 8 values as codes under scale byte e.

@@ -33,7 +33,7 @@ constexpr int kWideRows = 48;
 int row_blocks(const kh_paged &p) {
   const int rows = (p.top ? 1 : p.draft) * (p.heads / p.kv_heads);
   const int dt = padded_dim(p.dim);
-  if (p.cache_type != KH_TYPE_F32 && p.cache_type != KH_TYPE_MX4 && dt < 256 && rows >= kWideRows && p.batch <= kMaxWideBatch) return kWideBlocks;
+  if (p.cache_type != KH_TYPE_F32 && dt < 256 && rows >= kWideRows && p.batch <= kMaxWideBatch) return kWideBlocks;
   return rows <= 16 || dt == 256 ? 1 : 2;
 }
 
@@ -48,7 +48,7 @@ PagedWork work_of(const kh_paged &p) {
   w.items = p.kv_heads * w.per_head;
   w.half_shift = 0;
   while ((16 << w.half_shift) < p.page_size) ++w.half_shift;
-  w.tile = rm == 16 * kWideBlocks ? kWideTile : kPagedTile;
+  w.tile = rm == 16 * kWideBlocks || p.cache_type == KH_TYPE_MX4 ? kWideTile : kPagedTile;
   w.draft_tiles = (p.draft + w.tile - 1) / w.tile;
   w.sel_tiles = (int)(((int64_t)p.top * p.page_size + w.tile - 1) / w.tile);
   w.rounds = 0;

@@ -279,9 +279,6 @@ struct Cache<KH_TYPE_F16> {
 // 4-bit pages: values are bf16 ones (kh_mx4.hpp), the products bf16's
 template <>
 struct Cache<KH_TYPE_MX4> : Cache<KH_TYPE_BF16> {};
-// elements that pages are counted in
-template <int CT>
-using PageElement = std::conditional_t<CT == KH_TYPE_MX4, uint8_t, typename Cache<CT>::T>;
 
 // n (4 or 8) adjacent activations from element i, fp32 or T, 16-byte (8-byte) aligned
 template <class T, int N>
@@ -385,22 +382,6 @@ struct Tile {
   uint32_t v[8][VC][VW];
 };
 
-// 4-bit pages: K: codes of the DT / 4 dimensions from DT / 4 g on of key 16 h + li
-// (one 16-byte load where DT is 128), their blocks' scale bytes in a word; V:
-// codes of 8 dimensions of 4 keys (16 bytes that lie together; heads of 64: of
-// which this lane uses 4, its neighbour the others) and the keys' scales.
-template <int DT>
-struct Tile<KH_TYPE_MX4, DT> {
-  static constexpr int KS = DT / 32;
-  static constexpr int VD = DT >= 128 ? 8 : 4;
-  static constexpr int VC = DT / (16 * VD);
-  static constexpr int PD = DT / 4;                        // adjacent dimensions of a lane's key
-  static constexpr int PW = PD < 32 ? 2 : 4;               // words of one block's share of them
-  static constexpr int PB = PD < 32 ? 1 : PD / 32;         // blocks
-  uint32_t k[2][PB][PW], ke[2];
-  uint32_t v[2][VC][4], ve[2][VC];
-};
-
 template <int N>
 __device__ __forceinline__ void load_words(const void *p, uint32_t (&x)[N]) {
   if constexpr (N == 2) {
@@ -418,12 +399,10 @@ __device__ __forceinline__ void load_words(const void *p, uint32_t (&x)[N]) {
 }
 
 // Where a tile's halves lie (uniform over the wave): rows of `valid` keys each.
-// 4-bit pages: k and v are the page's of the head, slot the half's first token.
 template <class T>
 struct Source {
   const T *k[2], *v[2];
   int k_row, v_row;    // elements from a key to the next
-  int slot[2];
   int valid[2];
   int draft;           // index among the new tokens' tiles, -1 for a cached one
   int pos;             // a cached tile's first key
@@ -447,9 +426,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
   constexpr int WAVES = paged_waves(DT, RT, WHOLE);
   typedef typename Cache<CT>::T T;
   typedef Tile<CT, DT> Regs;
-  typedef PageElement<CT> E;
-  constexpr bool F32 = CT == KH_TYPE_F32, MX = CT == KH_TYPE_MX4;
-  typedef std::conditional_t<MX && NQ == 2, _Float16, T> A;   // 16-bit activations
+  constexpr bool F32 = CT == KH_TYPE_F32;
   constexpr int KS = Regs::KS, VD = Regs::VD, VC = Regs::VC;
   constexpr int RM = 16 * RT;
   constexpr int NT = DT / 16;                  // 16-wide tiles of O^T: (chunk, t)
@@ -520,11 +497,11 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 
     // -- where tile t lies; the first tile at or after t with a key, in steps of the waves
     const_work &wt = fresh();
-    const E *kp = static_cast<const E *>(wt.p.k_pages) + c * wt.p.kp_h, *vp = static_cast<const E *>(wt.p.v_pages) + c * wt.p.vp_h;
+    const T *kp = static_cast<const T *>(wt.p.k_pages) + c * wt.p.kp_h, *vp = static_cast<const T *>(wt.p.v_pages) + c * wt.p.vp_h;
     const int64_t kp_p = wt.p.kp_p, vp_p = wt.p.vp_p;
     const int kp_t = (int)wt.p.kp_t, vp_t = (int)wt.p.vp_t, half_shift = wt.half_shift, pages = wt.p.pages;
     const const_ints row_of_table = ints_of(wt.p.table) + s * wt.p.table_s;
-    auto find = [&](int &t, Source<E> &r) {
+    auto find = [&](int &t, Source<T> &r) {
       for (; t < t1; t += WAVES) {
         if (t >= cached) {
           const_work &w = fresh();
@@ -537,11 +514,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           for (int h = 0; h < 2; ++h) {
             r.valid[h] = min(max(w.p.draft - (n0 + 16 * h), 0), 16);
             const int n = r.valid[h] ? n0 + 16 * h : 0;
-            if constexpr (!MX) {
-              r.k[h] = static_cast<const T *>(w.p.k) + (s * w.p.k_s + c * w.p.k_h + n * w.p.k_n);
-              r.v[h] = static_cast<const T *>(w.p.v) + (s * w.p.v_s + c * w.p.v_h + n * w.p.v_n);
-            }
-            if constexpr (MX) r.slot[h] = n;
+            r.k[h] = static_cast<const T *>(w.p.k) + (s * w.p.k_s + c * w.p.k_h + n * w.p.k_n);
+            r.v[h] = static_cast<const T *>(w.p.v) + (s * w.p.v_s + c * w.p.v_h + n * w.p.v_n);
           }
           return;
         }
@@ -574,64 +548,17 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           in = in && page >= 0 && page < pages;
           r.valid[h] = in ? min(len - pos, 16) : 0;
           const int there = in ? page : 0;
-          if constexpr (MX) {
-            r.slot[h] = slot;
-            r.k[h] = kp + there * kp_p;
-            r.v[h] = vp + there * vp_p;
-          } else {
-            r.k[h] = kp + (there * kp_p + (int64_t)(slot * kp_t));
-            r.v[h] = vp + (there * vp_p + (int64_t)(slot * vp_t));
-          }
+          r.k[h] = kp + (there * kp_p + (int64_t)(slot * kp_t));
+          r.v[h] = vp + (there * vp_p + (int64_t)(slot * vp_t));
         }
         if (r.valid[0] | r.valid[1]) return;
       }
     };
 
     // a new tile of fp32 activations over a 16-bit cache is rounded as it is loaded
-    auto rounds = [&](const Source<E> &r) { return !F32 && !MX && act32 && r.draft >= 0; };
+    auto rounds = [&](const Source<T> &r) { return !F32 && act32 && r.draft >= 0; };
     const int dim = wt.p.dim;
-    const int page_size = wt.p.page_size;
-    auto load_k = [&](const Source<E> &r, Regs &x) {
-      if constexpr (MX) {
-        constexpr int PD = Regs::PD, PW = Regs::PW, PB = Regs::PB;
-        if (r.draft >= 0) {   // new tokens: as the cache will hold them
-          const_work &w = fresh();
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int64_t base = s * w.p.k_s + c * w.p.k_h + (int64_t)(r.slot[h] + min(li, max(r.valid[h], 1) - 1)) * w.p.k_n;
-            x.ke[h] = 0;
-#pragma unroll
-            for (int b = 0; b < PB; ++b) {
-              float y[8 * PW];
-#pragma unroll
-              for (int e = 0; e < PW; ++e) {
-                const int d = PD * g + 8 * (PW * b + e), in = d < dim ? d : 0;
-                load_acts<A>(w.p.k, base + in, act32, reinterpret_cast<float (&)[8]>(y[8 * e]));
-              }
-              uint32_t most = mx_most(y);
-              if constexpr (PD < 32) most = max(most, (uint32_t)__shfl_xor((int)most, 16));
-              const uint32_t e8 = mx_scale_of(most);
-              x.ke[h] |= e8 << (8 * b);
-#pragma unroll
-              for (int e = 0; e < PW; ++e) x.k[h][b][e] = mx_pack(reinterpret_cast<float (&)[8]>(y[8 * e]), e8);
-            }
-          }
-          return;
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int t = r.slot[h] + min(li, max(r.valid[h], 1) - 1);
-            x.ke[h] = 0;
-#pragma unroll
-            for (int b = 0; b < PB; ++b) {
-              const int d = PD * g + 32 * b, in = d < dim ? d : 0;
-              load_words(r.k[h] + (uint32_t)mx_key_code(t, in, dim), x.k[h][b]);
-              x.ke[h] |= (uint32_t)r.k[h][(uint32_t)mx_key_scale(t, in, dim, page_size)] << (8 * b);
-            }
-          }
-          return;
-        }
-      } else {
+    auto load_k = [&](const Source<T> &r, Regs &x) {
       const void *base = rounds(r) ? fresh().p.k : nullptr;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -652,46 +579,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           }
         }
       }
-      }
     };
-    auto load_v = [&](const Source<E> &r, Regs &x) {
-      if constexpr (MX) {
-        constexpr int PAIR = VD == 8 ? 1 : 2;   // lanes of a chunk of 8 dimensions
-        if (r.draft >= 0) {
-          const_work &w = fresh();
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int vc = 0; vc < VC; ++vc) {
-              const int d = 16 * VD * vc + 8 * (li / PAIR), in = d < dim ? d : 0;
-              x.ve[h][vc] = 0;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int64_t base = s * w.p.v_s + c * w.p.v_h + (int64_t)(r.slot[h] + min(4 * g + i, max(r.valid[h], 1) - 1)) * w.p.v_n;
-                float y[8];
-                load_acts<A>(w.p.v, base + in, act32, y);
-                uint32_t most = mx_most(y);
-                most = max(most, (uint32_t)__shfl_xor((int)most, PAIR));
-                most = max(most, (uint32_t)__shfl_xor((int)most, 2 * PAIR));
-                const uint32_t e8 = mx_scale_of(most);
-                x.ve[h][vc] |= e8 << (8 * i);
-                x.v[h][vc][i] = mx_pack(y, e8);
-              }
-            }
-          return;
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int vc = 0; vc < VC; ++vc) {
-              const int d = 16 * VD * vc + 8 * (li / PAIR), in = d < dim ? d : 0;
-              const int t = r.slot[h] + 4 * g;
-              load_words(r.v[h] + (uint32_t)mx_value_code(t, in, dim), x.v[h][vc]);
-              x.ve[h][vc] = *reinterpret_cast<const uint32_t *>(r.v[h] + (uint32_t)mx_value_scale(t, in, dim, page_size));
-            }
-          return;
-        }
-      } else {
+    auto load_v = [&](const Source<T> &r, Regs &x) {
       const void *base = rounds(r) ? fresh().p.v : nullptr;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -715,11 +604,10 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           }
         }
       }
-      }
     };
 
     Regs x;
-    Source<E> here;
+    Source<T> here;
     int t = t0 + wave;
     find(t, here);
     if (t < t1) {
@@ -750,9 +638,9 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       const int64_t base = s * wq.p.q_s + row_token[rt] * wq.p.q_n + row_head[rt] * wq.p.q_h;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int d = MX ? DT / 4 * g + 8 * ks : 32 * ks + 8 * g;
+        const int d = 32 * ks + 8 * g;
         const bool in = row_ok[rt] && (d < dim);
-        load_acts<A>(wq.p.q, base + (in ? d : 0), act32, y[ks]);
+        load_acts<T>(wq.p.q, base + (in ? d : 0), act32, y[ks]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[ks][j] = in ? y[ks][j] : 0.0f;
       }
@@ -802,10 +690,10 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 
     while (t < t1) {
       int t_next = t + WAVES;
-      Source<E> next;
+      Source<T> next;
       find(t_next, next);
 
-      if constexpr (!MX) if (dim < DT) {   // beyond dim: whatever was read meets q = 0, which needs it finite
+      if (dim < DT) {   // beyond dim: whatever was read meets q = 0, which needs it finite
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
           if (32 * ks + 8 * g >= dim) {
@@ -831,24 +719,6 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
               for (int h = 0; h < 2; ++h)
                 sc[rt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[h][ks][j]), q32[rt][ks][j], sc[rt][h], 0, 0, 0);
-      } else if constexpr (MX) {
-        // (dimensions beyond dim hold the first block's values, which meet q = 0)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          u32x4 a[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t word = x.k[h][ks / Regs::PW][ks % Regs::PW];
-            const float scale = mx_scale(x.ke[h] >> (8 * (ks / Regs::PW)) & 255u);
-            a[h] = u32x4{mx_pair<0>(word, scale), mx_pair<1>(word, scale), mx_pair<2>(word, scale), mx_pair<3>(word, scale)};
-          }
-#pragma unroll
-          for (int n = NQ - 1; n >= 0; --n)
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) sc[rt][h] = Cache<CT>::mma(a[h], q16[n][rt][ks], sc[rt][h]);
-        }
       } else {
 #pragma unroll
         for (int n = NQ - 1; n >= 0; --n)
@@ -890,22 +760,6 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           for (int j = 0; j < 8; ++j)
             if (!(see[rt] >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1)) sc[rt][j >> 2][j & 3] = -INFINITY;
         }
-        if constexpr (MX) {
-          // values behind the last key, and new ones or ones that not every row
-          // sees, of a block that is NaN: any scale will do for a weight of 0, and
-          // NaN is added by hand below
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int vc = 0; vc < VC; ++vc) {
-              const uint32_t e8 = x.ve[j >> 2][vc] >> (8 * (j & 3)) & 255u;
-              const bool behind = 4 * g + (j & 3) >= here.valid[j >> 2];
-              if (e8 == 255u && (behind || masked)) {
-                x.ve[j >> 2][vc] ^= (255u ^ 127u) << (8 * (j & 3));
-                if (!behind) odd |= 1u << (8 * vc + j);
-              }
-            }
-        } else {
         // values behind the last key (a page's unwritten slots): their weight
         // is 0, which needs them finite
 #pragma unroll
@@ -941,7 +795,6 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
                   }
                 }
               }
-        }
         }
       }
 
@@ -1001,24 +854,12 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
           for (int i0 = 0; i0 < VD; i0 += 4) {
             u32x4 a[4];   // 8 keys of dimensions i0 ..
-            uint32_t pairs[8][2];   // two dimensions each
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if constexpr (MX) {
-                const float scale = mx_scale(x.ve[j >> 2][vc] >> (8 * (j & 3)) & 255u);
-                const uint32_t word = x.v[j >> 2][vc][j & 3] >> (VD == 8 ? 0 : 16 * (li & 1));
-                pairs[j][0] = i0 ? mx_pair<2>(word, scale) : mx_pair<0>(word, scale);
-                pairs[j][1] = i0 ? mx_pair<3>(word, scale) : mx_pair<1>(word, scale);
-              } else {
-                pairs[j][0] = x.v[j][vc][i0 / 2];
-                pairs[j][1] = x.v[j][vc][i0 / 2 + 1];
-              }
-            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                a[i][e] = __builtin_amdgcn_perm(pairs[2 * e + 1][i / 2], pairs[2 * e][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                a[i][e] = __builtin_amdgcn_perm(x.v[2 * e + 1][vc][(i0 + i) / 2], x.v[2 * e][vc][(i0 + i) / 2],
+                                                i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
             for (int n = NW - 1; n >= 0; --n)
 #pragma unroll
@@ -1033,21 +874,6 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
         const_work &w = fresh();
         for (int key = 0; key < kTile; ++key) {   // the values taken out, by hand
           const int j = 4 * (key >> 4) + (key & 3), from = (key & 15) >> 2;
-          if constexpr (MX) {   // (all of a block at once: bit 8 vc + j of the lane that holds it)
-            if (!__any(g == from && (odd & (0x01010101u << j)) != 0)) continue;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const uint32_t theirs = (uint32_t)__shfl((int)odd, 4 * g + r + 16 * from);
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int vc = 0; vc < VC; ++vc)
-                  if ((theirs >> (8 * vc + j) & 1) && (see[rt] >> key & 1)) {
-#pragma unroll
-                    for (int i = 0; i < VD; ++i) o[rt][vc][i][r] = NAN;
-                  }
-            }
-          } else {
           if (!__any(g == from && (odd >> j & 1))) continue;
           const int n = min(kTile * here.draft + key, w.p.draft - 1);
           const int64_t row = s * w.p.v_s + c * w.p.v_h + n * w.p.v_n;
@@ -1075,7 +901,6 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
                   if (!(fabsf(z) < INFINITY)) o[rt][vc][i][r] += weight * z;
                 }
               }
-          }
           }
         }
       }
@@ -1162,7 +987,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
             } else if constexpr (!F32) {
 #pragma unroll
               for (int i = 0; i < VD; i += 4)
-                *reinterpret_cast<u32x2 *>(static_cast<A *>(w.p.out) + out + d + i) = u32x2{pack2<A>(y[i], y[i + 1]), pack2<A>(y[i + 2], y[i + 3])};
+                *reinterpret_cast<u32x2 *>(static_cast<T *>(w.p.out) + out + d + i) = u32x2{pack2<T>(y[i], y[i + 1]), pack2<T>(y[i + 2], y[i + 3])};
             }
           }
       }
@@ -1209,7 +1034,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int CT>
 __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
-  if constexpr (CT == KH_TYPE_BF16)
+  if constexpr (CT != KH_TYPE_F16)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -1242,6 +1067,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
   constexpr int RPI = 64 / CH;                 // rows of a copy
   constexpr int RM = 32 * kWaves;
   constexpr int PART = 16 * RB, SIDE = NH * PART;   // bytes of 16 keys, of a tile's K or V
+  constexpr bool MX = CT == KH_TYPE_MX4;
+  typedef std::conditional_t<MX && NQ == 2, _Float16, T> A;   // 16-bit activations
   constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NQ > 1;
   constexpr float kBias = CT == KH_TYPE_F16 ? kWeightExp : 0.0f;
 
@@ -1252,6 +1079,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
   __shared__ uint32_t spots[kWideSpots];
   __shared__ uint32_t odd_keys[kMaxDraft / TK][2];   // new tokens with a value that is not finite, by tile
   __shared__ uint32_t odd_edge[WIN ? 2 : 1];         // keys of a tile on a window's edge with such a value
+  __shared__ uint32_t nan_blocks[MX ? 2 : 1][MX ? TK : 1];   // 4-bit pages: [buffer][key], a byte per block whose values are set aside
 
   const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1349,7 +1177,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
       for (int ks = 0; ks < KS; ++ks) {
         const int d = 16 * ks + 8 * half;
         const bool in = row_ok && d < dim;
-        load_acts<T>(wq.p.q, base + (in ? d : 0), act32, y[ks]);
+        load_acts<A>(wq.p.q, base + (in ? d : 0), act32, y[ks]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[ks][j] = in ? y[ks][j] : 0.0f;
       }
@@ -1432,6 +1260,106 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
       }
       if (odd) atomicOr(&odd_keys[t - cached][wave >> 1], odd << (16 * (wave & 1)));
     };
+    // 4-bit pages: a thread takes 16 bytes of K (32 dimensions of a key) or V (8
+    // of 4 keys) a turn, loads them a tile ahead of the one that is written to
+    // the LDS, which is a tile ahead of the one in use
+    constexpr int TURNS = 4 * DT / kThreads, KN = DT / 32, VN = DT / 8;   // 16-byte pieces of a key's K, of 4 keys' V
+    u32x4 raw[MX ? TURNS : 1];
+    uint32_t raw_e[MX ? TURNS : 1];   // a scale byte, or 4
+    auto piece = [&](int i, bool &values) {
+      const int x = i * kThreads + (int)threadIdx.x;
+      values = DT == 128 ? i == 1 : wave >= 2;
+      return values ? x - 2 * DT : x;
+    };
+    auto load_raw = [&](int t, int c0) {
+      if (t >= cached) return;
+      const_work &w = fresh();
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        bool values;
+        const int x = piece(i, values);
+        const int key = values ? 4 * (x / VN) : x / KN, d = values ? 8 * (x % VN) : 32 * (x % KN), in = d < dim ? d : 0;
+        const int part = NH * (t < span.head ? t : t + span.skip) + (key >> 4), slot = (part & half_mask) * 16 + (key & 15);
+        const int64_t page = spots[NH * (t - c0) + (key >> 4)] >> 5;
+        const uint8_t *at = static_cast<const uint8_t *>(values ? w.p.v_pages : w.p.k_pages) +
+                            (values ? c * w.p.vp_h + page * w.p.vp_p : c * w.p.kp_h + page * w.p.kp_p);
+        raw[i] = *reinterpret_cast<const u32x4 *>(at + (uint32_t)(values ? mx_value_code(slot, in, dim) : mx_key_code(slot, in, dim)));
+        if (values) raw_e[i] = *reinterpret_cast<const uint32_t *>(at + (uint32_t)mx_value_scale(slot, in, dim, w.p.page_size));
+        else raw_e[i] = at[(uint32_t)mx_key_scale(slot, in, dim, w.p.page_size)];
+      }
+    };
+    // tile t, of `valid` keys, into buffer `to`; new tokens are read and rounded here
+    auto expand = [&](int t, int to, const int (&valid)[NH]) {
+      const_work &w = fresh();
+      const uint32_t k_lds = lds0 + (uint32_t)(to * 2 * SIDE), v_lds = k_lds + SIDE;
+      const bool masked = t >= cached || (WIN && on_edge<WIN>(w, len, TK * (t < span.head ? t : t + span.skip), TK));
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        bool values;
+        const int x = piece(i, values);
+        const int key = values ? 4 * (x / VN) : x / KN, d = values ? 8 * (x % VN) : 32 * (x % KN), in = d < dim ? d : 0;
+        if (t >= cached) {
+          const int n0 = TK * (t - cached);
+          if (values) raw_e[i] = 0;
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {   // 8 dimensions of K, or of one of V's 4 keys (rolled: its registers would come on top)
+            if (!values) break;
+            float y[8];
+            load_acts<A>(w.p.v, s * w.p.v_s + c * w.p.v_h + (int64_t)min(n0 + key + j, w.p.draft - 1) * w.p.v_n + in, act32, y);
+            uint32_t most = mx_most(y);
+            most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+            most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+            const uint32_t e8 = mx_scale_of(most), word = mx_pack(y, e8);
+            raw_e[i] |= e8 << (8 * j);
+            raw[i][0] = j == 0 ? word : raw[i][0];
+            raw[i][1] = j == 1 ? word : raw[i][1];
+            raw[i][2] = j == 2 ? word : raw[i][2];
+            raw[i][3] = j == 3 ? word : raw[i][3];
+          }
+          if (!values) {
+            const int64_t base = s * w.p.k_s + c * w.p.k_h + (int64_t)min(n0 + key, w.p.draft - 1) * w.p.k_n + in;
+            uint32_t most = 0;
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+              float y[8];
+              load_acts<A>(w.p.k, base + 8 * j, act32, y);
+              most = max(most, mx_most(y));
+            }
+            raw_e[i] = mx_scale_of(most);
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+              float y[8];
+              load_acts<A>(w.p.k, base + 8 * j, act32, y);
+              const uint32_t word = mx_pack(y, raw_e[i]);
+              raw[i][0] = j == 0 ? word : raw[i][0];
+              raw[i][1] = j == 1 ? word : raw[i][1];
+              raw[i][2] = j == 2 ? word : raw[i][2];
+              raw[i][3] = j == 3 ? word : raw[i][3];
+            }
+          }
+        }
+        const int h = key >> 4, there = h == 0 ? valid[0] : h == 1 ? valid[1] : h == 2 ? valid[2] : valid[3];
+        const float k_scale = mx_scale(raw_e[i] & 255u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // K: dimensions d + 8 j of the key; V: dimensions d of key + j
+          const int r = values ? key + j : key, chunk = values ? d / 8 : d / 8 + j;
+          const uint32_t e8 = raw_e[i] >> (8 * j) & 255u;
+          float scale = values ? mx_scale(e8) : k_scale;
+          uint32_t word = raw[i][j];
+          bool none = !values && d >= dim;       // K beyond dim meets q = 0, which needs it finite
+          if (values) {
+            const bool behind = (r & 15) >= there;   // (their weight is 0, which needs them finite)
+            const bool aside = masked && e8 > kMxMost && !behind;
+            if (masked && !(d & 31)) reinterpret_cast<uint8_t *>(&nan_blocks[to][r])[d >> 5] = aside && d < dim ? 1 : 0;
+            none = behind || aside;
+          }
+          u32x4 y = {mx_pair<0>(word, scale), mx_pair<1>(word, scale), mx_pair<2>(word, scale), mx_pair<3>(word, scale)};
+          if (none) y = u32x4{0, 0, 0, 0};
+          *(lds_u32x4 *)(uintptr_t)((values ? v_lds : k_lds) + (uint32_t)(r * RB + ((chunk ^ swz_wide<DT>(r)) * 16))) = y;
+        }
+      }
+    };
     // the tile at or after t that has a key; valid[] of its parts
     auto find = [&](int &t, int c0, int c1, int (&valid)[NH]) {
       for (; t < c1; ++t) {
@@ -1459,20 +1387,39 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
       __syncthreads();
       int t = c0, valid[NH];
       find(t, c0, c1, valid);
-      if (t < c1) fetch(t, c0, buffer);
+      if constexpr (MX) {
+        if (t < c1) {
+          load_raw(t, c0);
+          expand(t, buffer, valid);
+          int t_next = t + 1, valid_next[NH];
+          find(t_next, c0, c1, valid_next);
+          if (t_next < c1) load_raw(t_next, c0);
+        }
+      } else {
+        if (t < c1) fetch(t, c0, buffer);
+      }
       while (t < c1) {
         int t_next = t + 1, valid_next[NH];
         find(t_next, c0, c1, valid_next);
-        copies_landed();
+        if constexpr (!MX) copies_landed();
         __syncthreads();   // this tile is there, and no wave reads the other buffer
-        if (t_next < c1) fetch(t_next, c0, buffer ^ 1);
+        if constexpr (MX) {
+          if (t_next < c1) {
+            expand(t_next, buffer ^ 1, valid_next);
+            int t_then = t_next + 1, valid_then[NH];
+            find(t_then, c0, c1, valid_then);
+            if (t_then < c1) load_raw(t_then, c0);
+          }
+        } else {
+          if (t_next < c1) fetch(t_next, c0, buffer ^ 1);
+        }
         const uint32_t k_lds = lds0 + (uint32_t)(buffer * 2 * SIDE), v_lds = k_lds + SIDE;
         const int draft = t >= cached ? t - cached : -1;
         int fewest = valid[0] & valid[1] & valid[2] & valid[3];
         const int pos = TK * (t < span.head ? t : t + span.skip);
         const bool edge = WIN && draft < 0 && on_edge<WIN>(fresh(), len, pos, TK);
         const bool partly = draft >= 0 || edge || fewest < 16;
-        if (WIN && edge) {
+        if constexpr (WIN && !MX) if (edge) {
           // a value that is not finite must not reach rows that do not see its
           // key: set aside, as a new token's is
           if (threadIdx.x < 2) odd_edge[threadIdx.x] = 0;
@@ -1498,7 +1445,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
           }
           __syncthreads();
         }
-        if (draft < 0 && fewest < 16) {
+        if (!MX && draft < 0 && fewest < 16) {
           // values behind the last key (a page's unwritten slots): their weight
           // is 0, which needs them finite
 #pragma unroll
@@ -1509,7 +1456,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
           }
           __syncthreads();
         }
-        if (dim < DT) {   // K beyond dim meets q = 0, which needs it finite
+        if (!MX && dim < DT) {   // K beyond dim meets q = 0, which needs it finite
 #pragma unroll
           for (int i = 0; i < SIDE / (16 * kThreads); ++i) {
             const int chunk = i * kThreads + (int)threadIdx.x, r = chunk / CH, x = (chunk % CH) ^ swz_wide<DT>(r);
@@ -1621,7 +1568,23 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
           if (i & 1) __builtin_amdgcn_sched_barrier(0);
         }
 
-        if (draft >= 0 || (WIN && edge)) {
+        if constexpr (MX) {
+          if (draft >= 0 || (WIN && edge)) {
+            const uint32_t set_aside = nan_blocks[buffer][lane];
+            if (__builtin_expect(__any(set_aside != 0), 0)) {
+              for (int key = 0; key < TK; ++key) {
+                const uint32_t blocks = __builtin_amdgcn_readlane(set_aside, key);
+                if (!blocks || !((key >> 5 ? see[1] : see[0]) >> (key & 31) & 1)) continue;
+#pragma unroll
+                for (int t2 = 0; t2 < NT; ++t2)
+                  if (blocks >> (8 * t2) & 1) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[t2][r] = NAN;
+                  }
+              }
+            }
+          }
+        } else if (draft >= 0 || (WIN && edge)) {
           const uint32_t *set_aside = !WIN || draft >= 0 ? odd_keys[draft] : odd_edge;
           const uint32_t odd[2] = {set_aside[0], set_aside[1]};
           if (__builtin_expect(__any((odd[0] | odd[1]) != 0), 0)) {
@@ -1693,7 +1656,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[e] = done && l < 0.0f ? 0.0f : o[t2][4 * a + e] * norm;
           if (act32 || !done) *reinterpret_cast<f32x4 *>(to + d) = f32x4{y[0], y[1], y[2], y[3]};
-          else *reinterpret_cast<u32x2 *>(static_cast<T *>(we.p.out) + out + d) = u32x2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+          else *reinterpret_cast<u32x2 *>(static_cast<A *>(we.p.out) + out + d) = u32x2{pack2<A>(y[0], y[1]), pack2<A>(y[2], y[3])};
         }
     }
   }
@@ -1862,7 +1825,7 @@ template <int CT, int NQ, int NW, bool WIN>
 void launch_sizes(const PagedWork &w, int dt, int rt, hipStream_t stream) {
   if (dt == 256) launch_both<CT, NQ, NW, 256, 1, WIN>(w, stream);
   else if (rt == kWideBlocks) {
-    if constexpr (CT != KH_TYPE_F32 && CT != KH_TYPE_MX4) {
+    if constexpr (CT != KH_TYPE_F32) {
       if (dt == 128) launch_wide<CT, NQ, NW, 128, WIN>(w, stream);
       else launch_wide<CT, NQ, NW, 64, WIN>(w, stream);
     }

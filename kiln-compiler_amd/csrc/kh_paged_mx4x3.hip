@@ -1,11 +1,11 @@
 // kh_paged_mx4x3.hip - attention over a paged cache in 4 bits, fp32 activations: three bf16 parts of q and of the
-// weights (kh_paged_attn.hpp).
-#include "kh_paged_attn.hpp"
+// weights (kh_paged_mx4.hpp).
+#include "kh_paged_mx4.hpp"
 
 namespace kh {
 
 hipError_t launch_paged_mx4x3(const PagedWork &w, int dt, int rt, hipStream_t stream) {
-  return launch_passes<KH_TYPE_MX4, 3, 3>(w, dt, rt, stream);
+  return launch_mx4<3, 3>(w, dt, rt, stream);
 }
 
 }  // namespace kh

@@ -24,7 +24,7 @@ def block(x):
 
 
 def values(codes, e):
-    if e == 255:
+    if e > 252:
         return [math.nan] * 32
     return [(-1 if c > 7 else 1) * LEVELS[c % 8] * 2.0 ** (e - 127) for c in codes]
 
@@ -73,7 +73,7 @@ def unpack(pages, keys):
     code, scale = places(t, d, dim, page, keys)
     c, e = flat[:, code].long() >> 4 * (d % 2) & 15, flat[:, scale].double()
     x = torch.tensor(LEVELS, dtype=torch.float64)[c % 8] * torch.where(c > 7, -1.0, 1.0) * 2.0 ** (e - 127)
-    return torch.where(e == 255, math.nan, x).view(*pages.shape[:-1], dim)
+    return torch.where(e > 252, math.nan, x).view(*pages.shape[:-1], dim)
 
 
 def stored(x, dtype):

@@ -137,6 +137,12 @@ def test_drafts(draft, tree):
     check(ref.problem(gen(draft), act=torch.float16, draft=draft, heads=8, kv=1, tree=tree, lengths=(50, 3), dim=128, device="cuda"))
 
 
+def test_many_tokens_of_wide_heads():
+    # the new tokens' own pages in the LDS, at their largest
+    for act in ACTS:
+        check(ref.problem(gen(13), act=act, draft=256, heads=1, kv=1, dim=256, lengths=(50, 400), device="cuda"))
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_long_and_ragged(act):
     # ranges that end inside an item, and many items in one range
@@ -164,7 +170,7 @@ def test_what_is_masked_does_not_reach(act):
                 for pages, keys in ((p["k_pages"], True), (p["v_pages"], False)):
                     for d in range(0, dim, 32):
                         at = ref.places(t % 16, d, dim, 16, keys)[1]
-                        pages[page].view(2, -1)[:, at] = 255
+                        pages[page].view(2, -1)[:, at] = 253 + t % 3
         p["parents"] = torch.tensor([[-1, 0, 0, 1, 2, 4], [-1, -1, -1, -1, -1, -1]], dtype=torch.int32, device="cuda")
         p["v"][0, 1, 0, 3] = math.inf      # reaches tokens 1 and 3 of the first sequence alone
         p["v"][0, 4, 1] = math.nan         # tokens 4, 5
@@ -176,7 +182,10 @@ def test_what_is_masked_does_not_reach(act):
         p["v"][0, 1, 0, 3] = 0.0
         at = ref.places(5, 0, dim, 16, False)[1]
         p["v_pages"][int(p["table"][0, 1])].view(2, -1)[:, at] = 255   # a cached value: every row
-        check(p)
+        assert not torch.isfinite(check(p)[0, :, :, :32]).any()
+        at = ref.places(5, 0, dim, 16, True)[1]
+        p["k_pages"][int(p["table"][1, 0])].view(2, -1)[0, at] = 255   # a cached key: every row of its heads
+        assert not torch.isfinite(check(p)[1, :, :2]).any()
 
 
 def test_unused_rows_are_zeros():
