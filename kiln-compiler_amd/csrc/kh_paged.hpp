@@ -66,6 +66,11 @@ constexpr int kMaxWideBatch = 1024;
 constexpr int kPagedWaves = 4;     // waves of a workgroup
 // ... of paged_attn_kernel: eight where it takes whole items and two fit a SIMD
 constexpr int paged_waves(int dt, int rt, bool whole) { return whole && rt * dt <= 128 ? 8 : kPagedWaves; }
+// Tiles that an item over 4-bit pages counts for besides its own where ranges are
+// dealt out: beginning one is a few dependent loads, ending one a join and parts in
+// the workspace, together about as long as a workgroup takes for this many tiles.
+constexpr int kMxLead = 8;
+constexpr int kMxWideLead = 4;   // ... of 128 rows, whose tiles take longer
 constexpr int kMaxDraft = 256;     // new tokens of a sequence: a workgroup's table of paths fits the LDS
 constexpr int kMaxBatch = 4096;    // sequences of a call: each workgroup scans their lengths
 

@@ -21,6 +21,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 // on the device, so short sequences under a wide table run as ranges.
 constexpr int kWholeKeys = 1280, kWholeManyKeys = 4096, kWholeSlowKeys = 1024;
 
+// Over 4-bit pages (paged_mx4_kernel, tiles of 64 keys) the two meet elsewhere. 16
+// rows an item, eight waves, bf16, 8 heads of 128: 8 items of 2000 keys 18.4 (whole)
+// and 21.8 us (ranges), of 4000 keys 28.0 and 21.2; 128 items of 4000 keys 30.5 and
+// 31.5, of 8000 keys 53.9 and 43.3. 32 rows an item: four waves, 16 items of 1000
+// keys 23.2 and 30.1, of 2000 keys 33.8 and 30.5; 256 items of 4000 keys 57.6 and
+// 73.4, of 8000 keys 108 and 125 (heads of 64, eight waves: 71 and 102).
+constexpr int kMxWholeKeys = 2560, kMxWholeSlowKeys = 1536, kMxWholeManyKeys = 4096, kMxWholeManyRowsKeys = 8192;
+
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 // 16-row blocks of an item: one or two by its rows, what the registers of a
@@ -29,11 +37,29 @@ int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // blocks of 32 would read K and V twice (12 heads of 64, 1000 tokens, 4
 // sequences, bf16 under fp32 queries: 64 rows 29.5 us there, 32 rows 31.7 here).
 constexpr int kWideRows = 48;
+// Over 4-bit pages a row block's own reading of K and V costs little (they are
+// small and stay in the L2) and what splits 128 rows' keys much (64 KB of parts a
+// range), so paged_wide_kernel is for long ones, rows that fill its blocks, and 16-bit
+// activations (its parts of fp32 ones do not fit the registers): 16 sequences of 27
+// tokens, 108 rows a head, bf16 4000 keys 91.8 us there and 113 here, 1000 keys 60.3 and
+// 50.7; 64 rows a head, 8000 keys, 147 and 109; 108 rows, fp32, 8000 keys 316 and 254; 512
+// rows, fp16, 8000 keys 113 and 111, 32768 keys 254 and 335.
+constexpr int kMxWideKeys = 4096;
+
+// Keys of an item, at most: the table's or the picked pages', or the window's.
+int64_t most_keys(const kh_paged &p) {
+  const int64_t keys = (int64_t)(p.top ? p.top : p.width) * p.page_size;
+  return p.window ? std::min(keys, (int64_t)p.window + p.sinks) : keys;
+}
 
 int row_blocks(const kh_paged &p) {
   const int rows = (p.top ? 1 : p.draft) * (p.heads / p.kv_heads);
   const int dt = padded_dim(p.dim);
-  if (p.cache_type != KH_TYPE_F32 && dt < 256 && rows >= kWideRows && p.batch <= kMaxWideBatch) return kWideBlocks;
+  if (p.cache_type == KH_TYPE_MX4) {
+    const int filled = (rows + 16 * kWideBlocks - 1) / (16 * kWideBlocks) * 16 * kWideBlocks;
+    if (dt < 256 && 4 * rows >= 3 * filled && (p.act_type != KH_TYPE_F32 || p.one_pass) && most_keys(p) > kMxWideKeys && p.batch <= kMaxWideBatch)
+      return kWideBlocks;
+  } else if (p.cache_type != KH_TYPE_F32 && dt < 256 && rows >= kWideRows && p.batch <= kMaxWideBatch) return kWideBlocks;
   return rows <= 16 || dt == 256 ? 1 : 2;
 }
 
@@ -62,7 +88,11 @@ PagedWork work_of(const kh_paged &p) {
   // workgroups: one per item where none can have many tiles; else what the
   // chip holds at once, or a tile per wave of the most tiles the table has room for
   const bool eight = rm != 16 * kWideBlocks && paged_waves(padded_dim(p.dim), rm / 16, true) == 8;
-  const int64_t most_whole = !eight ? kWholeSlowKeys : 2 * items >= current_device().cus ? kWholeManyKeys : kWholeKeys;
+  const bool many = 2 * items >= current_device().cus;
+  const int64_t most_whole = p.cache_type == KH_TYPE_MX4 ? (many ? (rm == 16 ? kMxWholeManyKeys : kMxWholeManyRowsKeys) : eight ? kMxWholeKeys : kMxWholeSlowKeys)
+                             : !eight                    ? kWholeSlowKeys
+                             : many                      ? kWholeManyKeys
+                                                         : kWholeKeys;
   w.whole = per_item * w.tile <= most_whole;
   const bool two = rm == 16 * kWideBlocks || rm * padded_dim(p.dim) <= 16 * 128;   // workgroups of a CU
   const int cap = current_device().cus * (two ? 2 : 1);

@@ -132,15 +132,16 @@ __device__ __forceinline__ int tiles_of(W &w, int len) {
   return (w.sel_tiles ? w.sel_tiles : span_of<WIN>(w, len).tiles) + w.draft_tiles;
 }
 
-// first[s] = tiles of one item of the sequences before s, for s <= batch.
-template <bool WIN, class W>
+// first[s] = tiles of one item of the sequences before s, for s <= batch; LEAD: tiles
+// that an item counts for besides its own, in front of them (what beginning one costs).
+template <bool WIN, int LEAD, class W>
 __device__ __forceinline__ void scan_tiles(W &w, int *first, int *wave_sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = w.p.batch;
   const int per = (n + kThreads - 1) / kThreads;
   const int lo = threadIdx.x * per;
   int sum = 0;
-  for (int i = lo; i < min(lo + per, n); ++i) sum += tiles_of<WIN>(w, clamp_len(w, i));
+  for (int i = lo; i < min(lo + per, n); ++i) sum += tiles_of<WIN>(w, clamp_len(w, i)) + LEAD;
   int run = sum;   // inclusive over the wave
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -153,18 +154,19 @@ __device__ __forceinline__ void scan_tiles(W &w, int *first, int *wave_sums) {
   for (int i = 0; i < wave; ++i) at += wave_sums[i];
   for (int i = lo; i < min(lo + per, n); ++i) {
     first[i] = at;
-    at += tiles_of<WIN>(w, clamp_len(w, i));
+    at += tiles_of<WIN>(w, clamp_len(w, i)) + LEAD;
   }
   if (lo < n && lo + per >= n) first[n] = at;
   __syncthreads();
 }
 
-template <class W>
+template <int LEAD, class W>
 __device__ __forceinline__ Plan plan_of(W &w, const int *first) {
   Plan r;
   const uint32_t total = (uint32_t)__builtin_amdgcn_readfirstlane(first[w.p.batch]) * (uint32_t)w.items;
-  // a tile per wave at least
-  const uint32_t want = (total + kWaves - 1) / kWaves;
+  // a tile per wave at least, or as many tiles as a beginning counts for
+  const uint32_t least = LEAD ? 2 * LEAD : kWaves;
+  const uint32_t want = (total + least - 1) / least;
   r.count = (int)min(want, (uint32_t)w.grid);
   r.each = (int)(total / (uint32_t)r.count);
   r.extra = (int)(total - (uint32_t)r.each * r.count);
@@ -445,8 +447,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
   int me = blockIdx.x, at = 0, end = 1;
   if constexpr (!WHOLE) {
     const_work &w = fresh();
-    scan_tiles<WIN>(w, first, wave_sums);
-    const Plan plan = plan_of(w, first);
+    scan_tiles<WIN, 0>(w, first, wave_sums);
+    const Plan plan = plan_of<0>(w, first);
     if (me >= plan.count) return;
     // neighbouring ranges on the same XCD: they share row blocks' keys
     const int xcd = me & 7, per = plan.count >> 3, rest = plan.count & 7;
@@ -1068,6 +1070,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
   constexpr int RM = 32 * kWaves;
   constexpr int PART = 16 * RB, SIDE = NH * PART;   // bytes of 16 keys, of a tile's K or V
   constexpr bool MX = CT == KH_TYPE_MX4;
+  constexpr int LEAD = MX ? kMxWideLead : 0;
   typedef std::conditional_t<MX && NQ == 2, _Float16, T> A;   // 16-bit activations
   constexpr bool SCALED_Q = CT == KH_TYPE_F16 && NQ > 1;
   constexpr float kBias = CT == KH_TYPE_F16 ? kWeightExp : 0.0f;
@@ -1088,8 +1091,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
   const bool whole = fresh().whole;
   if (!whole) {
     const_work &w = fresh();
-    scan_tiles<WIN>(w, first, wave_sums);
-    const Plan plan = plan_of(w, first);
+    scan_tiles<WIN, LEAD>(w, first, wave_sums);
+    const Plan plan = plan_of<LEAD>(w, first);
     if (me >= plan.count) return;
     const int xcd = me & 7, per = plan.count >> 3, rest = plan.count & 7;
     me = xcd * per + min(xcd, rest) + (me >> 3);
@@ -1113,10 +1116,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
       len = clamp_len(w, s);
       tiles = tiles_of<WIN>(w, len);
       const int in_seq = at - __builtin_amdgcn_readfirstlane(first[s]) * w.items;
-      item = (int)((uint32_t)in_seq / (uint32_t)tiles);
-      t0 = in_seq - item * tiles;
-      t1 = min(tiles, t0 + (end - at));
+      item = (int)((uint32_t)in_seq / (uint32_t)(tiles + LEAD));
+      t0 = in_seq - item * (tiles + LEAD);
+      t1 = min(tiles + LEAD, t0 + (end - at));
       at += t1 - t0;
+      if constexpr (LEAD > 0) {
+        t0 = max(t0 - LEAD, 0);
+        t1 = max(t1 - LEAD, 0);
+        if (t1 == 0) continue;
+      }
     }
     const int cached = tiles - w.draft_tiles;
     const int c = (int)((uint32_t)item / (uint32_t)w.per_head);
@@ -1664,7 +1672,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
 
 // The parts of rows that few ranges share, joined: a wave per row, in range
 // order.
-template <int DT>
+template <int DT, int LEAD>
 __global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(const PagedWork w) {
   constexpr int RM = 32 * kWaves;
   constexpr int PER = DT / 64;
@@ -1673,11 +1681,11 @@ __global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(const PagedWo
   const kh_paged &p = w.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  scan_tiles<true>(w, first, wave_sums);
-  const Plan plan = plan_of(w, first);
+  scan_tiles<true, LEAD>(w, first, wave_sums);
+  const Plan plan = plan_of<LEAD>(w, first);
   const int s = blockIdx.x / w.items, item = blockIdx.x - s * w.items;
   const int tiles = tiles_of<true>(w, clamp_len(w, s));
-  const int x = first[s] * w.items + item * tiles;
+  const int x = first[s] * w.items + item * (tiles + LEAD) + LEAD;
   const int w0 = range_of(plan, x), w1 = range_of(plan, x + tiles - 1);
   if (w0 == w1) return;
   const int c = item / w.per_head, b = item - c * w.per_head;
@@ -1724,7 +1732,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(const PagedWo
 // The parts of the items that more than one range touched, joined: a
 // workgroup per row. Weights first, a part per lane, then the weighted sums,
 // every fourth part to a wave, then the waves' sums in order.
-template <int DT, int RT>
+template <int DT, int RT, int LEAD>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w) {
   constexpr int RM = 16 * RT;
   constexpr int PER = DT / 64;   // dimensions of a lane
@@ -1735,11 +1743,11 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedWork w)
   const kh_paged &p = w.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  scan_tiles<true>(w, first, wave_sums);
-  const Plan plan = plan_of(w, first);
+  scan_tiles<true, LEAD>(w, first, wave_sums);
+  const Plan plan = plan_of<LEAD>(w, first);
   const int s = blockIdx.x / w.items, item = blockIdx.x - s * w.items;
   const int tiles = tiles_of<true>(w, clamp_len(w, s));
-  const int x = first[s] * w.items + item * tiles;
+  const int x = first[s] * w.items + item * (tiles + LEAD) + LEAD;
   const int w0 = range_of(plan, x), w1 = range_of(plan, x + tiles - 1);
   if (w0 == w1) return;   // finished by its one range
   const int c = item / w.per_head, b = item - c * w.per_head;
@@ -1808,7 +1816,7 @@ void launch_both(const PagedWork &w, hipStream_t stream) {
   } else {
     paged_attn_kernel<CT, NQ, NW, DT, RT, false, WIN><<<w.grid, kThreads, 0, stream>>>(w);
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)std::min(w.rows, 16 * RT));
-    paged_join_kernel<DT, RT><<<grid, kThreads, 0, stream>>>(w);
+    paged_join_kernel<DT, RT, 0><<<grid, kThreads, 0, stream>>>(w);
   }
 }
 
@@ -1817,7 +1825,7 @@ void launch_wide(const PagedWork &w, hipStream_t stream) {
   paged_wide_kernel<CT, NQ, NW, DT, WIN><<<w.grid, kThreads, 0, stream>>>(w);
   if (!w.whole) {
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)((std::min(w.rows, 32 * kWaves) + kWaves - 1) / kWaves));
-    paged_join_rows_kernel<DT><<<grid, kThreads, 0, stream>>>(w);
+    paged_join_rows_kernel<DT, CT == KH_TYPE_MX4 ? kMxWideLead : 0><<<grid, kThreads, 0, stream>>>(w);
   }
 }
 

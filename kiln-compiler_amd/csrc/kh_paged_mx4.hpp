@@ -105,8 +105,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
   int me = blockIdx.x, at = 0, end = 1;
   if constexpr (!WHOLE) {
     const_work &w = fresh();
-    scan_tiles<WIN>(w, first, wave_sums);
-    const Plan plan = plan_of(w, first);
+    scan_tiles<WIN, kMxLead>(w, first, wave_sums);
+    const Plan plan = plan_of<kMxLead>(w, first);
     if (me >= plan.count) return;
     const int xcd = me & 7, per = plan.count >> 3, rest = plan.count & 7;
     me = xcd * per + min(xcd, rest) + (me >> 3);
@@ -132,10 +132,13 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       len = clamp_len(w, s);
       tiles = tiles_of<WIN>(w, len);
       const int in_seq = at - __builtin_amdgcn_readfirstlane(first[s]) * w.items;
-      item = (int)((uint32_t)in_seq / (uint32_t)tiles);
-      t0 = in_seq - item * tiles;
-      t1 = min(tiles, t0 + (end - at));
+      item = (int)((uint32_t)in_seq / (uint32_t)(tiles + kMxLead));
+      t0 = in_seq - item * (tiles + kMxLead);
+      t1 = min(tiles + kMxLead, t0 + (end - at));
       at += t1 - t0;
+      t0 = max(t0 - kMxLead, 0);
+      t1 = max(t1 - kMxLead, 0);
+      if (t1 == 0) continue;
     }
     const int cached = tiles - w.draft_tiles;
     const Span span = span_of<WIN>(w, len);
@@ -620,7 +623,7 @@ void launch_mx4_rows(const PagedWork &w, hipStream_t stream) {
   } else {
     paged_mx4_kernel<NQ, NW, DT, RT, false, WIN><<<w.grid, kThreads, lds, stream>>>(w);
     const dim3 grid((unsigned)(w.p.batch * w.items), (unsigned)std::min(w.rows, 16 * RT));
-    paged_join_kernel<DT, RT><<<grid, kThreads, 0, stream>>>(w);
+    paged_join_kernel<DT, RT, kMxLead><<<grid, kThreads, 0, stream>>>(w);
   }
 }
 
@@ -628,8 +631,10 @@ template <int NQ, int NW, bool WIN>
 void launch_mx4_sizes(const PagedWork &w, int dt, int rt, hipStream_t stream) {
   if (dt == 256) launch_mx4_rows<NQ, NW, 256, 1, WIN>(w, stream);
   else if (rt == kWideBlocks) {
-    if (dt == 128) launch_wide<KH_TYPE_MX4, NQ, NW, 128, WIN>(w, stream);
-    else launch_wide<KH_TYPE_MX4, NQ, NW, 64, WIN>(w, stream);
+    if constexpr (NQ < 3) {   // (not under fp32 activations)
+      if (dt == 128) launch_wide<KH_TYPE_MX4, NQ, NW, 128, WIN>(w, stream);
+      else launch_wide<KH_TYPE_MX4, NQ, NW, 64, WIN>(w, stream);
+    }
   } else if (dt == 128) {
     if (rt == 1) launch_mx4_rows<NQ, NW, 128, 1, WIN>(w, stream);
     else launch_mx4_rows<NQ, NW, 128, 2, WIN>(w, stream);

@@ -212,6 +212,34 @@ def test_tables_that_name_no_page():
     check(p, window=20, sinks=3)
 
 
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("tree", [True, False], ids=["tree", "chain"])
+def test_many_rows_over_long_caches(act, dim, tree):
+    # rows that share tiles; with a window, an unused token, NaN in the cache and among the new tokens
+    p = ref.problem(gen(14), act=act, batch=2, draft=26, heads=4, kv=1, dim=dim, page=64, lengths=(4700, 4200), tree=tree, device="cuda")
+    check(p)
+    if tree:
+        p["parents"][1, 3] = 3
+    p["v"][0, 25] = math.nan
+    p["k"][0, 24] = math.inf
+    for t in (100, 4300):                  # a value behind the window of every token, and one that some see
+        at = ref.places(t % 64, 0, dim, 64, False)[1]
+        p["v_pages"][int(p["table"][0, t // 64])].view(1, -1)[:, at] = 255
+    got = check(p, window=4097, sinks=33)
+    assert torch.isfinite(got[1]).all() and not torch.isfinite(got[0, :, :, :32]).any() and torch.isfinite(got[0, 0, :, 32:]).all()
+    for t in (4300,):
+        at = ref.places(t % 64, 0, dim, 64, False)[1]
+        p["v_pages"][int(p["table"][0, t // 64])].view(1, -1)[:, at] = 127
+    first = 4700 - 4200 + 1                # token 0's first key: the others do not see it
+    at = ref.places(first % 64, 32, dim, 64, False)[1]
+    p["v_pages"][int(p["table"][0, first // 64])].view(1, -1)[:, at] = 255
+    if not tree:
+        p["v"][0, 25], p["k"][0, 24] = 0.0, 0.0
+        got = check(p, window=4200, sinks=33)
+        assert not torch.isfinite(got[0, 0, :, 32:64]).any() and torch.isfinite(got[0, 1:]).all() and torch.isfinite(got[0, 0, :, :32]).all()
+
+
 # -- windows ---------------------------------------------------------------------------------------
 
 
