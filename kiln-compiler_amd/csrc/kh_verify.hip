@@ -93,11 +93,54 @@ __device__ __forceinline__ double left_of(double v, double q, const double *took
   return v;
 }
 
-__device__ __forceinline__ double add_lanes(double v) {
+// The weights that are left of probabilities p: a refusal at a time for all, so that
+// what it took is read once.
+template <int STEPS, int N>
+__device__ __forceinline__ void weigh(const float (&p)[STEPS][N], const float (&q)[STEPS][N], const double *took, int refusals, double (&v)[STEPS][N]) {
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+  for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[i][e] = p[i][e] > 0.0f ? (double)p[i][e] : 0.0;
+  for (int j = 0; j < refusals; ++j) {
+    const double r = took[j];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const double left = v[i][e] - r * q[i][e];
+        v[i][e] = left > 0.0 ? left : 0.0;
+      }
+  }
+}
+
+// v moved between lanes by a DPP control, 0 where nothing comes (DPP moves take a
+// few cycles where a permute through the LDS takes a hundred).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// A running sum over the lanes, own part included.
+__device__ __forceinline__ double scan_lanes(double v) {
+  v += moved<0x111, 0xF>(v);   // row_shr:1, 2, 4, 8
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  v += moved<0x142, 0xA>(v);   // row_bcast:15 to rows 1 and 3
+  v += moved<0x143, 0xC>(v);   // row_bcast:31 to rows 2 and 3
   return v;
 }
+
+__device__ __forceinline__ double lane_of(double v, int lane) {   // (a uniform lane: a scalar)
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+__device__ __forceinline__ double add_lanes(double v) { return lane_of(scan_lanes(v), 63); }
 
 // The sum of a stretch's weights, by one wave; the same in every lane.
 template <int PT, bool Q>
@@ -113,23 +156,14 @@ __device__ __forceinline__ double stretch_sum(const VerifyWork &w, const void *t
       load_probs<PT>(target, x, end, p[i]);
       if (Q && refusals) load_probs<PT>(draft, x, end, q[i]);
     }
+    double v[STEPS][N];
+    weigh(p, q, took, Q ? refusals : 0, v);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += left_of(p[i][e], Q && refusals ? q[i][e] : 0.0f, took, refusals);
+      for (int e = 0; e < N; ++e) sum += v[i][e];
   }
   return add_lanes(sum);
-}
-
-// A running sum over the lanes, own part included.
-__device__ __forceinline__ double scan_lanes(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const double o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
 }
 
 // The first token whose running sum passes `part` of the whole (the last with a
@@ -150,49 +184,55 @@ __device__ int find_token(const VerifyWork &w, const void *target, const void *d
     if (some) {   // (ballots are scalars)
       const int at = 63 - __builtin_clzll(some);
       last = c0 + at;
-      last_before = before + __shfl(run, at) - __shfl(mine, at);
+      last_before = before + lane_of(run, at) - lane_of(mine, at);
     }
     if (past) {
       const int at = __builtin_ctzll(past);
       found = c0 + at;
-      base = before + __shfl(run, at) - __shfl(mine, at);
+      base = before + lane_of(run, at) - lane_of(mine, at);
     }
-    before += __shfl(run, 63);
+    before += lane_of(run, 63);
   }
   if (found < 0) {
     if (last < 0) return -1;
     found = last;
     base = last_before;
   }
-  // the token
+  // the token: a lane looks at 16 that lie together
+  constexpr int STEPS = kStretch / (64 * N);
   const int x0 = found * w.stretch, end = min(w.p.vocab, x0 + w.stretch);
   int answer = -1, fallback = -1;
-  for (int x1 = x0; x1 < end && answer < 0; x1 += 64 * N) {
-    const int x = min(x1 + lane * N, end);
-    float p[N], q[N];
-    load_probs<PT>(target, x, end, p);
-    if (Q && refusals) load_probs<PT>(draft, x, end, q);
-    double v[N], mine = 0.0;
+  for (int x1 = x0; x1 < end && answer < 0; x1 += kStretch) {
+    const int x = min(x1 + lane * (kStretch / 64), end);
+    float p[STEPS][N], q[STEPS][N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      v[e] = left_of(p[e], Q && refusals ? q[e] : 0.0f, took, refusals);
-      mine += v[e];
+    for (int i = 0; i < STEPS; ++i) {
+      load_probs<PT>(target, min(x + i * N, end), end, p[i]);
+      if (Q && refusals) load_probs<PT>(draft, min(x + i * N, end), end, q[i]);
     }
+    double v[STEPS][N], mine = 0.0;
+    weigh(p, q, took, Q ? refusals : 0, v);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) mine += v[i][e];
     const double run = scan_lanes(mine);
     double at = base + (run - mine);
     int first = -1, any = -1;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      at += v[e];
-      if (v[e] > 0.0) {
-        any = x + e;
-        if (first < 0 && at > part) first = x + e;
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        at += v[i][e];
+        if (v[i][e] > 0.0) {
+          any = x + i * N + e;
+          if (first < 0 && at > part) first = any;
+        }
       }
-    }
     const uint64_t past = __ballot(first >= 0), some = __ballot(any >= 0);
-    if (past) answer = __shfl(first, __builtin_ctzll(past));
-    if (some) fallback = __shfl(any, 63 - __builtin_clzll(some));
-    base += __shfl(run, 63);
+    if (past) answer = __builtin_amdgcn_readlane(first, __builtin_ctzll(past));
+    if (some) fallback = __builtin_amdgcn_readlane(any, 63 - __builtin_clzll(some));
+    base += lane_of(run, 63);
   }
   return answer >= 0 ? answer : fallback;
 }
@@ -301,6 +341,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyWork w) {
   __shared__ double sums[kMaxStretches];
   __shared__ int drawn;
   const int s = blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  if (w.sums)
+    for (int c = threadIdx.x; c < w.stretches; c += blockDim.x) sums[c] = w.sums[(int64_t)s * w.stretches + c];
   load_walk<PT, Q>(w, s, t);
   const bool used = all_know(t.parent[0] == -1);
   Place r = {0, 0, used ? 1 : 0};
@@ -311,9 +353,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyWork w) {
   // the stretches' sums of the current row, and their whole
   auto add = [&](int refusals) {
     __syncthreads();   // (took, and nobody reads the old sums)
-    if (first) {
-      for (int c = threadIdx.x; c < w.stretches; c += blockDim.x) sums[c] = w.sums[(int64_t)s * w.stretches + c];
-    } else {
+    if (!first) {
       const void *target = row_of<PT>(w.p.target, s * w.p.target_s + r.now * w.p.target_n);
       const void *draft = row_of<PT>(w.p.drafted, s * w.p.drafted_s + r.now * w.p.drafted_n);
       for (int c = wave; c < w.stretches; c += waves) {
