@@ -422,10 +422,6 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyWork w) {
   }
 }
 
-// Sequences that leave compute units without work have the first sums of all
-// made beforehand.
-bool ahead(const kh_verify_op &p) { return p.batch < current_device().cus; }
-
 VerifyWork work_of(const kh_verify_op &p) {
   VerifyWork w;
   w.p = p;
@@ -434,6 +430,12 @@ VerifyWork work_of(const kh_verify_op &p) {
   w.sums = nullptr;
   return w;
 }
+
+// Sequences that leave compute units without work have the first sums of all
+// made beforehand, where that is more than four stretches a wave: a row of 50257 fp32
+// probabilities (and the draft's) takes one workgroup 10.5 us in all, 4.6 and 5.1
+// in two launches; 64 rows of 128000 23.0, and 14.3 and 7.9 us.
+bool ahead(const kh_verify_op &p) { return p.batch < current_device().cus && work_of(p).stretches > 4 * (kThreads / 64); }
 
 template <int PT, bool Q>
 void launch_of(const VerifyWork &w, hipStream_t stream) {

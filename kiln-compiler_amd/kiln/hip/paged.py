@@ -434,7 +434,8 @@ def _(k, v, k_pages, v_pages, table, lengths, rows, k_means):
 def _cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                 ends: torch.Tensor, tokens: int, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
     with torch.no_grad():
-        return run_read(k_pages, v_pages, table, starts, ends, tokens, dtype)
+        # (results of an operator share no memory)
+        return tuple(t.clone() for t in run_read(k_pages, v_pages, table, starts, ends, tokens, dtype))
 
 
 @_cache_read.register_fake
@@ -710,7 +711,7 @@ def run_read(k_pages, v_pages, table, starts, ends, tokens, dtype):
         rank = k_pages.dim()
         ks, vs = k_pages.stride(), v_pages.stride()
         if math.prod(shape) == 0:
-            return tuple(torch.empty(shape, dtype=dtype, device=k_pages.device) for _ in "kv")
+            return torch.empty((2, *shape), dtype=dtype, device=k_pages.device).unbind()
         if k_pages.shape[-4] == 0:
             raise ValueError("the cache has no pages")
         _ready(k_pages.device)
@@ -729,7 +730,7 @@ def run_read(k_pages, v_pages, table, starts, ends, tokens, dtype):
         _rows_in_place(k_pages, "k_pages")
         _rows_in_place(v_pages, "v_pages")
     device = k_pages.device
-    k, v = (torch.empty(found[1], dtype=dtype, device=device) for _ in "kv")
+    k, v = torch.empty((2, *found[1]), dtype=dtype, device=device).unbind()
     op.k, op.v, op.table, op.starts, op.ends = k.data_ptr(), v.data_ptr(), table.data_ptr(), starts.data_ptr(), ends.data_ptr()
     lib = kl.load()
     if device.type != "cuda":

@@ -81,15 +81,17 @@ def run_verify(tokens, target, uniforms, parents, draft):
             op.parents_s = parents.stride(0)
         size = ctypes.c_size_t()
         kl.check(kl.load().kh_verify_workspace_bytes(ctypes.byref(op), ctypes.byref(size)), "verify_tokens")
-        found = paged._keep(key, (bytes(op), size.value))
+        # one allocation holds the results and behind them, 16 bytes apart, the workspace
+        words = -(-batch * (n + 2) // 4) * 4
+        found = paged._keep(key, (bytes(op), size.value, words, (batch * n, batch, batch, words - batch * (n + 2) + size.value // 4)))
     elif tokens.device.type != "cuda" and not paged.interpreting():
         paged._one_device(tokens)
     op = kl.Verify.from_buffer_copy(found[0])
     device = tokens.device
     batch, n = op.batch, op.draft
-    # (one allocation: kept tokens, their number, the token after; and apart from them the sums)
-    out = torch.empty(batch * (n + 2), dtype=torch.int32, device=device)
-    rows, counts, after = out[:batch * n].view(batch, n), out[batch * n:batch * (n + 1)], out[batch * (n + 1):]
+    out = tokens.new_empty(found[2] + found[1] // 4, dtype=torch.int32)
+    rows, counts, after, _ = out.split_with_sizes(found[3])
+    rows = rows.view(batch, n)
     if batch == 0:
         return rows, counts, after
     op.tokens, op.target, op.uniforms = tokens.data_ptr(), target.data_ptr(), uniforms.data_ptr()
@@ -103,8 +105,7 @@ def run_verify(tokens, target, uniforms, parents, draft):
     if device.type != "cuda":
         rc = lib.kh_verify_host(ctypes.byref(op))
     else:
-        workspace = torch.empty(found[1], dtype=torch.uint8, device=device) if found[1] else None
-        rc = paged._on_device(device, lib.kh_verify_run, ctypes.byref(op), workspace.data_ptr() if found[1] else None, found[1])
+        rc = paged._on_device(device, lib.kh_verify_run, ctypes.byref(op), op.rows + 4 * found[2] if found[1] else None, found[1])
     if rc:
         kl.check(rc, "verify_tokens")
     return rows, counts, after
