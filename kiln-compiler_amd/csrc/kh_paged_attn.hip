@@ -60,7 +60,12 @@ int row_blocks(const kh_paged &p) {
     if (dt < 256 && 4 * rows >= 3 * filled && (p.act_type != KH_TYPE_F32 || p.one_pass) && most_keys(p) > kMxWideKeys && p.batch <= kMaxWideBatch)
       return kWideBlocks;
   } else if (p.cache_type != KH_TYPE_F32 && dt < 256 && rows >= kWideRows && p.batch <= kMaxWideBatch) return kWideBlocks;
-  return rows <= 16 || dt == 256 ? 1 : 2;
+  if (rows <= 16 || dt == 256) return 1;
+  // items of 32 rows that leave compute units without work are cut into 16: 64 rows of 8
+  // heads of 128, 250 keys 11.3 us and 16.1 in 32s, 8000 keys 26.3 and 30.6; of 16 sequences
+  // 20.6 and 15.7, 124 and 110
+  if (p.cache_type == KH_TYPE_MX4 && (int64_t)p.batch * p.kv_heads * (p.top ? p.draft : 1) * ((rows + 31) / 32) < current_device().cus) return 1;
+  return 2;
 }
 
 PagedWork work_of(const kh_paged &p) {
@@ -89,10 +94,11 @@ PagedWork work_of(const kh_paged &p) {
   // chip holds at once, or a tile per wave of the most tiles the table has room for
   const bool eight = rm != 16 * kWideBlocks && paged_waves(padded_dim(p.dim), rm / 16, true) == 8;
   const bool many = 2 * items >= current_device().cus;
-  const int64_t most_whole = p.cache_type == KH_TYPE_MX4 ? (many ? (rm == 16 ? kMxWholeManyKeys : kMxWholeManyRowsKeys) : eight ? kMxWholeKeys : kMxWholeSlowKeys)
-                             : !eight                    ? kWholeSlowKeys
-                             : many                      ? kWholeManyKeys
-                                                         : kWholeKeys;
+  const int64_t most_whole = p.cache_type == KH_TYPE_MX4 && rm != 16 * kWideBlocks
+                                 ? (many ? (rm == 16 ? kMxWholeManyKeys : kMxWholeManyRowsKeys) : eight ? kMxWholeKeys : kMxWholeSlowKeys)
+                             : !eight ? kWholeSlowKeys
+                             : many   ? kWholeManyKeys
+                                      : kWholeKeys;
   w.whole = per_item * w.tile <= most_whole;
   const bool two = rm == 16 * kWideBlocks || rm * padded_dim(p.dim) <= 16 * 128;   // workgroups of a CU
   const int cap = current_device().cus * (two ? 2 : 1);
