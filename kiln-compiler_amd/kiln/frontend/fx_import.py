@@ -16,7 +16,7 @@ and the HIP lowering recognises them (LayerNorm, softmax, bias + GELU):
   pow(x, 2)       mul(x, x)
 
 The operators over a paged cache (kiln/hip/paged.py) are one IR op each. Their
-pages may be bf16 or fp16 and their tables int32; those are inputs of the
+pages may be bf16, fp16 or uint8 (4 bits an element) and their tables int32; those are inputs of the
 compiled function (seen through views at most), everything else is float32.
 
 Python numbers become scalar constants, one per distinct value, created where
@@ -44,7 +44,8 @@ class Unsupported(NotImplementedError):
     """The graph uses something Kiln cannot compile."""
 
 
-_CACHE_TYPES = {torch.float32: "f32", torch.int32: "i32", torch.bfloat16: "bf16", torch.float16: "f16"}
+_CACHE_TYPES = {torch.float32: "f32", torch.int32: "i32", torch.bfloat16: "bf16", torch.float16: "f16",
+                torch.uint8: "u8"}
 
 
 def static_shape(node: torch.fx.Node, dtypes=(torch.float32,)) -> tuple:
@@ -328,13 +329,13 @@ def _typed(t, node, op, inputs, attrs):
 
 @translates(torch.ops.kiln.paged_attention.default)
 def _paged_attention(t, node, args, kwargs):
-    q, k, v, *cache, scale = args
-    *cache, parents, selected = cache
+    q, k, v, *cache, parents, selected, scale = args[:10]
+    window, sinks = (int(args[i] if len(args) > i else kwargs.get(name, 0)) for i, name in ((10, "window"), (11, "sinks")))
     optional = [x for x in (parents, selected) if x is not None]
     inputs = [t.value(x) for x in (q, k, v)] + [_cache_operand(t, node, x) for x in [*cache, *optional]]
     return _typed(t, node, "paged_attention", inputs,
                   dict(scale=float(scale), cache=inputs[3].type.dtype, parents=parents is not None,
-                       selected=selected is not None))
+                       selected=selected is not None, **(dict(window=window, sinks=sinks) if window else {})))
 
 
 @translates(torch.ops.kiln.select_pages.default)

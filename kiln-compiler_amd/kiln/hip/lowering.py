@@ -1780,10 +1780,11 @@ class _Lowerer:
             lists = list(n.inputs[7:])
             top = lists[-1].shape[3] if n.attrs["selected"] else 0
             operands = [*n.inputs[:7], n.out, *lists]
-            d.cfg[0] = {"f32": kl.TYPE_F32, "bf16": kl.TYPE_BF16, "f16": kl.TYPE_F16}[n.attrs["cache"]]
+            d.cfg[0] = {"f32": kl.TYPE_F32, "bf16": kl.TYPE_BF16, "f16": kl.TYPE_F16, "u8": kl.TYPE_MX4}[n.attrs["cache"]]
             d.cfg[2] = 1 if self.precision == "bf16" and d.cfg[0] != kl.TYPE_F32 else 0
             d.cfg[3] = 8 if n.attrs["parents"] else 0
             d.cfg[4] = 7 + len(lists) if n.attrs["selected"] else 0
+            d.cfg[5], d.cfg[6] = n.attrs.get("window", 0), n.attrs.get("sinks", 0)
             d.fparams[0] = n.attrs["scale"]
         for j, v in enumerate(operands):
             ref(j, v)
@@ -1793,7 +1794,8 @@ class _Lowerer:
         d.gemm[0], d.gemm[1], d.gemm[2] = pages, table.shape[1], top
         what = f"the best {top} of" if select else f"{top} picked of" if top else "over"
         self.add(d, k, f"{batch} x {draft} tokens, {heads} heads on {kv} of {dim}, {what} up to {table.shape[1]} pages "
-                       f"of {page}" + ("" if select else f", {n.attrs['cache']}{' one pass' if d.cfg[2] else ''}"))
+                       f"of {page}" + (f", a window of {d.cfg[5]} and {d.cfg[6]} sinks" if not select and d.cfg[5] else "")
+                 + ("" if select else f", {n.attrs['cache']}{' one pass' if d.cfg[2] else ''}"))
 
     # driver --------------------------------------------------------------------------------------
 

@@ -161,7 +161,7 @@ def host_constant(program, constants: dict, name: str) -> np.ndarray:
     return make(constants[src], offset, strides, batch, k, n).view(np.int16)
 
 
-TORCH_TYPES = {"f32": torch.float32, "i32": torch.int32, "bf16": torch.bfloat16, "f16": torch.float16}
+TORCH_TYPES = {"f32": torch.float32, "i32": torch.int32, "bf16": torch.bfloat16, "f16": torch.float16, "u8": torch.uint8}
 
 
 def check_cache_input(t, i, shape, dtype, device):

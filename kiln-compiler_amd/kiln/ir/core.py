@@ -22,13 +22,13 @@ from typing import NamedTuple
 import numpy as np
 
 
-ELEMENT_BYTES = {"f32": 4, "i32": 4, "bf16": 2, "f16": 2}
+ELEMENT_BYTES = {"f32": 4, "i32": 4, "bf16": 2, "f16": 2, "u8": 1}
 
 
 class TensorType(NamedTuple):
     """Static shape and element type: "f32", but for the operands of the paged
-    cache's operators (its pages may be "bf16" or "f16", tables and lists of
-    pages are "i32")."""
+    cache's operators (its pages may be "bf16", "f16" or, 4 bits an element,
+    "u8"; tables and lists of pages are "i32")."""
 
     shape: tuple
     dtype: str = "f32"

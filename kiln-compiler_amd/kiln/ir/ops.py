@@ -174,7 +174,8 @@ _add("expand", "view", 1, lambda shapes, attrs: broadcast_shapes(shapes[0], tupl
 # -- the paged cache (kiln/hip/paged.py says what the operators compute) -----------------------
 
 # paged_attention: q, k, v, k_pages, v_pages, table, lengths[, parents][, selected]
-#   {scale, cache (element type of the pages), parents, selected (whether given)}
+#   {scale, cache (element type of the pages; u8: 4 bits an element), parents, selected
+#   (whether given)[, window, sinks]}
 # select_pages: q, k_means, table, lengths {page_size, pages}
 
 
@@ -183,7 +184,8 @@ def _paged_attention_shape(shapes, attrs):
     given = 7 + bool(attrs["parents"]) + bool(attrs["selected"])
     s, n, heads, dim = q
     kv = k_pages[1]
-    ok = (len(shapes) == given and v_pages == k_pages and k_pages[3] == dim and k == v == (s, n, kv, dim)
+    row = dim // 32 * 17 if attrs["cache"] == "u8" and dim % 32 == 0 else dim   # (elements of a token's row)
+    ok = (len(shapes) == given and v_pages == k_pages and k_pages[3] == row and (attrs["cache"] != "u8" or dim % 32 == 0) and k == v == (s, n, kv, dim)
           and kv and heads % kv == 0 and table[0] == s and lengths == (s,))
     if ok and attrs["parents"]:
         ok = shapes[7] == (s, n)
@@ -201,7 +203,39 @@ def _select_pages_shape(shapes, attrs):
     return q[0], q[1], means[1], attrs["pages"]
 
 
+_LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6], np.float64)
+
+
+def _blocks(x):
+    """x [..., dim] as pages of 4 bits hold it (kiln/hip/paged.py)."""
+    x = x.astype(np.float64).reshape(*x.shape[:-1], -1, 32)
+    top = np.abs(x).max(-1, keepdims=True)
+    fine = np.isfinite(x).all(-1, keepdims=True)
+    _, power = np.frexp(np.where(fine, top, 1.0) / 7.0)        # the smallest 2^power above top / 7
+    step = np.ldexp(1.0, np.clip(power, -125, 125))
+    far = np.abs(np.abs(np.where(fine, x, 0.0) / step)[..., None] - _LEVELS)
+    near = (far + np.array([0.0, 1e-12] * 4)).argmin(-1)       # (a tie goes to the even code)
+    y = np.where(fine, np.copysign(_LEVELS[near], x) * step, np.nan)
+    return y.reshape(*y.shape[:-2], -1)
+
+
+def _unpacked(pages, keys):
+    """The values of pages of 4 bits (include/kiln_hip.h, kh_cache_append: how they lie)."""
+    ps, dim = pages.shape[-2], pages.shape[-1] // 17 * 32
+    flat = pages.astype(np.uint8).reshape(*pages.shape[:-2], -1)
+    t, d = np.arange(ps)[:, None], np.arange(dim)[None]
+    if keys:
+        code, scale = t * (dim // 2) + d // 2, t * (dim // 32) + d // 32
+    else:
+        code = t // 16 * 8 * dim + (t % 16 // 4 * (dim // 8) + d // 8) * 16 + t % 4 * 4 + d % 8 // 2
+        scale = t // 16 * (dim // 2) + (t % 16 // 4 * (dim // 32) + d // 32) * 4 + t % 4
+    c, e = flat[..., code] >> 4 * (d % 2).astype(np.uint8) & 15, flat[..., ps * dim // 2 + scale].astype(int)
+    return np.where(e > 252, np.nan, np.where(c > 7, -1.0, 1.0) * np.ldexp(_LEVELS[c & 7], e - 127))
+
+
 def _rounded(x, dtype):
+    if dtype == "u8":
+        return _blocks(x)
     if dtype == "f16":
         return x.astype(np.float16).astype(np.float64)
     if dtype == "bf16":   # nearest, ties to even
@@ -228,6 +262,9 @@ def _paged_attention(xs, attrs):
     batch, n, heads, dim = q.shape
     pages, kv, ps, _ = k_pages.shape
     new_k, new_v = _rounded(k, attrs["cache"]), _rounded(v, attrs["cache"])
+    if attrs["cache"] == "u8":
+        k_pages, v_pages = _unpacked(k_pages, True), _unpacked(v_pages, False)
+    window, sinks = attrs.get("window", 0), attrs.get("sinks", 0)
     out = np.zeros(q.shape)
     for s in range(batch):
         length = max(0, min(int(lengths[s]), table.shape[1] * ps))
@@ -240,10 +277,14 @@ def _paged_attention(xs, attrs):
                 if selected is not None:
                     row = [-1, *map(int, selected[s, i, c])]
                     columns = [b for a, b in zip(row, row[1:]) if b > a and 0 <= b < table.shape[1]]
-                spots = [(int(table[s, b]), min(ps, length - b * ps)) for b in columns if b * ps < length]
-                spots = [(p, m) for p, m in spots if 0 <= p < pages]
-                keys = np.concatenate([k_pages[p, c, :m] for p, m in spots] + [new_k[s, path, c]]).astype(np.float64)
-                values = np.concatenate([v_pages[p, c, :m] for p, m in spots] + [new_v[s, path, c]]).astype(np.float64)
+                spots = [(int(table[s, b]), b) for b in columns if b * ps < length]
+                spots = [(p, b, min(ps, length - b * ps)) for p, b in spots if 0 <= p < pages]
+                keys = np.concatenate([k_pages[p, c, :m] for p, _, m in spots] + [new_k[s, path, c]]).astype(np.float64)
+                values = np.concatenate([v_pages[p, c, :m] for p, _, m in spots] + [new_v[s, path, c]]).astype(np.float64)
+                if window:
+                    place = np.concatenate([np.arange(b * ps, b * ps + m) for _, b, m in spots] + [length + np.arange(len(path))])
+                    seen = (place < sinks) | (place > length + len(path) - 1 - window)
+                    keys, values = keys[seen], values[seen]
                 score = keys @ q[s, i, h].astype(np.float64) * attrs["scale"]
                 e = np.exp(score - score.max())
                 out[s, i, h] = e @ values / e.sum()

@@ -285,3 +285,166 @@ def test_what_is_behind_the_window_does_not_reach(cache, act, draft, heads):
 def test_window_of_everything():
     p = ref.problem(gen(12), cache=torch.bfloat16, act=torch.bfloat16, draft=5, lengths=(300, 7), device="cuda")
     assert torch.equal(kiln.tree_attention(**p, window=10 ** 6), kiln.tree_attention(**p))
+
+
+# -- in graphs, plans and beside other work ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("precision", ["fp32", "bf16"])
+@pytest.mark.parametrize("cache", [torch.uint8, torch.bfloat16])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (60, 3)])
+def test_compiled_block(precision, cache, window, sinks):
+    block = test_packed.gpt2_init_(test_packed.Block(128, 2, 16), seed=0).eval()
+    args = test_packed.block_operands(cache=cache, d=128, lengths=(500, 33))
+    model = test_packed.WindowBlock(block, 3, window, sinks)
+    on_gpu = tuple(t.cuda() for t in args)
+    compiled = kiln.compile(model, (args[0], *on_gpu[1:]), device="cuda", matmul_precision=precision)
+    got = compiled(*on_gpu)
+    if precision == "fp32":
+        want = test_packed.block_reference(block, *args, 3, window=window, sinks=sinks)
+        assert cache != torch.uint8 or all(test_packed.steps_agree(a, b) for a, b in zip(got[1:], want[1:]))
+        for a, b in zip(got, want):
+            torch.testing.assert_close(a.double().cpu(), b, rtol=1e-4, atol=1e-5)
+    else:
+        # the new tokens' keys and values as the plan's bf16 products made them (a 4-bit step may lie between those and
+        # the 64-bit ones), the rest of the block in 64 bits
+        q = block.double().c_attn(block.ln1(args[0].double())).detach()[:, :128].view(2, 3, 2, 64)
+        y = ref.attention(q.float(), got[1].float(), got[2].float(), *args[1:], window=window, sinks=sinks)
+        x = args[0].double() + block.c_proj(y.reshape(6, 128))
+        want = x + block.proj(torch.nn.functional.gelu(block.fc(block.ln2(x)), approximate="tanh"))
+        torch.testing.assert_close(got[0].double().cpu(), want, rtol=2e-2, atol=2e-2)
+
+
+def test_compiled_block_in_a_callers_graph():
+    block = test_packed.gpt2_init_(test_packed.Block(64, 2, 16), seed=1).eval()
+    args = test_packed.block_operands()
+    on_gpu = tuple(t.cuda() for t in args)
+    compiled = kiln.compile(test_packed.WindowBlock(block, 3, 30, 2), (args[0], *on_gpu[1:]), device="cuda")
+    compiled(*on_gpu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = compiled(*on_gpu)
+    for turn in range(4):
+        on_gpu[0].copy_(torch.randn(6, 64, generator=gen(turn)))
+        on_gpu[4].copy_(torch.tensor([40 - turn * 11, turn], dtype=torch.int32))
+        want = compiled(*on_gpu)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_torch_compile_backend(monkeypatch):
+    monkeypatch.setenv("KILN_STRICT", "1")
+    block = test_packed.gpt2_init_(test_packed.Block(64, 2, 16), seed=2).eval().cuda()
+    args = tuple(t.cuda() for t in test_packed.block_operands())
+    model = test_packed.WindowBlock(block, 3, 30, 2)
+    before = kiln.stats["compiled"]
+    with torch.no_grad():
+        got = torch.compile(model, backend=kiln.backend, dynamic=False)(*args)
+        want = model(*args)          # the operators as functions, torch's other kernels
+    assert kiln.stats["compiled"] > before
+    assert all(test_packed.steps_agree(a, b) for a, b in zip(got[1:], want[1:]))
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5)
+
+
+def test_calls_in_one_graph():
+    # ranges with a workspace, whole items, appends and reads: captured together, each with memory of its own
+    p = ref.problem(gen(20), act=torch.bfloat16, batch=2, draft=1, heads=8, kv=2, dim=128, page=64, lengths=(9000, 3000), device="cuda")
+    q = ref.problem(gen(21), act=torch.float32, batch=2, draft=4, heads=4, kv=2, dim=64, lengths=(90, 5), spare=6, device="cuda")
+    zero = torch.zeros(2, dtype=torch.int32, device="cuda")
+    out = {}
+
+    def step(pages):
+        out["long"] = kiln.tree_attention(**p)
+        out["window"] = kiln.tree_attention(**p, window=5000, sinks=4)
+        kiln.cache_append(q["k"], q["v"], pages[0], pages[1], q["table"], q["lengths"])
+        out["short"] = kiln.tree_attention(q["q"], q["k"], q["v"], *pages, q["table"], q["lengths"], q["parents"])
+        out["read"] = torch.stack(kiln.cache_read(*pages, q["table"], zero, q["lengths"], tokens=100))
+
+    mine = [q["k_pages"].clone(), q["v_pages"].clone()]
+    step(mine)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(mine)
+    captured = dict(out)
+    for turn in range(3):
+        g = gen(30 + turn)
+        p["q"].copy_(torch.randn(p["q"].shape, generator=g))
+        q["k"].copy_(torch.randn(q["k"].shape, generator=g))
+        q["lengths"].copy_(torch.tensor([80 - turn, 7 + turn], dtype=torch.int32))
+        other = [t.clone() for t in mine]
+        graph.replay()
+        step(other)
+        torch.cuda.synchronize()
+        for name, t in captured.items():
+            assert torch.equal(t.nan_to_num(), out[name].nan_to_num()), name
+        assert all(torch.equal(a, b) for a, b in zip(mine, other))
+
+
+def test_side_stream_and_threads():
+    import threading
+
+    p = ref.problem(gen(22), act=torch.bfloat16, batch=2, draft=3, heads=8, kv=2, dim=128, page=64, lengths=(7000, 100), device="cuda")
+    want = {w: kiln.tree_attention(**p, window=w) for w in (None, 40, 6000)}
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(w):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                if not torch.equal(kiln.tree_attention(**p, window=w), want[w]):
+                    bad.append(w)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(w,)) for w in (None, 40, 6000, None)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_other_strides_and_places():
+    p = ref.problem(gen(23), act=torch.float16, draft=5, heads=4, kv=2, dim=64, lengths=(40, 17), device="cuda")
+    want = kiln.tree_attention(**p, window=20, sinks=3)
+    q = dict(p)
+    q["q"] = torch.stack([p["q"]] * 2, 2)[:, :, 0]                              # rows apart
+    q["k"] = p["k"].transpose(1, 2).contiguous().transpose(1, 2)
+    q["v"] = torch.cat([p["v"], p["v"]], -1)[..., :64]
+    for name in ("k_pages", "v_pages"):
+        both = torch.zeros(len(p[name]), 3, 16, 34, dtype=torch.uint8, device="cuda")   # heads of a wider pool
+        both[:, 1:] = p[name]
+        q[name] = both[:, 1:]
+    q["table"] = torch.stack([p["table"]] * 2, -1)[..., 0]
+    q["lengths"] = torch.stack([p["lengths"]] * 2, -1)[:, 0]
+    assert torch.equal(kiln.tree_attention(**q, window=20, sinks=3), want)
+    layers = torch.stack([q["k_pages"], q["k_pages"]])
+    starts = torch.zeros(2, dtype=torch.int32, device="cuda")
+    a = kiln.cache_read(layers, layers, q["table"], starts, q["lengths"], tokens=41)
+    b = kiln.cache_read(p["k_pages"], p["k_pages"], p["table"], starts, p["lengths"], tokens=41)
+    assert all(torch.equal(x[0], y) and torch.equal(x[1], y) for x, y in zip(a, b))
+
+
+def test_another_cards_tensors_are_refused():
+    p = ref.problem(gen(24), device="cuda")
+    with pytest.raises(ValueError):
+        kiln.tree_attention(**dict(p, table=p["table"].cpu()))
+    with pytest.raises(ValueError):
+        kiln.cache_read(p["k_pages"], p["v_pages"], p["table"].cpu(), p["lengths"], p["lengths"], tokens=3)
+
+
+def test_as_operators_of_torch():
+    p = ref.problem(gen(25), device="cuda")
+    starts = torch.zeros(2, dtype=torch.int32, device="cuda")
+    pages = [p["k_pages"].clone(), p["v_pages"].clone()]
+    with torch.utils.flop_counter.FlopCounterMode(display=False):
+        got = kiln.tree_attention(**p, window=9, sinks=1)
+        kiln.cache_append(p["k"], p["v"], *pages, p["table"], p["lengths"])
+        k, v = kiln.cache_read(*pages, p["table"], starts, p["lengths"], tokens=30)
+    assert torch.equal(got, kiln.tree_attention(**p, window=9, sinks=1))
+    kiln.cache_append(p["k"], p["v"], p["k_pages"], p["v_pages"], p["table"], p["lengths"])
+    assert torch.equal(pages[0], p["k_pages"]) and torch.equal(pages[1], p["v_pages"])
+    assert torch.equal(k, kiln.cache_read(*pages, p["table"], starts, p["lengths"], tokens=30)[0])

@@ -10,12 +10,16 @@ sums differ by."""
 import math
 import random
 
+import numpy as np
 import pytest
 import torch
 
 import kiln
 import packed_reference as ref
-import paged_reference
+from kiln.frontend.fx_import import Unsupported, import_exported
+from kiln.ir import interpret, parse, verify
+from models.decoder import CachedBlock
+from models.transformer import Block, gpt2_init_
 
 FP4 = torch.float4_e2m1fn_x2
 
@@ -275,3 +279,94 @@ def test_release(interpreting):
         cache.release(99, window=3)
     cache.release(c, window=1)
     assert cache.free_pages == 11                 # (the last page has room)
+
+
+# -- through kiln.compile -----------------------------------------------------------------------------------
+
+
+class WindowBlock(CachedBlock):
+    """The cached block whose attention has a window."""
+
+    def __init__(self, block, tokens, window=None, sinks=0):
+        super().__init__(block, tokens)
+        self.window, self.sinks = window, sinks
+
+    def attend(self, x, k_pages, v_pages, table, lengths, parents, k_means):
+        b = self.block
+        split = (len(x) // self.tokens, self.tokens, b.nh, x.shape[-1] // b.nh)
+        q, k, v = (y.view(split) for y in b.c_attn(b.ln1(x)).split(x.shape[-1], dim=1))
+        y = kiln.tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents, window=self.window, sinks=self.sinks)
+        return x + b.c_proj(y.reshape(x.shape)), k, v
+
+
+def block_operands(cache=torch.uint8, seed=0, seqs=2, tokens=3, d=64, nh=2, lengths=(40, 17)):
+    p = ref.problem(gen(seed), cache=cache, batch=seqs, draft=tokens, heads=nh, kv=nh, dim=d // nh, lengths=lengths)
+    x = torch.randn(seqs * tokens, d, generator=gen(seed + 1))
+    return x, p["k_pages"], p["v_pages"], p["table"], p["lengths"], p["parents"]
+
+
+def block_reference(block, x, k_pages, v_pages, table, lengths, parents, tokens, **more):
+    """(the block's result, its keys and values) in 64 bits. (4-bit blocks have steps: a comparison is one only where
+    the keys and values round alike, steps_agree.)"""
+    b = block.double()
+    x = x.cpu().double()
+    shape = (len(x) // tokens, tokens, b.nh, x.shape[1] // b.nh)
+    with torch.no_grad():
+        q, k, v = (y.view(shape) for y in b.c_attn(b.ln1(x)).split(x.shape[1], 1))
+        y = ref.attention(q, k.float(), v.float(), k_pages, v_pages, table, lengths, parents, **more)
+        x = x + b.c_proj(y.reshape(x.shape))
+        out = x + b.proj(torch.nn.functional.gelu(b.fc(b.ln2(x)), approximate="tanh"))
+    block.float()
+    return out, k, v
+
+
+def steps_agree(got, want):
+    """Whether fp32 keys or values round to 4 bits as their 64-bit ones do."""
+    return torch.equal(ref.rounded(got.cpu().float()), ref.rounded(want.float()))
+
+
+@pytest.mark.parametrize("cache", [torch.uint8, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 3), (2, 0)])
+def test_compiled_block(interpreting, cache, window, sinks):
+    block = gpt2_init_(Block(64, 2, 16), seed=0).eval()
+    args = block_operands(cache=cache)
+    model = WindowBlock(block, 3, window, sinks)
+    compiled = kiln.compile(model, args, device="cuda")
+    assert compiled.report.lowering["families"]["paged"] == 1
+    got, want = compiled(*args), block_reference(block, *args, 3, window=window, sinks=sinks)
+    assert cache != torch.uint8 or all(steps_agree(a, b) for a, b in zip(got[1:], want[1:]))
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a.double(), b, rtol=1e-4, atol=1e-5)
+    args[4][0] = 31       # the cache is read in place, at each call anew
+    torch.testing.assert_close(compiled(*args)[0].double(), block_reference(block, *args, 3, window=window, sinks=sinks)[0], rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (5, 2)])
+def test_graph_text_and_meaning(window, sinks):
+    block = gpt2_init_(Block(64, 2, 16), seed=3).eval()
+    args = block_operands()
+    g = import_exported(torch.export.export(WindowBlock(block, 3, window, sinks), args).run_decompositions())
+    verify(g)
+    assert str(parse(str(g))) == str(g)
+    out = interpret(g, *[t.numpy() for t in args])
+    want = block_reference(block, *args, 3, window=window, sinks=sinks)
+    assert all(steps_agree(torch.tensor(a), b) for a, b in zip(out[1:], want[1:]))
+    np.testing.assert_allclose(out[0], want[0].numpy(), rtol=1e-4, atol=1e-5)
+
+
+def test_models_that_are_refused():
+    args = block_operands()
+
+    class Adds(torch.nn.Module):      # arithmetic on the pages' bytes
+        def forward(self, q, k_pages, table, lengths):
+            return kiln.tree_attention(q, q, q, k_pages + k_pages, k_pages, table, lengths)
+
+    class Verifies(torch.nn.Module):  # between steps, not in them
+        def forward(self, q, k_pages, table, lengths):
+            y = kiln.tree_attention(q, q, q, k_pages, k_pages, table, lengths)
+            return kiln.verify_tokens(table, y[:, :, 0].softmax(-1), y[:, :, 0, 0])[0]
+
+    q = torch.zeros(2, 3, 2, 32)
+    for model in (Adds(), Verifies()):
+        with pytest.raises(Unsupported):
+            import_exported(torch.export.export(model, (q, *args[1:2], *args[3:5])).run_decompositions())
