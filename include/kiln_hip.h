@@ -240,7 +240,8 @@ typedef struct kh_pass {
  *        of the table, picked pages per token (0: every page is read), 0};
  *        cfg[0] = cache type, cfg[1] = activation type (KH_TYPE_*), cfg[2] = 1:
  *        products on the cache type's own matrix instruction, one pass;
- *        cfg[5] = window, cfg[6] = sinks of ATTENTION; fparams[0] = scale. Refs, strides in elements of their own type:
+ *        cfg[5] = window, cfg[6] = sinks of ATTENTION; fparams[0] = scale. Refs,
+ *        strides in elements of their own type:
  *        ATTENTION 0 q, 1 k, 2 v over (sequence, token, head, d), 3, 4 the
  *        pages over (page, head, slot, d), 5 table over (sequence, column),
  *        6 lengths, 7 out (as q), then refs[cfg[3]] parents over (sequence,
@@ -453,11 +454,11 @@ int kh_paged_host(const kh_paged *op);
  * KH_TYPE_MX4 (dim a multiple of 32): a block is 32 adjacent dimensions of a
  * token, its elements a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6 (codes 0-7,
  * 8 more with the sign) times 2^(e - 127), e its scale byte: the smallest from
- * 2 to 252 for which the largest |x| is below 7 times it (or 252), 255
- * where an x is not finite (a byte above 252 is NaN); elements go to the nearest, ties to the even code. A page of a
- * head is page_size * 17 dim / 32 bytes, kp_p, kp_h (and vp_p, vp_h) count
- * bytes and kp_t, vp_t nothing: first the codes, element (t, d) the low half
- * (d even) or high half of byte
+ * 2 to 252 for which the largest |x| is below 7 times it (or 252), 255 (NaN)
+ * where an x is not finite; 253 and 254 are not scales. Elements go to the
+ * nearest, ties to the even code. A page of a head is page_size * 17 dim / 32
+ * bytes, kp_p, kp_h (and vp_p, vp_h) count bytes and kp_t, vp_t nothing: first
+ * the codes, element (t, d) the low half (d even) or high half of byte
  *   keys    t dim/2 + d/2
  *   values  (t/16) 8 dim + ((t%16)/4 dim/8 + d/8) 16 + (t%4) 4 + (d%8)/2
  * then, from byte page_size dim/2 on, the scale bytes, of (t, d) byte

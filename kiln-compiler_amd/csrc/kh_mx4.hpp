@@ -27,7 +27,7 @@
 namespace kh {
 
 constexpr int kMxBlock = 32;
-constexpr uint32_t kMxMost = 252;   // the largest scale byte of numbers: what is above stands for NaN
+constexpr uint32_t kMxMost = 252;   // the largest scale byte of numbers; 255 is NaN's, the two between nobody's
 
 // Byte offsets inside a page of a head, of token t's element d (its low half
 // where d is even) and of its block's scale byte.

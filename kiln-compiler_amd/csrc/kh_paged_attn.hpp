@@ -357,6 +357,24 @@ __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&out)[NP]) {
   }
 }
 
+// x (not negative) as parts that meet no infinite value: as split8, without what
+// that needs.
+template <class T, int NP>
+__device__ __forceinline__ void split_finite(const float (&x)[8], u32x4 (&out)[NP]) {
+  float rest[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) rest[j] = x[j];
+#pragma unroll
+  for (int part = 0; part < NP; ++part) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      out[part][m] = part + 1 < NP ? __builtin_amdgcn_perm(__float_as_uint(rest[2 * m + 1]), __float_as_uint(rest[2 * m]), 0x07060302u)
+                                   : pack2<T>(rest[2 * m], rest[2 * m + 1]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) rest[j] -= leading<T>(rest[j]);
+  }
+}
+
 __device__ __forceinline__ float max16x32(float v) {   // over the four lane groups of a query
   float2 p = row_pair(v);
   v = fmaxf(p.x, p.y);
@@ -1555,7 +1573,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = sc[i >> 1][8 * (i & 1) + e];
           u32x4 parts[NW];
-          split8<T, NW, false>(y, parts);
+          if constexpr (MX) split_finite<T, NW>(y, parts);
+          else split8<T, NW, false>(y, parts);
           u32x4 v[NT];
 #pragma unroll
           for (int t2 = 0; t2 < NT; ++t2) {
@@ -1578,7 +1597,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
 
         if constexpr (MX) {
           if (draft >= 0 || (WIN && edge)) {
-            const uint32_t set_aside = nan_blocks[buffer][lane];
+            const uint32_t set_aside = nan_blocks[buffer][lane] & (DT == 64 ? 0xffffu : ~0u);   // (bytes of its blocks)
             if (__builtin_expect(__any(set_aside != 0), 0)) {
               for (int key = 0; key < TK; ++key) {
                 const uint32_t blocks = __builtin_amdgcn_readlane(set_aside, key);

@@ -40,24 +40,6 @@ struct MxTile {
   uint32_t v[4][VC][4], ve[4][VC];
 };
 
-// x (not negative) as parts that meet no infinite value: as split8, without what
-// that needs.
-template <class T, int NP>
-__device__ __forceinline__ void split_finite(const float (&x)[8], u32x4 (&out)[NP]) {
-  float rest[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = x[j];
-#pragma unroll
-  for (int part = 0; part < NP; ++part) {
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-      out[part][m] = part + 1 < NP ? __builtin_amdgcn_perm(__float_as_uint(rest[2 * m + 1]), __float_as_uint(rest[2 * m]), 0x07060302u)
-                                   : pack2<T>(rest[2 * m], rest[2 * m + 1]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) rest[j] -= leading<T>(rest[j]);
-  }
-}
-
 // The new tokens of (s, c) into two 4-bit pages in the LDS, rounded as
 // kh_cache_append does: a thread takes 8 dimensions of a token, the 4 lanes of a
 // block agree on its largest.

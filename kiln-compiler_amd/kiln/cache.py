@@ -21,6 +21,7 @@ on tables made before can be captured). Not thread-safe.
 from __future__ import annotations
 
 import heapq
+import operator
 
 import torch
 
@@ -152,6 +153,7 @@ class PagedCache:
         ``sinks`` tokens'. Its length stays; ``batch`` names -1 in their place,
         and ``read`` gives zeros."""
         have = self._pages[self._known(seq)]
+        window, sinks = operator.index(window), operator.index(sinks)
         if window < 1 or sinks < 0:
             raise ValueError(f"a window of {window} tokens and {sinks} sinks")
         first = self._length[seq] - window + 1           # the next token's first key

@@ -24,11 +24,12 @@ NaN.
 The first three are also what a model given to ``kiln.compile`` or
 ``torch.compile(backend=kiln.backend)`` may call: they are the operators
 ``torch.ops.kiln.paged_attention`` and ``select_pages``, which the frontend
-translates. The last two change their arguments, which a compiled graph does
-not; they are called between the calls of a compiled step. Where a tracer or a
-dispatch mode watches (``torch.jit.trace``, ``make_fx``, a flop counter), a call
-goes through its operator in ``torch.ops.kiln``, which those see;
-``torch.jit.trace`` does not keep the last two, which refuse it.
+translates. ``cache_append`` and ``copy_pages`` change their arguments, which a
+compiled graph does not; they (and ``cache_read``) are called between the calls
+of a compiled step. Where a tracer or a dispatch mode watches
+(``torch.jit.trace``, ``make_fx``, a flop counter), a call goes through its
+operator in ``torch.ops.kiln``, which those see; ``torch.jit.trace`` does not
+keep those two, which refuse it.
 
 Each call runs on the current stream of its tensors' device, allocates its
 result and workspace from torch's allocator (so it can be captured into a
@@ -42,6 +43,7 @@ from __future__ import annotations
 import array
 import ctypes
 import math
+import operator
 
 import torch
 from torch.autograd import forward_ad
@@ -493,16 +495,18 @@ def tree_attention(q, k, v, k_pages, v_pages, table, lengths, parents=None, *, s
 
     Drafted keys and values are rounded to the cache's type first, so a token
     is attended to as it will be once it is appended. fp32 activations keep
-    fp32's accuracy over bf16 and fp16 caches too; 16-bit ones are exact in
-    the scores, their softmax weights keep 16 bits (bf16) or 22 (fp16), sums
-    are fp32, and the result is rounded once. Up to 256 tokens and 4096
+    fp32's accuracy over bf16, fp16 and 4-bit caches too; 16-bit ones are exact
+    in the scores, their softmax weights keep 16 bits (bf16, and 4-bit pages)
+    or 22 (fp16), sums are fp32, and the result is rounded once. Up to 256 tokens and 4096
     sequences, dim a multiple of 8 up to 256, page_size a power of two from
     16 to 1024. A table entry outside the pool holds no tokens.
     """
     scale = default_scale(scale, page_dim(k_pages))
-    if window is not None and window < 1:
+    if window is None:
+        window = 0
+    elif window < 1:
         raise ValueError(f"a window holds at least the token itself, got {window}")
-    window, sinks = 0 if window is None else int(window), int(sinks)
+    window, sinks = operator.index(window), operator.index(sinks)
     if _watched(q, k, v, k_pages, v_pages):
         return torch.ops.kiln.paged_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale, window, sinks)
     return run_attention(q, k, v, k_pages, v_pages, table, lengths, parents, None, scale, "tree_attention", window, sinks)
@@ -666,8 +670,8 @@ def cache_read(k_pages, v_pages, table, starts, ends, *, tokens, dtype=None):
     takes, of another cache too."""
     dtype = _read_type(k_pages, dtype)
     if _watched(k_pages, v_pages):
-        return torch.ops.kiln.cache_read(k_pages, v_pages, table, starts, ends, int(tokens), dtype)
-    return run_read(k_pages, v_pages, table, starts, ends, int(tokens), dtype)
+        return torch.ops.kiln.cache_read(k_pages, v_pages, table, starts, ends, operator.index(tokens), dtype)
+    return run_read(k_pages, v_pages, table, starts, ends, operator.index(tokens), dtype)
 
 
 def _read_type(k_pages, dtype):

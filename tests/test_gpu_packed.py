@@ -448,3 +448,21 @@ def test_as_operators_of_torch():
     kiln.cache_append(p["k"], p["v"], p["k_pages"], p["v_pages"], p["table"], p["lengths"])
     assert torch.equal(pages[0], p["k_pages"]) and torch.equal(pages[1], p["v_pages"])
     assert torch.equal(k, kiln.cache_read(*pages, p["table"], starts, p["lengths"], tokens=30)[0])
+
+
+@pytest.mark.parametrize("cache,act", [(torch.uint8, torch.bfloat16), (torch.bfloat16, torch.bfloat16)], ids=["fp4", "bf16"])
+def test_pools_past_32_bits(cache, act):
+    """The last pages of pools of more than 2^32 bytes."""
+    p = ref.problem(gen(26), cache=cache, act=act, draft=4, heads=4, kv=2, dim=128, lengths=(40, 17), device="cuda")
+    first = 2 ** 32 // p["k_pages"][0].nbytes
+    q = dict(p, table=p["table"] + first)
+    for name in ("k_pages", "v_pages"):
+        q[name] = torch.zeros((first + len(p[name]), *p[name].shape[1:]), dtype=cache, device="cuda")
+        q[name][first:] = p[name]
+    starts = torch.tensor([3, 0], dtype=torch.int32, device="cuda")
+    for more in (dict(), dict(window=20, sinks=3)):
+        assert torch.equal(kiln.tree_attention(**q, **more), kiln.tree_attention(**p, **more))
+    for x in (p, q):
+        kiln.cache_append(x["k"], x["v"], x["k_pages"], x["v_pages"], x["table"], x["lengths"])
+    a, b = (kiln.cache_read(x["k_pages"], x["v_pages"], x["table"], starts, x["lengths"] + 4, tokens=50) for x in (p, q))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

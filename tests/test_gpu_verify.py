@@ -89,6 +89,19 @@ def test_strides_and_odd_places():
     assert [t.tolist() for t in kiln.verify_tokens(**q)] == want
 
 
+@pytest.mark.parametrize("probs", [True, False], ids=["probs", "sampled"])
+def test_rows_past_32_bits(probs):
+    """A second sequence's rows more than 2^31 elements behind the first one's."""
+    p = ref.drafted(gen(7), 2, 4, 2050, torch.bfloat16, probs=probs, device="cuda")
+    want = [t.tolist() for t in kiln.verify_tokens(**p)]
+    far = 2 ** 31 + 64
+    for name in ("target", "draft"):
+        if p[name] is not None:
+            rows = torch.empty(far + 4 * 2050, dtype=torch.bfloat16, device="cuda").as_strided((2, 4, 2050), (far, 2050, 1))
+            p[name] = rows.copy_(p[name])
+    assert [t.tolist() for t in kiln.verify_tokens(**p)] == want
+
+
 def test_graph_and_streams():
     p = ref.drafted(gen(7), 4, 6, 5000, device="cuda")
     more = [ref.drafted(gen(8 + i), 4, 6, 5000, device="cuda") for i in range(4)]

@@ -157,6 +157,8 @@ def test_refusals(interpreting):
             ({}, dict(window=-1), ValueError),
             ({}, dict(sinks=4), ValueError),
             ({}, dict(window=4, sinks=-1), ValueError),
+            ({}, dict(window=2.5), TypeError),
+            ({}, dict(window=3, sinks=1.0), TypeError),
             ({}, dict(window=2 ** 31), ValueError)):
         with pytest.raises(error):
             kiln.tree_attention(**dict(p, **change), **more)
