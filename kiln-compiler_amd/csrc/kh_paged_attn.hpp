@@ -47,6 +47,10 @@
 // Tiles of 64 keys for 64-wide heads, and page numbers staged in the LDS, were
 // both slower (32.7 us there; 137 for the 32 sequences): the first tile waits
 // longer, and nothing that comes after was waiting for them.
+//
+// A window leaves tiles out and masks those on its edge row by row: 32 sequences
+// of up to 120000 bf16 tokens, a window of 4096 and 4 sinks, 102 us (536 MB, 5.3
+// TB/s) and 7 for the join, as much as caches of 4096 tokens take.
 #pragma once
 
 #include <algorithm>
@@ -1034,6 +1038,13 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 // without gain, with weights in one part: the second block's exponentials
 // between the first block's products (146 us; fp32 activations slower), eight
 // waves of 256 rows with two tiles copied ahead (150 us).
+//
+// Over 4-bit pages threads make a tile's bf16 values out of codes that were loaded
+// a tile before, where other caches copy to the LDS; q of fp16 takes two bf16 parts. 64
+// tokens of 4 sequences, 32 query heads on 4 of 128, up to 32768 tokens, fp16: 230
+// to 237 us and 13 for the join (8 more with split8, which is for caches that hold
+// infinities), 55% of the rate of a large matrix product. Without gain: one wave a SIMD
+// (292), the products' operands read a step ahead (231 to 238).
 
 // Chunk swizzle of K and V rows in the LDS, 16-byte chunks: a 128-bit read
 // meets in one LDS cycle rows {0-3, 12-15, 20-27}, distinct mod 16, so every

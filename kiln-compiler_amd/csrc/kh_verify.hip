@@ -11,7 +11,13 @@
 //
 // verify_kernel does all that with a workgroup per sequence. Where the
 // sequences alone do not fill the chip, sums_kernel does the first sum of every
-// sequence with a wave per stretch beforehand.
+// sequence with a wave per stretch beforehand: 64 chains over 128000 tokens of
+// fp32 14.6 us (the target's and the draft's row, 4.5 TB/s of the 5.2 that a copy
+// reaches) and 7.8 us for the walk, two dependent looks into the sums and one
+// stretch. One chain of 5 over 50257: 10.4 us, one workgroup reading 400 KB; 32
+// trees without the draft's probabilities, 2.3 rows a path one after the other:
+// 13 us. The sums of 64 bits cost what the loads wait for anyway; sums between
+// lanes by permutes through the LDS took 3 to 5 us more.
 #include <algorithm>
 #include <cmath>
 #include <exception>
