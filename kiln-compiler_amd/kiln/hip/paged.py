@@ -436,8 +436,7 @@ def _(k, v, k_pages, v_pages, table, lengths, rows, k_means):
 def _cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                 ends: torch.Tensor, tokens: int, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
     with torch.no_grad():
-        # (results of an operator share no memory)
-        return tuple(t.clone() for t in run_read(k_pages, v_pages, table, starts, ends, tokens, dtype))
+        return run_read(k_pages, v_pages, table, starts, ends, tokens, dtype)
 
 
 @_cache_read.register_fake
@@ -715,7 +714,7 @@ def run_read(k_pages, v_pages, table, starts, ends, tokens, dtype):
         rank = k_pages.dim()
         ks, vs = k_pages.stride(), v_pages.stride()
         if math.prod(shape) == 0:
-            return torch.empty((2, *shape), dtype=dtype, device=k_pages.device).unbind()
+            return tuple(torch.empty(shape, dtype=dtype, device=k_pages.device) for _ in range(2))
         if k_pages.shape[-4] == 0:
             raise ValueError("the cache has no pages")
         _ready(k_pages.device)
@@ -734,7 +733,8 @@ def run_read(k_pages, v_pages, table, starts, ends, tokens, dtype):
         _rows_in_place(k_pages, "k_pages")
         _rows_in_place(v_pages, "v_pages")
     device = k_pages.device
-    k, v = torch.empty((2, *found[1]), dtype=dtype, device=device).unbind()
+    k = torch.empty(found[1], dtype=dtype, device=device)
+    v = torch.empty_like(k)
     op.k, op.v, op.table, op.starts, op.ends = k.data_ptr(), v.data_ptr(), table.data_ptr(), starts.data_ptr(), ends.data_ptr()
     lib = kl.load()
     if device.type != "cuda":
