@@ -171,19 +171,20 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     }
 
     // -- where tiles lie: lane 4 i + h keeps part h of this wave's i-th tile from `batch` on
+    const int last = min(t1, cached);   // cached tiles end here
     int batch = t0 + wave;
     int spot_keys = 0;                  // its keys
-    uint64_t spot_k = 0, spot_v = 0;    // its page (a new token's part: nothing)
+    uint64_t spot_k = 0, spot_v = 0;    // its page (none: the first)
     uint64_t some = 0, full = 0;        // parts with keys, with 16 of them
     auto stage = [&] {
       const_work &w = fresh();
       const int t = batch + WAVES * (lane >> 2), h = lane & 3;
       spot_keys = 0;
       int page = 0;
-      if (t < cached) {
+      if (t < last) {
         const int real = t < span.head ? t : t + span.skip, j = 4 * real + h;
         int col = j >> half_shift, pos = 16 * j;
-        bool in = t < t1;
+        bool in = true;
         if (sel) {
           const int rank = col;
           in = in && rank < w.p.top;
@@ -198,8 +199,6 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
         in = in && page >= 0 && page < w.p.pages;
         spot_keys = in ? min(len - pos, 16) : 0;
         page = in ? page : 0;
-      } else if (t < t1) {
-        spot_keys = min(max(w.p.draft - (kMxTile * (t - cached) + 16 * h), 0), 16);
       }
       spot_k = (uint64_t)(page * w.p.kp_p);
       spot_v = (uint64_t)(page * w.p.vp_p);
@@ -208,9 +207,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     };
     struct Spot {
       int i;       // of the batch
-      int t;       // the tile, t1 and more: none
-      int draft;   // index among the new tokens' tiles, -1 for a cached one
-      int real;    // a cached tile's place in the sequence
+      int t;       // the tile, `last` and more: none
+      int real;    // its place in the sequence (a new one's: among the new ones)
       uint32_t keys;   // of its parts, a byte each: 0x10101010 where it has all 64
       uint32_t edge;   // not every row sees the same of its keys
     };
@@ -222,9 +220,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
         if (left) {
           r.i = from + (__builtin_ctzll(left) >> 2);
           r.t = batch + WAVES * r.i;
-          r.draft = r.t >= cached ? r.t - cached : -1;
           r.real = r.t < span.head ? r.t : r.t + span.skip;
-          r.edge = WIN && r.draft < 0 && on_edge<WIN>(fresh(), len, kMxTile * r.real, kMxTile);
+          r.edge = WIN && on_edge<WIN>(fresh(), len, kMxTile * r.real, kMxTile);
           r.keys = 0x10101010u;
           if ((full >> (4 * r.i) & 15) != 15) {
             r.keys = 0;
@@ -234,8 +231,9 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           return;
         }
         batch += 16 * WAVES;
-        if (batch >= t1) {
-          r.t = t1;
+        if (batch >= last) {
+          r.t = last;
+          r.i = r.real = 0;   // (a page of the pool's all the same)
           return;
         }
         stage();
@@ -245,32 +243,18 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     auto lane_of = [&](uint64_t x, int from) {
       return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, from));
     };
-    // first token of part h in its page
-    auto slot_of = [&](const Spot &r, int h) {
-      if (r.draft >= 0) return keys_of(r, h) ? kMxTile * r.draft + 16 * h : 0;
-      return ((4 * r.real + h) & ((1 << half_shift) - 1)) * 16;
-    };
     // (a page holds whole parts: rows behind the last key are read too, and masked)
     auto load_k = [&](const Spot &r, Regs &x) {
       int64_t page = 0;
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        const int slot = slot_of(r, h);
-        if (r.draft >= 0) {
-          const uint8_t *from = new_lds + slot * (dim / 2), *e = new_lds + new_page * (dim / 2) + slot * (dim / kMxBlock);
+        const int slot = ((4 * r.real + h) & ((1 << half_shift) - 1)) * 16;   // first token of the part in its page
+        if (h == 0 || half_shift < 2) page = lane_of(spot_k, 4 * r.i + h);    // (pages of 64 tokens hold the tile)
+        const uint8_t *from = kp + (page + slot * (dim / 2)), *e = kp + (page + page_size * (dim / 2) + slot * (dim / kMxBlock));
 #pragma unroll
-          for (int i = 0; i < PB; ++i) {
-            load_words(from + k_at[i], x.k[h][i]);
-            x.ke[h][i] = e[ke_at[i]];
-          }
-        } else {
-          if (h == 0 || half_shift < 2) page = lane_of(spot_k, 4 * r.i + h);   // (pages of 64 tokens hold the tile)
-          const uint8_t *from = kp + (page + slot * (dim / 2)), *e = kp + (page + page_size * (dim / 2) + slot * (dim / kMxBlock));
-#pragma unroll
-          for (int i = 0; i < PB; ++i) {
-            load_words(from + k_at[i], x.k[h][i]);
-            x.ke[h][i] = e[ke_at[i]];
-          }
+        for (int i = 0; i < PB; ++i) {
+          load_words(from + k_at[i], x.k[h][i]);
+          x.ke[h][i] = e[ke_at[i]];
         }
       }
     };
@@ -278,35 +262,43 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       int64_t page = 0;
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        const int slot = slot_of(r, h);
-        if (r.draft >= 0) {
-          const uint8_t *base = new_lds + mx_page_bytes(new_page, dim);
-          const uint8_t *from = base + slot * (dim / 2), *e = base + new_page * (dim / 2) + slot * (dim / kMxBlock);
+        const int slot = ((4 * r.real + h) & ((1 << half_shift) - 1)) * 16;
+        if (h == 0 || half_shift < 2) page = lane_of(spot_v, 4 * r.i + h);
+        const uint8_t *from = vp + (page + slot * (dim / 2)), *e = vp + (page + page_size * (dim / 2) + slot * (dim / kMxBlock));
 #pragma unroll
-          for (int vc = 0; vc < VC; ++vc) {
-            load_words(from + v_at[vc], x.v[h][vc]);
-            x.ve[h][vc] = *reinterpret_cast<const uint32_t *>(e + ve_at[vc]);
-          }
-        } else {
-          if (h == 0 || half_shift < 2) page = lane_of(spot_v, 4 * r.i + h);
-          const uint8_t *from = vp + (page + slot * (dim / 2)), *e = vp + (page + page_size * (dim / 2) + slot * (dim / kMxBlock));
+        for (int vc = 0; vc < VC; ++vc) {
+          load_words(from + v_at[vc], x.v[h][vc]);
+          x.ve[h][vc] = *reinterpret_cast<const uint32_t *>(e + ve_at[vc]);
+        }
+      }
+    };
+    // a tile of new tokens, from the LDS (parts behind the last hold the first's)
+    auto load_new = [&](const Spot &r, Regs &x) {
+      const uint8_t *values = new_lds + mx_page_bytes(new_page, dim);
 #pragma unroll
-          for (int vc = 0; vc < VC; ++vc) {
-            load_words(from + v_at[vc], x.v[h][vc]);
-            x.ve[h][vc] = *reinterpret_cast<const uint32_t *>(e + ve_at[vc]);
-          }
+      for (int h = 0; h < 4; ++h) {
+        const int slot = keys_of(r, h) ? kMxTile * r.real + 16 * h : 0, code = slot * (dim / 2), scale = new_page * (dim / 2) + slot * (dim / kMxBlock);
+#pragma unroll
+        for (int i = 0; i < PB; ++i) {
+          load_words(new_lds + code + k_at[i], x.k[h][i]);
+          x.ke[h][i] = new_lds[scale + ke_at[i]];
+        }
+#pragma unroll
+        for (int vc = 0; vc < VC; ++vc) {
+          load_words(values + code + v_at[vc], x.v[h][vc]);
+          x.ve[h][vc] = *reinterpret_cast<const uint32_t *>(values + scale + ve_at[vc]);
         }
       }
     };
 
     Regs x;
     Spot here;
-    here.t = t1;
-    if (batch < t1) {
+    here.t = last;
+    if (batch < last) {
       stage();
       find(here, 0);
     }
-    if (here.t < t1 && here.draft < 0) {
+    if (here.t < last) {
       load_k(here, x);
       load_v(here, x);
     }
@@ -314,10 +306,6 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       new_of = s * wt.p.kv_heads + c;
       store_new<A>(fresh(), s, c, new_page, new_lds);
       __syncthreads();
-    }
-    if (here.t < t1 && here.draft >= 0) {
-      load_k(here, x);
-      load_v(here, x);
     }
 
     // this lane's query rows
@@ -364,7 +352,11 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
         for (int i = 0; i < VD; ++i) o[rt][vc][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    while (here.t < t1) {
+    // A tile's products. The loads of the next one's K go between the first product
+    // and the softmax, of its V behind the second: always as many, so that a wait
+    // for this tile's V leaves the next one's K in flight.
+    auto consume = [&](const Spot &here, auto is_new, auto load_next_k, auto load_next_v) {
+      constexpr bool NEW = decltype(is_new)::value;
       f32x4 sc[RT][4];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -387,13 +379,11 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
             for (int h = 0; h < 4; ++h) sc[rt][h] = C::mma(a[h], q[n][rt][ks], sc[rt][h]);
       }
-      Spot next;
-      find(next, here.i + 1);
-      if (next.t < t1) load_k(next, x);
+      load_next_k();
 
       uint32_t odd = 0;        // bit 16 vc + 4 h + i: this lane's V of that key is NaN, and set aside
       uint32_t see[RT][2];
-      const bool masked = here.draft >= 0 || (WIN && here.edge);   // rows see different keys
+      const bool masked = NEW || (WIN && here.edge);   // rows see different keys
       const bool partly = masked || here.keys != 0x10101010u;
       if (partly) {
 #pragma unroll
@@ -402,8 +392,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
             see[rt][kb] = there;
-            if (here.draft >= 0) {
-              const int word = 2 * here.draft + kb, i = row_token[rt] - 32 * word;   // chain: the tokens up to its own
+            if constexpr (NEW) {
+              const int word = 2 * here.real + kb, i = row_token[rt] - 32 * word;   // chain: the tokens up to its own
               see[rt][kb] &= tree ? (word < kMaxDraft / 32 ? paths.bits[row_token[rt]][word] : 0u) : (i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1);
               if (WIN && !tree) {   // (a tree's bits know the window)
                 const_work &w = fresh();
@@ -498,7 +488,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) o[rt][vc][i0 + i] = C::mma(a[i], parts[rt][kb][n], o[rt][vc][i0 + i]);
           }
-      if (next.t < t1) load_v(next, x);
+      load_next_v();
 
       if (__builtin_expect(__any(odd != 0), 0)) {   // the blocks set aside, by hand
         for (int key = 0; key < kMxTile; ++key) {
@@ -518,7 +508,25 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
           }
         }
       }
+    };
+    while (here.t < last) {
+      Spot next;
+      consume(here, std::false_type(), [&] {
+        find(next, here.i + 1);
+        load_k(next, x);
+      }, [&] { load_v(next, x); });
       here = next;
+    }
+    if (has_draft) {   // new tokens' tiles of this wave
+      for (int t = max(cached, t0) + ((wave - (max(cached, t0) - t0)) & (WAVES - 1)); t < t1; t += WAVES) {
+        const_work &w = fresh();
+        here.real = t - cached;
+        here.keys = 0;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) here.keys |= (uint32_t)min(max(w.p.draft - (kMxTile * here.real + 16 * h), 0), 16) << (8 * h);
+        load_new(here, x);
+        consume(here, std::true_type(), [] {}, [] {});
+      }
     }
 
     // -- the waves' parts joined, in a fixed order
