@@ -52,26 +52,48 @@ struct MxTile {
   uint32_t v[4][VC][4], ve[4][VC];
 };
 
+// 8 adjacent activations as they lie in memory: asked for early, made floats later.
+struct Raw8 {
+  u32x4 w[2];
+};
+__device__ __forceinline__ void load_raw8(const void *p, int64_t i, bool fp32, Raw8 &r) {
+  if (fp32) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) r.w[j] = *reinterpret_cast<const u32x4 *>(static_cast<const float *>(p) + i + 4 * j);
+  } else {
+    r.w[0] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + i);
+  }
+}
+template <class A>
+__device__ __forceinline__ void raw_values(const Raw8 &r, bool fp32, float (&x)[8]) {
+  typedef A vec __attribute__((ext_vector_type(8)));
+  const vec a = __builtin_bit_cast(vec, r.w[0]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = fp32 ? __uint_as_float(r.w[j >> 2][j & 3]) : (float)a[j];
+}
+
 // The new tokens of (s, c) into two 4-bit pages in the LDS, rounded as
-// kh_cache_append does: a thread takes 8 dimensions of a token, the 4 lanes of a
-// block agree on its largest.
-template <class A, class W>
-__device__ __forceinline__ void store_new(W &w, int s, int c, int page, uint8_t *keys) {
-  const int dim = w.p.dim, chunks = dim / 8;
-  const bool act32 = w.p.act_type == KH_TYPE_F32;
+// kh_cache_append does: a thread takes 8 dimensions of a token (its i-th, of
+// draft dim / 8), the 4 lanes of a block agree on its largest.
+template <class W>
+__device__ __forceinline__ void load_new(W &w, int s, int c, int i, bool act32, Raw8 &k, Raw8 &v) {
+  const int chunks = w.p.dim / 8, t = i / chunks, d = (i - t * chunks) * 8;
+  load_raw8(w.p.k, s * w.p.k_s + c * w.p.k_h + t * w.p.k_n + d, act32, k);
+  load_raw8(w.p.v, s * w.p.v_s + c * w.p.v_h + t * w.p.v_n + d, act32, v);
+}
+template <class A>
+__device__ __forceinline__ void store_new(int dim, int i, int page, uint8_t *keys, bool act32, const Raw8 &k, const Raw8 &v) {
+  const int chunks = dim / 8, t = i / chunks, d = (i - t * chunks) * 8;
   uint8_t *values = keys + mx_page_bytes(page, dim);
-  for (int i = threadIdx.x; i < w.p.draft * chunks; i += blockDim.x) {   // (whole groups of 4 lanes)
-    const int t = i / chunks, d = (i - t * chunks) * 8;
-    float x[8], y[8];
-    load_acts<A>(w.p.k, s * w.p.k_s + c * w.p.k_h + t * w.p.k_n + d, act32, x);
-    load_acts<A>(w.p.v, s * w.p.v_s + c * w.p.v_h + t * w.p.v_n + d, act32, y);
-    const uint32_t ke = mx_scale_of(quad_max(mx_most(x))), ve = mx_scale_of(quad_max(mx_most(y)));
-    *reinterpret_cast<uint32_t *>(keys + mx_key_code(t, d, dim)) = mx_pack(x, ke);
-    *reinterpret_cast<uint32_t *>(values + mx_value_code(t, d, dim)) = mx_pack(y, ve);
-    if (!(d & 31)) {
-      keys[mx_key_scale(t, d, dim, page)] = (uint8_t)ke;
-      values[mx_value_scale(t, d, dim, page)] = (uint8_t)ve;
-    }
+  float x[8], y[8];
+  raw_values<A>(k, act32, x);
+  raw_values<A>(v, act32, y);
+  const uint32_t ke = mx_scale_of(quad_max(mx_most(x))), ve = mx_scale_of(quad_max(mx_most(y)));
+  *reinterpret_cast<uint32_t *>(keys + mx_key_code(t, d, dim)) = mx_pack(x, ke);
+  *reinterpret_cast<uint32_t *>(values + mx_value_code(t, d, dim)) = mx_pack(y, ve);
+  if (!(d & 31)) {
+    keys[mx_key_scale(t, d, dim, page)] = (uint8_t)ke;
+    values[mx_value_scale(t, d, dim, page)] = (uint8_t)ve;
   }
 }
 
@@ -141,8 +163,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     const bool sel = w.sel_tiles;
     const int token = sel ? (int)((uint32_t)b / (uint32_t)w.blocks) : 0;
     const int row0 = (sel ? b - token * w.blocks : b) * RM;
-    const bool act32 = w.p.act_type == KH_TYPE_F32;
-    const bool has_draft = t1 > cached;
+    const bool act32 = NQ == 3 || (NQ == 1 && w.p.act_type == KH_TYPE_F32);
+    const bool has_draft = WHOLE || t1 > cached;
     const bool tree = w.p.parents != nullptr;
     if ((has_draft || WIN) && tree && paths_of != s) {
       __syncthreads();   // the last item's rows have read the table
@@ -154,6 +176,31 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     const int dim = wt.p.dim, page_size = wt.p.page_size, half_shift = wt.half_shift;
     const int new_page = (wt.p.draft + 15) & ~15;
     const uint8_t *kp = static_cast<const uint8_t *>(wt.p.k_pages) + c * wt.p.kp_h, *vp = static_cast<const uint8_t *>(wt.p.v_pages) + c * wt.p.vp_h;
+
+    // this lane's query rows, and its share of the new tokens: asked for before the
+    // pages, whose loads wait for the table's
+    int row_token[RT], row_head[RT];
+    bool row_ok[RT];
+    Raw8 q_raw[RT][KS];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = row0 + rt * 16 + li;
+      row_ok[rt] = r < wt.rows;
+      const int rr = row_ok[rt] ? r : 0;
+      row_token[rt] = sel ? token : (int)((uint32_t)rr / (uint32_t)wt.group);
+      row_head[rt] = c * wt.group + (sel ? rr : rr - row_token[rt] * wt.group);
+      const int64_t base = s * wt.p.q_s + row_token[rt] * wt.p.q_n + row_head[rt] * wt.p.q_h;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d = PD * g + 8 * ks;
+        load_raw8(wt.p.q, base + (row_ok[rt] && d < dim ? d : 0), act32, q_raw[rt][ks]);
+      }
+    }
+    const bool make_new = has_draft && new_of != s * wt.p.kv_heads + c;
+    const bool mine = make_new && (int)threadIdx.x < wt.p.draft * (dim / 8);
+    Raw8 new_k, new_v;
+    if (mine) load_new(fresh(), s, c, threadIdx.x, act32, new_k, new_v);
+
     // where this lane's share of a part lies in it, and of its scales
     constexpr int PAIR = VD == 8 ? 1 : 2;   // lanes of 8 of V's dimensions
     uint32_t k_at[PB], ke_at[PB], v_at[VC], ve_at[VC];
@@ -273,7 +320,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       }
     };
     // a tile of new tokens, from the LDS (parts behind the last hold the first's)
-    auto load_new = [&](const Spot &r, Regs &x) {
+    auto load_new_tile = [&](const Spot &r, Regs &x) {
       const uint8_t *values = new_lds + mx_page_bytes(new_page, dim);
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
@@ -302,35 +349,30 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
       load_k(here, x);
       load_v(here, x);
     }
-    if (has_draft && new_of != s * wt.p.kv_heads + c) {
+    if (make_new) {
       new_of = s * wt.p.kv_heads + c;
-      store_new<A>(fresh(), s, c, new_page, new_lds);
+      if (mine) store_new<A>(dim, threadIdx.x, new_page, new_lds, act32, new_k, new_v);
+      for (int i = threadIdx.x + blockDim.x; i < wt.p.draft * (dim / 8); i += blockDim.x) {   // (whole groups of 4 lanes)
+        load_new(fresh(), s, c, i, act32, new_k, new_v);
+        store_new<A>(dim, i, new_page, new_lds, act32, new_k, new_v);
+      }
       __syncthreads();
     }
 
-    // this lane's query rows
-    const_work &wq = fresh();
-    int row_token[RT], row_head[RT];
-    bool row_ok[RT];
+    // the query rows' parts
     u32x4 q[NQ][RT][KS];
     // products to the base-2 domain; positive, so that a masked -inf stays one: q
     // takes a negative scale's sign, and a scale of zero is the smallest number
+    const_work &wq = fresh();
     const float mult = fmaxf(fabsf(wq.scale2), 0x1p-126f);
+    const float up = wq.scale2 < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = row0 + rt * 16 + li;
-      row_ok[rt] = r < wq.rows;
-      const int rr = row_ok[rt] ? r : 0;
-      row_token[rt] = sel ? token : (int)((uint32_t)rr / (uint32_t)wq.group);
-      row_head[rt] = c * wq.group + (sel ? rr : rr - row_token[rt] * wq.group);
-      const int64_t base = s * wq.p.q_s + row_token[rt] * wq.p.q_n + row_head[rt] * wq.p.q_h;
-      const float up = wq.scale2 < 0.0f ? -1.0f : 1.0f;
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int d = PD * g + 8 * ks;
-        const bool in = row_ok[rt] && d < dim;
+        const bool in = row_ok[rt] && PD * g + 8 * ks < dim;
         float y[8];
-        load_acts<A>(wq.p.q, base + (in ? d : 0), act32, y);
+        raw_values<A>(q_raw[rt][ks], act32, y);
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = in ? y[j] * up : 0.0f;
         u32x4 parts[NQ];
@@ -338,7 +380,6 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
         for (int n = 0; n < NQ; ++n) q[n][rt][ks] = parts[n];
       }
-    }
 
     f32x4 o[RT][VC][VD];
     float m[RT], l[RT];
@@ -524,7 +565,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
         here.keys = 0;
 #pragma unroll
         for (int h = 0; h < 4; ++h) here.keys |= (uint32_t)min(max(w.p.draft - (kMxTile * here.real + 16 * h), 0), 16) << (8 * h);
-        load_new(here, x);
+        load_new_tile(here, x);
         consume(here, std::true_type(), [] {}, [] {});
       }
     }
