@@ -68,8 +68,10 @@ constexpr int kPagedWaves = 4;     // waves of a workgroup
 constexpr int paged_waves(int dt, int rt, bool whole) { return whole && rt * dt <= 128 ? 8 : kPagedWaves; }
 // Tiles that an item over 4-bit pages counts for besides its own where ranges are
 // dealt out: beginning one is a few dependent loads, ending one a join and parts in
-// the workspace, together about as long as a workgroup takes for this many tiles.
-constexpr int kMxLead = 8;
+// the workspace, together about as long as a workgroup takes for this many tiles
+// (32 ragged sequences up to 8192 tokens: 50 us with 6, 42.8 with 8, 41.5 with 12; one of
+// 131072: 34.9, 34.6, 32.6).
+constexpr int kMxLead = 12;
 constexpr int kMxWideLead = 4;   // ... of 128 rows, whose tiles take longer
 constexpr int kMaxDraft = 256;     // new tokens of a sequence: a workgroup's table of paths fits the LDS
 constexpr int kMaxBatch = 4096;    // sequences of a call: each workgroup scans their lengths

@@ -17,16 +17,17 @@
 //   new tokens are rounded once an item, into pages of their own in the LDS.
 //
 // What it measured (one token, 8 kv heads of 128, 32 query heads, bf16): one
-// sequence of 131072 tokens 39 us, 3.7 TB/s of the 5.2 that a copy reaches; 32
-// ragged ones up to 8192, 45 us, 3.3 TB/s. The stream itself runs near the
-// copy's rate: what is missing is what beginning and ending an item takes, a
-// chain of dependent loads (length, page, codes) and a join, 6 to 8 us of a
-// workgroup's time that kMxLead counts. Two tiles in flight a wave (79 us ragged,
-// registers for two waves a SIMD alone) and ones of 32 keys (68) were slower; a
-// tenth of the vector instructions taken out changed nothing. Many rows under
-// fp32 activations (27 drafted tokens of 16 sequences, a window of 1021: 75 us, 17.5
-// of them products at the matrix cores' rate) are bound by one wave a SIMD: nine
-// products a pair of operands and their parts take 400 registers.
+// sequence of 131072 tokens 32.6 us, 4.4 TB/s of the 5.2 that a copy reaches; 32
+// ragged ones up to 8192, 41.5 us, 3.6 TB/s. What is missing is beginning and
+// ending an item, a chain of dependent loads (length, page, codes) and a join,
+// which kMxLead counts. Cached and new tokens' tiles are loops of their own, and
+// the cached one always asks for a next tile: while a wave could meet either, the
+// wait for this tile's V was one for the next one's K too (39 and 45 us). Two
+// tiles in flight a wave, registers for two waves a SIMD alone, and tiles of 32
+// keys were slower. Many rows under fp32 activations (27 drafted tokens of 16
+// sequences, a window of 1021: 68 us, 17.5 of them products at the matrix cores'
+// rate) are bound by one wave a SIMD: three products a pair of operands each way
+// and their parts take 400 registers.
 #pragma once
 
 #include "kh_paged_attn.hpp"
