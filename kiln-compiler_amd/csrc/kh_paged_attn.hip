@@ -22,11 +22,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWholeKeys = 1280, kWholeManyKeys = 4096, kWholeSlowKeys = 1024;
 
 // Over 4-bit pages (paged_mx4_kernel, tiles of 64 keys) the two meet elsewhere. 16
-// rows an item, eight waves, bf16, 8 heads of 128: 8 items of 2000 keys 18.4 (whole)
-// and 21.8 us (ranges), of 4000 keys 28.0 and 21.2; 128 items of 4000 keys 30.5 and
-// 31.5, of 8000 keys 53.9 and 43.3. 32 rows an item: four waves, 16 items of 1000
-// keys 23.2 and 30.1, of 2000 keys 33.8 and 30.5; 256 items of 4000 keys 57.6 and
-// 73.4, of 8000 keys 108 and 125 (heads of 64, eight waves: 71 and 102).
+// rows an item, eight waves, bf16, 8 heads of 128: 8 items of 2000 keys 17.7 (whole)
+// and 22.7 us (ranges), of 4000 keys 25.5 and 22.2; 128 items of 4000 keys 25.9 and
+// 28.6, of 8000 keys 44.2 and 39.4. 32 rows an item, four waves: 256 items of 4000
+// keys 45 and 62, of 8000 keys 92 and 103 (heads of 64, eight waves: 62 and 96). Four
+// waves and few items (heads of 256): half of what eight take.
 constexpr int kMxWholeKeys = 2560, kMxWholeSlowKeys = 1536, kMxWholeManyKeys = 4096, kMxWholeManyRowsKeys = 8192;
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
