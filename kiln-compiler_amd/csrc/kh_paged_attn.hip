@@ -26,7 +26,8 @@ constexpr int kWholeKeys = 1280, kWholeManyKeys = 4096, kWholeSlowKeys = 1024;
 // and 22.7 us (ranges), of 4000 keys 25.5 and 22.2; 128 items of 4000 keys 25.9 and
 // 28.6, of 8000 keys 44.2 and 39.4. 32 rows an item, four waves: 256 items of 4000
 // keys 45 and 62, of 8000 keys 92 and 103 (heads of 64, eight waves: 62 and 96). Four
-// waves and few items (heads of 256): half of what eight take.
+// waves and few items (heads of 256 now) as 16 items of 32 rows did: 1000 keys 23.2
+// and 30.1, 2000 keys 33.8 and 30.5.
 constexpr int kMxWholeKeys = 2560, kMxWholeSlowKeys = 1536, kMxWholeManyKeys = 4096, kMxWholeManyRowsKeys = 8192;
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
