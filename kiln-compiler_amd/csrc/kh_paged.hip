@@ -88,9 +88,10 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
   }
   const int64_t most = std::numeric_limits<int32_t>::max();
   const int64_t keys = (int64_t)p.width * p.page_size;
+  const int lead = mx ? kMxLead : 0;   // (ranges over 4-bit pages alone count an item's beginning)
   // (a length and a tile's keys are added in 32 bits)
   // (and under a window a new token's depth)
-  if (keys > most - std::max(kPagedTile, kWideTile) - (p.window ? kMaxDraft : 0) || (keys / 32 + 9 + kMxLead) * std::max(p.batch, 1) > most || (int64_t)p.top * p.page_size > most ||
+  if (keys > most - std::max(kPagedTile, kWideTile) - (p.window ? kMaxDraft : 0) || (keys / 32 + 9 + lead) * std::max(p.batch, 1) > most || (int64_t)p.top * p.page_size > most ||
       (int64_t)p.batch * p.draft * p.heads > most / 2 || p.top > (1 << 20)) {
     err = "more keys or query rows than 32-bit counts hold";
     return false;
@@ -100,7 +101,7 @@ bool check_paged(const kh_paged &p, std::string &err, bool &unsupported) {
     return false;
   }
   // (every query row of a token in a block of its own at the worst)
-  const int64_t tiles = (std::max(keys, p.top ? (int64_t)p.top * p.page_size : 0) / 32 + 10 + kMxLead) * std::max(p.batch, 1);
+  const int64_t tiles = (std::max(keys, p.top ? (int64_t)p.top * p.page_size : 0) / 32 + 10 + lead) * std::max(p.batch, 1);
   if (p.variant == KH_PAGED_ATTENTION && tiles * p.kv_heads > most / (((int64_t)p.draft * (p.heads / p.kv_heads) + 15) / 16 + p.draft)) {
     err = "more keys and query rows than 32-bit counts hold";
     return false;

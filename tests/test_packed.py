@@ -17,6 +17,7 @@ import torch
 import kiln
 import packed_reference as ref
 from kiln.frontend.fx_import import Unsupported, import_exported
+from kiln.hip import lib as kl
 from kiln.ir import interpret, parse, verify
 from models.decoder import CachedBlock
 from models.transformer import Block, gpt2_init_
@@ -180,6 +181,26 @@ def test_refusals(interpreting):
     assert kiln.cache_read(**dict(read, tokens=0))[0].shape == (2, 0, 2, 64)
     with pytest.raises(NotImplementedError):     # 48 dimensions: no block ends there
         kiln.PagedCache(1, 4, 16, 1, 48, dtype=FP4)
+
+
+@pytest.mark.parametrize("cache,act", [(0, 0), (1, 0), (1, 1), (2, 2)], ids=["fp32", "bf16-fp32", "bf16", "fp16"])
+def test_limits_of_other_caches(interpreting, cache, act):
+    # 32-bit counts of tiles: keys / 32 and 10 more a sequence, times the kv heads and their row blocks. What ranges
+    # over 4-bit pages count beside their tiles narrows 4-bit calls alone.
+    lib, size = kl.load(), kl.ctypes.c_size_t()
+
+    def of(cache, act, tokens, batch=4096, heads=32, kv_heads=8, variant=kl.PAGED_ATTENTION):
+        op = kl.Paged(variant, batch, 1, heads, kv_heads, 128, 64, 1000, tokens // 64, 0, cache, act, 0, 1.0)
+        return lib.kh_paged_workspace_bytes(op, size)
+
+    # (keys / 32 + 10) * 4096 * 8 <= (2^31 - 1) / 2: up to 32757 tiles
+    assert of(cache, act, 32757 // 2 * 64) == kl.OK
+    assert of(cache, act, 32757 // 2 * 64 + 64) == kl.ERR_UNSUPPORTED
+    assert of(kl.TYPE_MX4, act, 32757 // 2 * 64) == kl.ERR_UNSUPPORTED
+    assert of(kl.TYPE_MX4, act, (32757 - 12) // 2 * 64) == kl.OK
+    # (keys / 32 + 9) * batch <= 2^31 - 1
+    for tokens, want in ((524278 * 32, kl.OK), (524280 * 32, kl.ERR_UNSUPPORTED)):
+        assert of(kl.TYPE_F32, act, tokens, batch=4096, heads=1, kv_heads=1, variant=kl.PAGED_SELECT) == want
 
 
 def test_no_cpu_path():
