@@ -1763,6 +1763,8 @@ class _Lowerer:
                 raise NotImplementedError(f"HIP backend: value {v} has no storage")
             if lay.strides[-1] != 1 and lay.shape[-1] > 1:
                 raise NotImplementedError(f"HIP backend: the last dimension of operand {j} of {n.op} is not contiguous")
+            if v.type.dtype == "u8" and lay.strides[-2] != lay.shape[-1]:   # (its bytes are no rows of tokens)
+                raise NotImplementedError(f"HIP backend: the 4-bit pages of a head, operand {j} of {n.op}, are not contiguous")
             r = d.refs[j]
             r.base, r.index = self.slot_of(lay.base)
             r.offset = self.element_offset(v)

@@ -377,6 +377,47 @@ def test_graph_text_and_meaning(window, sinks):
     np.testing.assert_allclose(out[0], want[0].numpy(), rtol=1e-4, atol=1e-5)
 
 
+class Views(torch.nn.Module):
+    """Attention over what a view makes of the pages."""
+
+    def __init__(self, view):
+        super().__init__()
+        self.view = view
+
+    def forward(self, q, k, v, k_pages, v_pages, table, lengths):
+        return kiln.tree_attention(q, k, v, self.view(k_pages), self.view(v_pages), table, lengths)
+
+
+def view_operands(dim, make):
+    p = ref.problem(gen(21), dim=64, lengths=(40, 17))
+    q, k, v = (p[name][..., :dim].contiguous() for name in ("q", "k", "v"))
+    return q, k, v, make(p["k_pages"]), make(p["v_pages"]), p["table"], p["lengths"]
+
+
+@pytest.mark.parametrize("view,make", [
+    (lambda x: x[1], lambda x: torch.stack([x.flip(0), x])),              # a layer
+    (lambda x: x[1:], lambda x: torch.cat([x[:1], x])),                   # pages
+    (lambda x: x[:, 1:3], lambda x: torch.cat([x, x], 1)),                # heads
+    (lambda x: x[:, :, :16], lambda x: torch.cat([x, x], 2)),             # whole tokens, in a block all the same
+    (lambda x: x.view(-1, 2, 16, 34), lambda x: x.reshape(-1))])
+def test_views_of_pages_in_a_model(interpreting, view, make):
+    args = view_operands(64, make)
+    got = kiln.compile(Views(view), args, device="cuda")(*args)
+    want = ref.attention(*args[:3], *(view(t).contiguous() for t in args[3:5]), *args[5:])
+    torch.testing.assert_close(got.double(), want, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("view,make,dim", [
+    (lambda x: x[..., :17], lambda x: x, 32),                             # the first half of each token's bytes
+    (lambda x: x[:, :, ::2], lambda x: x.repeat_interleave(2, 2), 64),    # every other token's
+    (lambda x: x.transpose(1, 2), lambda x: x.transpose(1, 2).contiguous(), 64)])
+def test_views_that_part_a_heads_bytes(interpreting, view, make, dim):
+    # 4-bit pages of a head are one block of bytes: no view of it is another page
+    args = view_operands(dim, make)
+    with pytest.raises(NotImplementedError, match="4-bit pages of a head"):
+        kiln.compile(Views(view), args, device="cuda")
+
+
 def test_models_that_are_refused():
     args = block_operands()
 
