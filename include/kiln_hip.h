@@ -513,7 +513,8 @@ int kh_cache_read_host(const kh_cache_read_op *op);
  * the whole (r = target's row where R is 0). Without `drafted`, x is drawn so
  * from target's row with u[current]; a child that is x is kept and is the
  * current token, else next = x. All in 64 bits; a probability that is not above
- * 0 counts as 0, and next is -1 where a row has no weight or an infinite one.
+ * 0 counts as 0 (but a NaN of `drafted` takes all of its token's weight, and the
+ * token is refused), and next is -1 where a row has no weight or an infinite one.
  * rows [batch][draft]: the kept tokens, then -1; counts [batch]: their number.
  * The workspace as kh_paged_run's.
  */

@@ -88,10 +88,9 @@ __device__ __forceinline__ void load_probs(const void *row, int x, int end, floa
   }
 }
 
-// What is left of weight v after the refusals took their part of q: 0 where that
-// is not above it (or is no number).
+// What is left of weight v after the refusals took their part of q (not below 0): 0
+// where that is not above it (or is no number).
 __device__ __forceinline__ double left_of(double v, double q, const double *took, int refusals) {
-  if (!(v > 0.0)) v = 0.0;
   for (int j = 0; j < refusals; ++j) {
     const double r = v - took[j] * q;
     v = r > 0.0 ? r : 0.0;
@@ -99,14 +98,23 @@ __device__ __forceinline__ double left_of(double v, double q, const double *took
   return v;
 }
 
+// Probabilities as they count: of the target 0 where they are not above it (or no
+// number), of the draft 0 where they are below it; a NaN of the draft's stays, for
+// which its token is refused and nothing of it is left.
+__host__ __device__ inline float target_counted(float x) { return x > 0.0f ? x : 0.0f; }
+__host__ __device__ inline float draft_counted(float x) { return x < 0.0f ? 0.0f : x; }
+
 // The weights that are left of probabilities p: a refusal at a time for all, so that
 // what it took is read once.
 template <int STEPS, int N>
-__device__ __forceinline__ void weigh(const float (&p)[STEPS][N], const float (&q)[STEPS][N], const double *took, int refusals, double (&v)[STEPS][N]) {
+__device__ __forceinline__ void weigh(const float (&p)[STEPS][N], float (&q)[STEPS][N], const double *took, int refusals, double (&v)[STEPS][N]) {
 #pragma unroll
   for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[i][e] = p[i][e] > 0.0f ? (double)p[i][e] : 0.0;
+    for (int e = 0; e < N; ++e) {
+      v[i][e] = target_counted(p[i][e]);
+      if (refusals) q[i][e] = draft_counted(q[i][e]);
+    }
   for (int j = 0; j < refusals; ++j) {
     const double r = took[j];
 #pragma unroll
@@ -277,8 +285,8 @@ __device__ __forceinline__ void load_walk(const VerifyWork &w, int s, Walk &t) {
     t.token[i] = in ? (int)token : -1;
     t.parent[i] = up;
     if (Q && i > 0 && up >= 0) {
-      t.p[i] = (double)(float)static_cast<const T *>(w.p.target)[s * w.p.target_s + up * w.p.target_n + token];
-      t.q[i] = (double)(float)static_cast<const T *>(w.p.drafted)[s * w.p.drafted_s + up * w.p.drafted_n + token];
+      t.p[i] = target_counted((float)static_cast<const T *>(w.p.target)[s * w.p.target_s + up * w.p.target_n + token]);
+      t.q[i] = draft_counted((float)static_cast<const T *>(w.p.drafted)[s * w.p.drafted_s + up * w.p.drafted_n + token]);
     }
   }
   __syncthreads();
@@ -313,7 +321,7 @@ __device__ __forceinline__ void descend(const VerifyWork &w, Walk &t, Place &r) 
   for (;;) {
     r.at = next_child(w, t, r.at, r.now, -1);
     if (r.at >= w.p.draft) return;
-    if (!all_know(t.u[r.at] * t.q[r.at] < (t.p[r.at] > 0.0 ? t.p[r.at] : 0.0))) return;
+    if (!all_know(t.u[r.at] * t.q[r.at] < t.p[r.at])) return;
     r.now = r.at;
     t.path[r.count++] = r.now;   // (every thread the same)
   }
@@ -468,10 +476,10 @@ size_t workspace_bytes(const kh_verify_op &p) { return ahead(p) ? (size_t)p.batc
 
 // -- the meaning on the CPU ----------------------------------------------------------
 
-double prob(const void *p, int64_t i, int type) {
+float prob(const void *p, int64_t i, int type) {
   if (type == KH_TYPE_F32) return static_cast<const float *>(p)[i];
-  if (type == KH_TYPE_BF16) return (double)(float)static_cast<const __bf16 *>(p)[i];
-  return (double)(float)static_cast<const _Float16 *>(p)[i];
+  if (type == KH_TYPE_BF16) return (float)static_cast<const __bf16 *>(p)[i];
+  return (float)static_cast<const _Float16 *>(p)[i];
 }
 
 void host_verify(const kh_verify_op &p) {
@@ -490,8 +498,7 @@ void host_verify(const kh_verify_op &p) {
     auto fresh = [&] {
       double whole = 0.0;
       for (int x = 0; x < p.vocab; ++x) {
-        const double v = prob(p.target, s * p.target_s + now * p.target_n + x, p.type);
-        left[(size_t)x] = v > 0.0 ? v : 0.0;
+        left[(size_t)x] = target_counted(prob(p.target, s * p.target_s + now * p.target_n + x, p.type));
         whole += left[(size_t)x];
       }
       return whole;
@@ -522,10 +529,10 @@ void host_verify(const kh_verify_op &p) {
           if (c != token) continue;
         } else {
           const int64_t row = s * p.drafted_s + now * p.drafted_n;
-          if (!(uniform(i) * whole * prob(p.drafted, row + c, p.type) < left[(size_t)c])) {
+          if (!(uniform(i) * whole * draft_counted(prob(p.drafted, row + c, p.type)) < left[(size_t)c])) {
             double rest = 0.0;
             for (int x = 0; x < p.vocab; ++x) {
-              const double v = left[(size_t)x] - whole * prob(p.drafted, row + x, p.type);
+              const double v = left[(size_t)x] - whole * draft_counted(prob(p.drafted, row + x, p.type));
               left[(size_t)x] = v > 0.0 ? v : 0.0;
               rest += left[(size_t)x];
             }

@@ -154,8 +154,10 @@ def verify_tokens(tokens, target, uniforms, parents=None, *, draft=None):
     then -1: what ``cache_append`` takes), ``counts`` and the token after,
     ``[sequences]``. Sums are 64-bit. Probabilities that are not above 0 count
     as 0 and need not sum to 1; a row without any, or with an infinite one,
-    gives -1 as the token after. A token outside the vocabulary is not kept. Up
-    to 256 tokens, 65535 sequences and a vocabulary of 2^24."""
+    gives -1 as the token after. (A NaN of the draft's does not count as 0: its
+    token is refused, and a refusal leaves nothing of it.) A token outside the
+    vocabulary is not kept. Up to 256 tokens, 65535 sequences and a vocabulary
+    of 2^24."""
     if paged._watched(target, uniforms, draft):
         return torch.ops.kiln.verify_tokens(tokens, target, uniforms, parents, draft)
     return run_verify(tokens, target, uniforms, parents, draft)

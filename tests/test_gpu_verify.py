@@ -9,6 +9,7 @@ import torch
 
 import kiln
 import packed_reference as ref
+import test_verify
 
 pytestmark = pytest.mark.gpu
 
@@ -75,6 +76,16 @@ def test_odd_probabilities():
             p["draft"][6] = p["target"][6]
             p["uniforms"][6] = 1.0
         check(p)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [40, 3000])
+def test_draft_probabilities_that_count_as_nothing(dtype, vocab):
+    for seed in range(3):
+        p = ref.drafted(gen(seed), 6, 9, vocab, dtype, noise=2.0, device="cuda")
+        odd, want = test_verify.odd_drafts(p)
+        check(want)
+        assert [t.tolist() for t in kiln.verify_tokens(**odd)] == [t.tolist() for t in kiln.verify_tokens(**want)]
 
 
 def test_strides_and_odd_places():

@@ -68,6 +68,28 @@ def test_odd_probabilities(interpreting):
         check(p)
 
 
+def odd_drafts(p):
+    """The operands with probabilities of the draft that are negative, and with 0 in their places."""
+    draft = p["draft"].clone()
+    draft[:, :, ::3] *= -1.0
+    draft[0, 0, int(p["tokens"][0, 1])] = -0.5          # asked first, where the target has nothing
+    target = p["target"].clone()
+    target[0, 0, int(p["tokens"][0, 1])] = 0.0
+    p = dict(p, target=target)
+    return dict(p, draft=draft), dict(p, draft=torch.where(draft < 0, 0.0, draft))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_draft_probabilities_that_count_as_nothing(interpreting, dtype):
+    for seed in range(5):
+        p = ref.drafted(gen(seed), 6, 9, 40, dtype, noise=2.0)
+        p["uniforms"][0, 1] = 0.9
+        odd, want = odd_drafts(p)
+        rows, counts, _ = check(want)
+        assert [t.tolist() for t in kiln.verify_tokens(**odd)] == [t.tolist() for t in kiln.verify_tokens(**want)]
+        assert 1 not in rows[0].tolist() or int(p["parents"][0, 1]) != 0
+
+
 @pytest.mark.parametrize("probs", [True, False], ids=["probs", "sampled"])
 def test_distribution(interpreting, probs):
     # the token behind the root, kept or drawn, is distributed as the target's row: 40000 trials of a root with three
