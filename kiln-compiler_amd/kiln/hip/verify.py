@@ -81,17 +81,14 @@ def run_verify(tokens, target, uniforms, parents, draft):
             op.parents_s = parents.stride(0)
         size = ctypes.c_size_t()
         kl.check(kl.load().kh_verify_workspace_bytes(ctypes.byref(op), ctypes.byref(size)), "verify_tokens")
-        # one allocation holds the results and behind them, 16 bytes apart, the workspace
-        words = -(-batch * (n + 2) // 4) * 4
-        found = paged._keep(key, (bytes(op), size.value, words, (batch * n, batch, batch, words - batch * (n + 2) + size.value // 4)))
+        found = paged._keep(key, (bytes(op), size.value))
     elif tokens.device.type != "cuda" and not paged.interpreting():
         paged._one_device(tokens)
     op = kl.Verify.from_buffer_copy(found[0])
     device = tokens.device
     batch, n = op.batch, op.draft
-    out = tokens.new_empty(found[2] + found[1] // 4, dtype=torch.int32)
-    rows, counts, after, _ = out.split_with_sizes(found[3])
-    rows = rows.view(batch, n)
+    # (memory of their own: one that is kept or saved keeps no other, nor the workspace)
+    rows, counts, after = (tokens.new_empty(shape, dtype=torch.int32) for shape in ((batch, n), (batch,), (batch,)))
     if batch == 0:
         return rows, counts, after
     op.tokens, op.target, op.uniforms = tokens.data_ptr(), target.data_ptr(), uniforms.data_ptr()
@@ -99,13 +96,13 @@ def run_verify(tokens, target, uniforms, parents, draft):
         op.drafted = draft.data_ptr()
     if parents is not None:
         op.parents = parents.data_ptr()
-    op.rows = out.data_ptr()
-    op.counts, op.next = op.rows + 4 * batch * n, op.rows + 4 * batch * (n + 1)
+    op.rows, op.counts, op.next = rows.data_ptr(), counts.data_ptr(), after.data_ptr()
     lib = kl.load()
     if device.type != "cuda":
         rc = lib.kh_verify_host(ctypes.byref(op))
     else:
-        rc = paged._on_device(device, lib.kh_verify_run, ctypes.byref(op), op.rows + 4 * found[2] if found[1] else None, found[1])
+        workspace = torch.empty(found[1], dtype=torch.uint8, device=device) if found[1] else None
+        rc = paged._on_device(device, lib.kh_verify_run, ctypes.byref(op), workspace.data_ptr() if found[1] else None, found[1])
     if rc:
         kl.check(rc, "verify_tokens")
     return rows, counts, after
@@ -115,8 +112,7 @@ def run_verify(tokens, target, uniforms, parents, draft):
 def _verify_tokens(tokens: torch.Tensor, target: torch.Tensor, uniforms: torch.Tensor, parents: torch.Tensor | None,
                    draft: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     with torch.no_grad():
-        # (results of an operator share no memory)
-        return tuple(t.clone() for t in run_verify(tokens, target, uniforms, parents, draft))
+        return run_verify(tokens, target, uniforms, parents, draft)
 
 
 @_verify_tokens.register_fake

@@ -117,6 +117,13 @@ def test_strides(interpreting):
     assert [t.tolist() for t in kiln.verify_tokens(**dict(p, target=same))] == list(ref.verify(**dict(p, target=same)))
 
 
+def test_results_of_their_own(interpreting):
+    # a result that is kept or saved keeps no other, and no workspace
+    results = kiln.verify_tokens(**ref.drafted(gen(8), 3, 5, 17))
+    assert [t.untyped_storage().nbytes() for t in results] == [4 * 15, 4 * 3, 4 * 3]
+    assert all(t._base is None and t.is_contiguous() and t.storage_offset() == 0 for t in results)
+
+
 def test_refusals(interpreting):
     p = ref.drafted(gen(), 2, 3, 7)
     for change, error in (
