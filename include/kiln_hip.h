@@ -508,7 +508,8 @@ int kh_cache_read_host(const kh_cache_read_op *op);
  * uniforms[s][i] a number in [0, 1). With `drafted` the children c of the
  * current token are asked in order: with r = target's row and R = 1 at first, c
  * is kept where u[c] R q(c) < r(c), q = drafted's row; where not, r becomes
- * max(r - R q, 0) and R its sum. A kept child is the current token from then on.
+ * max(r - R q, 0) and R its sum (so both rows are taken to sum to 1; only without
+ * `drafted` need they not). A kept child is the current token from then on.
  * When none is left, next is the first x whose running sum of r passes u[0] of
  * the whole (r = target's row where R is 0). Without `drafted`, x is drawn so
  * from target's row with u[current]; a child that is x is kept and is the

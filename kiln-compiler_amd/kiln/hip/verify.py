@@ -148,12 +148,15 @@ def verify_tokens(tokens, target, uniforms, parents=None, *, draft=None):
 
     Returns int32 ``rows`` ``[sequences, tokens]`` (the kept tokens, root first,
     then -1: what ``cache_append`` takes), ``counts`` and the token after,
-    ``[sequences]``. Sums are 64-bit. Probabilities that are not above 0 count
-    as 0 and need not sum to 1; a row without any, or with an infinite one,
-    gives -1 as the token after. (A NaN of the draft's does not count as 0: its
-    token is refused, and a refusal leaves nothing of it.) A token outside the
-    vocabulary is not kept. Up to 256 tokens, 65535 sequences and a vocabulary
-    of 2^24."""
+    ``[sequences]``. Sums are 64-bit. With ``draft`` the rows of both are taken
+    to sum to 1, as the first comparison under a token weighs the two as they
+    are: tokens come out as the target's as nearly as the rows do (16-bit rows of
+    a large vocabulary only nearly). Without it, rows need not sum to 1.
+    Probabilities that are not above 0 count as 0; a target row without any, or
+    with an infinite one, gives -1 as the token after. (A NaN of the draft's does
+    not count as 0: its token is refused, and a refusal leaves nothing of it.) A
+    token outside the vocabulary is not kept. Up to 256 tokens, 65535 sequences
+    and a vocabulary of 2^24."""
     if paged._watched(target, uniforms, draft):
         return torch.ops.kiln.verify_tokens(tokens, target, uniforms, parents, draft)
     return run_verify(tokens, target, uniforms, parents, draft)

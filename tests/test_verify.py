@@ -106,6 +106,19 @@ def test_distribution(interpreting, probs):
     assert bool(((seen - trials * target).abs() <= 6 * (trials * target * (1 - target)).sqrt()).all()), seen
 
 
+def test_rows_that_do_not_sum_to_one(interpreting):
+    # a target of (0.6, 1.4): without the draft, token 0 for random numbers below 0.3; with it (0.5, 0.5) the two are
+    # compared as they are, so both tokens are kept
+    n = 100
+    target, draft = torch.tensor([0.6, 1.4]).expand(n, 2, 2), torch.tensor([0.5, 0.5]).expand(n, 2, 2)
+    u = ((torch.arange(n) + 0.5) / n).double()[:, None].expand(n, 2)
+    tokens = torch.tensor([[0, 0]]).expand(n, 2)
+    _, counts, after = kiln.verify_tokens(tokens, target, u)
+    assert counts.tolist() == [2] * 30 + [1] * 70 and after.tolist() == [0] * 30 + [1] * 70
+    for token in (0, 1):
+        assert kiln.verify_tokens(tokens + token, target, u, draft=draft)[1].tolist() == [2] * n
+
+
 def test_strides(interpreting):
     p = ref.drafted(gen(6), 3, 5, 17)
     want = [t.tolist() for t in kiln.verify_tokens(**p)]
