@@ -455,8 +455,10 @@ int kh_paged_host(const kh_paged *op);
  * token, its elements a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6 (codes 0-7,
  * 8 more with the sign) times 2^(e - 127), e its scale byte: the smallest from
  * 2 to 252 for which the largest |x| is below 7 times it (or 252), 255 (NaN)
- * where an x is not finite; 253 and 254 are not scales. Elements go to the
- * nearest, ties to the even code. A page of a head is page_size * 17 dim / 32
+ * where an x is not finite. 253 and 254 are not scales: what kh_cache_read and
+ * attention give for a block under one is not defined (NaN, infinities or
+ * numbers, by the kernel that reads it), in the rows that see its token alone.
+ * Elements go to the nearest, ties to the even code. A page of a head is page_size * 17 dim / 32
  * bytes, kp_p, kp_h (and vp_p, vp_h) count bytes and kp_t, vp_t nothing: first
  * the codes, element (t, d) the low half (d even) or high half of byte
  *   keys    t dim/2 + d/2

@@ -90,8 +90,10 @@ typedef float mx_f32x2 __attribute__((ext_vector_type(2)));
 // The power of two of a scale byte, or NaN.
 __device__ __forceinline__ float mx_scale(uint32_t e) { return __uint_as_float(e > kMxMost ? 0x7fc00000u : e << 23); }
 
-// ... left to the conversions, which take an exponent of 255 for NaN (253 and 254,
-// which no writer makes, for 2^126 and 2^127)
+// ... left to the conversions, which take an exponent of 255 for NaN. (253 and 254,
+// which no writer makes and whose blocks are not defined, they take for 2^126 and
+// 2^127: telling them apart would cost paged_mx4_kernel 1.2% of its time, 43.6
+// to 44.1 us for 32 ragged sequences.)
 __device__ __forceinline__ float mx_scale_raw(uint32_t e) { return __uint_as_float(e << 23); }
 
 // Codes 2 i and 2 i + 1 of a word as a pair of bf16, exact.

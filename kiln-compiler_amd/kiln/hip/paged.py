@@ -19,7 +19,7 @@ element is a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6 times it (17 / 64 of the
 bytes of bf16). The last two dimensions are one block of bytes, whose order is
 the kernels' own (include/kiln_hip.h, kh_cache_append): ``cache_append`` writes
 it, ``cache_read`` gives the values. A block with a value that is not finite is
-NaN.
+NaN (scale byte 255; pages made elsewhere must not hold 253 and 254).
 
 The first three are also what a model given to ``kiln.compile`` or
 ``torch.compile(backend=kiln.backend)`` may call: they are the operators

@@ -240,6 +240,23 @@ def test_many_rows_over_long_caches(act, dim, tree):
         assert not torch.isfinite(got[0, 0, :, 32:64]).any() and torch.isfinite(got[0, 1:]).all() and torch.isfinite(got[0, 0, :, :32]).all()
 
 
+@pytest.mark.parametrize("draft,heads,lengths,more", [
+    (1, 4, (150, 90), {}), (7, 2, (150, 90), {}), (7, 4, (150, 90), dict(window=60, sinks=5)),
+    (26, 8, (4300, 4200), {}), (26, 8, (4300, 4200), dict(window=4160, sinks=33))], ids=["one", "few", "window", "wide", "wide-window"])
+def test_blocks_that_are_nan(draft, heads, lengths, more):
+    # whichever kernel reads them, in whole tiles, the last one and one on a window's edge
+    p = ref.problem(gen(15), act=torch.bfloat16, batch=2, draft=draft, heads=heads, kv=2, dim=64, page=64, lengths=lengths, device="cuda")
+    for s, n in enumerate(lengths):
+        seen = [n - 1, n - 30, n - 50] + ([] if s == 0 else [70 if "window" not in more else n - more["window"] + 1])
+        for t in seen:                     # values of one head's second block
+            p["v_pages"][int(p["table"][s, t // 64]), 0].view(-1)[ref.places(t % 64, 32, 64, 64, False)[1]] = 255
+    page = int(p["table"][1, (lengths[1] - 20) // 64])
+    p["k_pages"][page, 1].view(-1)[ref.places((lengths[1] - 20) % 64, 0, 64, 64, True)[1]] = 255
+    got = check(p, **more).view(2, draft, 2, heads // 2, 64)
+    assert torch.isnan(got[:, :, 0, :, 32:]).all() and torch.isnan(got[1, :, 1]).all()
+    assert torch.isfinite(got[:, :, 0, :, :32]).all() and torch.isfinite(got[0, :, 1]).all()
+
+
 # -- windows ---------------------------------------------------------------------------------------
 
 
