@@ -10,12 +10,20 @@ import torch
 import kiln
 import packed_reference as ref
 import test_verify
+from kiln.hip import lib as kl
 
 pytestmark = pytest.mark.gpu
 
 
 def gen(seed=0):
     return torch.Generator().manual_seed(seed)
+
+
+def workspace(batch, n, vocab, type=kl.TYPE_F32):
+    """Bytes of a call's workspace: where there are some, the first sums are a launch of their own."""
+    size = kl.ctypes.c_size_t()
+    kl.check(kl.load().kh_verify_workspace_bytes(kl.Verify(batch, n, vocab, type), size), "")
+    return size.value
 
 
 def check(p):
@@ -36,6 +44,18 @@ def test_sizes(dtype, tree, probs, batch, n, vocab):
     check(dict(p, tokens=p["tokens"].to(torch.int32), uniforms=p["uniforms"].double()))
 
 
+# More than 65536 tokens: the first sums of few sequences are a launch of their own.
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tree", [True, False], ids=["tree", "chain"])
+@pytest.mark.parametrize("probs", [True, False], ids=["probs", "sampled"])
+@pytest.mark.parametrize("batch,n,vocab", [(1, 1, 65537), (3, 7, 70001), (2, 5, 128000)])
+def test_first_sums_beforehand(dtype, tree, probs, batch, n, vocab):
+    assert workspace(batch, n, vocab)
+    p = ref.drafted(gen(n), batch, n, vocab, dtype, tree, probs, device="cuda")
+    check(p)
+    check(dict(p, tokens=p["tokens"].to(torch.int32), uniforms=p["uniforms"].double()))
+
+
 @pytest.mark.parametrize("probs", [True, False], ids=["probs", "sampled"])
 def test_large_vocabulary(probs):
     # more stretches than are kept: longer ones
@@ -49,6 +69,54 @@ def test_refused_often():
         p = ref.drafted(gen(2), batch, 30, 700, noise=3.0, device="cuda")
         counts = check(p)[1]
         assert 1 <= int(counts.max()) < 30
+
+
+def test_refused_often_beside_the_first_sums():
+    # several refusals under one token, and tokens kept after a refusal, behind sums that were made beforehand
+    p = ref.drafted(gen(2), 4, 30, 70001, noise=3.0, device="cuda")
+    assert workspace(4, 30, 70001)
+    counts = check(p)[1]
+    assert 1 <= int(counts.max()) < 30
+    # the root's children 1 to 4 are refused, 5 is kept; 6 and 7, its own, too are refused and kept
+    p["parents"][0] = torch.tensor([-1, 0, 0, 0, 0, 0, 5, 5] + [7] * 22)
+    p["uniforms"][0, 1:5], p["uniforms"][0, 6] = 1.0, 1.0
+    p["uniforms"][0, 5], p["uniforms"][0, 7], p["uniforms"][0, 8:] = 0.0, 0.0, 1.0
+    for i, up in ((5, 0), (7, 5)):        # (something is left of these)
+        p["tokens"][0, i] = (p["target"][0, up] - 3 * p["draft"][0, up]).argmax()
+    for i, up in ((1, 0), (2, 0), (3, 0), (4, 0), (6, 5)):
+        p["tokens"][0, i] = p["draft"][0, up].argmax()
+        p["draft"][0, up, p["tokens"][0, i]] += p["target"][0, up, p["tokens"][0, i]]
+    rows, counts, _ = check(p)
+    assert rows[0].tolist()[:3] == [0, 5, 7]
+
+
+def test_unused_and_odd_tokens_beside_the_first_sums():
+    for probs in (True, False):
+        p = ref.drafted(gen(3), 5, 6, 70001, probs=probs, device="cuda")
+        p["parents"] = torch.tensor([[-2, 0, 0, 1, 2, 3], [-1, -1, -1, 0, 1, 2], [-1, 1, 5, 0, -7, 3], [0, 0, 0, 0, 0, 0], [-1, 0, 0, 0, 0, 0]],
+                                    dtype=torch.int32, device="cuda")
+        p["tokens"][4] = torch.tensor([0, -1, 70001, 2 ** 40, 3, 3])
+        counts = check(p)[1]
+        assert counts[0] == 0 and counts[3] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_odd_probabilities_beside_the_first_sums(dtype):
+    for probs in (True, False):
+        p = ref.drafted(gen(4), 7, 4, 70001, dtype, probs=probs, tree=False, device="cuda")
+        p["target"][0] = 0.0
+        p["target"][1, :, ::2] = math.nan
+        p["target"][2, :, 3] = math.inf
+        p["target"][3] *= -1.0
+        p["target"][4] = p["target"][4] * 0
+        p["target"][4, :, 69999] = 1.0
+        p["uniforms"][5] = torch.tensor([1.0, 0.0, math.nan, -3.0])
+        p["uniforms"][6] = 1.0 - 2.0 ** -24
+        if probs:
+            p["draft"][1, :, 5] = math.nan
+            p["draft"][6] = p["target"][6]
+            p["uniforms"][6] = 1.0
+        assert check(p)[2].tolist()[0] == -1
 
 
 def test_unused_and_odd_tokens():
@@ -134,6 +202,33 @@ def test_graph_and_streams():
         for a, b, c in zip(out, eager, ref.verify(**q)):
             assert a.tolist() == b.tolist() == c
         assert all(torch.equal(a, b) for a, b in zip(second, eager2))
+
+
+def test_graph_with_workspaces():
+    # two calls with a workspace each in one graph, and a second graph of one call: nothing is shared
+    sizes = (4, 6, 70001)
+    assert workspace(*sizes)
+    p, q = (ref.drafted(gen(i), *sizes, device="cuda") for i in (7, 17))
+    more = [ref.drafted(gen(8 + i), *sizes, device="cuda") for i in range(3)]
+    kiln.verify_tokens(**p)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.cuda.graph(graphs[0]):
+        first = kiln.verify_tokens(**p)
+        second = kiln.verify_tokens(**dict(p, draft=None))
+    with torch.cuda.graph(graphs[1]):
+        third = kiln.verify_tokens(**q)
+    for x in more:
+        for name, t in p.items():
+            t.copy_(x[name])
+        graphs[0].replay()
+        graphs[1].replay()
+        eager = kiln.verify_tokens(**p), kiln.verify_tokens(**dict(p, draft=None)), kiln.verify_tokens(**q)
+        torch.cuda.synchronize()
+        for got, want in zip((first, second, third), eager):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert [t.tolist() for t in first] == list(ref.verify(**x))
+    assert [t.tolist() for t in third] == list(ref.verify(**{k: t.cpu() for k, t in q.items()}))
 
 
 def test_as_an_operator_of_torch():

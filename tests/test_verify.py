@@ -158,6 +158,21 @@ def test_refusals(interpreting):
     assert rows.shape == (0, 3) and counts.shape == after.shape == (0,)
 
 
+def test_transforms_are_refused(interpreting):
+    from torch.autograd import forward_ad
+
+    p = ref.drafted(gen(), 2, 3, 7)
+    kiln.verify_tokens(**p)
+    for name, t in p.items():
+        with pytest.raises(RuntimeError):
+            torch.vmap(lambda t: kiln.verify_tokens(**dict(p, **{name: t})))(torch.stack([t] * 2))
+    for name in ("target", "uniforms", "draft"):
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(lambda t: kiln.verify_tokens(**dict(p, **{name: t}))[0].float(), (p[name],), (p[name],))
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            kiln.verify_tokens(**dict(p, **{name: forward_ad.make_dual(p[name], p[name])}))
+
+
 def test_no_cpu_path():
     with pytest.raises(NotImplementedError):
         kiln.verify_tokens(**ref.drafted(gen(), 2, 3, 7))
