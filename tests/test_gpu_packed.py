@@ -240,6 +240,67 @@ def test_many_rows_over_long_caches(act, dim, tree):
         assert not torch.isfinite(got[0, 0, :, 32:64]).any() and torch.isfinite(got[0, 1:]).all() and torch.isfinite(got[0, 0, :, :32]).all()
 
 
+def shared_cache(batch, draft, heads, kv, dim, page, length, act, spare=3):
+    """Sequences of equal length on the same pages, and their cached keys and values in 64 bits, [tokens, kv, dim]."""
+    g = gen(length)
+    pages = -(-length // page)
+    p = dict(q=torch.randn(batch, draft, heads, dim, generator=g).to(act), k=torch.randn(batch, draft, kv, dim, generator=g).to(act),
+             v=torch.randn(batch, draft, kv, dim, generator=g).to(act))
+    for name, keys in (("k_pages", True), ("v_pages", False)):
+        p[name] = ref.fast_pack(torch.empty(pages + spare, kv, page, dim), keys)
+    order = torch.randperm(pages + spare, generator=g)[:pages]
+    p["table"] = order.to(torch.int32).expand(batch, pages).contiguous()
+    p["lengths"] = torch.full((batch,), length, dtype=torch.int32)
+    held = [ref.unpack(p[name][order], keys).transpose(1, 2).reshape(-1, kv, dim)[:length] for name, keys in (("k_pages", True), ("v_pages", False))]
+    return {name: t.cuda() for name, t in p.items()}, *held
+
+
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("more", [{}, dict(window=35000, sinks=300)], ids=["all", "window"])
+def test_many_rows_over_ranges_of_many_tiles(act, more):
+    # 128 items of 40000 keys on 512 workgroups: ranges of more than the 128 tiles whose pages are looked up at once, and
+    # whole numbers of them do not end where items do
+    batch, draft, heads, kv, length = 64, 24, 8, 2, 40000
+    p, held_k, held_v = shared_cache(batch, draft, heads, kv, 128, 64, length, act)
+    for s in (0, 13, 63):                  # a stretch of pages that name none
+        p["table"][s, 200:420] = -1
+    got = kiln.tree_attention(**p, **more).double().cpu()
+    there = torch.arange(length)
+    for s, i, h in [(s, i, h) for s in (0, 1, 13, 40, 63) for i in (0, 11, 23) for h in (0, 3, 7)]:
+        c = h // (heads // kv)
+        seen = torch.ones(length, dtype=torch.bool)
+        if s in (0, 13, 63):
+            seen &= (there < 200 * 64) | (there >= 420 * 64)
+        if more:
+            seen &= (there < more["sinks"]) | (there > length + i - more["window"])
+        new_k, new_v = (ref.rounded(p[name][s, :i + 1, c].cpu()) for name in ("k", "v"))
+        kk, vv = torch.cat([held_k[seen, c], new_k]), torch.cat([held_v[seen, c], new_v])
+        want = torch.softmax(kk @ p["q"][s, i, h].double().cpu() / math.sqrt(128), 0) @ vv
+        torch.testing.assert_close(got[s, i, h], want, **tolerance(act))
+
+
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("more", [{}, dict(window=4200, sinks=20)], ids=["all", "window"])
+@pytest.mark.parametrize("tree", [True, False], ids=["tree", "chain"])
+def test_blocks_of_many_rows(act, more, tree):
+    # 300 rows of a head: two blocks of 128 and one that is not full
+    check(ref.problem(gen(16), act=act, batch=2, draft=50, heads=6, kv=1, dim=64, page=64, lengths=(4700, 130), tree=tree, device="cuda"), **more)
+
+
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_rows_over_picked_pages(act, dim):
+    # 104 query heads of one kv head, 70 of 79 pages picked for each token, some lists shorter
+    p = ref.problem(gen(17), act=act, batch=2, draft=2, heads=104, kv=1, dim=dim, page=64, lengths=(5000, 4100), device="cuda")
+    g, sel = gen(18), torch.full((2, 2, 1, 70), -1, dtype=torch.int32)
+    for s, columns in ((0, 79), (1, 65)):
+        for i in range(2):
+            n = min(70, columns) - 9 * i
+            sel[s, i, 0, :n] = torch.randperm(columns, generator=g)[:n].sort().values.to(torch.int32)
+    sel[0, 0, 0, 10] = sel[0, 0, 0, 9]     # named twice: counts once
+    check(p, selected=sel.cuda())
+
+
 @pytest.mark.parametrize("draft,heads,lengths,more", [
     (1, 4, (150, 90), {}), (7, 2, (150, 90), {}), (7, 4, (150, 90), dict(window=60, sinks=5)),
     (26, 8, (4300, 4200), {}), (26, 8, (4300, 4200), dict(window=4160, sinks=33))], ids=["one", "few", "window", "wide", "wide-window"])
@@ -255,6 +316,47 @@ def test_blocks_that_are_nan(draft, heads, lengths, more):
     got = check(p, **more).view(2, draft, 2, heads // 2, 64)
     assert torch.isnan(got[:, :, 0, :, 32:]).all() and torch.isnan(got[1, :, 1]).all()
     assert torch.isfinite(got[:, :, 0, :, :32]).all() and torch.isfinite(got[0, :, 1]).all()
+
+
+def test_fork_and_compact():
+    # pages of 17-byte rows: shared, copied when one of their sequences writes to them, moved to the front of the pool
+    g = gen(19)
+    cache = kiln.PagedCache(2, 12, 16, 2, 32, dtype=torch.float4_e2m1fn_x2, means=True, device="cuda")
+    first = cache.open()
+
+    def tokens(seqs, n):
+        k, v = (torch.randn(2, len(seqs), n, 2, 32, generator=g) for _ in "kv")
+        cache.append(seqs, k.cuda(), v.cuda())
+        for i, s in enumerate(seqs):
+            held[s] = tuple(torch.cat([old, ref.rounded(t[:, i])], 1) for old, t in zip(held[s], (k, v)))
+
+    def check_all():
+        got = cache.read(list(held), dtype=torch.float32)
+        for j, s in enumerate(held):
+            n = cache.length(s)
+            for t, want in zip(got, held[s]):
+                assert torch.equal(t[:, j, :n].double().cpu(), want) and not t[:, j, n:].any()
+            for column, page in enumerate(cache.pages_of(s)):
+                mean = held[s][0][:, 16 * column:16 * (column + 1)].mean(1)
+                torch.testing.assert_close(cache.means[:, page].double().cpu(), mean, rtol=0, atol=16 * 2 ** -24 * 8)
+
+    held = {first: (torch.zeros(2, 0, 2, 32, dtype=torch.float64),) * 2}
+    other = cache.open()
+    held[other] = held[first]
+    tokens([first, other], 39)
+    made = cache.fork(first, 2)
+    for s in made:
+        held[s] = held[first]
+    assert cache.free_pages == 6
+    tokens([made[0], first], 5)            # both write to a page that three have
+    assert cache.free_pages == 4
+    check_all()
+    cache.free(other)
+    del held[other]
+    assert cache.compact() == 5 and max(p for s in held for p in cache.pages_of(s)) == 4
+    check_all()
+    tokens([*made, first], 20)
+    check_all()
 
 
 # -- windows ---------------------------------------------------------------------------------------
@@ -330,6 +432,20 @@ def test_compiled_block(precision, cache, window, sinks):
         x = args[0].double() + block.c_proj(y.reshape(6, 128))
         want = x + block.proj(torch.nn.functional.gelu(block.fc(block.ln2(x)), approximate="tanh"))
         torch.testing.assert_close(got[0].double().cpu(), want, rtol=2e-2, atol=2e-2)
+
+
+def test_compiled_block_of_many_rows():
+    # fp32 activations rounded to bf16 once, over 4-bit pages: rows that share tiles
+    block = test_packed.gpt2_init_(test_packed.Block(128, 2, 16), seed=4).eval()
+    args = test_packed.block_operands(d=128, seqs=1, tokens=100, lengths=(4300,))
+    on_gpu = tuple(t.cuda() for t in args)
+    compiled = kiln.compile(test_packed.WindowBlock(block, 100), (args[0], *on_gpu[1:]), device="cuda", matmul_precision="bf16")
+    got = compiled(*on_gpu)
+    q = block.double().c_attn(block.ln1(args[0].double())).detach()[:, :128].view(1, 100, 2, 64)
+    y = ref.attention(q.float(), got[1].float(), got[2].float(), *args[1:])
+    x = args[0].double() + block.c_proj(y.reshape(100, 128))
+    want = x + block.proj(torch.nn.functional.gelu(block.fc(block.ln2(x)), approximate="tanh"))
+    torch.testing.assert_close(got[0].double().cpu(), want, rtol=2e-2, atol=2e-2)
 
 
 def test_compiled_block_in_a_callers_graph():

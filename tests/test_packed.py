@@ -203,6 +203,24 @@ def test_limits_of_other_caches(interpreting, cache, act):
         assert of(kl.TYPE_F32, act, tokens, batch=4096, heads=1, kv_heads=1, variant=kl.PAGED_SELECT) == want
 
 
+def test_transforms_are_refused(interpreting):
+    from torch.autograd import forward_ad
+
+    p = ref.problem(gen(), cache=torch.float32)
+    zero = torch.zeros(2, dtype=torch.int32)
+    read = dict(k_pages=p["k_pages"], v_pages=p["v_pages"], table=p["table"], starts=zero, ends=zero + 4, tokens=4)
+    kiln.cache_read(**read)                # (the form of a call that is known does not pass either)
+    for name in ("k_pages", "table", "ends"):
+        with pytest.raises(RuntimeError):
+            torch.vmap(lambda t: kiln.cache_read(**dict(read, **{name: t})))(torch.stack([read[name]] * 2))
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda t: kiln.cache_read(**dict(read, k_pages=t))[0], (p["k_pages"],), (p["k_pages"],))
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        kiln.cache_read(**dict(read, v_pages=forward_ad.make_dual(p["v_pages"], p["v_pages"])))
+    with pytest.raises(NotImplementedError):
+        torch.func.grad(lambda t: kiln.cache_read(**dict(read, k_pages=t))[0].sum())(p["k_pages"])
+
+
 def test_no_cpu_path():
     p = ref.problem(gen())
     with pytest.raises(NotImplementedError):
