@@ -248,7 +248,10 @@ MOST_FORMS = 4096
 
 def _keep(key, found):
     while len(_forms) >= MOST_FORMS:
-        _forms.pop(next(iter(_forms)), None)
+        try:
+            _forms.pop(next(iter(_forms)), None)
+        except (RuntimeError, StopIteration):   # another thread changed them meanwhile
+            pass
     _forms[key] = found
     return found
 

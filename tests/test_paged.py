@@ -472,6 +472,37 @@ def test_strides_past_32_bits_are_refused(interpreting):
     assert lib.kh_paged_workspace_bytes(op, size) == kl.ERR_UNSUPPORTED
 
 
+def test_kept_forms_of_several_threads(monkeypatch):
+    # the oldest goes where there are too many, while other threads do the same
+    import sys
+    import threading
+
+    from kiln.hip import paged
+
+    monkeypatch.setattr(paged, "MOST_FORMS", 4)
+    monkeypatch.setattr(paged, "_forms", {})
+    bad = []
+
+    def keep(i):
+        try:
+            for j in range(30000):
+                paged._keep((i, j), j)
+        except Exception as why:
+            bad.append(why)
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=keep, args=(i,)) for i in range(6)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    assert not bad and len(paged._forms) <= 4 + 6
+
+
 def test_a_cache_whose_append_fails_is_as_before(interpreting, monkeypatch):
     from kiln.hip import paged
 
