@@ -700,11 +700,12 @@ def check_read(k_pages, v_pages, table, starts, ends, tokens):
 
 def run_read(k_pages, v_pages, table, starts, ends, tokens, dtype):
     try:
-        key = ("read", _form(k_pages, v_pages, table, starts, ends), tokens, dtype)
+        # (without the number of tokens: sequences that are read as they grow have one form)
+        key = ("read", _form(k_pages, v_pages, table, starts, ends), dtype)
     except AttributeError:
         check_read(k_pages, v_pages, table, starts, ends, tokens)
         raise
-    found = _forms.get(key)
+    found = _forms.get(key) if 0 < tokens < 2 ** 31 else None
     if found is None:
         shape = check_read(k_pages, v_pages, table, starts, ends, tokens)
         _no_grad(k_pages, v_pages)
@@ -721,22 +722,23 @@ def run_read(k_pages, v_pages, table, starts, ends, tokens, dtype):
         if k_pages.shape[-4] == 0:
             raise ValueError("the cache has no pages")
         _ready(k_pages.device)
-        op = kl.CacheRead(k_pages.shape[0] if rank == 5 else 1, table.shape[0], tokens, k_pages.shape[-3], shape[-1],
+        op = kl.CacheRead(k_pages.shape[0] if rank == 5 else 1, table.shape[0], 0, k_pages.shape[-3], shape[-1],
                           k_pages.shape[-2], k_pages.shape[-4], table.shape[1], CACHE_TYPES[k_pages.dtype], TYPES[dtype],
                           None, None, None, None, None, None, None, ks[0] if rank == 5 else 0, *ks[rank - 4:-1],
                           vs[0] if rank == 5 else 0, *vs[rank - 4:-1], table.stride(0))
-        found = _keep(key, (bytes(op), shape))
+        found = _keep(key, (bytes(op), shape[:-3], shape[-2:]))
     elif k_pages.device.type != "cuda" and not interpreting():
         _one_device(k_pages)
     if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad):
         _no_grad(k_pages, v_pages)
     op = kl.CacheRead.from_buffer_copy(found[0])
+    op.tokens = tokens
     op.k_pages, op.v_pages = at = (k_pages.data_ptr(), v_pages.data_ptr())
     if (at[0] | at[1]) & 15:
         _rows_in_place(k_pages, "k_pages")
         _rows_in_place(v_pages, "v_pages")
     device = k_pages.device
-    k = torch.empty(found[1], dtype=dtype, device=device)
+    k = torch.empty((*found[1], tokens, *found[2]), dtype=dtype, device=device)
     v = torch.empty_like(k)
     op.k, op.v, op.table, op.starts, op.ends = k.data_ptr(), v.data_ptr(), table.data_ptr(), starts.data_ptr(), ends.data_ptr()
     lib = kl.load()

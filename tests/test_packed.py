@@ -101,6 +101,24 @@ def test_append_and_read(interpreting, dim, page):
     assert torch.equal(one[0], kiln.cache_read(k_pages, v_pages, table, starts, ends, tokens=5)[0][1])
 
 
+def test_reads_as_a_sequence_grows(interpreting, monkeypatch):
+    # one kept form, whatever the number of tokens: a long-lived program's reads push no other operator's out
+    from kiln.hip import paged
+
+    monkeypatch.setattr(paged, "_forms", {})
+    p = ref.problem(gen(6), cache=torch.bfloat16, lengths=(40, 17))
+    starts = torch.zeros(2, dtype=torch.int32)
+    pages = p["k_pages"], p["v_pages"]
+    want = ref.read(*(t[None] for t in pages), p["table"], starts, p["lengths"], 45)
+    for n in [*range(1, 46), 0, 7]:
+        got = kiln.cache_read(*pages, p["table"], starts, p["lengths"], tokens=n)
+        assert all(torch.equal(a.double(), b[0, :, :n]) for a, b in zip(got, want))
+    assert len(paged._forms) == 1
+    for n in (-1, 2 ** 31):
+        with pytest.raises(ValueError):
+            kiln.cache_read(*pages, p["table"], starts, p["lengths"], tokens=n)
+
+
 @pytest.mark.parametrize("cache", [torch.float32, torch.bfloat16, torch.float16])
 def test_read_of_other_types(interpreting, cache):
     g = gen(5)
