@@ -88,7 +88,8 @@ def run_verify(tokens, target, uniforms, parents, draft):
     device = tokens.device
     batch, n = op.batch, op.draft
     # (memory of their own: one that is kept or saved keeps no other, nor the workspace)
-    rows, counts, after = (tokens.new_empty(shape, dtype=torch.int32) for shape in ((batch, n), (batch,), (batch,)))
+    rows = tokens.new_empty((batch, n), dtype=torch.int32)
+    counts, after = rows.new_empty(batch), rows.new_empty(batch)
     if batch == 0:
         return rows, counts, after
     op.tokens, op.target, op.uniforms = tokens.data_ptr(), target.data_ptr(), uniforms.data_ptr()
