@@ -654,7 +654,8 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     u32x4 q16[F32 ? 1 : NQ][RT][KS];
     float q32[F32 ? RT : 1][F32 ? KS : 1][8];
     // products to the base-2 domain; positive, so that a masked -inf stays one: q
-    // takes a negative scale's sign, and a scale of zero is the smallest number
+    // takes a negative scale's sign, or a zero (so that 0 inf is NaN), under which
+    // the smallest number does
     float mult[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -668,7 +669,7 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[ks][j] = in ? y[ks][j] : 0.0f;
       }
-      float up = wq.scale2 < 0.0f ? -1.0f : 1.0f;
+      float up = wq.scale2 > 0.0f ? 1.0f : wq.scale2 < 0.0f ? -1.0f : wq.scale2;
       mult[rt] = fabsf(wq.scale2);
       if constexpr (SCALED_Q) {
         float most = 0.0f;
@@ -1218,7 +1219,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(const PagedWork
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[ks][j] = in ? y[ks][j] : 0.0f;
       }
-      float up = wq.scale2 < 0.0f ? -1.0f : 1.0f;
+      float up = wq.scale2 > 0.0f ? 1.0f : wq.scale2 < 0.0f ? -1.0f : wq.scale2;
       if constexpr (SCALED_Q) {
         float most = 0.0f;
 #pragma unroll

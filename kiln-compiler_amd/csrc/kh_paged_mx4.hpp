@@ -363,10 +363,11 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
     // the query rows' parts
     u32x4 q[NQ][RT][KS];
     // products to the base-2 domain; positive, so that a masked -inf stays one: q
-    // takes a negative scale's sign, and a scale of zero is the smallest number
+    // takes a negative scale's sign, or a zero (so that 0 inf is NaN), under which
+    // the smallest number does
     const_work &wq = fresh();
     const float mult = fmaxf(fabsf(wq.scale2), 0x1p-126f);
-    const float up = wq.scale2 < 0.0f ? -1.0f : 1.0f;
+    const float up = wq.scale2 > 0.0f ? 1.0f : wq.scale2 < 0.0f ? -1.0f : wq.scale2;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll

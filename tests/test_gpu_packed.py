@@ -359,6 +359,24 @@ def test_fork_and_compact():
     check_all()
 
 
+@pytest.mark.parametrize("cache,act", CACHES, ids=IDS)
+@pytest.mark.parametrize("draft,heads,lengths", [(1, 2, (70, 33)), (33, 4, (4300, 200))], ids=["one", "many"])
+def test_a_scale_of_zero(cache, act, draft, heads, lengths):
+    # every key alike; one whose product with the query is not finite makes the row NaN, and no other
+    p = ref.problem(gen(27), cache=cache, act=act, draft=draft, heads=heads, kv=1, dim=64, lengths=lengths, tree=False, device="cuda")
+    for more in (dict(), dict(window=50, sinks=3)):
+        check(p, scale=0.0, **more)
+    p["q"][0, 0, 1, 5] = -math.inf
+    page, slot = int(p["table"][1, (lengths[1] - 1) // 16]), (lengths[1] - 1) % 16
+    if cache == torch.uint8:
+        p["k_pages"][page].view(1, -1)[:, ref.places(slot, 0, 64, 16, True)[1]] = 255
+    else:
+        p["k_pages"][page, 0, slot, 9] = math.inf
+    for more in (dict(), dict(window=50, sinks=3)):
+        got = check(p, scale=0.0, **more)
+        assert torch.isnan(got[0, 0, 1]).all() and torch.isfinite(got[0, 0, 0]).all() and torch.isnan(got[1]).all()
+
+
 # -- windows ---------------------------------------------------------------------------------------
 
 
