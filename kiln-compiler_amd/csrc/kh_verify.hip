@@ -107,21 +107,18 @@ __host__ __device__ inline float draft_counted(float x) { return __builtin_eleme
 // The weights that are left of probabilities p: a refusal at a time for all, so that
 // what it took is read once.
 template <int STEPS, int N>
-__device__ __forceinline__ void weigh(const float (&p)[STEPS][N], float (&q)[STEPS][N], const double *took, int refusals, double (&v)[STEPS][N]) {
+__device__ __forceinline__ void weigh(const float (&p)[STEPS][N], const float (&q)[STEPS][N], const double *took, int refusals, double (&v)[STEPS][N]) {
 #pragma unroll
   for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      v[i][e] = target_counted(p[i][e]);
-      if (refusals) q[i][e] = draft_counted(q[i][e]);
-    }
+    for (int e = 0; e < N; ++e) v[i][e] = target_counted(p[i][e]);
   for (int j = 0; j < refusals; ++j) {
     const double r = took[j];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const double left = v[i][e] - r * q[i][e];
+        const double left = v[i][e] - r * draft_counted(q[i][e]);
         v[i][e] = left > 0.0 ? left : 0.0;
       }
   }
