@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const kh_cache_append_
 
 // Append into 4-bit pages: as append_kernel, the 4 lanes of a block agree on its
 // largest. The mean is that of the values stored. 12 layers of 16 prompts of 256
-// tokens, 8 heads of 128, bf16: 255 MB in 64 to 83 us (3.1 to 4 TB/s), bound by
+// tokens, 8 heads of 128, bf16: 255 MB in 84 us (3 TB/s; 65 and 3.9 at best), bound by
 // the rows' loads; 1 or 4 rows ahead (kPair) were no faster than 2.
 template <int AT>
 __global__ __launch_bounds__(kThreads) void append_mx4_kernel(const kh_cache_append_op a) {

@@ -1042,9 +1042,9 @@ __global__ __launch_bounds__(64 * paged_waves(DT, RT, WHOLE), RT * DT > 128 ? 1 
 //
 // Over 4-bit pages threads make a tile's bf16 values out of codes that were loaded
 // a tile before, where other caches copy to the LDS; q of fp16 takes two bf16 parts. 64
-// tokens of 4 sequences, 32 query heads on 4 of 128, up to 32768 tokens, fp16: 230
-// to 237 us and 13 for the join (8 more with split8, which is for caches that hold
-// infinities), 55% of the rate of a large matrix product. Without gain: one wave a SIMD
+// tokens of 4 sequences, 32 query heads on 4 of 128, up to 32768 tokens, fp16: 235
+// to 242 us (228 at best) and 13.5 for the join (8 more with split8, which is for caches
+// that hold infinities), 53% of the rate of a large matrix product. Without gain: one wave a SIMD
 // (292), the products' operands read a step ahead (231 to 238).
 
 // Chunk swizzle of K and V rows in the LDS, 16-byte chunks: a 128-bit read

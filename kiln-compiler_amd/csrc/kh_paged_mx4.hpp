@@ -17,8 +17,8 @@
 //   new tokens are rounded once an item, into pages of their own in the LDS.
 //
 // What it measured (one token, 8 kv heads of 128, 32 query heads, bf16): one
-// sequence of 131072 tokens 32.6 us, 4.4 TB/s of the 5.2 that a copy reaches; 32
-// ragged ones up to 8192, 41.5 us, 3.6 TB/s. What is missing is beginning and
+// sequence of 131072 tokens 33 us, 4.3 TB/s of the 5.2 that a copy reaches; 32
+// ragged ones up to 8192, 41.5 us, 3.6 TB/s (medians; 31.3 and 38.8 at best). What is missing is beginning and
 // ending an item, a chain of dependent loads (length, page, codes) and a join,
 // which kMxLead counts. Cached and new tokens' tiles are loops of their own, and
 // the cached one always asks for a next tile: while a wave could meet either, the

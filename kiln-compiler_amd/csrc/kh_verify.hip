@@ -14,7 +14,7 @@
 // sequence with a wave per stretch beforehand: 64 chains over 128000 tokens of
 // fp32 14.6 us (the target's and the draft's row, 4.5 TB/s of the 5.2 that a copy
 // reaches) and 7.8 us for the walk, two dependent looks into the sums and one
-// stretch. One chain of 5 over 50257: 10.4 us, one workgroup reading 400 KB; 32
+// stretch. One chain of 5 over 50257: 10.8 us, one workgroup reading 400 KB; 32
 // trees without the draft's probabilities, 2.3 rows a path one after the other:
 // 13 us. The sums of 64 bits cost what the loads wait for anyway; sums between
 // lanes by permutes through the LDS took 3 to 5 us more.
@@ -444,7 +444,7 @@ VerifyWork work_of(const kh_verify_op &p) {
 
 // Sequences that leave compute units without work have the first sums of all
 // made beforehand, where that is more than four stretches a wave: a row of 50257 fp32
-// probabilities (and the draft's) takes one workgroup 10.5 us in all, 4.6 and 5.1
+// probabilities (and the draft's) takes one workgroup 10.8 us in all, 4.6 and 5.1
 // in two launches; 64 rows of 128000 23.0, and 14.3 and 7.9 us.
 bool ahead(const kh_verify_op &p) { return p.batch < current_device().cus && work_of(p).stretches > 4 * (kThreads / 64); }
 
